@@ -34,6 +34,12 @@ class DsMoeDesc(Structure):
                 ("out_f32", c_int32)]
 
 
+class DsGatedFfn(Structure):
+    _fields_ = [("tokens", c_int64), ("hidden", c_int32), ("inter", c_int32), ("dtype", c_int32), ("limit", c_float),
+                ("x", c_void_p), ("w1", c_void_p), ("w3", c_void_p), ("w2", c_void_p),
+                ("ld_x", c_int64), ("ld_w1", c_int64), ("ld_w3", c_int64), ("ld_w2", c_int64)]
+
+
 # name -> (restype, argtypes); every symbol include/deepseeker_b200.h declares
 SIGNATURES: dict[str, tuple] = {
     "ds_last_error_string": (c_char_p, []),
@@ -83,6 +89,12 @@ SIGNATURES: dict[str, tuple] = {
                              c_void_p, c_void_p, c_size_t, c_void_p]),
     "ds_ep_status": (c_int, [c_void_p, POINTER(c_int32)]),
     "ds_ep_destroy": (c_int, [c_void_p]),
+    "ds_gated_ffn_workspace_size": (c_int, [POINTER(DsGatedFfn), c_int, POINTER(c_size_t)]),
+    "ds_gated_ffn": (c_int, [POINTER(DsGatedFfn), c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "ds_gated_ffn_backward_workspace_size": (c_int, [POINTER(DsGatedFfn), c_void_p, c_int64, POINTER(c_size_t)]),
+    "ds_gated_ffn_backward": (c_int, [POINTER(DsGatedFfn), c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
+                                      c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "ds_gated_ffn_status": (c_int, [c_void_p, c_void_p]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -416,6 +416,50 @@ int ds_ep_decode(DsEp* ep, const DsMoeDesc* desc, int32_t first_expert, const vo
 int ds_ep_status(DsEp* ep, int32_t* err);
 int ds_ep_destroy(DsEp* ep);
 
+/* ---------------------------------------------------------------------------
+ * Dense gated feed-forward block over 16-bit weights, forward and backward
+ * (the shared expert of a layer, or a layer without routing; the reference's
+ * is four separate products, src/deepseeker/mlx_runner.py:776-781, and has no
+ * backward pass):
+ *   g = x W1^T, u = x W3^T, h = silu(min(g, L)) * clip(u, -L, L), y = h W2^T.
+ * Products accumulate in f32; h and the gradients of g and u are rounded once
+ * to the 16-bit type, g and u are kept in f32 between the passes.  NaN passes
+ * through the clamps.  Any sizes, row strides and 2-byte alignments; operands
+ * whose base is no multiple of 16 bytes or whose row stride is no multiple of
+ * 8 elements are first copied into the workspace.  Results do not depend on
+ * timing (no atomics). */
+typedef struct DsGatedFfn {
+  int64_t tokens;             /* T, 0 <= T <= 2^22                                 */
+  int32_t hidden, inter;      /* H, I, 1 .. 2^17                                   */
+  int32_t dtype;              /* DS_BF16 or DS_F16: x, weights, y, gradients        */
+  float limit;                /* L > 0, or 0: no clamps                            */
+  const void* x;              /* [T, H], rows ld_x elements apart                   */
+  const void* w1;             /* [I, H] gate                                       */
+  const void* w3;             /* [I, H] up                                         */
+  const void* w2;             /* [H, I] down                                       */
+  int64_t ld_x, ld_w1, ld_w3, ld_w2;
+} DsGatedFfn;
+
+/* Workspace bytes of ds_gated_ffn; keeps_h: the call gets an h buffer. */
+int ds_gated_ffn_workspace_size(const DsGatedFfn* desc, int keeps_h, size_t* bytes);
+/* y [T, H] contiguous.  For a later backward pass: h [T, Ip] 16 bit and
+ * pre [2][T, Ip] f32 (g, then u), Ip = inter rounded up to a multiple of 8
+ * (columns from inter on are not written); both NULL otherwise. */
+int ds_gated_ffn(const DsGatedFfn* desc, void* y, void* h, float* pre, void* workspace,
+                 size_t workspace_bytes, void* stream);
+
+/* Backward pass from dy [T, H] (rows ld_dy elements apart) and the h and pre
+ * that ds_gated_ffn left: dx [T, H], dw1 and dw3 [I, H], dw2 [H, I], each
+ * contiguous and 16 bit; NULL skips one, with the products only it needs. */
+int ds_gated_ffn_backward_workspace_size(const DsGatedFfn* desc, const void* dy, int64_t ld_dy, size_t* bytes);
+int ds_gated_ffn_backward(const DsGatedFfn* desc, const void* h, const float* pre, const void* dy,
+                          int64_t ld_dy, void* dx, void* dw1, void* dw3, void* dw2, void* workspace,
+                          size_t workspace_bytes, void* stream);
+/* Copies the current device's error word of these calls into *err (host or
+ * device memory; read it after the stream has finished) and clears it.  Bit 1:
+ * a bounded device wait gave up, and that call's outputs are undefined. */
+int ds_gated_ffn_status(int32_t* err, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
