@@ -1,0 +1,596 @@
+// Microscaled 4-bit dense operators: quantisation of activations, the product
+// of two quantised matrices and the gated feed-forward block over quantised
+// weights.
+//
+// Product y[n, m] = sum_k x[n, k] W[m, k] on tcgen05 kind::mxf4: packed codes
+// straight from memory (two per byte, K-major, 128-byte swizzle), both scale
+// sets in tensor memory, f32 accumulate.  Products of two codes and a power
+// of two are exact, so the only error is that of the f32 sums.
+//
+// Tile kernel: one CTA computes 128 features (lanes) x NT rows of x over a
+// slice of the contraction; the slices of a tile are the CTAs of a cluster
+// and are added in slice order through distributed shared memory.  In the
+// gated block 32 consecutive lanes are one block of h, so a warp quantises it
+// with one maximum over its lanes.
+#include <algorithm>
+#include <cooperative_groups.h>
+#include <string.h>
+
+#include "mx4.cuh"
+
+namespace ds {
+namespace mx4 {
+namespace {
+
+namespace cg = cooperative_groups;
+
+__device__ int g_err;   // bit 1: a bounded wait gave up
+
+// ---------------------------------------------------------------- quantisation
+
+template <typename T>
+__device__ __forceinline__ float load_one(const T* p) {
+  if constexpr (sizeof(T) == 4) return *p;
+  else if constexpr (std::is_same<T, __half>::value) return __half2float(*p);
+  else return __bfloat162float(*p);
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+      } else {
+        v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      }
+    }
+  }
+}
+
+// A thread takes 8 values, four neighbours a block: a 16-byte load (two in
+// f32), a maximum over four lanes and a 4-byte store each, so a warp's loads
+// and code stores are whole lines.  `slab` rows per CTA.
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ld,
+                                                       int vec, int slab, uint32_t* __restrict__ packed,
+                                                       uint8_t* __restrict__ scales, uint8_t* __restrict__ atoms) {
+  launch_dependents();
+  const int blocks = (cols + 31) / 32, per_row = blocks * 4, chunks = (blocks + 3) / 4;
+  const int64_t r0 = (int64_t)blockIdx.x * slab;
+  const int count = (int)min((int64_t)slab, rows - r0) * per_row;
+  for (int i = threadIdx.x; i < (count + 31) / 32 * 32; i += blockDim.x) {
+    const int r = i / per_row, g = i - r * per_row;
+    const int64_t row = r0 + r;
+    const bool live = i < count;
+    const T* src = x + row * ld + g * 8;
+    float v[8];
+    if (live && vec && g * 8 + 8 <= cols) {
+      load8(src, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = live && g * 8 + j < cols ? load_one(src + j) : 0.0f;
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    if (!live) continue;
+    const int s = scale_byte(top);
+    const float inv = inv_scale(s);
+    uint32_t w = 0;
+    if (s != 255) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w |= tc5::f32x2_to_e2m1x2(v[2 * j] * inv, v[2 * j + 1] * inv) << (8 * j);
+      w = no_negative_zero(w);
+    }
+    packed[row * per_row + g] = w;
+    if ((g & 3) == 0) {
+      const int b = g >> 2;
+      if (scales) scales[row * blocks + b] = (uint8_t)s;
+      if (atoms) {
+        atoms[atom_at(row, b, chunks)] = (uint8_t)s;
+        if (b == blocks - 1)   // blocks that fill up the last chunk: any scale but NaN
+          for (int e = blocks; e < chunks * 4; ++e) atoms[atom_at(row, e, chunks)] = 0;
+      }
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) scale_atoms_kernel(const uint8_t* __restrict__ scales, int64_t rows, int blocks,
+                                                          uint8_t* __restrict__ atoms) {
+  const int chunks = (blocks + 3) / 4;
+  const int64_t n = rows * chunks;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t row = i / chunks;
+    const int c = (int)(i - row * chunks);
+    uint32_t w = 0;
+    for (int b = 0; b < 4; ++b)
+      if (c * 4 + b < blocks) w |= (uint32_t)scales[row * blocks + c * 4 + b] << (8 * b);
+    *reinterpret_cast<uint32_t*>(atoms + atom_at(row, c * 4, chunks)) = w;
+  }
+}
+
+// ---------------------------------------------------------------- product
+
+enum Mode { LINEAR, GATED };
+
+struct TileParams {
+  CUtensorMap a[2], b;         // weights (gated: W1, W3), rows of x
+  const uint8_t* sa[2];        // their scale atoms
+  const uint8_t* sb;
+  int M, N;                    // features, rows of x
+  int blocks;                  // blocks of 32 along the contraction
+  void* out;                   // LINEAR: out[n * ldo + m]
+  int64_t ldo;
+  int out_dtype;
+  uint8_t* hq;                 // GATED: codes and atoms of h
+  uint8_t* hs;
+  float limit;
+  int* err;
+};
+
+template <int MODE, int NT>
+struct TileShape {
+  static constexpr int kMats = MODE == GATED ? 2 : 1;
+  static constexpr int kOps = kMats * 16384 + NT * 128;              // 256 codes of 128 features and NT rows
+  static constexpr int kSf = (kMats + 1) * 2 * kAtom;
+  static constexpr int kStage = kOps + (kSf + 1023) / 1024 * 1024;
+  static constexpr int kStages = std::min(6, 200 * 1024 / kStage);
+  static constexpr int kSmem = 1024 + kStages * kStage;
+  static constexpr int kAcc = kMats * NT;
+  static constexpr int kSfCols = (kMats + 1) * 8;
+  static constexpr int kNeed = kAcc + 2 * kSfCols;
+  static constexpr int kCols = kNeed <= 64 ? 64 : kNeed <= 128 ? 128 : kNeed <= 256 ? 256 : 512;
+  static_assert(kOps % 1024 == 0 && kStages * kStage >= kMats * NT * 128 * 4, "stages hold the partial tile");
+};
+
+constexpr int kTileThreads = 192;   // warp 0 copies, warp 1 MMA, warps 2-5 epilogue
+
+__device__ __forceinline__ float gate_unit(float g, float u, float limit) {
+  if (limit > 0.0f) {   // comparisons keep a NaN
+    g = g > limit ? limit : g;
+    u = u > limit ? limit : (u < -limit ? -limit : u);
+  }
+  return g / (1.0f + expf(-g)) * u;
+}
+
+// One element of the tile: row n of x, feature m (lane of a full warp).
+template <int MODE>
+__device__ __forceinline__ void tile_store(const TileParams& p, int m, int n, float v0, float v1) {
+  if constexpr (MODE == LINEAR) {
+    if (m >= p.M) return;
+    const int64_t at = (int64_t)n * p.ldo + m;
+    if (p.out_dtype == DS_F32) static_cast<float*>(p.out)[at] = v0;
+    else if (p.out_dtype == DS_F16) static_cast<__half*>(p.out)[at] = __float2half_rn(v0);
+    else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v0);
+  } else {
+    // lanes past the features hold products with unset scales: no part of the block
+    const float h = m < p.M ? gate_unit(v0, v1, p.limit) : 0.0f;
+    const int s = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7FFFFFFFu));
+    const int lane = threadIdx.x & 31, block = m >> 5, blocks = (p.M + 31) / 32, chunks = (blocks + 3) / 4;
+    uint32_t w = s == 255 ? 0u : tc5::f32x2_to_e2m1x2(h * inv_scale(s), 0.0f) & 0xFu;
+    if (w == 8u) w = 0u;
+    w |= __shfl_down_sync(0xffffffffu, w, 1) << 4;
+    if (block < blocks && (lane & 1) == 0) p.hq[((int64_t)n * blocks + block) * 16 + lane / 2] = (uint8_t)w;
+    if (lane == 0) p.hs[atom_at(n, block, chunks)] = (uint8_t)s;
+  }
+}
+
+template <int MODE, int NT>
+__global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_constant__ TileParams p) {
+  using C = TileShape<MODE, NT>;
+  constexpr int S = C::kStages, kMats = C::kMats;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  __shared__ __align__(8) uint64_t full[S], empty[S], accfull;
+  __shared__ uint32_t tmem_base;
+  __shared__ int abort_flag;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int slices = cluster.dim_blocks().x, slice = cluster.block_rank();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int mt = blockIdx.x / slices, m0 = mt * 128, n0 = blockIdx.y * NT;
+  const int chunks = (p.blocks + 3) / 4, ksteps = (chunks + 1) / 2;   // a stage is two chunks of 128 codes
+  const int it0 = (int)((int64_t)ksteps * slice / slices), it1 = (int)((int64_t)ksteps * (slice + 1) / slices);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(&accfull, 1);
+    abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) tc5::alloc(&tmem_base, C::kCols);
+  tc5::fence_before();
+  __syncthreads();
+  tc5::fence_after();
+  const uint32_t tb = tmem_base;
+  volatile int* abort = &abort_flag;
+  launch_dependents();
+  wait_prior_grid();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int g = 0;
+      for (int it = it0; it < it1; ++it, ++g) {
+        const int s = g % S;
+        if (g >= S && !grouped::wait_or_abort(&empty[s], ((g / S) - 1) & 1, abort, p.err)) break;
+        uint8_t* st = smem + s * C::kStage;
+        uint8_t* sf = st + C::kOps;
+        const int na = min(2, chunks - 2 * it);   // atoms of this stage
+        mbar_arrive_expect_tx(&full[s], C::kOps + (kMats + 1) * na * kAtom);
+#pragma unroll
+        for (int t = 0; t < kMats; ++t) {
+          tma_load_2d(st + t * 16384, &p.a[t], it * 128, m0, &full[s]);
+          bulk_g2s(sf + t * 2 * kAtom, p.sa[t] + ((int64_t)mt * chunks + 2 * it) * kAtom, na * kAtom, &full[s]);
+        }
+        tma_load_2d(st + kMats * 16384, &p.b, it * 128, n0, &full[s]);
+        bulk_g2s(sf + kMats * 2 * kAtom, p.sb + ((int64_t)(n0 >> 7) * chunks + 2 * it) * kAtom, na * kAtom, &full[s]);
+      }
+      // never leave with copies in flight into this CTA's shared memory
+      for (int j = g - S < 0 ? 0 : g - S; j < g; ++j) mbar_wait_bounded(&full[j % S], (j / S) & 1, 200000000ull);
+    }
+  } else if (warp == 1) {
+    const uint32_t idesc[2] = {tc5::idesc_mxf4(NT, 0), tc5::idesc_mxf4(NT, 2)};
+    const uint64_t ops = tc5::sdesc_sw128(smem_u32(smem));
+    for (int g = 0; g < it1 - it0; ++g) {
+      const int s = g % S;
+      if (!grouped::warp_wait(&full[s], (g / S) & 1, abort, p.err)) break;
+      tc5::fence_after();
+      if (elect_one()) {
+        const int left = p.blocks - 8 * (it0 + g);     // blocks from this stage on
+        const int steps = min(4, (left + 1) / 2);      // MMAs of 64 codes (two blocks)
+        const uint32_t sf = smem_u32(smem) + s * C::kStage + C::kOps;
+        const uint32_t tsf = tb + C::kAcc + (g & 1) * C::kSfCols;   // [W (, W3), x][two atoms]
+        for (int a = 0; a < (steps + 1) / 2; ++a)
+#pragma unroll
+          for (int t = 0; t <= kMats; ++t) copy_atom(tsf + 4 * (2 * t + a), sf + (2 * t + a) * kAtom);
+        const uint64_t ad = ops + (uint64_t)((s * C::kStage) >> 4), bd = ad + ((kMats * 16384) >> 4);
+        for (int kk = 0; kk < steps; ++kk)
+#pragma unroll
+          for (int t = 0; t < kMats; ++t)
+            tc5::mma_mxf4(tb + t * NT, ad + t * (16384 >> 4) + 2 * kk, bd + 2 * kk, idesc[kk & 1],
+                          tsf + 4 * (2 * t + (kk >> 1)), tsf + 4 * (2 * kMats + (kk >> 1)), (g | kk) != 0);
+        tc5::commit(&empty[s]);
+      }
+      __syncwarp();
+    }
+    // all issued MMAs complete before the accumulators are read or released
+    if (elect_one()) tc5::commit(&accfull);
+    __syncwarp();
+    grouped::warp_wait(&accfull, 0, abort, p.err);
+  } else {
+    grouped::warp_wait(&accfull, 0, abort, p.err);
+  }
+  tc5::fence_after();
+
+  // ---- epilogue: thread = one feature (lane of tensor memory)
+  const int q = warp & 3, mi = q * 32 + lane, m = m0 + mi;
+  const int nv = min(NT, p.N - n0);
+  float* part = reinterpret_cast<float*>(smem);   // [mats][NT][128]
+  if (warp >= 2) {
+    for (int c0 = 0; c0 < nv; c0 += 16) {
+      float v[kMats][16];
+#pragma unroll
+      for (int t = 0; t < kMats; ++t) tc5::ld_x16_nowait(tc5::lane_quarter(tb + t * NT + c0, q), v[t]);
+      tc5::wait_ld();
+      if (slices > 1) {
+#pragma unroll
+        for (int t = 0; t < kMats; ++t)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) part[(t * NT + c0 + j) * 128 + mi] = v[t][j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (c0 + j < nv) tile_store<MODE>(p, m, n0 + c0 + j, v[0][j], v[kMats - 1][j]);
+      }
+    }
+  }
+  if (slices > 1) {
+    cluster.sync();
+    if (warp >= 2) {
+      for (int n = slice; n < nv; n += slices) {
+        float v0 = 0.0f, v1 = 0.0f;
+        for (int r = 0; r < slices; ++r) {
+          const float* src = cluster.map_shared_rank(part, r);
+          v0 += src[n * 128 + mi];
+          if (kMats == 2) v1 += src[(NT + n) * 128 + mi];
+        }
+        tile_store<MODE>(p, m, n0 + n, v0, v1);
+      }
+    }
+    cluster.sync();   // partial tiles stay until every CTA has read them
+  }
+  tc5::fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc5::fence_after();
+    tc5::dealloc(tb, C::kCols);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+
+int64_t blocks_of(int64_t cols) { return (cols + 31) / 32; }
+size_t atoms_bytes(int64_t rows, int64_t cols) {
+  return (size_t)((rows + 127) / 128) * ((cols + 127) / 128) * kAtom;
+}
+size_t packed_bytes(int64_t rows, int64_t cols) { return (size_t)rows * blocks_of(cols) * 16; }
+
+// Codes of a matrix as bytes [rows, 16 blocks]; a box is 128 bytes (256 codes) x box_rows.
+bool map_codes(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int box_rows) {
+  const cuuint64_t dims[2] = {(cuuint64_t)blocks_of(cols) * 16, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)blocks_of(cols) * 16};
+  const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  const cuuint32_t es[2] = {1, 1};
+  return grouped::encode_fn()(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, es,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int* err_word() {
+  void* p = nullptr;
+  return cudaGetSymbolAddress(&p, g_err) == cudaSuccess ? static_cast<int*>(p) : nullptr;
+}
+
+int launch_quantize(const void* x, int dtype, int64_t rows, int cols, int64_t ld, uint8_t* packed, uint8_t* scales,
+                    uint8_t* atoms, cudaStream_t s) {
+  const int per_row = (int)blocks_of(cols) * 4, es = dtype == DS_F32 ? 4 : 2;
+  const int vec = ds::aligned(x, 16) && (rows == 1 || ld * es % 16 == 0);
+  // about four groups of 8 values per thread; one where that leaves SMs idle
+  int slab = std::max(1, 1024 / per_row);
+  if ((rows + slab - 1) / slab < 2 * ds::sm_count()) slab = std::max(1, 256 / per_row);
+  const int64_t grid = (rows + slab - 1) / slab;
+  uint32_t* pk = reinterpret_cast<uint32_t*>(packed);
+  if (dtype == DS_F32)
+    quantize_kernel<<<(unsigned)grid, 256, 0, s>>>(static_cast<const float*>(x), rows, cols, ld, vec, slab, pk, scales,
+                                                   atoms);
+  else if (dtype == DS_F16)
+    quantize_kernel<<<(unsigned)grid, 256, 0, s>>>(static_cast<const __half*>(x), rows, cols, ld, vec, slab, pk,
+                                                   scales, atoms);
+  else
+    quantize_kernel<<<(unsigned)grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(x), rows, cols, ld, vec, slab, pk,
+                                                   scales, atoms);
+  DS_CHECK_LAUNCH("mx4 quantize_kernel");
+  return DS_OK;
+}
+
+template <int MODE, int NT>
+int launch_tiles(const TileParams& p, int slices, cudaStream_t s, bool chained) {
+  using C = TileShape<MODE, NT>;
+  DS_CHECK_CUDA(cudaFuncSetAttribute(tile_kernel<MODE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((p.M + 127) / 128 * slices), (unsigned)((p.N + NT - 1) / NT));
+  cfg.blockDim = dim3(kTileThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)slices;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = chained ? 2 : 1;
+  DS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, tile_kernel<MODE, NT>, p));
+  return DS_OK;
+}
+
+// Rows of x per tile (a single tile below 128, so a tile starts at row 0 of a scale atom).
+int row_tile(int64_t n) { return n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 128; }
+
+template <int MODE>
+int run_tiles(const TileParams& p, int nt, cudaStream_t s, bool chained) {
+  const int64_t tiles = (int64_t)((p.M + 127) / 128) * ((p.N + nt - 1) / nt);
+  const int ksteps = (p.blocks + 7) / 8;
+  int slices = 1;   // enough to give every SM a CTA, at least two stages each
+  while (slices < 8 && tiles * slices * 2 <= ds::sm_count() && ksteps / (slices * 2) >= 2) slices *= 2;
+  if (nt == 16) return launch_tiles<MODE, 16>(p, slices, s, chained);
+  if (nt == 32) return launch_tiles<MODE, 32>(p, slices, s, chained);
+  if (nt == 64) return launch_tiles<MODE, 64>(p, slices, s, chained);
+  return launch_tiles<MODE, 128>(p, slices, s, chained);
+}
+
+int validate_weight(const DsMx4* w, const char* what) {
+  DS_REQUIRE(w && w->packed && w->atoms, DS_EINVAL, "%s: null weight", what);
+  DS_REQUIRE(w->rows >= 1 && w->rows <= (1 << 20) && w->cols >= 1 && w->cols <= (1 << 20), DS_ERANGE,
+             "%s: weight rows and cols must be in [1, 2^20]", what);
+  DS_REQUIRE(ds::aligned(w->packed, 16) && ds::aligned(w->atoms, 16), DS_EALIGN,
+             "%s: weight codes and atoms must be 16-byte aligned", what);
+  return DS_OK;
+}
+
+int validate_x(const void* x, const uint8_t* atoms, int dtype, int64_t rows, int cols, int64_t ld, const char* what) {
+  DS_REQUIRE(dtype == DS_F32 || dtype == DS_BF16 || dtype == DS_F16 || (dtype == DS_U8 && atoms), DS_EINVAL,
+             "%s: x must be f32, bf16 or f16, or codes (u8) with atoms", what);
+  DS_REQUIRE(rows >= 0 && rows <= (1 << 22), DS_ERANGE, "%s: rows must be in [0, 2^22]", what);
+  DS_REQUIRE(rows == 0 || x, DS_EINVAL, "%s: null x", what);
+  DS_REQUIRE(dtype == DS_U8 || rows <= 1 || ld >= cols, DS_EINVAL, "%s: row stride of x below its columns", what);
+  DS_REQUIRE(ds::aligned(x, dtype == DS_U8 ? 16 : dtype == DS_F32 ? 4 : 2) && ds::aligned(atoms, 16), DS_EALIGN,
+             "%s: x must be aligned to its elements, codes and atoms to 16 bytes", what);
+  return DS_OK;
+}
+
+size_t quantized_bytes(int64_t rows, int64_t cols) {
+  return grouped::up(packed_bytes(rows, cols), 256) + grouped::up(atoms_bytes(rows, cols), 256);
+}
+
+// Codes and atoms of x: as given, or quantised into the workspace.
+int quantized_x(const void*& x, const uint8_t*& atoms, int dtype, int64_t rows, int cols, int64_t ld, uint8_t*& ws,
+                cudaStream_t s) {
+  if (dtype == DS_U8) return DS_OK;
+  uint8_t* sa = ws + grouped::up(packed_bytes(rows, cols), 256);
+  const int st = launch_quantize(x, dtype, rows, cols, ld, ws, nullptr, sa, s);
+  if (st != DS_OK) return st;
+  x = ws;
+  atoms = sa;
+  ws += quantized_bytes(rows, cols);
+  return DS_OK;
+}
+
+}  // namespace
+}  // namespace mx4
+}  // namespace ds
+
+using namespace ds::mx4;
+
+extern "C" int ds_mx4_atoms_size(int64_t rows, int64_t cols, size_t* bytes) {
+  DS_REQUIRE(bytes && rows >= 0 && cols >= 1, DS_EINVAL, "mx4_atoms_size: rows >= 0, cols >= 1 and an output expected");
+  *bytes = atoms_bytes(rows, cols);
+  return DS_OK;
+}
+
+extern "C" int ds_mx4_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ld, uint8_t* packed,
+                               uint8_t* scales, uint8_t* atoms, void* stream) {
+  DS_REQUIRE(x_dtype == DS_F32 || x_dtype == DS_BF16 || x_dtype == DS_F16, DS_EINVAL,
+             "mx4_quantize: x must be f32, bf16 or f16");
+  DS_REQUIRE(rows >= 0 && rows < ((int64_t)1 << 31) && cols >= 1 && cols <= (1 << 20), DS_ERANGE,
+             "mx4_quantize: rows must be in [0, 2^31), cols in [1, 2^20]");
+  DS_REQUIRE(rows <= 1 || ld >= cols, DS_EINVAL, "mx4_quantize: row stride below cols");
+  if (rows == 0) return DS_OK;
+  DS_REQUIRE(x && packed && scales, DS_EINVAL, "mx4_quantize: null pointer");
+  DS_REQUIRE(ds::aligned(x, x_dtype == DS_F32 ? 4 : 2) && ds::aligned(packed, 16) && ds::aligned(atoms, 16), DS_EALIGN,
+             "mx4_quantize: x must be aligned to its elements, codes and atoms to 16 bytes");
+  return launch_quantize(x, x_dtype, rows, (int)cols, ld, packed, scales, atoms, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int ds_mx4_scale_atoms(const uint8_t* scales, int64_t rows, int64_t cols, uint8_t* atoms, void* stream) {
+  DS_REQUIRE(rows >= 0 && rows < ((int64_t)1 << 31) && cols >= 1 && cols <= (1 << 20), DS_ERANGE,
+             "mx4_scale_atoms: rows must be in [0, 2^31), cols in [1, 2^20]");
+  if (rows == 0) return DS_OK;
+  DS_REQUIRE(scales && atoms, DS_EINVAL, "mx4_scale_atoms: null pointer");
+  DS_REQUIRE(ds::aligned(atoms, 16), DS_EALIGN, "mx4_scale_atoms: atoms must be 16-byte aligned");
+  const int64_t n = rows * ((cols + 127) / 128);
+  const int grid = (int)std::min<int64_t>((n + 255) / 256, (int64_t)ds::sm_count() * 16);
+  scale_atoms_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(scales, rows, (int)blocks_of(cols), atoms);
+  DS_CHECK_LAUNCH("mx4 scale_atoms_kernel");
+  return DS_OK;
+}
+
+extern "C" int ds_mx4_linear_workspace_size(int64_t rows, int64_t cols, size_t* bytes) {
+  DS_REQUIRE(bytes && rows >= 0 && cols >= 1, DS_EINVAL,
+             "mx4_linear_workspace_size: rows >= 0, cols >= 1 and an output expected");
+  *bytes = quantized_bytes(rows, cols);
+  return DS_OK;
+}
+
+extern "C" int ds_mx4_linear(const void* x, const uint8_t* x_atoms, int x_dtype, int64_t rows, int64_t ld,
+                             const DsMx4* w, void* out, int out_dtype, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+  int st = validate_weight(w, "mx4_linear");
+  if (st != DS_OK) return st;
+  if ((st = validate_x(x, x_atoms, x_dtype, rows, (int)w->cols, ld, "mx4_linear")) != DS_OK) return st;
+  DS_REQUIRE(out_dtype == DS_F32 || out_dtype == DS_BF16 || out_dtype == DS_F16, DS_EINVAL,
+             "mx4_linear: out must be f32, bf16 or f16");
+  if (rows == 0) return DS_OK;
+  const size_t need = x_dtype == DS_U8 ? 0 : quantized_bytes(rows, w->cols);
+  DS_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), DS_EINVAL,
+             "mx4_linear: workspace %zu bytes < required %zu", workspace_bytes, need);
+  DS_REQUIRE(out && ds::aligned(out, out_dtype == DS_F32 ? 4 : 2) && ds::aligned(workspace, 256), DS_EALIGN,
+             "mx4_linear: out must be aligned to its elements, the workspace to 256 bytes");
+  DS_REQUIRE(ds::grouped::encode_fn() != nullptr, DS_ECUDA, "mx4_linear: cuTensorMapEncodeTiled unavailable");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if ((st = quantized_x(x, x_atoms, x_dtype, rows, (int)w->cols, ld, ws, s)) != DS_OK) return st;
+
+  const int nt = row_tile(rows);
+  TileParams p;
+  memset(&p, 0, sizeof(p));
+  p.err = err_word();
+  DS_REQUIRE(p.err != nullptr, DS_ECUDA, "mx4_linear: error word unavailable");
+  const bool ok = map_codes(&p.a[0], w->packed, w->rows, w->cols, 128) && map_codes(&p.b, x, rows, w->cols, nt);
+  DS_REQUIRE(ok, DS_ECUDA, "mx4_linear: tensor map encoding failed");
+  p.sa[0] = w->atoms;
+  p.sb = x_atoms;
+  p.M = (int)w->rows;
+  p.N = (int)rows;
+  p.blocks = (int)blocks_of(w->cols);
+  p.out = out;
+  p.ldo = w->rows;
+  p.out_dtype = out_dtype;
+  return run_tiles<LINEAR>(p, nt, s, x_dtype != DS_U8);
+}
+
+extern "C" int ds_mx4_gated_ffn_workspace_size(int64_t rows, int64_t hidden, int64_t inter, size_t* bytes) {
+  DS_REQUIRE(bytes && rows >= 0 && hidden >= 1 && inter >= 1, DS_EINVAL,
+             "mx4_gated_ffn_workspace_size: rows >= 0, hidden >= 1, inter >= 1 and an output expected");
+  *bytes = quantized_bytes(rows, hidden) + quantized_bytes(rows, inter);
+  return DS_OK;
+}
+
+extern "C" int ds_mx4_gated_ffn(const void* x, const uint8_t* x_atoms, int x_dtype, int64_t rows, int64_t ld,
+                                const DsMx4* w1, const DsMx4* w3, const DsMx4* w2, float limit, void* out,
+                                int out_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  int st;
+  for (const DsMx4* w : {w1, w3, w2})
+    if ((st = validate_weight(w, "mx4_gated_ffn")) != DS_OK) return st;
+  const int64_t H = w1->cols, I = w1->rows;
+  DS_REQUIRE(w3->rows == I && w3->cols == H && w2->rows == H && w2->cols == I, DS_EINVAL,
+             "mx4_gated_ffn: w1 and w3 [I, H] and w2 [H, I] expected");
+  if ((st = validate_x(x, x_atoms, x_dtype, rows, (int)H, ld, "mx4_gated_ffn")) != DS_OK) return st;
+  DS_REQUIRE(out_dtype == DS_F32 || out_dtype == DS_BF16 || out_dtype == DS_F16, DS_EINVAL,
+             "mx4_gated_ffn: out must be f32, bf16 or f16");
+  DS_REQUIRE(limit >= 0.0f, DS_EINVAL, "mx4_gated_ffn: limit must be >= 0 (0: no clamps)");
+  if (rows == 0) return DS_OK;
+  const size_t need = (x_dtype == DS_U8 ? 0 : quantized_bytes(rows, H)) + quantized_bytes(rows, I);
+  DS_REQUIRE(workspace && workspace_bytes >= need, DS_EINVAL, "mx4_gated_ffn: workspace %zu bytes < required %zu",
+             workspace_bytes, need);
+  DS_REQUIRE(out && ds::aligned(out, out_dtype == DS_F32 ? 4 : 2) && ds::aligned(workspace, 256), DS_EALIGN,
+             "mx4_gated_ffn: out must be aligned to its elements, the workspace to 256 bytes");
+  DS_REQUIRE(ds::grouped::encode_fn() != nullptr, DS_ECUDA, "mx4_gated_ffn: cuTensorMapEncodeTiled unavailable");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if ((st = quantized_x(x, x_atoms, x_dtype, rows, (int)H, ld, ws, s)) != DS_OK) return st;
+  uint8_t* hq = ws;
+  uint8_t* hs = ws + ds::grouped::up(packed_bytes(rows, I), 256);
+
+  const int nt = row_tile(rows);
+  TileParams p;
+  memset(&p, 0, sizeof(p));
+  p.err = err_word();
+  DS_REQUIRE(p.err != nullptr, DS_ECUDA, "mx4_gated_ffn: error word unavailable");
+  bool ok = map_codes(&p.a[0], w1->packed, I, H, 128) && map_codes(&p.a[1], w3->packed, I, H, 128) &&
+            map_codes(&p.b, x, rows, H, nt);
+  DS_REQUIRE(ok, DS_ECUDA, "mx4_gated_ffn: tensor map encoding failed (gate / up)");
+  p.sa[0] = w1->atoms;
+  p.sa[1] = w3->atoms;
+  p.sb = x_atoms;
+  p.M = (int)I;
+  p.N = (int)rows;
+  p.blocks = (int)blocks_of(H);
+  p.hq = hq;
+  p.hs = hs;
+  p.limit = limit;
+  if ((st = run_tiles<GATED>(p, nt, s, x_dtype != DS_U8)) != DS_OK) return st;
+
+  ok = map_codes(&p.a[0], w2->packed, H, I, 128) && map_codes(&p.b, hq, rows, I, nt);
+  DS_REQUIRE(ok, DS_ECUDA, "mx4_gated_ffn: tensor map encoding failed (down)");
+  p.sa[0] = w2->atoms;
+  p.sb = hs;
+  p.M = (int)H;
+  p.blocks = (int)blocks_of(I);
+  p.out = out;
+  p.ldo = H;
+  p.out_dtype = out_dtype;
+  return run_tiles<LINEAR>(p, nt, s, true);
+}
+
+extern "C" int ds_mx4_status(int32_t* err, void* stream) {
+  DS_REQUIRE(err != nullptr, DS_EINVAL, "mx4_status: null output");
+  int* w = err_word();
+  DS_REQUIRE(w != nullptr, DS_ECUDA, "mx4_status: error word unavailable");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  DS_CHECK_CUDA(cudaMemcpyAsync(err, w, sizeof(int), cudaMemcpyDefault, s));
+  DS_CHECK_CUDA(cudaMemsetAsync(w, 0, sizeof(int), s));
+  return DS_OK;
+}

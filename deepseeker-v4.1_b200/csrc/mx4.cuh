@@ -1,0 +1,55 @@
+// Microscaled 4-bit format shared by the dense kernels in mx4.cu: scale rule,
+// rounding, the tensor-core scale atoms and the copy of an atom into tensor
+// memory.
+//
+// A row of K values is ceil(K / 32) blocks.  A block keeps 32 e2m1 codes (16
+// bytes, low nibble first, zeros behind an uneven end) and one ue8m0 scale
+// 2^(s - 127), s the smallest that brings the block's largest magnitude to 6
+// or less (127 for a block of zeros).  A block that holds a NaN or an infinity
+// gets s = 255, the format's NaN, so the value is not lost.
+#pragma once
+
+#include "grouped.cuh"
+#include "tc5.cuh"
+
+namespace ds {
+namespace mx4 {
+
+using namespace ds::ptx;
+
+constexpr int kAtom = grouped::kSfAtom;   // scales of 128 rows x 4 blocks
+
+// Scale byte from the bits of the block's largest magnitude.
+__device__ __forceinline__ int scale_byte(uint32_t top) {
+  const int ef = (int)(top >> 23);
+  if (ef == 255) return 255;
+  if (ef == 0) return top == 0u ? 127 : 0;
+  return max((top & 0x7FFFFFu) <= 0x400000u ? ef - 2 : ef - 1, 0);
+}
+
+// 2^(127 - s), s <= 253; 0 for the NaN scale (the codes are then all 0).
+__device__ __forceinline__ float inv_scale(int s) { return s == 255 ? 0.0f : __uint_as_float((uint32_t)(254 - s) << 23); }
+
+// Clears the sign of codes that rounded to 0: one code stands for 0.
+__device__ __forceinline__ uint32_t no_negative_zero(uint32_t w) {
+  const uint32_t nz = (w | (w >> 1) | (w >> 2)) & 0x11111111u;
+  return w & (0x77777777u | (nz << 3));
+}
+
+// Byte of (row, block) in a matrix's atoms [ceil(rows / 128)][chunks][512],
+// chunks = ceil(blocks / 4).
+__device__ __forceinline__ int64_t atom_at(int64_t row, int block, int chunks) {
+  return ((row >> 7) * chunks + (block >> 2)) * kAtom + grouped::atom_off((int)(row & 127), block & 3);
+}
+
+// One atom from shared memory into four tensor-memory columns, replicated to
+// the four lane quarters.  Ordered before the MMAs that this thread issues next.
+__device__ __forceinline__ void copy_atom(uint32_t taddr, uint32_t saddr) {
+  uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)8 << 32;   // 128 bytes between groups of 8 rows x 16 bytes
+  d |= (uint64_t)1 << 46;   // no swizzle
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+}
+
+}  // namespace mx4
+}  // namespace ds

@@ -40,6 +40,10 @@ class DsGatedFfn(Structure):
                 ("ld_x", c_int64), ("ld_w1", c_int64), ("ld_w3", c_int64), ("ld_w2", c_int64)]
 
 
+class DsMx4(Structure):
+    _fields_ = [("packed", c_void_p), ("atoms", c_void_p), ("rows", c_int64), ("cols", c_int64)]
+
+
 # name -> (restype, argtypes); every symbol include/deepseeker_b200.h declares
 SIGNATURES: dict[str, tuple] = {
     "ds_last_error_string": (c_char_p, []),
@@ -95,6 +99,16 @@ SIGNATURES: dict[str, tuple] = {
     "ds_gated_ffn_backward": (c_int, [POINTER(DsGatedFfn), c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
                                       c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "ds_gated_ffn_status": (c_int, [c_void_p, c_void_p]),
+    "ds_mx4_atoms_size": (c_int, [c_int64, c_int64, POINTER(c_size_t)]),
+    "ds_mx4_quantize": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "ds_mx4_scale_atoms": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
+    "ds_mx4_linear_workspace_size": (c_int, [c_int64, c_int64, POINTER(c_size_t)]),
+    "ds_mx4_linear": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, POINTER(DsMx4), c_void_p, c_int, c_void_p,
+                              c_size_t, c_void_p]),
+    "ds_mx4_gated_ffn_workspace_size": (c_int, [c_int64, c_int64, c_int64, POINTER(c_size_t)]),
+    "ds_mx4_gated_ffn": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, POINTER(DsMx4), POINTER(DsMx4),
+                                 POINTER(DsMx4), c_float, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "ds_mx4_status": (c_int, [c_void_p, c_void_p]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -1,0 +1,190 @@
+"""Microscaled 4-bit dense operators: e2m1 codes, one ue8m0 scale per 32 values of a row.
+
+  quantize     activations (f32, bf16, f16) -> MX4Tensor
+  from_packed  stored codes and scales (the FP4 bank layout, one expert's matrix) -> MX4Tensor
+  linear       x W^T on the tensor cores' 4-bit rate, x quantised on the way or already
+  gated_ffn    the gated block (deepseeker.gated) over quantised weights
+
+Serving only: the results have no gradients, and an input that asks for one is refused.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _abi, metal_fp4
+from ._dev import stream_handle
+from .gated import _rows
+
+BLOCK = 32
+_DTYPES = {torch.float32: _abi.DS_F32, torch.bfloat16: _abi.DS_BF16, torch.float16: _abi.DS_F16}
+
+
+def _blocks(cols: int) -> int:
+    return (cols + BLOCK - 1) // BLOCK
+
+
+def _atoms_bytes(rows: int, cols: int) -> int:
+    return -(-rows // 128) * -(-cols // 128) * 512
+
+
+class MX4Tensor:
+    """A quantised matrix: ``packed`` u8 [rows, 16 ceil(cols/32)] (two codes per
+    byte, low nibble first), ``scales`` u8 [rows, ceil(cols/32)] (2^(b-127), 255
+    = NaN), ``atoms`` (the scales as the tensor cores read them); ``shape``:
+    the shape it stands for, leading dimensions included."""
+
+    __slots__ = ("packed", "scales", "atoms", "rows", "cols", "shape", "_c")
+
+    def __init__(self, packed, scales, atoms, shape):
+        self.packed, self.scales, self.atoms = packed, scales, atoms
+        self.shape = torch.Size(shape)
+        self.rows, self.cols = packed.shape[0], self.shape[-1]
+        self._c = _abi.DsMx4(packed.data_ptr(), atoms.data_ptr(), self.rows, self.cols)
+
+    @property
+    def device(self) -> torch.device:
+        return self.packed.device
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values that the codes stand for, f32 or bf16 (both exact)."""
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("dtype must be torch.float32 or torch.bfloat16")
+        v = metal_fp4.dequant(self.packed, self.scales, dtype).view(self.rows, _blocks(self.cols) * BLOCK)
+        return v[:, : self.cols].reshape(self.shape)
+
+
+def _check_x(x) -> None:
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _DTYPES:
+        raise ValueError("x must be a f32, bf16 or f16 CUDA tensor (or an MX4Tensor where one is taken)")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("x must be [..., cols] with at least one column")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError("4-bit operators have no backward pass: detach x or use torch.no_grad()")
+
+
+def quantize(x: torch.Tensor) -> MX4Tensor:
+    """x [..., cols] -> MX4Tensor.  A block's scale is the smallest power of two
+    that brings its largest magnitude to 6 or less (1 for zeros); values round
+    to the nearest code, ties to the even one.  A NaN or an infinity makes its
+    whole block NaN."""
+    _check_x(x)
+    cols = x.shape[-1]
+    rows, ld = _rows(x.reshape(-1, cols))
+    n = rows.shape[0]
+    packed = torch.empty(n, _blocks(cols) * 16, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(n, _blocks(cols), dtype=torch.uint8, device=x.device)
+    atoms = torch.empty(_atoms_bytes(n, cols), dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        _abi.call("ds_mx4_quantize", rows.data_ptr(), _DTYPES[x.dtype], n, cols, ld, packed.data_ptr(),
+                  scales.data_ptr(), atoms.data_ptr(), stream_handle(x.device))
+    return MX4Tensor(packed, scales, atoms, x.shape)
+
+
+def from_packed(packed: torch.Tensor, scales: torch.Tensor, cols: int | None = None) -> MX4Tensor:
+    """MX4Tensor over stored codes u8 [rows, 16 ceil(cols/32)] and scales u8
+    [rows, ceil(cols/32)] (used in place where contiguous; the scale atoms are
+    built once here).  ``cols`` defaults to 32 per scale."""
+    for name, t in (("packed", packed), ("scales", scales)):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.uint8 or t.dim() != 2:
+            raise ValueError(f"{name} must be a 2-D u8 CUDA tensor")
+    rows, nb = scales.shape
+    cols = nb * BLOCK if cols is None else cols
+    if rows < 1 or cols < 1 or _blocks(cols) != nb or packed.shape != (rows, nb * 16) or packed.device != scales.device:
+        raise ValueError("packed [rows, 16 ceil(cols/32)] and scales [rows, ceil(cols/32)] expected, on one device")
+    packed, scales = packed.contiguous(), scales.contiguous()
+    if packed.data_ptr() % 16:
+        packed = packed.clone()
+    atoms = torch.empty(_atoms_bytes(rows, cols), dtype=torch.uint8, device=packed.device)
+    with torch.cuda.device(packed.device):
+        _abi.call("ds_mx4_scale_atoms", scales.data_ptr(), rows, cols, atoms.data_ptr(), stream_handle(packed.device))
+    return MX4Tensor(packed, scales, atoms, (rows, cols))
+
+
+def _weight(w, name: str, device) -> None:
+    if not isinstance(w, MX4Tensor) or len(w.shape) != 2 or w.device != device:
+        raise ValueError(f"{name} must be a 2-D MX4Tensor on x's device")
+
+
+def _input(x, cols: int):
+    """(tensor kept alive, pointer, atoms pointer, type, rows, row stride) of x, quantised or not."""
+    if isinstance(x, MX4Tensor):
+        if x.cols != cols:
+            raise ValueError(f"x must be [..., {cols}]")
+        return x, x.packed.data_ptr(), x.atoms.data_ptr(), _abi.DS_U8, x.rows, 0
+    _check_x(x)
+    if x.shape[-1] != cols:
+        raise ValueError(f"x must be [..., {cols}]")
+    rows, ld = _rows(x.reshape(-1, cols))
+    return rows, rows.data_ptr(), None, _DTYPES[x.dtype], rows.shape[0], ld
+
+
+def _out(x, rows: int, cols: int, out_dtype):
+    if out_dtype is None:
+        out_dtype = torch.bfloat16 if isinstance(x, MX4Tensor) else x.dtype
+    if out_dtype not in _DTYPES:
+        raise ValueError("out_dtype must be f32, bf16 or f16")
+    return torch.empty(rows, cols, dtype=out_dtype, device=x.device), _DTYPES[out_dtype]
+
+
+def _device_of(x):
+    if not isinstance(x, MX4Tensor):
+        _check_x(x)
+    return x.device
+
+
+def linear(x, w: MX4Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """x [..., K] (a tensor, quantised on the way, or an MX4Tensor) times W^T,
+    W [N, K] -> [..., N] in out_dtype (default: x's type; bf16 for an
+    MX4Tensor).  Exact up to the f32 accumulation and the final rounding."""
+    dev = _device_of(x)
+    _weight(w, "w", dev)
+    hold, px, pa, dt, rows, ld = _input(x, w.cols)
+    out, odt = _out(x, rows, w.rows, out_dtype)
+    ws = None
+    n = 0
+    if dt != _abi.DS_U8:
+        n = _up(rows * _blocks(w.cols) * 16) + _up(_atoms_bytes(rows, w.cols))
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        _abi.call("ds_mx4_linear", px, pa, dt, rows, ld, ctypes.byref(w._c), out.data_ptr(), odt,
+                  None if ws is None else ws.data_ptr(), n, stream_handle(dev))
+    return out.view(*x.shape[:-1], w.rows)
+
+
+def gated_ffn(x, w1: MX4Tensor, w3: MX4Tensor, w2: MX4Tensor, limit: float | None = None,
+              out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """(silu(min(x W1^T, L)) * clip(x W3^T, -L, L)) W2^T with x and the product
+    of the gate quantised; w1 and w3 [I, H], w2 [H, I].  Clamps as in
+    ``deepseeker.gated.gated_ffn``."""
+    dev = _device_of(x)
+    for name, w in (("w1", w1), ("w3", w3), ("w2", w2)):
+        _weight(w, name, dev)
+    if w3.shape != w1.shape or w2.shape != (w1.cols, w1.rows):
+        raise ValueError("w1 [I, H], w3 [I, H], w2 [H, I] expected")
+    if limit is not None and not limit > 0:
+        raise ValueError("limit must be positive, or None for no clamps")
+    hold, px, pa, dt, rows, ld = _input(x, w1.cols)
+    out, odt = _out(x, rows, w2.rows, out_dtype)
+    n = _up(rows * _blocks(w1.rows) * 16) + _up(_atoms_bytes(rows, w1.rows))
+    n += 0 if dt == _abi.DS_U8 else _up(rows * _blocks(w1.cols) * 16) + _up(_atoms_bytes(rows, w1.cols))
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        _abi.call("ds_mx4_gated_ffn", px, pa, dt, rows, ld, ctypes.byref(w1._c), ctypes.byref(w3._c),
+                  ctypes.byref(w2._c), limit or 0.0, out.data_ptr(), odt, ws.data_ptr(), n, stream_handle(dev))
+    return out.view(*x.shape[:-1], w2.rows)
+
+
+def _up(n: int) -> int:
+    return (n + 255) // 256 * 256
+
+
+def status(device: torch.device | None = None) -> int:
+    """Error bits of this module's calls on `device` since the last query (2: a
+    bounded device wait gave up; outputs are then undefined).  Waits for the stream."""
+    err = torch.zeros(1, dtype=torch.int32)
+    with torch.cuda.device(device):
+        _abi.call("ds_mx4_status", err.data_ptr(), stream_handle(device))
+        torch.cuda.current_stream(device).synchronize()
+    return int(err[0])

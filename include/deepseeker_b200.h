@@ -460,6 +460,54 @@ int ds_gated_ffn_backward(const DsGatedFfn* desc, const void* h, const float* pr
  * a bounded device wait gave up, and that call's outputs are undefined. */
 int ds_gated_ffn_status(int32_t* err, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Microscaled 4-bit dense operators over the FP4 layout above (the reference
+ * only dequantises such weights, src/deepseeker/metal_fp4.py:28-66; products
+ * of two quantised matrices have no counterpart there).
+ * A row of K values is ceil(K / 32) blocks: 16 bytes of codes (zeros behind an
+ * uneven end) and one ue8m0 scale each, the smallest power of two that brings
+ * the block's largest magnitude to 6 or less (1 for zeros; the rule of
+ * ds_fp4_quantize).  Rounding is to nearest, ties to the even code; 0 has one
+ * code.  A block with a NaN or an infinity gets scale 255 (NaN), so products
+ * with it are NaN.  Magnitudes that round to 2^128 (above 2.9e38) stand for a
+ * value outside f32.
+ * Beside the scales, the tensor cores read them as atoms
+ * [ceil(rows/128)][ceil(K/128)][512 B]: byte (r%32)*16 + (r/32)*4 + b is the
+ * scale of row r, block b of a 128 x 128 tile (as ds_fp4_scale_atoms, for any
+ * sizes; rows past the matrix are not written). */
+int ds_mx4_atoms_size(int64_t rows, int64_t cols, size_t* bytes);
+/* x [rows, cols] f32, bf16 or f16, rows ld elements apart -> packed
+ * [rows, 16 ceil(cols/32)], scales [rows, ceil(cols/32)], atoms (or NULL). */
+int ds_mx4_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ld, uint8_t* packed,
+                    uint8_t* scales, uint8_t* atoms, void* stream);
+/* Atoms of stored scales [rows, ceil(cols/32)]: once per weight matrix. */
+int ds_mx4_scale_atoms(const uint8_t* scales, int64_t rows, int64_t cols, uint8_t* atoms, void* stream);
+
+typedef struct DsMx4 {
+  const uint8_t* packed;
+  const uint8_t* atoms;
+  int64_t rows, cols;         /* 1 .. 2^20 each */
+} DsMx4;
+
+/* out [rows, w->rows] (f32, bf16 or f16, contiguous) = x W^T, f32 accumulate.
+ * x_dtype f32 / bf16 / f16: x [rows, w->cols], rows ld elements apart, is
+ * quantised into the workspace first (x_atoms NULL); DS_U8: x is codes and
+ * x_atoms its atoms, and no workspace is needed.  rows in [0, 2^22]. */
+int ds_mx4_linear_workspace_size(int64_t rows, int64_t cols, size_t* bytes);
+int ds_mx4_linear(const void* x, const uint8_t* x_atoms, int x_dtype, int64_t rows, int64_t ld, const DsMx4* w,
+                  void* out, int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The gated block (ds_gated_ffn's formula) over quantised weights: x is
+ * quantised (or given as codes), h = silu(min(g, limit)) * clip(u, +-limit) is
+ * computed from the f32 sums and quantised in the product's epilogue; limit 0:
+ * no clamps.  out [rows, hidden] f32, bf16 or f16. */
+int ds_mx4_gated_ffn_workspace_size(int64_t rows, int64_t hidden, int64_t inter, size_t* bytes);
+int ds_mx4_gated_ffn(const void* x, const uint8_t* x_atoms, int x_dtype, int64_t rows, int64_t ld, const DsMx4* w1,
+                     const DsMx4* w3, const DsMx4* w2, float limit, void* out, int out_dtype, void* workspace,
+                     size_t workspace_bytes, void* stream);
+/* As ds_gated_ffn_status, for the calls of this group. */
+int ds_mx4_status(int32_t* err, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,18 +1,18 @@
 """Dense gated feed-forward block (deepseeker.gated): forward and gradients
 against the formulas in 64 bits.
 
-Tolerances.  Let u be the 16-bit type's unit roundoff (2^-9 bf16, 2^-12 f16).
-Every output is a sum of products a b of which one factor a (h, dg or du) was
-rounded once, and is rounded once itself.  The last rounding is off by at most
-u |output|.  The first adds sum_k d_k a_k b_k with |d_k| <= u, independent
-and of mean square at most u^2 / 3: 0.58 u R in the root mean square, with
+Tolerances.  Let v be half the 16-bit type's unit roundoff (2^-9 bf16, 2^-12
+f16): rounding to nearest is off by at most 2 v of the value, and by 0.85 v in
+the root mean square over values of all mantissas.  Every output is a sum of
+products a b of which one factor a (h, dg or du) was rounded once, and is
+rounded once itself: independent errors of 0.85 v |output| and 0.85 v R with
 R^2 = sum_k a_k^2 b_k^2 (about the output's own square unless the sum
-cancels).  Over n independent errors the 2-norm exceeds its mean by the factor
-1 + 3 / sqrt(n) only beyond three deviations; n is the smaller of the number
-of outputs and of rounded factors.  Asserted:
-  |error|_2 <= u |output|_2 + 0.58 u (1 + 3 / sqrt(n)) |R|_2
-plus ATOL per value (f16's spacing at 0, 2^-24, once per rounding).  The f32
-accumulation of a few thousand terms adds 1e-3 u.
+cancels).  Where R = |output| that is 1.2 v |output| together; asserted is
+  |error|_2 <= v |output|_2 + 0.58 v (1 + 3 / sqrt(n)) |R|_2,
+1.58 v there, the last factor for the spread of the 2-norm of n independent
+errors (n: the smaller of the number of outputs and of rounded factors), plus
+ATOL per value (f16's spacing at 0, 2^-24, once per rounding).  The f32
+accumulation of a few thousand terms adds 1e-3 v.
 """
 from __future__ import annotations
 
@@ -22,7 +22,7 @@ import torch
 from deepseeker import gated
 
 pytestmark = pytest.mark.gpu
-UNIT = {torch.bfloat16: 2.0 ** -9, torch.float16: 2.0 ** -12}
+HALF_UNIT = {torch.bfloat16: 2.0 ** -9, torch.float16: 2.0 ** -12}
 ATOL = 2.0 ** -24
 
 
@@ -55,7 +55,7 @@ def scales(x, w1, w3, w2, dy, limit):
 def check(got, want, dtype, scale, what):
     got, want = got.double(), want.double()
     assert got.shape == want.shape
-    (R, n), u = scale, UNIT[dtype]
+    (R, n), u = scale, HALF_UNIT[dtype]
     err = float((got - want).norm())
     bound = u * float(want.norm()) + 0.58 * u * (1 + 3 / n ** 0.5) * R + 2 * ATOL * want.numel() ** 0.5
     assert err <= bound, f"{what}: {err} > {bound} (relative {err / max(float(want.norm()), 1e-30):.2e})"
@@ -117,8 +117,8 @@ def test_gradient_against_differences(cuda):
     L(p) = sum(y dy).  With step s along a unit-scale direction the central
     difference of the 64-bit formula is off by O(s^2) and 1e-16 / s: s = 1e-5
     leaves less than 1e-9 relative.  The kernel's gradients are off by at most
-    2 u |grad| (above: 1.58 u and the factor's few per cent), so <grad, v> is
-    within 2 u |grad| |v| of it."""
+    2 v |grad| (above: 1.58 v and the factor's few per cent), so <grad, d> along
+    a direction d is within 2 v |grad| |d| of it."""
     ins, dy = make(24, 96, 64, torch.float16, cuda, seed=3)
     got, _ = both(ins, dy, 1.0)
     base = [t.double() for t in ins]
@@ -128,7 +128,7 @@ def test_gradient_against_differences(cuda):
         f = lambda s: (formula(*[b + s * v if j == i else b for j, b in enumerate(base)], 1.0) * dy.double()).sum()  # noqa: E731,B023
         diff = float((f(1e-5) - f(-1e-5)) / 2e-5)
         grad = got[1 + i].double()
-        bound = 2 * UNIT[torch.float16] * float(grad.norm()) * float(v.norm())
+        bound = 2 * HALF_UNIT[torch.float16] * float(grad.norm()) * float(v.norm())
         assert abs(float((grad * v).sum()) - diff) <= bound
 
 
@@ -174,7 +174,7 @@ def test_shared_and_frozen_weights(cuda):
     b = w1.double().requires_grad_()
     gw, = torch.autograd.grad(formula(x.double(), b, b, w2.double(), None), b, dy.double())
     # two rounded gradients and their rounded sum
-    assert float((g.double() - gw).norm()) <= 4 * UNIT[torch.bfloat16] * float(gw.norm())
+    assert float((g.double() - gw).norm()) <= 4 * HALF_UNIT[torch.bfloat16] * float(gw.norm())
 
 
 def test_no_tokens(cuda):
