@@ -76,7 +76,9 @@ inline bool map16(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, 
 // ---------------------------------------------------------------- the gated unit
 
 // h = silu(min(g, L)) * clip(u, -L, L); L = 0: no clamps.  The comparisons
-// keep a NaN (fminf would drop it).
+// keep a NaN (fminf would drop it).  The fast exponential and division are
+// good to about 2^-20, far below the 16-bit rounding that follows; both have
+// the right limits (0 for g towards -infinity).
 __device__ __forceinline__ void gate_clamp(float& g, float& u, float limit) {
   if (limit > 0.0f) {
     g = g > limit ? limit : g;
@@ -86,7 +88,7 @@ __device__ __forceinline__ void gate_clamp(float& g, float& u, float limit) {
 
 __device__ __forceinline__ float gate_unit(float g, float u, float limit) {
   gate_clamp(g, u, limit);
-  return g / (1.0f + expf(-g)) * u;
+  return __fdividef(g, 1.0f + __expf(-g)) * u;
 }
 
 // Gradients of the unclamped g and u from dh.  With s = sigmoid(g'):
@@ -95,7 +97,7 @@ __device__ __forceinline__ float gate_unit(float g, float u, float limit) {
 __device__ __forceinline__ void gate_grad(float g, float u, float dh, float limit, float& dg, float& du) {
   float gc = g, uc = u;
   gate_clamp(gc, uc, limit);
-  const float s = 1.0f / (1.0f + expf(-gc));
+  const float s = __fdividef(1.0f, 1.0f + __expf(-gc));
   dg = dh * uc * (s * (1.0f + gc * (1.0f - s)));
   du = dh * (gc * s);
   if (limit > 0.0f) {
@@ -107,6 +109,15 @@ __device__ __forceinline__ void gate_grad(float g, float u, float dh, float limi
 // f32 -> 16-bit (round to nearest even), the low half of the result.
 __device__ __forceinline__ uint16_t to16(float v, int f16) {
   return f16 ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
+
+__device__ __forceinline__ uint32_t pack16(float lo, float hi, int f16) {
+  if (f16) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&b);
 }
 
 }  // namespace dense

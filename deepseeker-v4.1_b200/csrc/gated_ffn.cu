@@ -21,15 +21,13 @@
 #include <cooperative_groups.h>
 #include <string.h>
 
-#include "dense16.cuh"
+#include "gated_pair.cuh"
 
 namespace ds {
 namespace dense {
 namespace {
 
 namespace cg = cooperative_groups;
-
-enum Mode { GATED, PLAIN, DHID, DX, DW };
 
 template <int MODE>
 struct ModeOf {
@@ -326,6 +324,41 @@ int run_tiles(const TileParams& p, int nt, cudaStream_t s, bool chained) {
   return launch_tiles<MODE, 128>(p, max_m, max_n, slices, s, chained);
 }
 
+// ---- pair kernel
+
+// Tiles of an [M, N] result in the pair kernel.
+template <int MODE>
+int64_t pair_tiles(int64_t M, int64_t N) {
+  constexpr int c = pair::Shape<MODE>::kCols;
+  return (M + 255) / 256 * ((N + c - 1) / c);
+}
+
+// The pair kernel takes the products with at least PAIR_MIN tiles.
+constexpr int kPairMin = 37;
+
+template <int MODE>
+int run_pairs(PairParams& p, cudaStream_t s, bool chained) {
+  using C = pair::Shape<MODE>;
+  int64_t tiles = 0;
+  for (int z = 0; z < C::kProblems; ++z) {
+    tiles += p.M[z] && p.N[z] ? pair_tiles<MODE>(p.M[z], p.N[z]) : 0;
+    p.tiles[z] = (int)tiles;
+  }
+  DS_CHECK_CUDA(cudaFuncSetAttribute(pair::pair_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, pair::kSmem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, ds::sm_count() / 2)));
+  cfg.blockDim = dim3(pair::kThreads);
+  cfg.dynamicSmemBytes = pair::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = chained ? 1 : 0;
+  DS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, pair::pair_kernel<MODE>, p));
+  return DS_OK;
+}
+
 int validate(const DsGatedFfn* d) {
   DS_REQUIRE(d != nullptr, DS_EINVAL, "gated_ffn: null descriptor");
   DS_REQUIRE(d->tokens >= 0 && d->tokens <= (1 << 22), DS_ERANGE, "gated_ffn: tokens must be in [0, 2^22]");
@@ -403,33 +436,50 @@ extern "C" int ds_gated_ffn(const DsGatedFfn* desc, void* y, void* h, float* pre
     if ((st = place(*q, ws, s)) != DS_OK) return st;
   if (!h) h = ws;
   const int64_t ldm = up8(I);
+  int* err = err_word();
+  DS_REQUIRE(err != nullptr, DS_ECUDA, "gated_ffn: error word unavailable");
+  const int f16 = desc->dtype == DS_F16;
+  float* pre_u = pre ? pre + (int64_t)T * ldm : nullptr;
   const int nt = token_tile(T);
 
-  TileParams p;
-  memset(&p, 0, sizeof(p));
-  p.f16 = desc->dtype == DS_F16;
-  p.limit = desc->limit;
-  p.err = err_word();
-  DS_REQUIRE(p.err != nullptr, DS_ECUDA, "gated_ffn: error word unavailable");
-  bool ok = map16(&p.a[0], o.w1.p, I, H, o.w1.ld, 128) && map16(&p.a[1], o.w3.p, I, H, o.w3.ld, 128) &&
-            map16(&p.b[0], o.x.p, T, H, o.x.ld, nt);
-  DS_REQUIRE(ok, DS_ECUDA, "gated_ffn: tensor map encoding failed (gate / up)");
-  p.M[0] = I;
-  p.N[0] = T;
-  p.K = H;
-  p.out[0] = h;
-  p.ldo[0] = ldm;
-  p.g = pre;
-  p.u = pre ? pre + (int64_t)T * ldm : nullptr;
-  p.ldp = ldm;
-  if ((st = run_tiles<GATED>(p, nt, s, false)) != DS_OK) return st;
+  if (pair_tiles<GATED>(T, I) >= kPairMin) {
+    PairParams p = {};
+    p.f16 = f16, p.limit = desc->limit, p.err = err;
+    const bool ok = map16(&p.a[0], o.x.p, T, H, o.x.ld, 128) && map16(&p.b[0], o.w1.p, I, H, o.w1.ld, 128) &&
+                    map16(&p.b[1], o.w3.p, I, H, o.w3.ld, 128);
+    DS_REQUIRE(ok, DS_ECUDA, "gated_ffn: tensor map encoding failed (gate / up)");
+    p.M[0] = T, p.N[0] = I, p.K = H;
+    p.out[0] = h, p.ldo[0] = ldm;
+    p.g = pre, p.u = pre_u, p.ldp = ldm;
+    st = run_pairs<GATED>(p, s, false);
+  } else {
+    TileParams p = {};
+    p.f16 = f16, p.limit = desc->limit, p.err = err;
+    const bool ok = map16(&p.a[0], o.w1.p, I, H, o.w1.ld, 128) && map16(&p.a[1], o.w3.p, I, H, o.w3.ld, 128) &&
+                    map16(&p.b[0], o.x.p, T, H, o.x.ld, nt);
+    DS_REQUIRE(ok, DS_ECUDA, "gated_ffn: tensor map encoding failed (gate / up)");
+    p.M[0] = I, p.N[0] = T, p.K = H;
+    p.out[0] = h, p.ldo[0] = ldm;
+    p.g = pre, p.u = pre_u, p.ldp = ldm;
+    st = run_tiles<GATED>(p, nt, s, false);
+  }
+  if (st != DS_OK) return st;
 
-  ok = map16(&p.a[0], o.w2.p, H, I, o.w2.ld, 128) && map16(&p.b[0], h, T, I, ldm, nt);
+  if (pair_tiles<PLAIN>(T, H) >= kPairMin) {
+    PairParams p = {};
+    p.f16 = f16, p.err = err;
+    const bool ok = map16(&p.a[0], h, T, I, ldm, 128) && map16(&p.b[0], o.w2.p, H, I, o.w2.ld, 128);
+    DS_REQUIRE(ok, DS_ECUDA, "gated_ffn: tensor map encoding failed (down)");
+    p.M[0] = T, p.N[0] = H, p.K = I;
+    p.out[0] = y, p.ldo[0] = H;
+    return run_pairs<PLAIN>(p, s, true);
+  }
+  TileParams p = {};
+  p.f16 = f16, p.err = err;
+  const bool ok = map16(&p.a[0], o.w2.p, H, I, o.w2.ld, 128) && map16(&p.b[0], h, T, I, ldm, nt);
   DS_REQUIRE(ok, DS_ECUDA, "gated_ffn: tensor map encoding failed (down)");
-  p.M[0] = H;
-  p.K = I;
-  p.out[0] = y;
-  p.ldo[0] = H;
+  p.M[0] = H, p.N[0] = T, p.K = I;
+  p.out[0] = y, p.ldo[0] = H;
   return run_tiles<PLAIN>(p, nt, s, true);
 }
 
@@ -472,59 +522,90 @@ extern "C" int ds_gated_ffn_backward(const DsGatedFfn* desc, const void* h, cons
   const int64_t ldm = up8(I);
   void* dg = ws;
   void* du = ws + mid_bytes(desc);
+  int* err = err_word();
+  DS_REQUIRE(err != nullptr, DS_ECUDA, "gated_ffn_backward: error word unavailable");
+  const int f16 = desc->dtype == DS_F16;
+  float* g = const_cast<float*>(pre);
+  float* u = g + (int64_t)T * ldm;
   const int nt = token_tile(T);
+  bool ok, chained = false;
 
-  TileParams p;
-  memset(&p, 0, sizeof(p));
-  p.f16 = desc->dtype == DS_F16;
-  p.limit = desc->limit;
-  p.err = err_word();
-  DS_REQUIRE(p.err != nullptr, DS_ECUDA, "gated_ffn_backward: error word unavailable");
-  const bool need_mid = dx || dw1 || dw3;
-  bool ok;
-  if (need_mid) {
-    ok = map16(&p.a[0], o.w2.p, H, I, o.w2.ld, 64) && map16(&p.b[0], gy.p, T, H, gy.ld, nt);
-    DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (hidden gradient)");
-    p.M[0] = I;
-    p.N[0] = T;
-    p.K = H;
-    p.out[0] = dg;
-    p.out[1] = du;
-    p.ldo[0] = p.ldo[1] = ldm;
-    p.g = const_cast<float*>(pre);
-    p.u = p.g + (int64_t)T * ldm;
-    p.ldp = ldm;
-    if ((st = run_tiles<DHID>(p, nt, s, false)) != DS_OK) return st;
+  if (dx || dw1 || dw3) {
+    if (pair_tiles<DHID>(T, I) >= kPairMin) {
+      PairParams p = {};
+      p.f16 = f16, p.limit = desc->limit, p.err = err;
+      ok = map16(&p.a[0], gy.p, T, H, gy.ld, 128) && map16(&p.b[0], o.w2.p, H, I, o.w2.ld, 64);
+      DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (hidden gradient)");
+      p.M[0] = T, p.N[0] = I, p.K = H;
+      p.out[0] = dg, p.out[1] = du, p.ldo[0] = p.ldo[1] = ldm;
+      p.g = g, p.u = u, p.ldp = ldm;
+      st = run_pairs<DHID>(p, s, false);
+    } else {
+      TileParams p = {};
+      p.f16 = f16, p.limit = desc->limit, p.err = err;
+      ok = map16(&p.a[0], o.w2.p, H, I, o.w2.ld, 64) && map16(&p.b[0], gy.p, T, H, gy.ld, nt);
+      DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (hidden gradient)");
+      p.M[0] = I, p.N[0] = T, p.K = H;
+      p.out[0] = dg, p.out[1] = du, p.ldo[0] = p.ldo[1] = ldm;
+      p.g = g, p.u = u, p.ldp = ldm;
+      st = run_tiles<DHID>(p, nt, s, false);
+    }
+    if (st != DS_OK) return st;
+    chained = true;
   }
   if (dx) {
-    ok = map16(&p.a[0], o.w1.p, I, H, o.w1.ld, 64) && map16(&p.a[1], o.w3.p, I, H, o.w3.ld, 64) &&
-         map16(&p.b[0], dg, T, I, ldm, nt) && map16(&p.b[1], du, T, I, ldm, nt);
-    DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (dx)");
-    p.M[0] = H;
-    p.N[0] = T;
-    p.K = I;
-    p.out[0] = dx;
-    p.ldo[0] = H;
-    if ((st = run_tiles<DX>(p, nt, s, need_mid)) != DS_OK) return st;
+    if (pair_tiles<DX>(T, H) >= kPairMin) {
+      PairParams p = {};
+      p.f16 = f16, p.err = err;
+      ok = map16(&p.a[0], dg, T, I, ldm, 128) && map16(&p.a[1], du, T, I, ldm, 128) &&
+           map16(&p.b[0], o.w1.p, I, H, o.w1.ld, 64) && map16(&p.b[1], o.w3.p, I, H, o.w3.ld, 64);
+      DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (dx)");
+      p.M[0] = T, p.N[0] = H, p.K = I;
+      p.out[0] = dx, p.ldo[0] = H;
+      st = run_pairs<DX>(p, s, chained);
+    } else {
+      TileParams p = {};
+      p.f16 = f16, p.err = err;
+      ok = map16(&p.a[0], o.w1.p, I, H, o.w1.ld, 64) && map16(&p.a[1], o.w3.p, I, H, o.w3.ld, 64) &&
+           map16(&p.b[0], dg, T, I, ldm, nt) && map16(&p.b[1], du, T, I, ldm, nt);
+      DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (dx)");
+      p.M[0] = H, p.N[0] = T, p.K = I;
+      p.out[0] = dx, p.ldo[0] = H;
+      st = run_tiles<DX>(p, nt, s, chained);
+    }
+    if (st != DS_OK) return st;
   }
   if (dw1 || dw3 || dw2) {
-    // dW1[i, h] and dW3: lanes h (x), columns i (dg, du); dW2[h, i]: lanes i (h), columns h (dy)
+    // dW1 and dW3 [I, H]: x against dg and du; dW2 [H, I]: h against dy
     void* outs[3] = {dw1, dw3, dw2};
-    const void* bs[3] = {dg, du, gy.p};
-    const int64_t ldb[3] = {ldm, ldm, gy.ld};
+    const Operand grads[3] = {{dg, T, I, ldm}, {du, T, I, ldm}, gy};
+    const Operand acts[3] = {o.x, o.x, {h, T, I, ldm}};
+    int64_t tiles = 0;
+    for (int z = 0; z < 3; ++z) tiles += outs[z] ? pair_tiles<DW>(grads[z].cols, acts[z].cols) : 0;
+    if (tiles >= kPairMin) {
+      PairParams p = {};
+      p.f16 = f16, p.err = err, p.K = T;
+      for (int z = 0; z < 3; ++z) {
+        if (!outs[z]) continue;   // M = 0: no tiles
+        p.M[z] = (int)grads[z].cols, p.N[z] = (int)acts[z].cols;
+        p.out[z] = outs[z], p.ldo[z] = acts[z].cols;
+        ok = map16(&p.a[z], grads[z].p, T, grads[z].cols, grads[z].ld, 64) &&
+             map16(&p.b[z], acts[z].p, T, acts[z].cols, acts[z].ld, 64);
+        DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (weight gradients)");
+      }
+      return run_pairs<DW>(p, s, chained);
+    }
+    TileParams p = {};
+    p.f16 = f16, p.err = err, p.K = T;
     for (int z = 0; z < 3; ++z) {
-      const bool down = z == 2;
-      p.M[z] = outs[z] ? (down ? I : H) : 0;   // M = 0: the problem's CTAs return at once
-      p.N[z] = down ? H : I;
-      p.out[z] = outs[z];
-      p.ldo[z] = down ? I : H;
-      if (!outs[z]) continue;
-      ok = map16(&p.a[z], down ? h : o.x.p, T, down ? I : H, down ? ldm : o.x.ld, 64) &&
-           map16(&p.b[z], bs[z], T, down ? H : I, ldb[z], 64);
+      if (!outs[z]) continue;     // M = 0: the problem's CTAs return at once
+      p.M[z] = (int)acts[z].cols, p.N[z] = (int)grads[z].cols;
+      p.out[z] = outs[z], p.ldo[z] = acts[z].cols;
+      ok = map16(&p.a[z], acts[z].p, T, acts[z].cols, acts[z].ld, 64) &&
+           map16(&p.b[z], grads[z].p, T, grads[z].cols, grads[z].ld, 64);
       DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (weight gradients)");
     }
-    p.K = T;
-    if ((st = run_tiles<DW>(p, 128, s, need_mid)) != DS_OK) return st;
+    return run_tiles<DW>(p, 128, s, chained);
   }
   return DS_OK;
 }

@@ -444,7 +444,7 @@ typedef struct DsGatedFfn {
 int ds_gated_ffn_workspace_size(const DsGatedFfn* desc, int keeps_h, size_t* bytes);
 /* y [T, H] contiguous.  For a later backward pass: h [T, Ip] 16 bit and
  * pre [2][T, Ip] f32 (g, then u), Ip = inter rounded up to a multiple of 8
- * (columns from inter on are not written); both NULL otherwise. */
+ * (columns from inter on hold nothing); both NULL otherwise. */
 int ds_gated_ffn(const DsGatedFfn* desc, void* y, void* h, float* pre, void* workspace,
                  size_t workspace_bytes, void* stream);
 
