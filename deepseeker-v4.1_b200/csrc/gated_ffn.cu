@@ -29,11 +29,13 @@ namespace {
 
 namespace cg = cooperative_groups;
 
+enum Mode { GATE_UP, PLAIN, DHID, DX, DW };
+
 template <int MODE>
 struct ModeOf {
   static constexpr bool kAMn = MODE == DHID || MODE == DX || MODE == DW;   // A stored with m running fastest
   static constexpr bool kBMn = MODE == DW;
-  static constexpr int kMats = MODE == GATED ? 2 : 1;                      // accumulators (W1 and W3 share x)
+  static constexpr int kMats = MODE == GATE_UP ? 2 : 1;                      // accumulators (W1 and W3 share x)
   static constexpr int kSegs = MODE == DX ? 2 : 1;                         // dg W1 and du W3 in one accumulator
   static constexpr int kProblems = MODE == DW ? 3 : 1;
 };
@@ -73,7 +75,7 @@ constexpr int kTileThreads = 192;   // warp 0 copies, warp 1 MMA, warps 2-5 epil
 template <int MODE>
 __device__ __forceinline__ void tile_store(const TileParams& p, int z, int m, int n, float v0, float v1) {
   uint16_t* out = static_cast<uint16_t*>(p.out[z]) + (int64_t)n * p.ldo[z] + m;
-  if constexpr (MODE == GATED) {
+  if constexpr (MODE == GATE_UP) {
     if (p.g) {
       p.g[(int64_t)n * p.ldp + m] = v0;
       p.u[(int64_t)n * p.ldp + m] = v1;
@@ -327,26 +329,40 @@ int run_tiles(const TileParams& p, int nt, cudaStream_t s, bool chained) {
 // ---- pair kernel
 
 // Tiles of an [M, N] result in the pair kernel.
-template <int MODE>
-int64_t pair_tiles(int64_t M, int64_t N) {
-  constexpr int c = pair::Shape<MODE>::kCols;
+int64_t pair_tiles(int epi, int64_t M, int64_t N) {
+  const int c = pair::tile_cols(epi);
   return (M + 255) / 256 * ((N + c - 1) / c);
 }
 
-// The pair kernel takes the products with at least PAIR_MIN tiles.
+// The pair kernel takes the products with at least this many tiles.
 constexpr int kPairMin = 37;
 
-template <int MODE>
+// Adds the problem c = a b^T (a and b given with their own layouts; k the
+// contraction) to a launch.
+Problem* add(PairParams& p, int epi, int64_t M, int64_t N, int64_t k, void* c, int64_t ldc) {
+  Problem& q = p.pr[p.n++];
+  q.epi = epi, q.M = (int)M, q.N = (int)N;
+  q.ksteps = (int)((k + kBK - 1) / kBK), q.segs = 1;
+  q.c[0] = c, q.ldc = ldc;
+  q.tiles = (int)(pair_tiles(epi, M, N) + (p.n > 1 ? p.pr[p.n - 2].tiles : 0));
+  return &q;
+}
+
+// Boxes of the result where its rows allow them.
+bool box_result(Problem& q) {
+  q.boxed = q.epi == STORE && direct(q.c[0], q.ldc);
+  return !q.boxed || map16(&q.out, q.c[0], q.M, q.N, q.ldc, 32);
+}
+
+// Operand maps: box rows by the way the operand is stored.
+bool side(CUtensorMap* m, const Operand& o, int mn) { return map16(m, o.p, o.rows, o.cols, o.ld, mn ? 64 : 128); }
+
+template <int EPI>
 int run_pairs(PairParams& p, cudaStream_t s, bool chained) {
-  using C = pair::Shape<MODE>;
-  int64_t tiles = 0;
-  for (int z = 0; z < C::kProblems; ++z) {
-    tiles += p.M[z] && p.N[z] ? pair_tiles<MODE>(p.M[z], p.N[z]) : 0;
-    p.tiles[z] = (int)tiles;
-  }
-  DS_CHECK_CUDA(cudaFuncSetAttribute(pair::pair_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, pair::kSmem));
+  if (p.split == 0) p.split = p.n;
+  DS_CHECK_CUDA(cudaFuncSetAttribute(pair::pair_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, pair::kSmem));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, ds::sm_count() / 2)));
+  cfg.gridDim = dim3((unsigned)(2 * std::min(p.pr[p.n - 1].tiles, ds::sm_count() / 2)));
   cfg.blockDim = dim3(pair::kThreads);
   cfg.dynamicSmemBytes = pair::kSmem;
   cfg.stream = s;
@@ -355,7 +371,7 @@ int run_pairs(PairParams& p, cudaStream_t s, bool chained) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = chained ? 1 : 0;
-  DS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, pair::pair_kernel<MODE>, p));
+  DS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, pair::pair_kernel<EPI>, p));
   return DS_OK;
 }
 
@@ -442,15 +458,13 @@ extern "C" int ds_gated_ffn(const DsGatedFfn* desc, void* y, void* h, float* pre
   float* pre_u = pre ? pre + (int64_t)T * ldm : nullptr;
   const int nt = token_tile(T);
 
-  if (pair_tiles<GATED>(T, I) >= kPairMin) {
+  if (pair_tiles(GATED, T, I) >= kPairMin) {
     PairParams p = {};
-    p.f16 = f16, p.limit = desc->limit, p.err = err;
-    const bool ok = map16(&p.a[0], o.x.p, T, H, o.x.ld, 128) && map16(&p.b[0], o.w1.p, I, H, o.w1.ld, 128) &&
-                    map16(&p.b[1], o.w3.p, I, H, o.w3.ld, 128);
+    p.f16 = f16, p.limit = desc->limit, p.err = err, p.keep = pre != nullptr;
+    Problem& q = *add(p, GATED, T, I, H, h, ldm);
+    const bool ok = side(&q.a[0], o.x, 0) && side(&q.b[0], o.w1, 0) && side(&q.b[1], o.w3, 0) &&
+                    (!pre || (map32(&p.g, pre, T, I, ldm) && map32(&p.u, pre_u, T, I, ldm)));
     DS_REQUIRE(ok, DS_ECUDA, "gated_ffn: tensor map encoding failed (gate / up)");
-    p.M[0] = T, p.N[0] = I, p.K = H;
-    p.out[0] = h, p.ldo[0] = ldm;
-    p.g = pre, p.u = pre_u, p.ldp = ldm;
     st = run_pairs<GATED>(p, s, false);
   } else {
     TileParams p = {};
@@ -461,18 +475,18 @@ extern "C" int ds_gated_ffn(const DsGatedFfn* desc, void* y, void* h, float* pre
     p.M[0] = I, p.N[0] = T, p.K = H;
     p.out[0] = h, p.ldo[0] = ldm;
     p.g = pre, p.u = pre_u, p.ldp = ldm;
-    st = run_tiles<GATED>(p, nt, s, false);
+    st = run_tiles<GATE_UP>(p, nt, s, false);
   }
   if (st != DS_OK) return st;
 
-  if (pair_tiles<PLAIN>(T, H) >= kPairMin) {
+  const Operand oh = {h, T, I, ldm};
+  if (pair_tiles(STORE, T, H) >= kPairMin) {
     PairParams p = {};
     p.f16 = f16, p.err = err;
-    const bool ok = map16(&p.a[0], h, T, I, ldm, 128) && map16(&p.b[0], o.w2.p, H, I, o.w2.ld, 128);
+    Problem& q = *add(p, STORE, T, H, I, y, H);
+    const bool ok = side(&q.a[0], oh, 0) && side(&q.b[0], o.w2, 0) && box_result(q);
     DS_REQUIRE(ok, DS_ECUDA, "gated_ffn: tensor map encoding failed (down)");
-    p.M[0] = T, p.N[0] = H, p.K = I;
-    p.out[0] = y, p.ldo[0] = H;
-    return run_pairs<PLAIN>(p, s, true);
+    return run_pairs<STORE>(p, s, true);
   }
   TileParams p = {};
   p.f16 = f16, p.err = err;
@@ -528,79 +542,98 @@ extern "C" int ds_gated_ffn_backward(const DsGatedFfn* desc, const void* h, cons
   float* g = const_cast<float*>(pre);
   float* u = g + (int64_t)T * ldm;
   const int nt = token_tile(T);
-  bool ok, chained = false;
+  const Operand og = {dg, T, I, ldm}, ou = {du, T, I, ldm}, oh = {h, T, I, ldm};
+  const bool need_mid = dx || dw1 || dw3;
+  const int64_t wtiles = pair_tiles(STORE, H, I);
+  bool ok = true, chained = false;
 
-  if (dx || dw1 || dw3) {
-    if (pair_tiles<DHID>(T, I) >= kPairMin) {
-      PairParams p = {};
-      p.f16 = f16, p.limit = desc->limit, p.err = err;
-      ok = map16(&p.a[0], gy.p, T, H, gy.ld, 128) && map16(&p.b[0], o.w2.p, H, I, o.w2.ld, 64);
-      DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (hidden gradient)");
-      p.M[0] = T, p.N[0] = I, p.K = H;
-      p.out[0] = dg, p.out[1] = du, p.ldo[0] = p.ldo[1] = ldm;
-      p.g = g, p.u = u, p.ldp = ldm;
-      st = run_pairs<DHID>(p, s, false);
-    } else {
-      TileParams p = {};
-      p.f16 = f16, p.limit = desc->limit, p.err = err;
-      ok = map16(&p.a[0], o.w2.p, H, I, o.w2.ld, 64) && map16(&p.b[0], gy.p, T, H, gy.ld, nt);
-      DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (hidden gradient)");
-      p.M[0] = I, p.N[0] = T, p.K = H;
-      p.out[0] = dg, p.out[1] = du, p.ldo[0] = p.ldo[1] = ldm;
-      p.g = g, p.u = u, p.ldp = ldm;
-      st = run_tiles<DHID>(p, nt, s, false);
+  // first launch: dg and du from dy, and beside them dW2, which needs neither
+  const bool mid_pair = need_mid && pair_tiles(HIDDEN, T, I) >= kPairMin;
+  const bool dw2_pair = dw2 && wtiles * ((dw1 != nullptr) + (dw3 != nullptr) + 1) >= kPairMin;
+  if (mid_pair || dw2_pair) {
+    PairParams p = {};
+    p.f16 = f16, p.limit = desc->limit, p.err = err;
+    const bool long_first = T >= H;   // the longer tiles are dealt first
+    for (int k = 0; k < 2; ++k) {
+      if ((k == 0) == long_first) {
+        if (!dw2_pair) continue;
+        Problem& q = *add(p, STORE, H, I, T, dw2, I);
+        q.a_mn = q.b_mn = 1;
+        ok = ok && side(&q.a[0], gy, 1) && side(&q.b[0], oh, 1) && box_result(q);
+      } else if (mid_pair) {
+        Problem& q = *add(p, HIDDEN, T, I, H, dg, ldm);
+        q.c[1] = du, q.b_mn = 1;
+        ok = ok && side(&q.a[0], gy, 0) && side(&q.b[0], o.w2, 1) && map32(&p.g, g, T, I, ldm) &&
+             map32(&p.u, u, T, I, ldm);
+      }
+      if (k == 0) p.split = p.n;
     }
-    if (st != DS_OK) return st;
+    DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (hidden gradient)");
+    if ((st = run_pairs<HIDDEN>(p, s, false)) != DS_OK) return st;
     chained = true;
   }
-  if (dx) {
-    if (pair_tiles<DX>(T, H) >= kPairMin) {
-      PairParams p = {};
-      p.f16 = f16, p.err = err;
-      ok = map16(&p.a[0], dg, T, I, ldm, 128) && map16(&p.a[1], du, T, I, ldm, 128) &&
-           map16(&p.b[0], o.w1.p, I, H, o.w1.ld, 64) && map16(&p.b[1], o.w3.p, I, H, o.w3.ld, 64);
-      DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (dx)");
-      p.M[0] = T, p.N[0] = H, p.K = I;
-      p.out[0] = dx, p.ldo[0] = H;
-      st = run_pairs<DX>(p, s, chained);
-    } else {
-      TileParams p = {};
-      p.f16 = f16, p.err = err;
-      ok = map16(&p.a[0], o.w1.p, I, H, o.w1.ld, 64) && map16(&p.a[1], o.w3.p, I, H, o.w3.ld, 64) &&
-           map16(&p.b[0], dg, T, I, ldm, nt) && map16(&p.b[1], du, T, I, ldm, nt);
-      DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (dx)");
-      p.M[0] = H, p.N[0] = T, p.K = I;
-      p.out[0] = dx, p.ldo[0] = H;
-      st = run_tiles<DX>(p, nt, s, chained);
-    }
-    if (st != DS_OK) return st;
+  if (need_mid && !mid_pair) {
+    TileParams p = {};
+    p.f16 = f16, p.limit = desc->limit, p.err = err;
+    ok = map16(&p.a[0], o.w2.p, H, I, o.w2.ld, 64) && map16(&p.b[0], gy.p, T, H, gy.ld, nt);
+    DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (hidden gradient)");
+    p.M[0] = I, p.N[0] = T, p.K = H;
+    p.out[0] = dg, p.out[1] = du, p.ldo[0] = p.ldo[1] = ldm;
+    p.g = g, p.u = u, p.ldp = ldm;
+    if ((st = run_tiles<DHID>(p, nt, s, chained)) != DS_OK) return st;
+    chained = true;
   }
-  if (dw1 || dw3 || dw2) {
-    // dW1 and dW3 [I, H]: x against dg and du; dW2 [H, I]: h against dy
-    void* outs[3] = {dw1, dw3, dw2};
-    const Operand grads[3] = {{dg, T, I, ldm}, {du, T, I, ldm}, gy};
-    const Operand acts[3] = {o.x, o.x, {h, T, I, ldm}};
-    int64_t tiles = 0;
-    for (int z = 0; z < 3; ++z) tiles += outs[z] ? pair_tiles<DW>(grads[z].cols, acts[z].cols) : 0;
-    if (tiles >= kPairMin) {
-      PairParams p = {};
-      p.f16 = f16, p.err = err, p.K = T;
-      for (int z = 0; z < 3; ++z) {
-        if (!outs[z]) continue;   // M = 0: no tiles
-        p.M[z] = (int)grads[z].cols, p.N[z] = (int)acts[z].cols;
-        p.out[z] = outs[z], p.ldo[z] = acts[z].cols;
-        ok = map16(&p.a[z], grads[z].p, T, grads[z].cols, grads[z].ld, 64) &&
-             map16(&p.b[z], acts[z].p, T, acts[z].cols, acts[z].ld, 64);
-        DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (weight gradients)");
+
+  // second launch: dW1 and dW3, and beside them dx
+  void* const dw[2] = {dw1, dw3};
+  const Operand* const mid[2] = {&og, &ou};
+  const int64_t w13 = wtiles * ((dw1 != nullptr) + (dw3 != nullptr));
+  const bool dx_pair = dx && pair_tiles(STORE, T, H) >= kPairMin, dw_pair = w13 >= kPairMin;
+  if (dx_pair || dw_pair) {
+    PairParams p = {};
+    p.f16 = f16, p.err = err;
+    const bool long_first = T >= 2 * I;
+    for (int k = 0; k < 2; ++k) {
+      if ((k == 0) == long_first) {
+        for (int z = 0; z < 2 && dw_pair; ++z) {
+          if (!dw[z]) continue;
+          Problem& q = *add(p, STORE, I, H, T, dw[z], H);
+          q.a_mn = q.b_mn = 1;
+          ok = ok && side(&q.a[0], *mid[z], 1) && side(&q.b[0], o.x, 1) && box_result(q);
+        }
+      } else if (dx_pair) {
+        Problem& q = *add(p, STORE, T, H, I, dx, H);
+        q.b_mn = 1, q.segs = 2;
+        ok = ok && side(&q.a[0], og, 0) && side(&q.a[1], ou, 0) && side(&q.b[0], o.w1, 1) && side(&q.b[1], o.w3, 1) &&
+             box_result(q);
       }
-      return run_pairs<DW>(p, s, chained);
+      if (k == 0) p.split = p.n;
     }
+    DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (dx, dW1, dW3)");
+    if ((st = run_pairs<STORE>(p, s, chained)) != DS_OK) return st;
+    chained = true;
+  }
+  if (dx && !dx_pair) {
+    TileParams p = {};
+    p.f16 = f16, p.err = err;
+    ok = map16(&p.a[0], o.w1.p, I, H, o.w1.ld, 64) && map16(&p.a[1], o.w3.p, I, H, o.w3.ld, 64) &&
+         map16(&p.b[0], dg, T, I, ldm, nt) && map16(&p.b[1], du, T, I, ldm, nt);
+    DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (dx)");
+    p.M[0] = H, p.N[0] = T, p.K = I;
+    p.out[0] = dx, p.ldo[0] = H;
+    if ((st = run_tiles<DX>(p, nt, s, chained)) != DS_OK) return st;
+    chained = true;
+  }
+  // what weight gradients are left: dW1 and dW3 [I, H] from x against dg and du, dW2 [H, I] from h against dy
+  void* const left[3] = {dw_pair ? nullptr : dw1, dw_pair ? nullptr : dw3, dw2_pair ? nullptr : dw2};
+  if (left[0] || left[1] || left[2]) {
+    const Operand grads[3] = {og, ou, gy}, acts[3] = {o.x, o.x, oh};
     TileParams p = {};
     p.f16 = f16, p.err = err, p.K = T;
     for (int z = 0; z < 3; ++z) {
-      if (!outs[z]) continue;     // M = 0: the problem's CTAs return at once
+      if (!left[z]) continue;     // M = 0: the problem's CTAs return at once
       p.M[z] = (int)acts[z].cols, p.N[z] = (int)grads[z].cols;
-      p.out[z] = outs[z], p.ldo[z] = acts[z].cols;
+      p.out[z] = left[z], p.ldo[z] = acts[z].cols;
       ok = map16(&p.a[z], acts[z].p, T, acts[z].cols, acts[z].ld, 64) &&
            map16(&p.b[z], grads[z].p, T, grads[z].cols, grads[z].ld, 64);
       DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (weight gradients)");

@@ -11,8 +11,15 @@
 // Persistent, one cluster per two SMs, 320 threads a CTA: warp 0 copies
 // (both CTAs signal the leader's barrier), warp 1 of the leader issues the
 // MMAs, warps 2-9 empty one 256-column accumulator while the other fills.
-// Lanes are rows here, so a thread owns runs of 32 columns of its row and
-// stores them 16 bytes at a time.
+// Lanes are rows here.  The f32 pre-activations go out (and come back in the
+// backward pass) as 32 x 32 boxes through 8 KB of shared memory per epilogue
+// warp: a thread's own 16-byte stores to 32 rows at a time made the epilogue
+// longer than the 64 stages of a tile (gate / up of 8192 x 4096 x 2048: 212
+// us with them, 176 us when nothing was kept).
+//
+// A launch may hold two groups of problems with different contractions (the
+// gradient of W2 beside that of the hidden values; those of W1 and W3 beside
+// dx), so that the last wave of tiles is one of the shorter ones.
 #pragma once
 
 #include "dense16.cuh"
@@ -20,40 +27,42 @@
 namespace ds {
 namespace dense {
 
-enum Mode { GATED, PLAIN, DHID, DX, DW };
+enum Epilogue { STORE, GATED, HIDDEN };   // plain result; h (and g, u); dg and du
+
+struct Problem {
+  CUtensorMap a[2], b[2];      // operands of the segments; GATED: b = W1, W3
+  CUtensorMap out;             // STORE with boxed = 1: the result in boxes of 64 columns x 32 rows
+  void* c[2];                  // result [m * ldc + n], 16 bit (HIDDEN: dg, du)
+  int64_t ldc;
+  int M, N;                    // rows and columns of the result
+  int ksteps, segs;            // stages of one segment, segments
+  int a_mn, b_mn;              // operand stored with m / n running fastest
+  int epi, boxed;
+  int tiles;                   // filled by the launch
+};
 
 struct PairParams {
-  CUtensorMap a[3], b[3];      // GATED: b = W1, W3; DX: segments; DW: three problems
-  int M[3], N[3];              // rows and columns of each problem's result
-  void* out[3];                // out[m * ldo + n], 16 bit (DHID: dg, du)
-  int64_t ldo[3];
-  int tiles[3];                // tiles of the problems up to and with this one
-  int K;                       // contraction of one segment
+  Problem pr[3];
+  int n, split;                // problems; the first `split` form group 0
+  CUtensorMap g, u;            // f32 pre-activations, boxes of 32 x 32
+  int keep;                    // GATED: write them
   int f16;
   float limit;
-  float* g;                    // f32 pre-activations [m * ldp + n]: written (GATED, may be null), read (DHID)
-  float* u;
-  int64_t ldp;
   int* err;
 };
 
 namespace pair {
 
-constexpr int kStages = 6;
+constexpr int kStages = 5;
 constexpr int kOperand = 2 * kBoxBytes;          // 128 rows x 64
 constexpr int kStage = 2 * kOperand;
-constexpr int kSmem = 1024 + kStages * kStage;
-constexpr int kThreads = 320;
 constexpr int kEpiWarps = 8;
+constexpr int kBox = 4096;                       // 32 rows of 128 bytes
+constexpr int kSmem = 1024 + kStages * kStage + kEpiWarps * 2 * kBox;
+constexpr int kThreads = 32 * (2 + kEpiWarps);
+static_assert(kSmem <= 227 * 1024 - 1024, "shared memory of an SM");
 
-template <int MODE>
-struct Shape {
-  static constexpr bool kAMn = MODE == DW;
-  static constexpr bool kBMn = MODE == DHID || MODE == DX || MODE == DW;
-  static constexpr int kSegs = MODE == DX ? 2 : 1;
-  static constexpr int kProblems = MODE == DW ? 3 : 1;
-  static constexpr int kCols = MODE == GATED ? 128 : 256;   // result columns of a tile
-};
+__host__ __device__ constexpr int tile_cols(int epi) { return epi == GATED ? 128 : 256; }
 
 __device__ __forceinline__ uint32_t leader_addr(const void* p) {
   uint32_t r;
@@ -61,16 +70,23 @@ __device__ __forceinline__ uint32_t leader_addr(const void* p) {
   return r;
 }
 
-// A tile load whose bytes are counted on the leader's barrier.
+// Half a tile's operand (128 rows x 64), its bytes counted on the leader's barrier.
+__device__ __forceinline__ void load_box(uint8_t* dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
+
 template <bool MN>
 __device__ __forceinline__ void load_half(uint8_t* dst, const CUtensorMap* map, int r0, int k0, uint32_t bar) {
-#pragma unroll
-  for (int b = 0; b < (MN ? 2 : 1); ++b)
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
-        "[%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst + b * kBoxBytes)),
-        "l"(map), "r"(MN ? r0 + 64 * b : k0), "r"(MN ? k0 : r0), "r"(bar)
-        : "memory");
+  if (MN) {
+    load_box(dst, map, r0, k0, bar);
+    load_box(dst + kBoxBytes, map, r0 + 64, k0, bar);
+  } else {
+    load_box(dst, map, k0, r0, bar);
+  }
 }
 
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -129,50 +145,142 @@ __device__ __forceinline__ void store16(uint16_t* dst, const float (&v)[32], int
   }
 }
 
-// f32 rows of the saved pre-activations: their stride is a multiple of 8, so
-// whole groups of four may be moved where at least one column is inside.
-__device__ __forceinline__ void store_pre(float* dst, const float (&v)[32], int n) {
-#pragma unroll
-  for (int c = 0; c < 8; ++c)
-    if (4 * c < n) *reinterpret_cast<float4*>(dst + 4 * c) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+// A box of 32 lines of 128 bytes in shared memory, 16-byte pieces swizzled:
+// lane = line, piece c of it.
+__device__ __forceinline__ uint4* box_at(uint8_t* box, int lane, int c) {
+  return reinterpret_cast<uint4*>(box + lane * 128 + ((c ^ (lane & 7)) << 4));
 }
 
-__device__ __forceinline__ void load_pre(const float* src, float (&v)[32], int n) {
+__device__ __forceinline__ void box_put(uint8_t* box, int lane, const float (&v)[32]) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    *box_at(box, lane, c) = make_uint4(__float_as_uint(v[4 * c]), __float_as_uint(v[4 * c + 1]),
+                                       __float_as_uint(v[4 * c + 2]), __float_as_uint(v[4 * c + 3]));
+}
+
+__device__ __forceinline__ void box_get(uint8_t* box, int lane, float (&v)[32]) {
 #pragma unroll
   for (int c = 0; c < 8; ++c) {
-    const float4 t = 4 * c < n ? *reinterpret_cast<const float4*>(src + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
-    v[4 * c] = t.x, v[4 * c + 1] = t.y, v[4 * c + 2] = t.z, v[4 * c + 3] = t.w;
+    const uint4 w = *box_at(box, lane, c);
+    v[4 * c] = __uint_as_float(w.x), v[4 * c + 1] = __uint_as_float(w.y);
+    v[4 * c + 2] = __uint_as_float(w.z), v[4 * c + 3] = __uint_as_float(w.w);
   }
 }
 
-// A tile: problem z, first row and first column of the result.  Rows run
-// fastest inside bands of 16 row tiles, so the CTAs at work at one time share
-// both operands in L2.
-template <int MODE>
-__device__ __forceinline__ void locate(const PairParams& p, int tile, int& z, int& m0, int& n0) {
-  z = 0;
-  if (Shape<MODE>::kProblems > 1)
-    while (z < Shape<MODE>::kProblems - 1 && tile >= p.tiles[z]) ++z;
-  if (z) tile -= p.tiles[z - 1];
-  const int mt = (p.M[z] + 255) / 256, nt = (p.N[z] + Shape<MODE>::kCols - 1) / Shape<MODE>::kCols;
+// One thread: the box goes to columns x.., rows y.. (clipped to the matrix).
+__device__ __forceinline__ void box_store(const CUtensorMap* map, int x, int y, const uint8_t* box) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x),
+               "r"(y), "r"(smem_u32(box))
+               : "memory");
+}
+__device__ __forceinline__ void box_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// This thread's stores but the last N have read their boxes.
+template <int N>
+__device__ __forceinline__ void box_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void box_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// The i-th tile of pair c.  Group 0 is dealt round robin.  A tile of group 1
+// goes to the pair that is free first (ties: fewer tiles of group 0, then the
+// lower index), which a pair can tell for itself: x pairs have one tile of
+// group 0 more than the others, a tile of group 0 takes `a` stages and one of
+// group 1 `b`, so the m-th tile of one of the y others comes after m * y + c'
+// of theirs and the ceil(m - a / b) * x that start before it, and so on.
+// Returns -1 after the last.
+struct Dealer {
+  int t0, t1, pairs, c, own0;
+  int64_t a, b;
+  __device__ __forceinline__ Dealer(const PairParams& p, int pairs_, int c_) : pairs(pairs_), c(c_) {
+    t0 = p.pr[p.split - 1].tiles;
+    t1 = p.pr[p.n - 1].tiles - t0;
+    a = (int64_t)p.pr[0].ksteps * p.pr[0].segs;
+    b = (int64_t)p.pr[p.n - 1].ksteps * p.pr[p.n - 1].segs;
+    own0 = t0 / pairs + (c < t0 % pairs ? 1 : 0);
+  }
+  __device__ __forceinline__ int tile(int i) const {
+    if (i < own0) return c + i * pairs;
+    const int64_t m = i - own0, x = t0 % pairs, y = pairs - x;
+    int64_t rank;
+    if (c < x) rank = m * x + c + ((m * b + a) / b + 1) * y;
+    else rank = m * y + (c - x) + (m * b > a ? (m * b - a + b - 1) / b : 0) * x;
+    return rank < t1 ? t0 + (int)rank : -1;
+  }
+};
+
+// A tile's problem, first row and first column of its result.  Rows run
+// fastest inside bands of 16 row tiles, so the pairs at work at one time
+// share both operands in L2.
+__device__ __forceinline__ int locate(const PairParams& p, int tile, int& m0, int& n0) {
+  int z = 0;
+  while (z < p.n - 1 && tile >= p.pr[z].tiles) ++z;
+  if (z) tile -= p.pr[z - 1].tiles;
+  const Problem& q = p.pr[z];
+  const int cols = tile_cols(q.epi), mt = (q.M + 255) / 256, nt = (q.N + cols - 1) / cols;
   const int band = tile / (16 * nt), in = tile - band * 16 * nt, rows = min(16, mt - 16 * band);
-  n0 = (in / rows) * Shape<MODE>::kCols;
+  n0 = (in / rows) * cols;
   m0 = (16 * band + in % rows) * 256;
+  return z;
 }
 
-template <int MODE>
+struct Rings {
+  uint64_t *full, *empty;
+  uint8_t* smem;
+  volatile int* abort;
+  int* err;
+};
+
+// The copies of one tile, stages g on.  False: a wait gave up.
+template <bool AMN, bool BMN, bool GATE>
+__device__ __forceinline__ bool copy_tile(const Rings& r, const Problem& q, int rank, int m0, int n0, int& g) {
+  const int ksteps = q.ksteps, its = ksteps * q.segs, am = m0 + 128 * rank, bn = GATE ? n0 : n0 + 128 * rank;
+  for (int it = 0; it < its; ++it, ++g) {
+    const int s = g % kStages;
+    if (g >= kStages && !grouped::wait_or_abort(&r.empty[s], ((g / kStages) - 1) & 1, r.abort, r.err)) return false;
+    const int seg = it >= ksteps ? 1 : 0, k0 = (it - seg * ksteps) * kBK;
+    uint8_t* st = r.smem + s * kStage;
+    const uint32_t bar = leader_addr(&r.full[s]);
+    if (rank == 0) mbar_arrive_expect_tx(&r.full[s], 2 * kStage);
+    load_half<AMN>(st, &q.a[seg], am, k0, bar);
+    load_half<BMN>(st + kOperand, &q.b[GATE ? rank : seg], bn, k0, bar);
+  }
+  return true;
+}
+
+// The MMAs of one tile, issued by an elected lane of a warp-uniform loop with
+// descriptors that differ by constants (held in uniform registers; operand
+// layouts read at run time instead made the 64 stages of a tile a fifth slower).
+template <bool AMN, bool BMN>
+__device__ __forceinline__ bool mma_tile(const Rings& r, int its, int f16, uint32_t acc, int& g) {
+  const uint32_t idesc = idesc16(f16, AMN, BMN, 256, 256);
+  const uint64_t a0 = tile_desc<AMN>(smem_u32(r.smem)), b0 = tile_desc<BMN>(smem_u32(r.smem) + kOperand);
+  for (int it = 0; it < its; ++it, ++g) {
+    const int s = g % kStages;
+    if (!grouped::warp_wait(&r.full[s], (g / kStages) & 1, r.abort, r.err)) return false;
+    tc5::fence_after();
+    if (elect_one()) {
+      const uint64_t ad = a0 + (uint64_t)((s * kStage) >> 4), bd = b0 + (uint64_t)((s * kStage) >> 4);
+#pragma unroll
+      for (int kk = 0; kk < kBK / 16; ++kk) mma(acc, ad + kk * kStep16<AMN>, bd + kk * kStep16<BMN>, idesc, (it | kk) != 0);
+      commit(&r.empty[s]);
+    }
+    __syncwarp();
+  }
+  return true;
+}
+
+// EPI: the launch's epilogue beside STORE.
+template <int EPI>
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_kernel(const __grid_constant__ PairParams p) {
-  using C = Shape<MODE>;
   constexpr int S = kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  __shared__ __align__(8) uint64_t full[S], empty[S], accfull[2], accempty[2];
+  __shared__ __align__(8) uint64_t full[S], empty[S], accfull[2], accempty[2], boxfull[kEpiWarps];
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = blockIdx.x & 1, pairs = gridDim.x >> 1, first = blockIdx.x >> 1;
-  const int n_tiles = p.tiles[C::kProblems - 1];
-  const int ksteps = (p.K + kBK - 1) / kBK, its = C::kSegs * ksteps;
+  const int rank = blockIdx.x & 1;
+  const Dealer dealer(p, gridDim.x >> 1, blockIdx.x >> 1);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -183,6 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
       mbar_init(&accfull[b], 1);
       mbar_init(&accempty[b], 2 * kEpiWarps);
     }
+    for (int w = 0; w < kEpiWarps; ++w) mbar_init(&boxfull[w], 1);
     abort_flag = 0;
     fence_barrier_init();
   }
@@ -200,26 +309,21 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
   launch_dependents();
   wait_prior_grid();
 
+  const Rings r = {full, empty, smem, abort, p.err};
+
   if (warp == 0) {
     // ------------------------------------------------------------ copies
     if (lane == 0) {
       int g = 0;
-      for (int tile = first; tile < n_tiles; tile += pairs) {
-        int z, m0, n0;
-        locate<MODE>(p, tile, z, m0, n0);
-        for (int it = 0; it < its; ++it, ++g) {
-          const int s = g % S;
-          if (g >= S && !grouped::wait_or_abort(&empty[s], ((g / S) - 1) & 1, abort, p.err)) goto drain;
-          const int seg = C::kSegs > 1 && it >= ksteps ? 1 : 0, k0 = (it - seg * ksteps) * kBK;
-          uint8_t* st = smem + s * kStage;
-          const uint32_t bar = leader_addr(&full[s]);
-          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kStage);
-          load_half<C::kAMn>(st, &p.a[z + seg], m0 + 128 * rank, k0, bar);
-          load_half<C::kBMn>(st + kOperand, &p.b[MODE == GATED ? rank : z + seg],
-                             MODE == GATED ? n0 : n0 + 128 * rank, k0, bar);
-        }
+      bool ok = true;
+      for (int i = 0, tile; ok && (tile = dealer.tile(i)) >= 0; ++i) {
+        int m0, n0;
+        const Problem& q = p.pr[locate(p, tile, m0, n0)];
+        if (EPI == GATED) ok = copy_tile<false, false, true>(r, q, rank, m0, n0, g);
+        else if (q.a_mn) ok = copy_tile<true, true, false>(r, q, rank, m0, n0, g);
+        else if (q.b_mn) ok = copy_tile<false, true, false>(r, q, rank, m0, n0, g);
+        else ok = copy_tile<false, false, false>(r, q, rank, m0, n0, g);
       }
-    drain:
       // every stage has been read by the MMAs, and the signal of that has
       // arrived, before this CTA's shared memory goes
       for (int j = g - S < 0 ? 0 : g - S; j < g; ++j) mbar_wait_bounded(&empty[j % S], (j / S) & 1, 200000000ull);
@@ -227,100 +331,144 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMAs, by the leader
     if (rank == 0) {
-      const uint32_t idesc = idesc16(p.f16, C::kAMn, C::kBMn, 256, 256);
-      const uint64_t a0 = tile_desc<C::kAMn>(smem_u32(smem)), b0 = tile_desc<C::kBMn>(smem_u32(smem) + kOperand);
-      int g = 0, li = 0;
-      for (int tile = first; tile < n_tiles; tile += pairs, ++li) {
-        const int b = li & 1;
-        if (li >= 2 && !grouped::warp_wait(&accempty[b], ((li >> 1) - 1) & 1, abort, p.err)) break;
+      int g = 0;
+      bool ok = true;
+      for (int i = 0, tile; ok && (tile = dealer.tile(i)) >= 0; ++i) {
+        int m0, n0;
+        const Problem& q = p.pr[locate(p, tile, m0, n0)];
+        const int its = q.ksteps * q.segs, b = i & 1;
+        if (i >= 2 && !grouped::warp_wait(&accempty[b], ((i >> 1) - 1) & 1, abort, p.err)) break;
         tc5::fence_after();
-        for (int it = 0; it < its; ++it, ++g) {
-          const int s = g % S;
-          if (!grouped::warp_wait(&full[s], (g / S) & 1, abort, p.err)) goto mma_out;
-          tc5::fence_after();
-          if (elect_one()) {
-            const uint64_t ad = a0 + (uint64_t)((s * kStage) >> 4), bd = b0 + (uint64_t)((s * kStage) >> 4);
-#pragma unroll
-            for (int kk = 0; kk < kBK / 16; ++kk)
-              mma(tb + b * 256, ad + kk * kStep16<C::kAMn>, bd + kk * kStep16<C::kBMn>, idesc, (it | kk) != 0);
-            commit(&empty[s]);
-          }
-          __syncwarp();
-        }
-        if (elect_one()) commit(&accfull[b]);
+        const uint32_t acc = tb + b * 256;
+        if (EPI != GATED && q.a_mn) ok = mma_tile<true, true>(r, its, p.f16, acc, g);
+        else if (EPI != GATED && q.b_mn) ok = mma_tile<false, true>(r, its, p.f16, acc, g);
+        else ok = mma_tile<false, false>(r, its, p.f16, acc, g);
+        if (ok && elect_one()) commit(&accfull[b]);
         __syncwarp();
       }
-    mma_out:;
     }
   } else {
     // ------------------------------------------------------------ epilogue
-    const int q = warp & 3, half = (warp - 2) >> 2;
-    const uint32_t bar[2] = {leader_addr(&accempty[0]), leader_addr(&accempty[1])};
-    int li = 0;
-    for (int tile = first; tile < n_tiles; tile += pairs, ++li) {
-      int z, m0, n0;
-      locate<MODE>(p, tile, z, m0, n0);
-      const int b = li & 1;
-      const int m = m0 + 128 * rank + 32 * q + lane;
-      const bool row = m < p.M[z];
-      const uint32_t acc = tc5::lane_quarter(tb + b * 256, q);
-      uint16_t* out = static_cast<uint16_t*>(p.out[z]) + (int64_t)m * p.ldo[z];
-      const bool vec = ((reinterpret_cast<uintptr_t>(p.out[z]) | (uintptr_t)(p.ldo[z] * 2)) & 15) == 0;
-      constexpr int kPer = C::kCols / 2;                    // columns of this warp
-      if constexpr (MODE == DHID) {
-        // the first pre-activations are on their way while the MMAs still run
-        const int n = n0 + half * kPer;
-        if (row && n < p.N[0]) {
-          asm volatile("prefetch.global.L2 [%0];" ::"l"(p.g + (int64_t)m * p.ldp + n));
-          asm volatile("prefetch.global.L2 [%0];" ::"l"(p.u + (int64_t)m * p.ldp + n));
+    const int q4 = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* box0 = smem + S * kStage + (warp - 2) * 2 * kBox;
+    uint8_t* box1 = box0 + kBox;
+    uint64_t* loaded = &boxfull[warp - 2];
+    int loads = 0, turn = 0;
+    for (int i = 0, tile; (tile = dealer.tile(i)) >= 0; ++i) {
+      int m0, n0;
+      const Problem& q = p.pr[locate(p, tile, m0, n0)];
+      const int b = i & 1, mw = m0 + 128 * rank + 32 * q4, m = mw + lane;
+      const bool row = m < q.M, hidden = EPI == HIDDEN && q.epi == HIDDEN;
+      const uint32_t acc = tc5::lane_quarter(tb + b * 256, q4);
+      const int per = EPI == GATED ? 64 : 128, nw = n0 + half * per;   // this warp's columns
+      const int nc = mw < q.M ? min(per, q.N - nw) : 0;                // those inside the result
+      uint16_t* out = static_cast<uint16_t*>(q.c[0]) + (int64_t)m * q.ldc;
+      const bool vec = ((reinterpret_cast<uintptr_t>(q.c[0]) | (uintptr_t)(q.ldc * 2)) & 15) == 0;
+      // the pre-activations of 32 columns come in while the accumulator of
+      // the previous ones (or the MMAs) are still at work
+      auto fetch = [&](int c) {
+        if (lane == 0) {
+          mbar_arrive_expect_tx(loaded, 2 * kBox);
+          tma_load_2d(box0, &p.g, nw + c, mw, loaded);
+          tma_load_2d(box1, &p.u, nw + c, mw, loaded);
         }
+      };
+      if (hidden && nc > 0) fetch(0);
+      if (!grouped::warp_wait(&accfull[b], (i >> 1) & 1, abort, p.err)) {
+        if (hidden && nc > 0 && lane == 0) mbar_wait_bounded(loaded, loads & 1, 200000000ull);
+        break;
       }
-      if (!grouped::warp_wait(&accfull[b], (li >> 1) & 1, abort, p.err)) break;
       tc5::fence_after();
+      if (EPI == GATED) {
 #pragma unroll 1
-      for (int c = 0; c < kPer; c += 32) {
-        const int col = half * kPer + c, n = n0 + col, left = p.N[z] - n;
-        const bool in = row && left > 0;
-        __syncwarp();
-        if (MODE == GATED) {
+        for (int c = 0; c < nc; c += 32) {
           float gv[32], uv[32];
-          ld_x32(acc + col, gv);
-          ld_x32(acc + 128 + col, uv);
+          __syncwarp();
+          ld_x32(acc + half * per + c, gv);
+          ld_x32(acc + 128 + half * per + c, uv);
           tc5::wait_ld();
-          if (in) {
-            if (p.g) {
-              store_pre(p.g + (int64_t)m * p.ldp + n, gv, left);
-              store_pre(p.u + (int64_t)m * p.ldp + n, uv, left);
+          if (p.keep) {
+            if (lane == 0) box_wait_read<0>();
+            __syncwarp();
+            box_put(box0, lane, gv);
+            box_put(box1, lane, uv);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              box_store(&p.g, nw + c, mw, box0);
+              box_store(&p.u, nw + c, mw, box1);
+              box_commit();
             }
-#pragma unroll
-            for (int j = 0; j < 32; ++j) gv[j] = gate_unit(gv[j], uv[j], p.limit);
-            store16(out + n, gv, left, vec, p.f16);
           }
-        } else if (MODE == DHID) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) gv[j] = gate_unit(gv[j], uv[j], p.limit);
+          if (row) store16(out + nw + c, gv, nc - c, vec, p.f16);
+        }
+      } else if (hidden) {
+        uint16_t* out1 = static_cast<uint16_t*>(q.c[1]) + (int64_t)m * q.ldc;
+#pragma unroll 1
+        for (int c = 0; c < nc; c += 32) {
           float v[32], gv[32], uv[32];
-          if (in) {
-            load_pre(p.g + (int64_t)m * p.ldp + n, gv, left);
-            load_pre(p.u + (int64_t)m * p.ldp + n, uv, left);
-          }
-          ld_x32(acc + col, v);
+          if (!grouped::warp_wait(loaded, loads & 1, abort, p.err)) break;
+          ++loads;
+          box_get(box0, lane, gv);
+          box_get(box1, lane, uv);
+          // every lane's reads are done before the next boxes may land (without
+          // the fence, reads still queued met the newer values)
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (c + 32 < nc) fetch(c + 32);
+          __syncwarp();
+          ld_x32(acc + half * per + c, v);
           tc5::wait_ld();
-          if (in) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) gate_grad(gv[j], uv[j], v[j], p.limit, gv[j], uv[j]);
-            store16(out + n, gv, left, vec, p.f16);
-            store16(static_cast<uint16_t*>(p.out[1]) + (int64_t)m * p.ldo[1] + n, uv, left, vec, p.f16);
+          for (int j = 0; j < 32; ++j) gate_grad(gv[j], uv[j], v[j], p.limit, gv[j], uv[j]);
+          if (row) {
+            store16(out + nw + c, gv, nc - c, vec, p.f16);
+            store16(out1 + nw + c, uv, nc - c, vec, p.f16);
           }
-        } else {
+        }
+      } else if (q.boxed) {
+#pragma unroll 1
+        for (int c = 0; c < nc; c += 64) {
+          uint8_t* box = turn++ & 1 ? box1 : box0;   // the store before the last has read its box
+          if (lane == 0) box_wait_read<1>();
+          __syncwarp();
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float v[32];
+            ld_x32(acc + half * per + c + 32 * e, v);
+            tc5::wait_ld();
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              *box_at(box, lane, 4 * e + k) =
+                  make_uint4(pack16(v[8 * k], v[8 * k + 1], p.f16), pack16(v[8 * k + 2], v[8 * k + 3], p.f16),
+                             pack16(v[8 * k + 4], v[8 * k + 5], p.f16), pack16(v[8 * k + 6], v[8 * k + 7], p.f16));
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            box_store(&q.out, nw + c, mw, box);
+            box_commit();
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < nc; c += 32) {
           float v[32];
-          ld_x32(acc + col, v);
+          __syncwarp();
+          ld_x32(acc + half * per + c, v);
           tc5::wait_ld();
-          if (in) store16(out + n, v, left, vec, p.f16);
+          if (row) store16(out + nw + c, v, nc - c, false, p.f16);
         }
       }
+      // the boxes are free again before a later tile's loads overwrite them
+      if (EPI == HIDDEN && !hidden && lane == 0) box_wait_read<0>();
       tc5::fence_before();
       __syncwarp();
-      if (lane == 0) arrive_leader(bar[b]);
+      if (lane == 0) arrive_leader(leader_addr(&accempty[b]));
     }
+    if (lane == 0) box_wait_all();
   }
   tc5::fence_before();
   __syncthreads();
