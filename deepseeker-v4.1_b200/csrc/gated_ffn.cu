@@ -29,22 +29,20 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-enum Mode { GATE_UP, PLAIN, DHID, DX, DW };
+enum Mode { GATE_UP, PLAIN, DHID, DX };
 
 template <int MODE>
 struct ModeOf {
-  static constexpr bool kAMn = MODE == DHID || MODE == DX || MODE == DW;   // A stored with m running fastest
-  static constexpr bool kBMn = MODE == DW;
+  static constexpr bool kAMn = MODE == DHID || MODE == DX;                // A stored with m running fastest
   static constexpr int kMats = MODE == GATE_UP ? 2 : 1;                      // accumulators (W1 and W3 share x)
   static constexpr int kSegs = MODE == DX ? 2 : 1;                         // dg W1 and du W3 in one accumulator
-  static constexpr int kProblems = MODE == DW ? 3 : 1;
 };
 
 struct TileParams {
-  CUtensorMap a[3], b[3];
-  int M[3], N[3];              // features (lanes) and tokens / columns of each problem
-  void* out[3];                // out[n * ldo + m], 16 bit
-  int64_t ldo[3];
+  CUtensorMap a[2], b[2];      // GATE_UP: a = W1, W3; DX: segments
+  int M, N;                    // features (lanes) and tokens
+  void* out[2];                // out[n * ldo + m], 16 bit (DHID: dg, du)
+  int64_t ldo;
   int K;                       // contraction of one segment
   int f16;
   float limit;
@@ -66,28 +64,46 @@ struct TileShape {
   static constexpr int kSmem = 1024 + kStages * kStage;
   static constexpr int kCols = Md::kMats * NT < 32 ? 32 : Md::kMats * NT;
   static_assert(kStage % 1024 == 0 && kStages * kStage >= Md::kMats * NT * 128 * 4, "stages hold the partial tile");
-  static_assert(!Md::kBMn || NT % 64 == 0, "MN-major tiles come in boxes of 64");
 };
 
 constexpr int kTileThreads = 192;   // warp 0 copies, warp 1 MMA, warps 2-5 epilogue
 
-// What becomes of one element (m, n) of the accumulator(s).
-template <int MODE>
-__device__ __forceinline__ void tile_store(const TileParams& p, int z, int m, int n, float v0, float v1) {
-  uint16_t* out = static_cast<uint16_t*>(p.out[z]) + (int64_t)n * p.ldo[z] + m;
-  if constexpr (MODE == GATE_UP) {
-    if (p.g) {
-      p.g[(int64_t)n * p.ldp + m] = v0;
-      p.u[(int64_t)n * p.ldp + m] = v1;
+// What becomes of the elements (m, n0 .. n0 + J - 1) of the accumulator(s), nv
+// of them inside the result.  Lanes are features, so a warp's accesses are
+// runs of 32; all reads come before the first write, which could alias them
+// for all the compiler knows (one column after the other, the reads' latency
+// made the hidden gradient of 1024 x 4096 x 2048 five times slower).
+template <int MODE, int J>
+__device__ __forceinline__ void tile_store(const TileParams& p, int m, int n0, int nv, const float (&v0)[J],
+                                           const float (&v1)[J]) {
+  uint16_t* out = static_cast<uint16_t*>(p.out[0]) + (int64_t)n0 * p.ldo + m;
+  const int64_t at = (int64_t)n0 * p.ldp + m;
+  if constexpr (MODE == DHID) {
+    float g[J], u[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      g[j] = j < nv ? p.g[at + j * p.ldp] : 0.0f;
+      u[j] = j < nv ? p.u[at + j * p.ldp] : 0.0f;
     }
-    *out = to16(gate_unit(v0, v1, p.limit), p.f16);
-  } else if constexpr (MODE == DHID) {
-    float dg, du;
-    gate_grad(p.g[(int64_t)n * p.ldp + m], p.u[(int64_t)n * p.ldp + m], v0, p.limit, dg, du);
-    *out = to16(dg, p.f16);
-    static_cast<uint16_t*>(p.out[1])[(int64_t)n * p.ldo[1] + m] = to16(du, p.f16);
+    uint16_t* out1 = static_cast<uint16_t*>(p.out[1]) + (int64_t)n0 * p.ldo + m;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      gate_grad(g[j], u[j], v0[j], p.limit, g[j], u[j]);
+      if (j < nv) {
+        out[j * p.ldo] = to16(g[j], p.f16);
+        out1[j * p.ldo] = to16(u[j], p.f16);
+      }
+    }
   } else {
-    *out = to16(v0, p.f16);
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if (j >= nv) continue;
+      if (MODE == GATE_UP && p.g) {
+        p.g[at + j * p.ldp] = v0[j];
+        p.u[at + j * p.ldp] = v1[j];
+      }
+      out[j * p.ldo] = to16(MODE == GATE_UP ? gate_unit(v0[j], v1[j], p.limit) : v0[j], p.f16);
+    }
   }
 }
 
@@ -104,9 +120,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
   cg::cluster_group cluster = cg::this_cluster();
   const int slices = cluster.dim_blocks().x, slice = cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int z = blockIdx.z;
   const int m0 = (blockIdx.x / slices) * 128, n0 = blockIdx.y * NT;
-  if (m0 >= p.M[z] || n0 >= p.N[z]) return;   // the whole cluster: its CTAs share m0 and n0
   const int ksteps = (p.K + kBK - 1) / kBK;
   const int it0 = (int)((int64_t)Md::kSegs * ksteps * slice / slices);
   const int it1 = (int)((int64_t)Md::kSegs * ksteps * (slice + 1) / slices);
@@ -138,16 +152,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
         const int seg = it / ksteps, k0 = (it - seg * ksteps) * kBK;
         uint8_t* st = smem + s * C::kStage;
         mbar_arrive_expect_tx(&full[s], C::kStage);
-        load_tile<Md::kAMn, 128>(st, &p.a[z + seg], m0, k0, &full[s]);
+        load_tile<Md::kAMn, 128>(st, &p.a[seg], m0, k0, &full[s]);
         if (Md::kMats == 2) load_tile<Md::kAMn, 128>(st + 2 * kBoxBytes, &p.a[1], m0, k0, &full[s]);
-        load_tile<Md::kBMn, NT>(st + C::kA, &p.b[z + seg], n0, k0, &full[s]);
+        load_tile<false, NT>(st + C::kA, &p.b[seg], n0, k0, &full[s]);
       }
       // never leave with copies in flight into this CTA's shared memory
       for (int j = g - S < 0 ? 0 : g - S; j < g; ++j) mbar_wait_bounded(&full[j % S], (j / S) & 1, 200000000ull);
     }
   } else if (warp == 1) {
-    const uint32_t idesc = idesc16(p.f16, Md::kAMn, Md::kBMn, 128, NT);
-    const uint64_t a0 = tile_desc<Md::kAMn>(smem_u32(smem)), b0 = tile_desc<Md::kBMn>(smem_u32(smem) + C::kA);
+    const uint32_t idesc = idesc16(p.f16, Md::kAMn, false, 128, NT);
+    const uint64_t a0 = tile_desc<Md::kAMn>(smem_u32(smem)), b0 = tile_desc<false>(smem_u32(smem) + C::kA);
     for (int g = 0; g < it1 - it0; ++g) {
       const int s = g % S;
       if (!grouped::warp_wait(&full[s], (g / S) & 1, abort, p.err)) break;
@@ -156,10 +170,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
         const uint64_t ad = a0 + (uint64_t)((s * C::kStage) >> 4), bd = b0 + (uint64_t)((s * C::kStage) >> 4);
 #pragma unroll
         for (int kk = 0; kk < kBK / 16; ++kk) {
-          tc5::mma_bf16(tb, ad + kk * kStep16<Md::kAMn>, bd + kk * kStep16<Md::kBMn>, idesc, (g | kk) != 0);
+          tc5::mma_bf16(tb, ad + kk * kStep16<Md::kAMn>, bd + kk * kStep16<false>, idesc, (g | kk) != 0);
           if (Md::kMats == 2)
             tc5::mma_bf16(tb + NT, ad + ((2 * kBoxBytes) >> 4) + kk * kStep16<Md::kAMn>,
-                          bd + kk * kStep16<Md::kBMn>, idesc, (g | kk) != 0);
+                          bd + kk * kStep16<false>, idesc, (g | kk) != 0);
         }
         tc5::commit(&empty[s]);
       }
@@ -176,7 +190,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
 
   // ---- epilogue: thread = one feature (lane of tensor memory)
   const int q = warp & 3, mi = q * 32 + lane, m = m0 + mi;
-  const int nv = min(NT, p.N[z] - n0);
+  const int nv = min(NT, p.N - n0);
   float* part = reinterpret_cast<float*>(smem);   // [mats][NT][128]
   if (warp >= 2) {
     for (int c0 = 0; c0 < nv; c0 += 16) {
@@ -189,24 +203,28 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
         for (int t = 0; t < Md::kMats; ++t)
 #pragma unroll
           for (int j = 0; j < 16; ++j) part[(t * NT + c0 + j) * 128 + mi] = v[t][j];
-      } else if (m < p.M[z]) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (c0 + j < nv) tile_store<MODE>(p, z, m, n0 + c0 + j, v[0][j], v[Md::kMats - 1][j]);
+      } else if (m < p.M) {
+        tile_store<MODE>(p, m, n0 + c0, nv - c0, v[0], v[Md::kMats - 1]);
       }
     }
   }
   if (slices > 1) {
     cluster.sync();
-    if (warp >= 2 && m < p.M[z]) {
-      for (int n = slice; n < nv; n += slices) {
-        float v0 = 0.0f, v1 = 0.0f;
+    if (warp >= 2 && m < p.M) {
+      // this CTA's share of the columns, four at a time
+      const int share = (nv + slices - 1) / slices, end = min(nv, (slice + 1) * share);
+      for (int n = slice * share; n < end; n += 4) {
+        float v[2][4] = {};
         for (int r = 0; r < slices; ++r) {
-          const float* src = cluster.map_shared_rank(part, r);
-          v0 += src[n * 128 + mi];
-          if (Md::kMats == 2) v1 += src[(NT + n) * 128 + mi];
+          const float* src = cluster.map_shared_rank(part, r) + mi;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (n + j >= end) continue;
+            v[0][j] += src[(n + j) * 128];
+            if (Md::kMats == 2) v[1][j] += src[(NT + n + j) * 128];
+          }
         }
-        tile_store<MODE>(p, z, m, n0 + n, v0, v1);
+        tile_store<MODE>(p, m, n0 + n, end - n, v[0], v[1]);
       }
     }
     cluster.sync();   // partial tiles stay until every CTA has read them
@@ -276,12 +294,11 @@ int* err_word() {
 }
 
 template <int MODE, int NT>
-int launch_tiles(const TileParams& p, int max_m, int max_n, int slices, cudaStream_t s, bool chained) {
+int launch_tiles(const TileParams& p, int slices, cudaStream_t s, bool chained) {
   using C = TileShape<MODE, NT>;
   DS_CHECK_CUDA(cudaFuncSetAttribute(tile_kernel<MODE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((max_m + 127) / 128 * slices), (unsigned)((max_n + NT - 1) / NT),
-                     ModeOf<MODE>::kProblems);
+  cfg.gridDim = dim3((unsigned)((p.M + 127) / 128 * slices), (unsigned)((p.N + NT - 1) / NT));
   cfg.blockDim = dim3(kTileThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = s;
@@ -309,70 +326,101 @@ int slices_for(int64_t tiles, int ksteps) {
 
 template <int MODE>
 int run_tiles(const TileParams& p, int nt, cudaStream_t s, bool chained) {
-  using Md = ModeOf<MODE>;
-  int max_m = 0, max_n = 0;
-  int64_t tiles = 0;
-  for (int z = 0; z < Md::kProblems; ++z) {
-    max_m = std::max(max_m, p.M[z]);
-    max_n = std::max(max_n, p.N[z]);
-    tiles += (int64_t)((p.M[z] + 127) / 128) * ((p.N[z] + nt - 1) / nt);
-  }
-  const int slices = slices_for(tiles, Md::kSegs * ((p.K + kBK - 1) / kBK));
-  if constexpr (MODE != DW) {
-    if (nt == 16) return launch_tiles<MODE, 16>(p, max_m, max_n, slices, s, chained);
-    if (nt == 32) return launch_tiles<MODE, 32>(p, max_m, max_n, slices, s, chained);
-    if (nt == 64) return launch_tiles<MODE, 64>(p, max_m, max_n, slices, s, chained);
-  }
-  return launch_tiles<MODE, 128>(p, max_m, max_n, slices, s, chained);
+  const int64_t tiles = (int64_t)((p.M + 127) / 128) * ((p.N + nt - 1) / nt);
+  const int slices = slices_for(tiles, ModeOf<MODE>::kSegs * ((p.K + kBK - 1) / kBK));
+  if (nt == 16) return launch_tiles<MODE, 16>(p, slices, s, chained);
+  if (nt == 32) return launch_tiles<MODE, 32>(p, slices, s, chained);
+  if (nt == 64) return launch_tiles<MODE, 64>(p, slices, s, chained);
+  return launch_tiles<MODE, 128>(p, slices, s, chained);
 }
 
 // ---- pair kernel
 
-// Tiles of an [M, N] result in the pair kernel.
-int64_t pair_tiles(int epi, int64_t M, int64_t N) {
-  const int c = pair::tile_cols(epi);
-  return (M + 255) / 256 * ((N + c - 1) / c);
+// The pair kernel takes the products of at least this many rows; weight
+// gradients always.
+constexpr int kPairRows = 129;
+
+int64_t tiles_of(const Problem& q, int nt) {
+  const int c = pair::tile_cols(q.epi, nt);
+  return (q.M + 255) / 256 * (int64_t)((q.N + c - 1) / c);
 }
 
-// The pair kernel takes the products with at least this many tiles.
-constexpr int kPairMin = 37;
-
-// Adds the problem c = a b^T (a and b given with their own layouts; k the
-// contraction) to a launch.
-Problem* add(PairParams& p, int epi, int64_t M, int64_t N, int64_t k, void* c, int64_t ldc) {
+// Adds the problem c = a b^T to a launch (k: the contraction).  Problems of
+// one contraction form a group; the longer one is given first.
+Problem* add(PairParams& p, int epi, int64_t M, int64_t N, int64_t k, int segs, void* c, int64_t ldc) {
   Problem& q = p.pr[p.n++];
   q.epi = epi, q.M = (int)M, q.N = (int)N;
-  q.ksteps = (int)((k + kBK - 1) / kBK), q.segs = 1;
+  q.ksteps = (int)((k + kBK - 1) / kBK), q.segs = segs;
   q.c[0] = c, q.ldc = ldc;
-  q.tiles = (int)(pair_tiles(epi, M, N) + (p.n > 1 ? p.pr[p.n - 2].tiles : 0));
   return &q;
 }
 
-// Boxes of the result where its rows allow them.
-bool box_result(Problem& q) {
-  q.boxed = q.epi == STORE && direct(q.c[0], q.ldc);
-  return !q.boxed || map16(&q.out, q.c[0], q.M, q.N, q.ldc, 32);
+// One of a launch's problems with its operands; W3's map of a gate / up
+// product in b1.
+struct Sides {
+  Problem* q;
+  Operand a0, b0, a1, b1;
+};
+
+// Time of a launch in tensor cycles for tiles of nt columns: a stage takes 2 nt
+// of them, or what its bytes take at the ~70 bytes a cycle that an SM gets
+// from L2; a tile's epilogue is hidden but for the last; whole tiles per pair.
+int64_t cycles_of(const PairParams& p, int nt, int pairs) {
+  const int64_t stage = nt == 256 ? 512 : nt == 128 ? 350 : 300;
+  int64_t work = 0, longest = 0, tiles = 0;
+  for (int z = 0; z < p.n; ++z) {
+    const int64_t its = (int64_t)p.pr[z].ksteps * p.pr[z].segs, n = tiles_of(p.pr[z], nt), tile = its * stage + 400;
+    work += n * tile;
+    tiles += n;
+    longest = std::max(longest, tile);
+  }
+  const int64_t level = (work + pairs - 1) / pairs;
+  return p.split == p.n ? (tiles + pairs - 1) / pairs * longest : std::max(longest, level + longest / 4);
 }
 
-// Operand maps: box rows by the way the operand is stored.
-bool side(CUtensorMap* m, const Operand& o, int mn) { return map16(m, o.p, o.rows, o.cols, o.ld, mn ? 64 : 128); }
-
-template <int EPI>
-int run_pairs(PairParams& p, cudaStream_t s, bool chained) {
-  if (p.split == 0) p.split = p.n;
-  DS_CHECK_CUDA(cudaFuncSetAttribute(pair::pair_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, pair::kSmem));
+template <int EPI, int NT>
+int launch_pairs(PairParams& p, Sides* sides, cudaStream_t s, bool chained) {
+  using C = pair::Shape<NT>;
+  int64_t tiles = 0;
+  for (int z = 0; z < p.n; ++z) {
+    Problem& q = p.pr[z];
+    const Sides& d = sides[z];
+    auto side = [&](CUtensorMap* m, const Operand& o, int mn, int rows) {
+      return !o.p || map16(m, o.p, o.rows, o.cols, o.ld, mn ? 64 : rows);
+    };
+    q.boxed = q.epi == STORE && direct(q.c[0], q.ldc);
+    const bool ok = side(&q.a[0], d.a0, q.a_mn, 128) && side(&q.a[1], d.a1, q.a_mn, 128) &&
+                    side(&q.b[0], d.b0, q.b_mn, NT / 2) && side(&q.b[1], d.b1, q.b_mn, NT / 2) &&
+                    (!q.boxed || map16(&q.out, q.c[0], q.M, q.N, q.ldc, 32));
+    DS_REQUIRE(ok, DS_ECUDA, "gated_ffn: tensor map encoding failed");
+    tiles += tiles_of(q, NT);
+    DS_REQUIRE(tiles < ((int64_t)1 << 31), DS_ERANGE, "gated_ffn: too many tiles");
+    q.tiles = (int)tiles;
+  }
+  DS_CHECK_CUDA(cudaFuncSetAttribute(pair::pair_kernel<EPI, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(2 * std::min(p.pr[p.n - 1].tiles, ds::sm_count() / 2)));
+  cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, ds::sm_count() / 2)));
   cfg.blockDim = dim3(pair::kThreads);
-  cfg.dynamicSmemBytes = pair::kSmem;
+  cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = chained ? 1 : 0;
-  DS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, pair::pair_kernel<EPI>, p));
+  DS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, pair::pair_kernel<EPI, NT>, p));
   return DS_OK;
+}
+
+// Runs the problems with the tile width that takes least time.
+template <int EPI>
+int run_pairs(PairParams& p, Sides* sides, cudaStream_t s, bool chained) {
+  if (p.split == 0) p.split = p.n;
+  const int pairs = ds::sm_count() / 2;
+  const int64_t t256 = cycles_of(p, 256, pairs), t128 = cycles_of(p, 128, pairs), t64 = cycles_of(p, 64, pairs);
+  if (t256 <= t128 && t256 <= t64) return launch_pairs<EPI, 256>(p, sides, s, chained);
+  if (t128 <= t64) return launch_pairs<EPI, 128>(p, sides, s, chained);
+  return launch_pairs<EPI, 64>(p, sides, s, chained);
 }
 
 int validate(const DsGatedFfn* d) {
@@ -456,44 +504,34 @@ extern "C" int ds_gated_ffn(const DsGatedFfn* desc, void* y, void* h, float* pre
   DS_REQUIRE(err != nullptr, DS_ECUDA, "gated_ffn: error word unavailable");
   const int f16 = desc->dtype == DS_F16;
   float* pre_u = pre ? pre + (int64_t)T * ldm : nullptr;
-  const int nt = token_tile(T);
+  const Operand oh = {h, T, I, ldm}, none = {};
 
-  if (pair_tiles(GATED, T, I) >= kPairMin) {
+  if (T >= kPairRows) {
     PairParams p = {};
     p.f16 = f16, p.limit = desc->limit, p.err = err, p.keep = pre != nullptr;
-    Problem& q = *add(p, GATED, T, I, H, h, ldm);
-    const bool ok = side(&q.a[0], o.x, 0) && side(&q.b[0], o.w1, 0) && side(&q.b[1], o.w3, 0) &&
-                    (!pre || (map32(&p.g, pre, T, I, ldm) && map32(&p.u, pre_u, T, I, ldm)));
-    DS_REQUIRE(ok, DS_ECUDA, "gated_ffn: tensor map encoding failed (gate / up)");
-    st = run_pairs<GATED>(p, s, false);
-  } else {
-    TileParams p = {};
-    p.f16 = f16, p.limit = desc->limit, p.err = err;
-    const bool ok = map16(&p.a[0], o.w1.p, I, H, o.w1.ld, 128) && map16(&p.a[1], o.w3.p, I, H, o.w3.ld, 128) &&
-                    map16(&p.b[0], o.x.p, T, H, o.x.ld, nt);
-    DS_REQUIRE(ok, DS_ECUDA, "gated_ffn: tensor map encoding failed (gate / up)");
-    p.M[0] = I, p.N[0] = T, p.K = H;
-    p.out[0] = h, p.ldo[0] = ldm;
-    p.g = pre, p.u = pre_u, p.ldp = ldm;
-    st = run_tiles<GATE_UP>(p, nt, s, false);
+    Sides up[1] = {{add(p, GATED, T, I, H, 1, h, ldm), o.x, o.w1, none, o.w3}};
+    DS_REQUIRE(!pre || (map32(&p.g, pre, T, I, ldm) && map32(&p.u, pre_u, T, I, ldm)), DS_ECUDA,
+               "gated_ffn: tensor map encoding failed (pre-activations)");
+    if ((st = run_pairs<GATED>(p, up, s, false)) != DS_OK) return st;
+    PairParams d = {};
+    d.f16 = f16, d.err = err;
+    Sides down[1] = {{add(d, STORE, T, H, I, 1, y, H), oh, o.w2, none, none}};
+    return run_pairs<STORE>(d, down, s, true);
   }
-  if (st != DS_OK) return st;
-
-  const Operand oh = {h, T, I, ldm};
-  if (pair_tiles(STORE, T, H) >= kPairMin) {
-    PairParams p = {};
-    p.f16 = f16, p.err = err;
-    Problem& q = *add(p, STORE, T, H, I, y, H);
-    const bool ok = side(&q.a[0], oh, 0) && side(&q.b[0], o.w2, 0) && box_result(q);
-    DS_REQUIRE(ok, DS_ECUDA, "gated_ffn: tensor map encoding failed (down)");
-    return run_pairs<STORE>(p, s, true);
-  }
+  const int nt = token_tile(T);
   TileParams p = {};
-  p.f16 = f16, p.err = err;
-  const bool ok = map16(&p.a[0], o.w2.p, H, I, o.w2.ld, 128) && map16(&p.b[0], h, T, I, ldm, nt);
+  p.f16 = f16, p.limit = desc->limit, p.err = err;
+  bool ok = map16(&p.a[0], o.w1.p, I, H, o.w1.ld, 128) && map16(&p.a[1], o.w3.p, I, H, o.w3.ld, 128) &&
+            map16(&p.b[0], o.x.p, T, H, o.x.ld, nt);
+  DS_REQUIRE(ok, DS_ECUDA, "gated_ffn: tensor map encoding failed (gate / up)");
+  p.M = I, p.N = T, p.K = H;
+  p.out[0] = h, p.ldo = ldm;
+  p.g = pre, p.u = pre_u, p.ldp = ldm;
+  if ((st = run_tiles<GATE_UP>(p, nt, s, false)) != DS_OK) return st;
+  ok = map16(&p.a[0], o.w2.p, H, I, o.w2.ld, 128) && map16(&p.b[0], h, T, I, ldm, nt);
   DS_REQUIRE(ok, DS_ECUDA, "gated_ffn: tensor map encoding failed (down)");
-  p.M[0] = H, p.N[0] = T, p.K = I;
-  p.out[0] = y, p.ldo[0] = H;
+  p.M = H, p.K = I;
+  p.out[0] = y, p.ldo = H;
   return run_tiles<PLAIN>(p, nt, s, true);
 }
 
@@ -541,106 +579,76 @@ extern "C" int ds_gated_ffn_backward(const DsGatedFfn* desc, const void* h, cons
   const int f16 = desc->dtype == DS_F16;
   float* g = const_cast<float*>(pre);
   float* u = g + (int64_t)T * ldm;
-  const int nt = token_tile(T);
-  const Operand og = {dg, T, I, ldm}, ou = {du, T, I, ldm}, oh = {h, T, I, ldm};
-  const bool need_mid = dx || dw1 || dw3;
-  const int64_t wtiles = pair_tiles(STORE, H, I);
-  bool ok = true, chained = false;
+  const Operand og = {dg, T, I, ldm}, ou = {du, T, I, ldm}, oh = {h, T, I, ldm}, none = {};
+  const bool need_mid = dx || dw1 || dw3, wide = T >= kPairRows;
+  auto grad = [&](PairParams& p, Sides* sd, void* dw, int64_t M, int64_t N, const Operand& dy_, const Operand& act) {
+    Problem* q = add(p, STORE, M, N, T, 1, dw, N);   // dw [M, N] = dy_^T act
+    q->a_mn = q->b_mn = 1;
+    sd[p.n - 1] = {q, dy_, act, none, none};
+  };
+  bool chained = false;
 
-  // first launch: dg and du from dy, and beside them dW2, which needs neither
-  const bool mid_pair = need_mid && pair_tiles(HIDDEN, T, I) >= kPairMin;
-  const bool dw2_pair = dw2 && wtiles * ((dw1 != nullptr) + (dw3 != nullptr) + 1) >= kPairMin;
-  if (mid_pair || dw2_pair) {
+  if (wide) {
+    // first launch: dg and du from dy, and beside them dW2, which needs neither
     PairParams p = {};
     p.f16 = f16, p.limit = desc->limit, p.err = err;
-    const bool long_first = T >= H;   // the longer tiles are dealt first
+    Sides sd[3];
     for (int k = 0; k < 2; ++k) {
-      if ((k == 0) == long_first) {
-        if (!dw2_pair) continue;
-        Problem& q = *add(p, STORE, H, I, T, dw2, I);
-        q.a_mn = q.b_mn = 1;
-        ok = ok && side(&q.a[0], gy, 1) && side(&q.b[0], oh, 1) && box_result(q);
-      } else if (mid_pair) {
-        Problem& q = *add(p, HIDDEN, T, I, H, dg, ldm);
-        q.c[1] = du, q.b_mn = 1;
-        ok = ok && side(&q.a[0], gy, 0) && side(&q.b[0], o.w2, 1) && map32(&p.g, g, T, I, ldm) &&
-             map32(&p.u, u, T, I, ldm);
+      if ((k == 0) == (T >= H)) {
+        if (dw2) grad(p, sd, dw2, H, I, gy, oh);
+      } else if (need_mid) {
+        Problem* q = add(p, HIDDEN, T, I, H, 1, dg, ldm);
+        q->c[1] = du, q->b_mn = 1;
+        sd[p.n - 1] = {q, gy, o.w2, none, none};
       }
       if (k == 0) p.split = p.n;
     }
-    DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (hidden gradient)");
-    if ((st = run_pairs<HIDDEN>(p, s, false)) != DS_OK) return st;
-    chained = true;
-  }
-  if (need_mid && !mid_pair) {
+    if (p.n) {
+      DS_REQUIRE(map32(&p.g, g, T, I, ldm) && map32(&p.u, u, T, I, ldm), DS_ECUDA,
+                 "gated_ffn_backward: tensor map encoding failed (pre-activations)");
+      if ((st = run_pairs<HIDDEN>(p, sd, s, false)) != DS_OK) return st;
+      chained = true;
+    }
+  } else {
+    const int nt = token_tile(T);
     TileParams p = {};
     p.f16 = f16, p.limit = desc->limit, p.err = err;
-    ok = map16(&p.a[0], o.w2.p, H, I, o.w2.ld, 64) && map16(&p.b[0], gy.p, T, H, gy.ld, nt);
-    DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (hidden gradient)");
-    p.M[0] = I, p.N[0] = T, p.K = H;
-    p.out[0] = dg, p.out[1] = du, p.ldo[0] = p.ldo[1] = ldm;
-    p.g = g, p.u = u, p.ldp = ldm;
-    if ((st = run_tiles<DHID>(p, nt, s, chained)) != DS_OK) return st;
-    chained = true;
-  }
-
-  // second launch: dW1 and dW3, and beside them dx
-  void* const dw[2] = {dw1, dw3};
-  const Operand* const mid[2] = {&og, &ou};
-  const int64_t w13 = wtiles * ((dw1 != nullptr) + (dw3 != nullptr));
-  const bool dx_pair = dx && pair_tiles(STORE, T, H) >= kPairMin, dw_pair = w13 >= kPairMin;
-  if (dx_pair || dw_pair) {
-    PairParams p = {};
-    p.f16 = f16, p.err = err;
-    const bool long_first = T >= 2 * I;
-    for (int k = 0; k < 2; ++k) {
-      if ((k == 0) == long_first) {
-        for (int z = 0; z < 2 && dw_pair; ++z) {
-          if (!dw[z]) continue;
-          Problem& q = *add(p, STORE, I, H, T, dw[z], H);
-          q.a_mn = q.b_mn = 1;
-          ok = ok && side(&q.a[0], *mid[z], 1) && side(&q.b[0], o.x, 1) && box_result(q);
-        }
-      } else if (dx_pair) {
-        Problem& q = *add(p, STORE, T, H, I, dx, H);
-        q.b_mn = 1, q.segs = 2;
-        ok = ok && side(&q.a[0], og, 0) && side(&q.a[1], ou, 0) && side(&q.b[0], o.w1, 1) && side(&q.b[1], o.w3, 1) &&
-             box_result(q);
-      }
-      if (k == 0) p.split = p.n;
+    p.N = T, p.g = g, p.u = u, p.ldp = ldm;
+    if (need_mid) {
+      const bool ok = map16(&p.a[0], o.w2.p, H, I, o.w2.ld, 64) && map16(&p.b[0], gy.p, T, H, gy.ld, nt);
+      DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (hidden gradient)");
+      p.M = I, p.K = H;
+      p.out[0] = dg, p.out[1] = du, p.ldo = ldm;
+      if ((st = run_tiles<DHID>(p, nt, s, false)) != DS_OK) return st;
+      chained = true;
     }
-    DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (dx, dW1, dW3)");
-    if ((st = run_pairs<STORE>(p, s, chained)) != DS_OK) return st;
-    chained = true;
-  }
-  if (dx && !dx_pair) {
-    TileParams p = {};
-    p.f16 = f16, p.err = err;
-    ok = map16(&p.a[0], o.w1.p, I, H, o.w1.ld, 64) && map16(&p.a[1], o.w3.p, I, H, o.w3.ld, 64) &&
-         map16(&p.b[0], dg, T, I, ldm, nt) && map16(&p.b[1], du, T, I, ldm, nt);
-    DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (dx)");
-    p.M[0] = H, p.N[0] = T, p.K = I;
-    p.out[0] = dx, p.ldo[0] = H;
-    if ((st = run_tiles<DX>(p, nt, s, chained)) != DS_OK) return st;
-    chained = true;
-  }
-  // what weight gradients are left: dW1 and dW3 [I, H] from x against dg and du, dW2 [H, I] from h against dy
-  void* const left[3] = {dw_pair ? nullptr : dw1, dw_pair ? nullptr : dw3, dw2_pair ? nullptr : dw2};
-  if (left[0] || left[1] || left[2]) {
-    const Operand grads[3] = {og, ou, gy}, acts[3] = {o.x, o.x, oh};
-    TileParams p = {};
-    p.f16 = f16, p.err = err, p.K = T;
-    for (int z = 0; z < 3; ++z) {
-      if (!left[z]) continue;     // M = 0: the problem's CTAs return at once
-      p.M[z] = (int)acts[z].cols, p.N[z] = (int)grads[z].cols;
-      p.out[z] = left[z], p.ldo[z] = acts[z].cols;
-      ok = map16(&p.a[z], acts[z].p, T, acts[z].cols, acts[z].ld, 64) &&
-           map16(&p.b[z], grads[z].p, T, grads[z].cols, grads[z].ld, 64);
-      DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (weight gradients)");
+    if (dx) {
+      const bool ok = map16(&p.a[0], o.w1.p, I, H, o.w1.ld, 64) && map16(&p.a[1], o.w3.p, I, H, o.w3.ld, 64) &&
+                      map16(&p.b[0], dg, T, I, ldm, nt) && map16(&p.b[1], du, T, I, ldm, nt);
+      DS_REQUIRE(ok, DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (dx)");
+      p.M = H, p.K = I;
+      p.out[0] = dx, p.ldo = H;
+      if ((st = run_tiles<DX>(p, nt, s, chained)) != DS_OK) return st;
     }
-    return run_tiles<DW>(p, 128, s, chained);
   }
-  return DS_OK;
+  // last launch: dW1 and dW3, and beside them dx, or dW2 of few rows
+  PairParams p = {};
+  p.f16 = f16, p.err = err;
+  Sides sd[3];
+  for (int k = 0; k < 2; ++k) {
+    if (!wide || (k == 0) == (T >= 2 * I)) {
+      if (k == 1 && !wide) break;
+      if (dw1) grad(p, sd, dw1, I, H, og, o.x);
+      if (dw3) grad(p, sd, dw3, I, H, ou, o.x);
+      if (dw2 && !wide) grad(p, sd, dw2, H, I, gy, oh);
+    } else if (dx) {
+      Problem* q = add(p, STORE, T, H, I, 2, dx, H);
+      q->b_mn = 1;
+      sd[p.n - 1] = {q, og, o.w1, ou, o.w3};
+    }
+    if (k == 0) p.split = p.n;
+  }
+  return p.n ? run_pairs<STORE>(p, sd, s, chained) : DS_OK;
 }
 
 extern "C" int ds_gated_ffn_status(int32_t* err, void* stream) {

@@ -1,16 +1,17 @@
 // Pair kernel of the dense gated block: the products of many rows.
 //
-// A cluster of two CTAs computes 256 rows x 256 columns with one
-// tcgen05.mma.cta_group::2 (M = 256, N = 256, K = 16): each CTA stages its
-// 128 rows of A and half of B's 256 rows and holds its rows' accumulators, so
-// a stage of 64 along k costs each SM 32 KB of L2 reads per 512 tensor
-// cycles (a CTA alone on 128 x 256 would need 48 KB).  In the gate / up
-// product the halves of B are 128 rows of W1 and the same 128 rows of W3, so
-// every CTA ends up with g and u of the same features.
+// A cluster of two CTAs computes 256 rows x NT columns (256, or 128 or 64
+// where that would leave SMs without a tile) with one tcgen05.mma.cta_group::2
+// (M = 256, N = NT, K = 16): each CTA stages its 128 rows of A and half of B's
+// NT rows and holds its rows' accumulators, so at NT = 256 a stage of 64
+// along k costs each SM 32 KB of L2 reads per 512 tensor cycles (a CTA alone
+// on 128 x 256 would need 48 KB).  In the gate / up product the halves of B
+// are NT / 2 rows of W1 and the same rows of W3, so every CTA ends up with g
+// and u of the same features.
 //
 // Persistent, one cluster per two SMs, 320 threads a CTA: warp 0 copies
 // (both CTAs signal the leader's barrier), warp 1 of the leader issues the
-// MMAs, warps 2-9 empty one 256-column accumulator while the other fills.
+// MMAs, warps 2-9 empty one NT-column accumulator while the other fills.
 // Lanes are rows here.  The f32 pre-activations go out (and come back in the
 // backward pass) as 32 x 32 boxes through 8 KB of shared memory per epilogue
 // warp: a thread's own 16-byte stores to 32 rows at a time made the epilogue
@@ -53,16 +54,23 @@ struct PairParams {
 
 namespace pair {
 
-constexpr int kStages = 5;
 constexpr int kOperand = 2 * kBoxBytes;          // 128 rows x 64
-constexpr int kStage = 2 * kOperand;
 constexpr int kEpiWarps = 8;
 constexpr int kBox = 4096;                       // 32 rows of 128 bytes
-constexpr int kSmem = 1024 + kStages * kStage + kEpiWarps * 2 * kBox;
 constexpr int kThreads = 32 * (2 + kEpiWarps);
-static_assert(kSmem <= 227 * 1024 - 1024, "shared memory of an SM");
 
-__host__ __device__ constexpr int tile_cols(int epi) { return epi == GATED ? 128 : 256; }
+template <int NT>
+struct Shape {
+  // half of B: NT / 2 rows x 64; MN-major boxes are 64 wide whatever NT
+  static constexpr int kHalf = NT == 256 ? kOperand : kBoxBytes;
+  static constexpr int kStage = kOperand + kHalf;
+  static constexpr int kStages = NT == 256 ? 5 : 6;
+  static constexpr int kSmem = 1024 + kStages * kStage + kEpiWarps * 2 * kBox;
+  static_assert(kSmem <= 226 * 1024, "shared memory of an SM");
+};
+
+// Result columns of a tile.
+__host__ __device__ constexpr int tile_cols(int epi, int nt) { return epi == GATED ? nt / 2 : nt; }
 
 __device__ __forceinline__ uint32_t leader_addr(const void* p) {
   uint32_t r;
@@ -70,7 +78,7 @@ __device__ __forceinline__ uint32_t leader_addr(const void* p) {
   return r;
 }
 
-// Half a tile's operand (128 rows x 64), its bytes counted on the leader's barrier.
+// A CTA's rows of an operand, their bytes counted on the leader's barrier.
 __device__ __forceinline__ void load_box(uint8_t* dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
@@ -79,11 +87,13 @@ __device__ __forceinline__ void load_box(uint8_t* dst, const CUtensorMap* map, i
       : "memory");
 }
 
-template <bool MN>
+// ROWS of them; a K-major box holds them all, MN-major ones 64 each (of 32
+// rows the rest of the box is not used).
+template <bool MN, int ROWS>
 __device__ __forceinline__ void load_half(uint8_t* dst, const CUtensorMap* map, int r0, int k0, uint32_t bar) {
   if (MN) {
     load_box(dst, map, r0, k0, bar);
-    load_box(dst + kBoxBytes, map, r0 + 64, k0, bar);
+    if (ROWS > 64) load_box(dst + kBoxBytes, map, r0 + 64, k0, bar);
   } else {
     load_box(dst, map, k0, r0, bar);
   }
@@ -211,12 +221,13 @@ struct Dealer {
 // A tile's problem, first row and first column of its result.  Rows run
 // fastest inside bands of 16 row tiles, so the pairs at work at one time
 // share both operands in L2.
+template <int NT>
 __device__ __forceinline__ int locate(const PairParams& p, int tile, int& m0, int& n0) {
   int z = 0;
   while (z < p.n - 1 && tile >= p.pr[z].tiles) ++z;
   if (z) tile -= p.pr[z - 1].tiles;
   const Problem& q = p.pr[z];
-  const int cols = tile_cols(q.epi), mt = (q.M + 255) / 256, nt = (q.N + cols - 1) / cols;
+  const int cols = tile_cols(q.epi, NT), mt = (q.M + 255) / 256, nt = (q.N + cols - 1) / cols;
   const int band = tile / (16 * nt), in = tile - band * 16 * nt, rows = min(16, mt - 16 * band);
   n0 = (in / rows) * cols;
   m0 = (16 * band + in % rows) * 256;
@@ -231,18 +242,20 @@ struct Rings {
 };
 
 // The copies of one tile, stages g on.  False: a wait gave up.
-template <bool AMN, bool BMN, bool GATE>
+template <bool AMN, bool BMN, bool GATE, int NT>
 __device__ __forceinline__ bool copy_tile(const Rings& r, const Problem& q, int rank, int m0, int n0, int& g) {
-  const int ksteps = q.ksteps, its = ksteps * q.segs, am = m0 + 128 * rank, bn = GATE ? n0 : n0 + 128 * rank;
+  using C = Shape<NT>;
+  constexpr uint32_t kBytes = kOperand + (BMN ? (NT == 256 ? 2 : 1) * kBoxBytes : NT / 2 * 128);
+  const int ksteps = q.ksteps, its = ksteps * q.segs, am = m0 + 128 * rank, bn = GATE ? n0 : n0 + NT / 2 * rank;
   for (int it = 0; it < its; ++it, ++g) {
-    const int s = g % kStages;
-    if (g >= kStages && !grouped::wait_or_abort(&r.empty[s], ((g / kStages) - 1) & 1, r.abort, r.err)) return false;
+    const int s = g % C::kStages;
+    if (g >= C::kStages && !grouped::wait_or_abort(&r.empty[s], ((g / C::kStages) - 1) & 1, r.abort, r.err)) return false;
     const int seg = it >= ksteps ? 1 : 0, k0 = (it - seg * ksteps) * kBK;
-    uint8_t* st = r.smem + s * kStage;
+    uint8_t* st = r.smem + s * C::kStage;
     const uint32_t bar = leader_addr(&r.full[s]);
-    if (rank == 0) mbar_arrive_expect_tx(&r.full[s], 2 * kStage);
-    load_half<AMN>(st, &q.a[seg], am, k0, bar);
-    load_half<BMN>(st + kOperand, &q.b[GATE ? rank : seg], bn, k0, bar);
+    if (rank == 0) mbar_arrive_expect_tx(&r.full[s], 2 * kBytes);
+    load_half<AMN, 128>(st, &q.a[seg], am, k0, bar);
+    load_half<BMN, NT / 2>(st + kOperand, &q.b[GATE ? rank : seg], bn, k0, bar);
   }
   return true;
 }
@@ -250,16 +263,17 @@ __device__ __forceinline__ bool copy_tile(const Rings& r, const Problem& q, int 
 // The MMAs of one tile, issued by an elected lane of a warp-uniform loop with
 // descriptors that differ by constants (held in uniform registers; operand
 // layouts read at run time instead made the 64 stages of a tile a fifth slower).
-template <bool AMN, bool BMN>
+template <bool AMN, bool BMN, int NT>
 __device__ __forceinline__ bool mma_tile(const Rings& r, int its, int f16, uint32_t acc, int& g) {
-  const uint32_t idesc = idesc16(f16, AMN, BMN, 256, 256);
+  using C = Shape<NT>;
+  const uint32_t idesc = idesc16(f16, AMN, BMN, 256, NT);
   const uint64_t a0 = tile_desc<AMN>(smem_u32(r.smem)), b0 = tile_desc<BMN>(smem_u32(r.smem) + kOperand);
   for (int it = 0; it < its; ++it, ++g) {
-    const int s = g % kStages;
-    if (!grouped::warp_wait(&r.full[s], (g / kStages) & 1, r.abort, r.err)) return false;
+    const int s = g % C::kStages;
+    if (!grouped::warp_wait(&r.full[s], (g / C::kStages) & 1, r.abort, r.err)) return false;
     tc5::fence_after();
     if (elect_one()) {
-      const uint64_t ad = a0 + (uint64_t)((s * kStage) >> 4), bd = b0 + (uint64_t)((s * kStage) >> 4);
+      const uint64_t ad = a0 + (uint64_t)((s * C::kStage) >> 4), bd = b0 + (uint64_t)((s * C::kStage) >> 4);
 #pragma unroll
       for (int kk = 0; kk < kBK / 16; ++kk) mma(acc, ad + kk * kStep16<AMN>, bd + kk * kStep16<BMN>, idesc, (it | kk) != 0);
       commit(&r.empty[s]);
@@ -270,9 +284,9 @@ __device__ __forceinline__ bool mma_tile(const Rings& r, int its, int f16, uint3
 }
 
 // EPI: the launch's epilogue beside STORE.
-template <int EPI>
+template <int EPI, int NT>
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_kernel(const __grid_constant__ PairParams p) {
-  constexpr int S = kStages;
+  constexpr int S = Shape<NT>::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   __shared__ __align__(8) uint64_t full[S], empty[S], accfull[2], accempty[2], boxfull[kEpiWarps];
@@ -318,11 +332,11 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
       bool ok = true;
       for (int i = 0, tile; ok && (tile = dealer.tile(i)) >= 0; ++i) {
         int m0, n0;
-        const Problem& q = p.pr[locate(p, tile, m0, n0)];
-        if (EPI == GATED) ok = copy_tile<false, false, true>(r, q, rank, m0, n0, g);
-        else if (q.a_mn) ok = copy_tile<true, true, false>(r, q, rank, m0, n0, g);
-        else if (q.b_mn) ok = copy_tile<false, true, false>(r, q, rank, m0, n0, g);
-        else ok = copy_tile<false, false, false>(r, q, rank, m0, n0, g);
+        const Problem& q = p.pr[locate<NT>(p, tile, m0, n0)];
+        if (EPI == GATED) ok = copy_tile<false, false, true, NT>(r, q, rank, m0, n0, g);
+        else if (q.a_mn) ok = copy_tile<true, true, false, NT>(r, q, rank, m0, n0, g);
+        else if (q.b_mn) ok = copy_tile<false, true, false, NT>(r, q, rank, m0, n0, g);
+        else ok = copy_tile<false, false, false, NT>(r, q, rank, m0, n0, g);
       }
       // every stage has been read by the MMAs, and the signal of that has
       // arrived, before this CTA's shared memory goes
@@ -335,14 +349,14 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
       bool ok = true;
       for (int i = 0, tile; ok && (tile = dealer.tile(i)) >= 0; ++i) {
         int m0, n0;
-        const Problem& q = p.pr[locate(p, tile, m0, n0)];
+        const Problem& q = p.pr[locate<NT>(p, tile, m0, n0)];
         const int its = q.ksteps * q.segs, b = i & 1;
         if (i >= 2 && !grouped::warp_wait(&accempty[b], ((i >> 1) - 1) & 1, abort, p.err)) break;
         tc5::fence_after();
-        const uint32_t acc = tb + b * 256;
-        if (EPI != GATED && q.a_mn) ok = mma_tile<true, true>(r, its, p.f16, acc, g);
-        else if (EPI != GATED && q.b_mn) ok = mma_tile<false, true>(r, its, p.f16, acc, g);
-        else ok = mma_tile<false, false>(r, its, p.f16, acc, g);
+        const uint32_t acc = tb + b * NT;
+        if (EPI != GATED && q.a_mn) ok = mma_tile<true, true, NT>(r, its, p.f16, acc, g);
+        else if (EPI != GATED && q.b_mn) ok = mma_tile<false, true, NT>(r, its, p.f16, acc, g);
+        else ok = mma_tile<false, false, NT>(r, its, p.f16, acc, g);
         if (ok && elect_one()) commit(&accfull[b]);
         __syncwarp();
       }
@@ -350,18 +364,18 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
   } else {
     // ------------------------------------------------------------ epilogue
     const int q4 = warp & 3, half = (warp - 2) >> 2;
-    uint8_t* box0 = smem + S * kStage + (warp - 2) * 2 * kBox;
+    uint8_t* box0 = smem + S * Shape<NT>::kStage + (warp - 2) * 2 * kBox;
     uint8_t* box1 = box0 + kBox;
     uint64_t* loaded = &boxfull[warp - 2];
     int loads = 0, turn = 0;
     for (int i = 0, tile; (tile = dealer.tile(i)) >= 0; ++i) {
       int m0, n0;
-      const Problem& q = p.pr[locate(p, tile, m0, n0)];
+      const Problem& q = p.pr[locate<NT>(p, tile, m0, n0)];
       const int b = i & 1, mw = m0 + 128 * rank + 32 * q4, m = mw + lane;
       const bool row = m < q.M, hidden = EPI == HIDDEN && q.epi == HIDDEN;
-      const uint32_t acc = tc5::lane_quarter(tb + b * 256, q4);
-      const int per = EPI == GATED ? 64 : 128, nw = n0 + half * per;   // this warp's columns
-      const int nc = mw < q.M ? min(per, q.N - nw) : 0;                // those inside the result
+      const uint32_t acc = tc5::lane_quarter(tb + b * NT, q4);
+      // the two warps of a lane quarter take turns at the columns inside the result
+      const int nc = mw < q.M ? min(tile_cols(EPI, NT), q.N - n0) : 0;
       uint16_t* out = static_cast<uint16_t*>(q.c[0]) + (int64_t)m * q.ldc;
       const bool vec = ((reinterpret_cast<uintptr_t>(q.c[0]) | (uintptr_t)(q.ldc * 2)) & 15) == 0;
       // the pre-activations of 32 columns come in while the accumulator of
@@ -369,23 +383,23 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
       auto fetch = [&](int c) {
         if (lane == 0) {
           mbar_arrive_expect_tx(loaded, 2 * kBox);
-          tma_load_2d(box0, &p.g, nw + c, mw, loaded);
-          tma_load_2d(box1, &p.u, nw + c, mw, loaded);
+          tma_load_2d(box0, &p.g, n0 + c, mw, loaded);
+          tma_load_2d(box1, &p.u, n0 + c, mw, loaded);
         }
       };
-      if (hidden && nc > 0) fetch(0);
+      if (hidden && half * 32 < nc) fetch(half * 32);
       if (!grouped::warp_wait(&accfull[b], (i >> 1) & 1, abort, p.err)) {
-        if (hidden && nc > 0 && lane == 0) mbar_wait_bounded(loaded, loads & 1, 200000000ull);
+        if (hidden && half * 32 < nc && lane == 0) mbar_wait_bounded(loaded, loads & 1, 200000000ull);
         break;
       }
       tc5::fence_after();
       if (EPI == GATED) {
 #pragma unroll 1
-        for (int c = 0; c < nc; c += 32) {
+        for (int c = half * 32; c < nc; c += 64) {
           float gv[32], uv[32];
           __syncwarp();
-          ld_x32(acc + half * per + c, gv);
-          ld_x32(acc + 128 + half * per + c, uv);
+          ld_x32(acc + c, gv);
+          ld_x32(acc + NT / 2 + c, uv);
           tc5::wait_ld();
           if (p.keep) {
             if (lane == 0) box_wait_read<0>();
@@ -395,19 +409,19 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-              box_store(&p.g, nw + c, mw, box0);
-              box_store(&p.u, nw + c, mw, box1);
+              box_store(&p.g, n0 + c, mw, box0);
+              box_store(&p.u, n0 + c, mw, box1);
               box_commit();
             }
           }
 #pragma unroll
           for (int j = 0; j < 32; ++j) gv[j] = gate_unit(gv[j], uv[j], p.limit);
-          if (row) store16(out + nw + c, gv, nc - c, vec, p.f16);
+          if (row) store16(out + n0 + c, gv, nc - c, vec, p.f16);
         }
       } else if (hidden) {
         uint16_t* out1 = static_cast<uint16_t*>(q.c[1]) + (int64_t)m * q.ldc;
 #pragma unroll 1
-        for (int c = 0; c < nc; c += 32) {
+        for (int c = half * 32; c < nc; c += 64) {
           float v[32], gv[32], uv[32];
           if (!grouped::warp_wait(loaded, loads & 1, abort, p.err)) break;
           ++loads;
@@ -417,27 +431,27 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
           // the fence, reads still queued met the newer values)
           fence_proxy_async_smem();
           __syncwarp();
-          if (c + 32 < nc) fetch(c + 32);
+          if (c + 64 < nc) fetch(c + 64);
           __syncwarp();
-          ld_x32(acc + half * per + c, v);
+          ld_x32(acc + c, v);
           tc5::wait_ld();
 #pragma unroll
           for (int j = 0; j < 32; ++j) gate_grad(gv[j], uv[j], v[j], p.limit, gv[j], uv[j]);
           if (row) {
-            store16(out + nw + c, gv, nc - c, vec, p.f16);
-            store16(out1 + nw + c, uv, nc - c, vec, p.f16);
+            store16(out + n0 + c, gv, nc - c, vec, p.f16);
+            store16(out1 + n0 + c, uv, nc - c, vec, p.f16);
           }
         }
       } else if (q.boxed) {
 #pragma unroll 1
-        for (int c = 0; c < nc; c += 64) {
+        for (int c = half * 64; c < nc; c += 128) {
           uint8_t* box = turn++ & 1 ? box1 : box0;   // the store before the last has read its box
           if (lane == 0) box_wait_read<1>();
           __syncwarp();
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             float v[32];
-            ld_x32(acc + half * per + c + 32 * e, v);
+            ld_x32(acc + c + 32 * e, v);
             tc5::wait_ld();
 #pragma unroll
             for (int k = 0; k < 4; ++k)
@@ -448,18 +462,18 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            box_store(&q.out, nw + c, mw, box);
+            box_store(&q.out, n0 + c, mw, box);
             box_commit();
           }
         }
       } else {
 #pragma unroll 1
-        for (int c = 0; c < nc; c += 32) {
+        for (int c = half * 32; c < nc; c += 64) {
           float v[32];
           __syncwarp();
-          ld_x32(acc + half * per + c, v);
+          ld_x32(acc + c, v);
           tc5::wait_ld();
-          if (row) store16(out + nw + c, v, nc - c, false, p.f16);
+          if (row) store16(out + n0 + c, v, nc - c, false, p.f16);
         }
       }
       // the boxes are free again before a later tile's loads overwrite them

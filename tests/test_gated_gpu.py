@@ -85,7 +85,7 @@ def both(ins, dy, limit):
 
 
 SIZES = [(1, 64, 64), (1, 4096, 2048), (2, 128, 96), (15, 72, 200), (16, 256, 128), (17, 1000, 711), (33, 513, 40),
-         (64, 640, 1280), (65, 8, 8), (127, 1, 1), (128, 384, 257), (129, 2048, 512), (255, 96, 1024), (257, 1024, 264),
+         (64, 640, 1280), (65, 8, 8), (127, 1, 1), (130, 64, 4096), (200, 4096, 72), (384, 1288, 1000), (640, 2048, 2048), (128, 384, 257), (129, 2048, 512), (255, 96, 1024), (257, 1024, 264),
          (300, 30, 2050), (1, 7, 3), (1000, 512, 520), (2049, 256, 328)]
 
 
