@@ -14,9 +14,8 @@
 // with one maximum over its lanes.
 #include <algorithm>
 #include <cooperative_groups.h>
-#include <string.h>
 
-#include "mx4.cuh"
+#include "mx4_pair.cuh"
 
 namespace ds {
 namespace mx4 {
@@ -154,14 +153,6 @@ struct TileShape {
 };
 
 constexpr int kTileThreads = 192;   // warp 0 copies, warp 1 MMA, warps 2-5 epilogue
-
-__device__ __forceinline__ float gate_unit(float g, float u, float limit) {
-  if (limit > 0.0f) {   // comparisons keep a NaN
-    g = g > limit ? limit : g;
-    u = u > limit ? limit : (u < -limit ? -limit : u);
-  }
-  return g / (1.0f + expf(-g)) * u;
-}
 
 // One element of the tile: row n of x, feature m (lane of a full warp).
 template <int MODE>
@@ -401,6 +392,102 @@ int run_tiles(const TileParams& p, int nt, cudaStream_t s, bool chained) {
   return launch_tiles<MODE, 128>(p, slices, s, chained);
 }
 
+// ---- pair kernel
+
+// The pair kernel takes products of at least this many rows of x.
+constexpr int kPairRows = 129;
+
+// Scale atoms as lines of 512 bytes (128 words); a box is two lines.
+bool map_atoms(CUtensorMap* m, const void* base, int64_t rows, int64_t cols) {
+  const cuuint64_t dims[2] = {128, (cuuint64_t)(atoms_bytes(rows, cols) / kAtom)};
+  const cuuint64_t strides[1] = {kAtom};
+  const cuuint32_t box[2] = {128, 2};
+  const cuuint32_t es[2] = {1, 1};
+  return grouped::encode_fn()(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, es,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Result [rows, cols] in boxes of 128 bytes x 32 rows; false where its rows do not start on 16 bytes.
+bool map_result(CUtensorMap* m, void* y, int64_t rows, int64_t cols, int dtype) {
+  const int es_ = dtype == DS_F32 ? 4 : 2;
+  if (!ds::aligned(y, 16) || cols * es_ % 16 != 0) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(cols * es_)};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / es_), 32};
+  const cuuint32_t es[2] = {1, 1};
+  return grouped::encode_fn()(m, dtype == DS_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2,
+                              y, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool GATED>
+int run_pairs(const PairParams& p, cudaStream_t s, bool chained) {
+  constexpr int cols = GATED ? 128 : 256;
+  const int64_t tiles = (p.M + 255) / 256 * (int64_t)((p.N + cols - 1) / cols);
+  DS_REQUIRE(tiles < ((int64_t)1 << 31), DS_ERANGE, "mx4: too many tiles");
+  DS_CHECK_CUDA(cudaFuncSetAttribute(pairs::pair_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, pairs::kSmem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, ds::sm_count() / 2)));
+  cfg.blockDim = dim3(pairs::kThreads);
+  cfg.dynamicSmemBytes = pairs::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = chained ? 1 : 0;
+  DS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, pairs::pair_kernel<GATED>, p));
+  return DS_OK;
+}
+
+// y = x W^T of quantised operands.
+int product(const void* x, const uint8_t* x_atoms, int64_t rows, const DsMx4& w, void* y, int out_dtype, int* err,
+            cudaStream_t s, bool chained) {
+  if (rows >= kPairRows) {
+    PairParams p = {};
+    const bool ok = map_codes(&p.a, x, rows, w.cols, 128) && map_codes(&p.b[0], w.packed, w.rows, w.cols, 128) &&
+                    map_atoms(&p.sa, x_atoms, rows, w.cols) && map_atoms(&p.sb[0], w.atoms, w.rows, w.cols);
+    DS_REQUIRE(ok, DS_ECUDA, "mx4: tensor map encoding failed");
+    p.boxed = map_result(&p.out, y, rows, w.rows, out_dtype);
+    p.y = y, p.ldy = w.rows, p.out_dtype = out_dtype;
+    p.M = (int)rows, p.N = (int)w.rows, p.blocks = (int)blocks_of(w.cols), p.err = err;
+    return run_pairs<false>(p, s, chained);
+  }
+  const int nt = row_tile(rows);
+  TileParams p = {};
+  const bool ok = map_codes(&p.a[0], w.packed, w.rows, w.cols, 128) && map_codes(&p.b, x, rows, w.cols, nt);
+  DS_REQUIRE(ok, DS_ECUDA, "mx4: tensor map encoding failed");
+  p.sa[0] = w.atoms, p.sb = x_atoms;
+  p.M = (int)w.rows, p.N = (int)rows, p.blocks = (int)blocks_of(w.cols), p.err = err;
+  p.out = y, p.ldo = w.rows, p.out_dtype = out_dtype;
+  return run_tiles<LINEAR>(p, nt, s, chained);
+}
+
+// Codes and atoms of h = the gated unit of x W1^T and x W3^T.
+int gate_up(const void* x, const uint8_t* x_atoms, int64_t rows, const DsMx4& w1, const DsMx4& w3, float limit,
+            uint8_t* hq, uint8_t* hs, int* err, cudaStream_t s, bool chained) {
+  if (rows >= kPairRows) {
+    PairParams p = {};
+    const bool ok = map_codes(&p.a, x, rows, w1.cols, 128) && map_codes(&p.b[0], w1.packed, w1.rows, w1.cols, 128) &&
+                    map_codes(&p.b[1], w3.packed, w1.rows, w1.cols, 128) && map_atoms(&p.sa, x_atoms, rows, w1.cols) &&
+                    map_atoms(&p.sb[0], w1.atoms, w1.rows, w1.cols) && map_atoms(&p.sb[1], w3.atoms, w1.rows, w1.cols);
+    DS_REQUIRE(ok, DS_ECUDA, "mx4: tensor map encoding failed");
+    p.hq = hq, p.hs = hs, p.limit = limit;
+    p.M = (int)rows, p.N = (int)w1.rows, p.blocks = (int)blocks_of(w1.cols), p.err = err;
+    return run_pairs<true>(p, s, chained);
+  }
+  const int nt = row_tile(rows);
+  TileParams p = {};
+  const bool ok = map_codes(&p.a[0], w1.packed, w1.rows, w1.cols, 128) &&
+                  map_codes(&p.a[1], w3.packed, w1.rows, w1.cols, 128) && map_codes(&p.b, x, rows, w1.cols, nt);
+  DS_REQUIRE(ok, DS_ECUDA, "mx4: tensor map encoding failed");
+  p.sa[0] = w1.atoms, p.sa[1] = w3.atoms, p.sb = x_atoms;
+  p.M = (int)w1.rows, p.N = (int)rows, p.blocks = (int)blocks_of(w1.cols), p.err = err;
+  p.hq = hq, p.hs = hs, p.limit = limit;
+  return run_tiles<GATED>(p, nt, s, chained);
+}
+
 int validate_weight(const DsMx4* w, const char* what) {
   DS_REQUIRE(w && w->packed && w->atoms, DS_EINVAL, "%s: null weight", what);
   DS_REQUIRE(w->rows >= 1 && w->rows <= (1 << 20) && w->cols >= 1 && w->cols <= (1 << 20), DS_ERANGE,
@@ -503,22 +590,9 @@ extern "C" int ds_mx4_linear(const void* x, const uint8_t* x_atoms, int x_dtype,
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   if ((st = quantized_x(x, x_atoms, x_dtype, rows, (int)w->cols, ld, ws, s)) != DS_OK) return st;
 
-  const int nt = row_tile(rows);
-  TileParams p;
-  memset(&p, 0, sizeof(p));
-  p.err = err_word();
-  DS_REQUIRE(p.err != nullptr, DS_ECUDA, "mx4_linear: error word unavailable");
-  const bool ok = map_codes(&p.a[0], w->packed, w->rows, w->cols, 128) && map_codes(&p.b, x, rows, w->cols, nt);
-  DS_REQUIRE(ok, DS_ECUDA, "mx4_linear: tensor map encoding failed");
-  p.sa[0] = w->atoms;
-  p.sb = x_atoms;
-  p.M = (int)w->rows;
-  p.N = (int)rows;
-  p.blocks = (int)blocks_of(w->cols);
-  p.out = out;
-  p.ldo = w->rows;
-  p.out_dtype = out_dtype;
-  return run_tiles<LINEAR>(p, nt, s, x_dtype != DS_U8);
+  int* err = err_word();
+  DS_REQUIRE(err != nullptr, DS_ECUDA, "mx4_linear: error word unavailable");
+  return product(x, x_atoms, rows, *w, out, out_dtype, err, s, x_dtype != DS_U8);
 }
 
 extern "C" int ds_mx4_gated_ffn_workspace_size(int64_t rows, int64_t hidden, int64_t inter, size_t* bytes) {
@@ -554,35 +628,10 @@ extern "C" int ds_mx4_gated_ffn(const void* x, const uint8_t* x_atoms, int x_dty
   uint8_t* hq = ws;
   uint8_t* hs = ws + ds::grouped::up(packed_bytes(rows, I), 256);
 
-  const int nt = row_tile(rows);
-  TileParams p;
-  memset(&p, 0, sizeof(p));
-  p.err = err_word();
-  DS_REQUIRE(p.err != nullptr, DS_ECUDA, "mx4_gated_ffn: error word unavailable");
-  bool ok = map_codes(&p.a[0], w1->packed, I, H, 128) && map_codes(&p.a[1], w3->packed, I, H, 128) &&
-            map_codes(&p.b, x, rows, H, nt);
-  DS_REQUIRE(ok, DS_ECUDA, "mx4_gated_ffn: tensor map encoding failed (gate / up)");
-  p.sa[0] = w1->atoms;
-  p.sa[1] = w3->atoms;
-  p.sb = x_atoms;
-  p.M = (int)I;
-  p.N = (int)rows;
-  p.blocks = (int)blocks_of(H);
-  p.hq = hq;
-  p.hs = hs;
-  p.limit = limit;
-  if ((st = run_tiles<GATED>(p, nt, s, x_dtype != DS_U8)) != DS_OK) return st;
-
-  ok = map_codes(&p.a[0], w2->packed, H, I, 128) && map_codes(&p.b, hq, rows, I, nt);
-  DS_REQUIRE(ok, DS_ECUDA, "mx4_gated_ffn: tensor map encoding failed (down)");
-  p.sa[0] = w2->atoms;
-  p.sb = hs;
-  p.M = (int)H;
-  p.blocks = (int)blocks_of(I);
-  p.out = out;
-  p.ldo = H;
-  p.out_dtype = out_dtype;
-  return run_tiles<LINEAR>(p, nt, s, true);
+  int* err = err_word();
+  DS_REQUIRE(err != nullptr, DS_ECUDA, "mx4_gated_ffn: error word unavailable");
+  if ((st = gate_up(x, x_atoms, rows, *w1, *w3, limit, hq, hs, err, s, x_dtype != DS_U8)) != DS_OK) return st;
+  return product(hq, hs, rows, *w2, out, out_dtype, err, s, true);
 }
 
 extern "C" int ds_mx4_status(int32_t* err, void* stream) {

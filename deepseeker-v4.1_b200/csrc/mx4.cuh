@@ -51,5 +51,16 @@ __device__ __forceinline__ void copy_atom(uint32_t taddr, uint32_t saddr) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
 }
 
+// The gated unit (ds_gated_ffn's), from f32 sums: the clamps keep a NaN; the
+// fast exponential and division are good to about 2^-20, and what follows
+// rounds to three bits.
+__device__ __forceinline__ float gate_unit(float g, float u, float limit) {
+  if (limit > 0.0f) {
+    g = g > limit ? limit : g;
+    u = u > limit ? limit : (u < -limit ? -limit : u);
+  }
+  return __fdividef(g, 1.0f + __expf(-g)) * u;
+}
+
 }  // namespace mx4
 }  // namespace ds
