@@ -27,79 +27,202 @@ __device__ int g_err;   // bit 1: a bounded wait gave up
 
 // ---------------------------------------------------------------- quantisation
 
+// Eight values of a row as they are stored: 16-bit types two a word.
 template <typename T>
-__device__ __forceinline__ float load_one(const T* p) {
-  if constexpr (sizeof(T) == 4) return *p;
-  else if constexpr (std::is_same<T, __half>::value) return __half2float(*p);
-  else return __bfloat162float(*p);
-}
+struct Eight {
+  static constexpr bool kF32 = sizeof(T) == 4, kF16 = std::is_same<T, __half>::value;
+  uint32_t w[kF32 ? 8 : 4];
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  } else {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (std::is_same<T, __half>::value) {
+    for (int i = 0; i < (kF32 ? 8 : 4); ++i) w[i] = 0u;
+  }
+  // All eight, 16-byte aligned.
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (kF32 ? 2 : 1); ++i) {
+      const uint4 a = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = a.x, w[4 * i + 1] = a.y, w[4 * i + 2] = a.z, w[4 * i + 3] = a.w;
+    }
+  }
+  // The first n.
+  __device__ __forceinline__ void load_some(const T* p, int n) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j >= n) continue;
+      if constexpr (kF32) w[j] = __float_as_uint(p[j]);
+      else w[j >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[j] << (16 * (j & 1));
+    }
+  }
+  // Bits of the largest magnitude as f32 (the bits of non-negative values
+  // order as the values, infinities and NaN above), over the four threads of a block.
+  __device__ __forceinline__ uint32_t top() const {
+    if constexpr (kF32) {
+      uint32_t t = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t = max(t, w[i] & 0x7FFFFFFFu);
+      t = max(t, __shfl_xor_sync(0xffffffffu, t, 1));
+      return max(t, __shfl_xor_sync(0xffffffffu, t, 2));
+    } else {
+      uint32_t t = w[0] & 0x7FFF7FFFu;
+#pragma unroll
+      for (int i = 1; i < 4; ++i) t = __vmaxu2(t, w[i] & 0x7FFF7FFFu);
+      t = __vmaxu2(t, __shfl_xor_sync(0xffffffffu, t, 1));
+      t = __vmaxu2(t, __shfl_xor_sync(0xffffffffu, t, 2));
+      t = max(t & 0xFFFFu, t >> 16);
+      return kF16 ? __float_as_uint(__half2float(__ushort_as_half((uint16_t)t))) : t << 16;
+    }
+  }
+  // Codes of the values times inv, a power of two.
+  __device__ __forceinline__ uint32_t codes(float inv) const {
+    float v[8];
+    if constexpr (kF32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]) * inv;
+    } else if constexpr (kF16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        v[2 * i] = f.x, v[2 * i + 1] = f.y;
-      } else {
-        v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        v[2 * i] = f.x * inv, v[2 * i + 1] = f.y * inv;
       }
+    } else {
+      // exact in bf16 too, which has f32's exponents; what leaves its normal
+      // range rounds to code 0 either way
+      const __nv_bfloat162 k = __float2bfloat162_rn(inv);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 m = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), k);
+        const uint32_t u = *reinterpret_cast<const uint32_t*>(&m);
+        v[2 * i] = __uint_as_float(u << 16), v[2 * i + 1] = __uint_as_float(u & 0xFFFF0000u);
+      }
+    }
+    return e2m1x8(v);
+  }
+};
+
+// How the rows of x lie: groups of 8 that follow one another through the whole
+// matrix, 16-byte aligned groups in rows of any stride, or neither.
+enum Rows { WHOLE, ALIGNED, ANY };
+
+// A group is 8 values, four neighbours a block: a 16-byte load (two in f32),
+// a maximum over four lanes and a 4-byte store each, so a warp's loads and
+// code stores are whole lines.  A thread has its GROUPS loads in flight
+// together.  What is left to bound it is the number of instructions per group
+// (164 made it 47 us for 16384 x 4096 bf16, of which memory needs 27), so
+// codes and scales are addressed by the group's number alone, two 16-bit
+// magnitudes share a maximum, and a place in the matrix is only worked out
+// where it is needed, without a division per group.
+template <typename T, int GROUPS, int ROWS>
+__global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ld,
+                                                       uint32_t* __restrict__ packed, uint8_t* __restrict__ scales,
+                                                       uint8_t* __restrict__ atoms) {
+  launch_dependents();
+  const uint32_t blocks = (cols + 31) / 32, per_row = blocks * 4;
+  const int64_t first = (int64_t)blockIdx.x * (256 * GROUPS), row0 = first / per_row;
+  const int tid = threadIdx.x, count = (int)min((int64_t)(256 * GROUPS), rows * per_row - first);
+  const uint32_t t0 = (uint32_t)(first - row0 * per_row) + tid;
+  const uint32_t rs = 256 / per_row, gs = 256 - rs * per_row;   // 256 groups on: rows, and groups of a row
+  Eight<T> v[GROUPS];
+  if (ROWS == WHOLE) {
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) {
+      v[k].clear();
+      if (tid + 256 * k < count) v[k].load(x + (first + tid) * 8 + 2048 * k);
+    }
+  } else {
+    int64_t r = row0 + t0 / per_row;
+    uint32_t g = t0 % per_row;
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) {
+      v[k].clear();
+      const int left = tid + 256 * k < count ? cols - (int)g * 8 : 0;
+      if (ROWS == ANY) v[k].load_some(x + r * ld + g * 8, left);
+      else if (left > 0) v[k].load(x + r * ld + g * 8);
+      r += rs, g += gs;
+      if (g >= per_row) g -= per_row, ++r;
+    }
+  }
+  uint32_t s[GROUPS];
+#pragma unroll
+  for (int k = 0; k < GROUPS; ++k) {
+    s[k] = scale_byte(v[k].top());
+    const uint32_t w = s[k] == 255u ? 0u : v[k].codes(inv_scale(s[k]));
+    if (tid + 256 * k < count) packed[first + tid + 256 * k] = w;
+  }
+  if (tid & 3) return;
+  if (scales) {
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k)
+      if (tid + 256 * k < count) scales[(first + tid) / 4 + 64 * k] = (uint8_t)s[k];
+  }
+  if (atoms) {
+    const uint32_t chunks = (blocks + 3) / 4;
+    int64_t row = row0 + t0 / per_row;
+    uint32_t g = t0 % per_row;
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) {
+      if (tid + 256 * k < count) {
+        uint8_t* at = atoms + atom_at(row, g >> 2, chunks);
+        *at = (uint8_t)s[k];
+        if (g == per_row - 4)   // blocks that fill up the last chunk: any scale but NaN
+            for (uint32_t e = blocks; e < chunks * 4; ++e) at[e - blocks + 1] = 0;
+      }
+      row += rs, g += gs;
+      if (g >= per_row) g -= per_row, ++row;
     }
   }
 }
 
-// A thread takes 8 values, four neighbours a block: a 16-byte load (two in
-// f32), a maximum over four lanes and a 4-byte store each, so a warp's loads
-// and code stores are whole lines.  `slab` rows per CTA.
-template <typename T>
-__global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ld,
-                                                       int vec, int slab, uint32_t* __restrict__ packed,
-                                                       uint8_t* __restrict__ scales, uint8_t* __restrict__ atoms) {
-  launch_dependents();
-  const int blocks = (cols + 31) / 32, per_row = blocks * 4, chunks = (blocks + 3) / 4;
-  const int64_t r0 = (int64_t)blockIdx.x * slab;
-  const int count = (int)min((int64_t)slab, rows - r0) * per_row;
-  for (int i = threadIdx.x; i < (count + 31) / 32 * 32; i += blockDim.x) {
-    const int r = i / per_row, g = i - r * per_row;
-    const int64_t row = r0 + r;
-    const bool live = i < count;
-    const T* src = x + row * ld + g * 8;
+// The values of 8 codes a thread: a 4-byte load, 16 or 32 bytes stored, whole
+// lines a warp.  Exact: a code times a power of two; the added 0 turns the
+// second code of zero into +0.
+template <typename T, int GROUPS>
+__global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restrict__ packed,
+                                                         const uint8_t* __restrict__ scales, int64_t rows, int cols,
+                                                         int vec, T* __restrict__ out) {
+  const uint32_t blocks = (cols + 31) / 32, per_row = blocks * 4;
+  const int64_t first = (int64_t)blockIdx.x * (256 * GROUPS), row0 = first / per_row;
+  const uint32_t rem = (uint32_t)(first - row0 * per_row) + threadIdx.x;
+  uint32_t w[GROUPS], sc[GROUPS];
+#pragma unroll
+  for (int k = 0; k < GROUPS; ++k) {
+    const uint32_t t = rem + 256 * k, r = t / per_row, g = t - r * per_row;
+    const int64_t row = row0 + r;
+    w[k] = row < rows ? __ldcs(packed + row * per_row + g) : 0u;
+    sc[k] = row < rows ? scales[row * blocks + (g >> 2)] : 0u;
+  }
+#pragma unroll
+  for (int k = 0; k < GROUPS; ++k) {
+    const uint32_t t = rem + 256 * k, r = t / per_row, g = t - r * per_row;
+    const int64_t row = row0 + r;
+    if (row >= rows) continue;
+    const float s = ds::u8m0_value(sc[k]);
+    uint32_t h[4];
+    e2m1x8_to_f16x2(w[k], h);
     float v[8];
-    if (live && vec && g * 8 + 8 <= cols) {
-      load8(src, v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+      v[2 * j] = fmaf(f.x, s, 0.0f), v[2 * j + 1] = fmaf(f.y, s, 0.0f);
+    }
+    T* dst = out + row * cols + g * 8;
+    if (vec && (int)(g * 8 + 8) <= cols) {
+      if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+      } else {
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+          o[j] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = live && g * 8 + j < cols ? load_one(src + j) : 0.0f;
-    }
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    if (!live) continue;
-    const int s = scale_byte(top);
-    const float inv = inv_scale(s);
-    uint32_t w = 0;
-    if (s != 255) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w |= tc5::f32x2_to_e2m1x2(v[2 * j] * inv, v[2 * j + 1] * inv) << (8 * j);
-      w = no_negative_zero(w);
-    }
-    packed[row * per_row + g] = w;
-    if ((g & 3) == 0) {
-      const int b = g >> 2;
-      if (scales) scales[row * blocks + b] = (uint8_t)s;
-      if (atoms) {
-        atoms[atom_at(row, b, chunks)] = (uint8_t)s;
-        if (b == blocks - 1)   // blocks that fill up the last chunk: any scale but NaN
-          for (int e = blocks; e < chunks * 4; ++e) atoms[atom_at(row, e, chunks)] = 0;
-      }
+      for (int j = 0; j < 8; ++j)
+        if ((int)(g * 8) + j < cols) dst[j] = (T)v[j];
     }
   }
 }
@@ -334,24 +457,37 @@ int* err_word() {
   return cudaGetSymbolAddress(&p, g_err) == cudaSuccess ? static_cast<int*>(p) : nullptr;
 }
 
+// Groups of 8 values per thread: four, or one where that leaves SMs idle.
+template <typename F>
+int by_groups(int64_t rows, int64_t cols, F launch) {
+  const int64_t groups = rows * blocks_of(cols) * 4;
+  const int per = groups >= (int64_t)ds::sm_count() * 4 * 1024 ? 4 : 1;
+  const int64_t grid = (groups + 256 * per - 1) / (256 * per);
+  DS_REQUIRE(grid < ((int64_t)1 << 31), DS_ERANGE, "mx4: matrix too large");
+  if (per == 4) launch(std::integral_constant<int, 4>(), (unsigned)grid);
+  else launch(std::integral_constant<int, 1>(), (unsigned)grid);
+  return DS_OK;
+}
+
 int launch_quantize(const void* x, int dtype, int64_t rows, int cols, int64_t ld, uint8_t* packed, uint8_t* scales,
                     uint8_t* atoms, cudaStream_t s) {
-  const int per_row = (int)blocks_of(cols) * 4, es = dtype == DS_F32 ? 4 : 2;
-  const int vec = ds::aligned(x, 16) && (rows == 1 || ld * es % 16 == 0);
-  // about four groups of 8 values per thread; one where that leaves SMs idle
-  int slab = std::max(1, 1024 / per_row);
-  if ((rows + slab - 1) / slab < 2 * ds::sm_count()) slab = std::max(1, 256 / per_row);
-  const int64_t grid = (rows + slab - 1) / slab;
+  const int es = dtype == DS_F32 ? 4 : 2;
+  const bool vec = ds::aligned(x, 16) && cols % 8 == 0 && (rows == 1 || ld * es % 16 == 0);
+  const bool whole = vec && cols % 32 == 0 && (rows == 1 || ld == cols);
   uint32_t* pk = reinterpret_cast<uint32_t*>(packed);
-  if (dtype == DS_F32)
-    quantize_kernel<<<(unsigned)grid, 256, 0, s>>>(static_cast<const float*>(x), rows, cols, ld, vec, slab, pk, scales,
-                                                   atoms);
-  else if (dtype == DS_F16)
-    quantize_kernel<<<(unsigned)grid, 256, 0, s>>>(static_cast<const __half*>(x), rows, cols, ld, vec, slab, pk,
-                                                   scales, atoms);
-  else
-    quantize_kernel<<<(unsigned)grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(x), rows, cols, ld, vec, slab, pk,
-                                                   scales, atoms);
+  const int st = by_groups(rows, cols, [&](auto per, unsigned grid) {
+    constexpr int G = decltype(per)::value;
+    auto run = [&](auto* src) {
+      using T = std::remove_const_t<std::remove_pointer_t<decltype(src)>>;
+      if (whole) quantize_kernel<T, G, WHOLE><<<grid, 256, 0, s>>>(src, rows, cols, ld, pk, scales, atoms);
+      else if (vec) quantize_kernel<T, G, ALIGNED><<<grid, 256, 0, s>>>(src, rows, cols, ld, pk, scales, atoms);
+      else quantize_kernel<T, G, ANY><<<grid, 256, 0, s>>>(src, rows, cols, ld, pk, scales, atoms);
+    };
+    if (dtype == DS_F32) run(static_cast<const float*>(x));
+    else if (dtype == DS_F16) run(static_cast<const __half*>(x));
+    else run(static_cast<const __nv_bfloat16*>(x));
+  });
+  if (st != DS_OK) return st;
   DS_CHECK_LAUNCH("mx4 quantize_kernel");
   return DS_OK;
 }
@@ -549,6 +685,31 @@ extern "C" int ds_mx4_quantize(const void* x, int x_dtype, int64_t rows, int64_t
   DS_REQUIRE(ds::aligned(x, x_dtype == DS_F32 ? 4 : 2) && ds::aligned(packed, 16) && ds::aligned(atoms, 16), DS_EALIGN,
              "mx4_quantize: x must be aligned to its elements, codes and atoms to 16 bytes");
   return launch_quantize(x, x_dtype, rows, (int)cols, ld, packed, scales, atoms, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int ds_mx4_dequantize(const uint8_t* packed, const uint8_t* scales, int64_t rows, int64_t cols, void* out,
+                                 int out_dtype, void* stream) {
+  DS_REQUIRE(out_dtype == DS_F32 || out_dtype == DS_BF16, DS_EINVAL, "mx4_dequantize: out must be f32 or bf16");
+  DS_REQUIRE(rows >= 0 && rows < ((int64_t)1 << 31) && cols >= 1 && cols <= (1 << 20), DS_ERANGE,
+             "mx4_dequantize: rows must be in [0, 2^31), cols in [1, 2^20]");
+  if (rows == 0) return DS_OK;
+  DS_REQUIRE(packed && scales && out, DS_EINVAL, "mx4_dequantize: null pointer");
+  DS_REQUIRE(ds::aligned(packed, 16) && ds::aligned(out, out_dtype == DS_F32 ? 4 : 2), DS_EALIGN,
+             "mx4_dequantize: codes must be 16-byte aligned, out to its elements");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int vec = ds::aligned(out, 16) && cols * (out_dtype == DS_F32 ? 4 : 2) % 16 == 0;
+  const uint32_t* pk = reinterpret_cast<const uint32_t*>(packed);
+  const int st = by_groups(rows, cols, [&](auto per, unsigned grid) {
+    constexpr int G = decltype(per)::value;
+    if (out_dtype == DS_F32)
+      dequantize_kernel<float, G><<<grid, 256, 0, s>>>(pk, scales, rows, (int)cols, vec, static_cast<float*>(out));
+    else
+      dequantize_kernel<__nv_bfloat16, G><<<grid, 256, 0, s>>>(pk, scales, rows, (int)cols, vec,
+                                                               static_cast<__nv_bfloat16*>(out));
+  });
+  if (st != DS_OK) return st;
+  DS_CHECK_LAUNCH("mx4 dequantize_kernel");
+  return DS_OK;
 }
 
 extern "C" int ds_mx4_scale_atoms(const uint8_t* scales, int64_t rows, int64_t cols, uint8_t* atoms, void* stream) {

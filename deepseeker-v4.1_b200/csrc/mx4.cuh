@@ -21,10 +21,9 @@ constexpr int kAtom = grouped::kSfAtom;   // scales of 128 rows x 4 blocks
 
 // Scale byte from the bits of the block's largest magnitude.
 __device__ __forceinline__ int scale_byte(uint32_t top) {
-  const int ef = (int)(top >> 23);
-  if (ef == 255) return 255;
-  if (ef == 0) return top == 0u ? 127 : 0;
-  return max((top & 0x7FFFFFu) <= 0x400000u ? ef - 2 : ef - 1, 0);
+  // adding the mantissa bits above 1.5 carries into the exponent: ef - 2 or ef - 1
+  const int s = max((int)((top + 0x3FFFFFu) >> 23) - 2, 0);
+  return top >= 0x7F800000u ? 255 : top == 0u ? 127 : s;
 }
 
 // 2^(127 - s), s <= 253; 0 for the NaN scale (the codes are then all 0).
@@ -34,6 +33,21 @@ __device__ __forceinline__ float inv_scale(int s) { return s == 255 ? 0.0f : __u
 __device__ __forceinline__ uint32_t no_negative_zero(uint32_t w) {
   const uint32_t nz = (w | (w >> 1) | (w >> 2)) & 0x11111111u;
   return w & (0x77777777u | (nz << 3));
+}
+
+// Eight scaled values to codes, the first in the lowest bits: to nearest, ties
+// to the even code, at most 6 in magnitude.
+__device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
+  uint32_t w;
+  asm("{ .reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3}; }"
+      : "=r"(w)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return no_negative_zero(w);
 }
 
 // Byte of (row, block) in a matrix's atoms [ceil(rows / 128)][chunks][512],

@@ -128,10 +128,10 @@ __device__ __forceinline__ uint4 quantize_block(const float* h, int& s) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    w[i] = 0;
+    float v[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[i] |= tc5::f32x2_to_e2m1x2(h[8 * i + 2 * j] * inv, h[8 * i + 2 * j + 1] * inv) << (8 * j);
-    w[i] = s == 255 ? 0u : no_negative_zero(w[i]);
+    for (int j = 0; j < 8; ++j) v[j] = h[8 * i + j] * inv;
+    w[i] = s == 255 ? 0u : e2m1x8(v);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }

@@ -101,6 +101,7 @@ SIGNATURES: dict[str, tuple] = {
     "ds_gated_ffn_status": (c_int, [c_void_p, c_void_p]),
     "ds_mx4_atoms_size": (c_int, [c_int64, c_int64, POINTER(c_size_t)]),
     "ds_mx4_quantize": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "ds_mx4_dequantize": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p]),
     "ds_mx4_scale_atoms": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
     "ds_mx4_linear_workspace_size": (c_int, [c_int64, c_int64, POINTER(c_size_t)]),
     "ds_mx4_linear": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, POINTER(DsMx4), c_void_p, c_int, c_void_p,

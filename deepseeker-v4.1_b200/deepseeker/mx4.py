@@ -13,7 +13,7 @@ import ctypes
 
 import torch
 
-from . import _abi, metal_fp4
+from . import _abi
 from ._dev import stream_handle
 from .gated import _rows
 
@@ -51,8 +51,11 @@ class MX4Tensor:
         """The values that the codes stand for, f32 or bf16 (both exact)."""
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError("dtype must be torch.float32 or torch.bfloat16")
-        v = metal_fp4.dequant(self.packed, self.scales, dtype).view(self.rows, _blocks(self.cols) * BLOCK)
-        return v[:, : self.cols].reshape(self.shape)
+        out = torch.empty(self.rows, self.cols, dtype=dtype, device=self.device)
+        with torch.cuda.device(self.device):
+            _abi.call("ds_mx4_dequantize", self.packed.data_ptr(), self.scales.data_ptr(), self.rows, self.cols,
+                      out.data_ptr(), _DTYPES[dtype], stream_handle(self.device))
+        return out.view(self.shape)
 
 
 def _check_x(x) -> None:

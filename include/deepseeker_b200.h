@@ -480,6 +480,10 @@ int ds_mx4_atoms_size(int64_t rows, int64_t cols, size_t* bytes);
  * [rows, 16 ceil(cols/32)], scales [rows, ceil(cols/32)], atoms (or NULL). */
 int ds_mx4_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ld, uint8_t* packed,
                     uint8_t* scales, uint8_t* atoms, void* stream);
+/* The values that codes and scales stand for, out [rows, cols] f32 or bf16
+ * contiguous (both exact; scale 255 gives NaN). */
+int ds_mx4_dequantize(const uint8_t* packed, const uint8_t* scales, int64_t rows, int64_t cols, void* out,
+                      int out_dtype, void* stream);
 /* Atoms of stored scales [rows, ceil(cols/32)]: once per weight matrix. */
 int ds_mx4_scale_atoms(const uint8_t* scales, int64_t rows, int64_t cols, uint8_t* atoms, void* stream);
 
