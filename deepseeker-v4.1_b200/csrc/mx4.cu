@@ -27,62 +27,64 @@ __device__ int g_err;   // bit 1: a bounded wait gave up
 
 // ---------------------------------------------------------------- quantisation
 
-// Eight values of a row as they are stored: 16-bit types two a word.
+// Sixteen values of a row, half a block, as they are stored: 16-bit types two
+// a word.
 template <typename T>
-struct Eight {
+struct Half {
   static constexpr bool kF32 = sizeof(T) == 4, kF16 = std::is_same<T, __half>::value;
-  uint32_t w[kF32 ? 8 : 4];
+  static constexpr int kWords = kF32 ? 16 : 8;
+  uint32_t w[kWords];
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < (kF32 ? 8 : 4); ++i) w[i] = 0u;
+    for (int i = 0; i < kWords; ++i) w[i] = 0u;
   }
-  // All eight, 16-byte aligned.
-  __device__ __forceinline__ void load(const T* p) {
+  // The first n, a multiple of 8, 16-byte aligned.
+  __device__ __forceinline__ void load(const T* p, int n) {
 #pragma unroll
-    for (int i = 0; i < (kF32 ? 2 : 1); ++i) {
+    for (int i = 0; i < kWords / 4; ++i) {
+      if (i * 8 >= n * (kF32 ? 2 : 1)) continue;
       const uint4 a = reinterpret_cast<const uint4*>(p)[i];
       w[4 * i] = a.x, w[4 * i + 1] = a.y, w[4 * i + 2] = a.z, w[4 * i + 3] = a.w;
     }
   }
-  // The first n.
+  // The first n, one by one.
   __device__ __forceinline__ void load_some(const T* p, int n) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < 16; ++j) {
       if (j >= n) continue;
       if constexpr (kF32) w[j] = __float_as_uint(p[j]);
       else w[j >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[j] << (16 * (j & 1));
     }
   }
-  // Bits of the largest magnitude as f32 (the bits of non-negative values
-  // order as the values, infinities and NaN above), over the four threads of a block.
+  // Bits of the block's largest magnitude as f32 (the bits of non-negative
+  // values order as the values, infinities and NaN above); the other half is
+  // the neighbouring lane's.
   __device__ __forceinline__ uint32_t top() const {
     if constexpr (kF32) {
       uint32_t t = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) t = max(t, w[i] & 0x7FFFFFFFu);
-      t = max(t, __shfl_xor_sync(0xffffffffu, t, 1));
-      return max(t, __shfl_xor_sync(0xffffffffu, t, 2));
+      for (int i = 0; i < 16; ++i) t = max(t, w[i] & 0x7FFFFFFFu);
+      return max(t, __shfl_xor_sync(0xffffffffu, t, 1));
     } else {
       uint32_t t = w[0] & 0x7FFF7FFFu;
 #pragma unroll
-      for (int i = 1; i < 4; ++i) t = __vmaxu2(t, w[i] & 0x7FFF7FFFu);
-      t = __vmaxu2(t, __shfl_xor_sync(0xffffffffu, t, 1));
-      t = __vmaxu2(t, __shfl_xor_sync(0xffffffffu, t, 2));
+      for (int i = 1; i < 8; ++i) t = __vmaxu2(t, w[i] & 0x7FFF7FFFu);
       t = max(t & 0xFFFFu, t >> 16);
+      t = max(t, __shfl_xor_sync(0xffffffffu, t, 1));
       return kF16 ? __float_as_uint(__half2float(__ushort_as_half((uint16_t)t))) : t << 16;
     }
   }
-  // Codes of the values times inv, a power of two.
-  __device__ __forceinline__ uint32_t codes(float inv) const {
+  // Codes of values 8 h .. 8 h + 7 times inv, a power of two.
+  __device__ __forceinline__ uint32_t codes(int h, float inv) const {
     float v[8];
     if constexpr (kF32) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]) * inv;
+      for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[8 * h + i]) * inv;
     } else if constexpr (kF16) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[4 * h + i]));
         v[2 * i] = f.x * inv, v[2 * i + 1] = f.y * inv;
       }
     } else {
@@ -91,7 +93,7 @@ struct Eight {
       const __nv_bfloat162 k = __float2bfloat162_rn(inv);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 m = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), k);
+        const __nv_bfloat162 m = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[4 * h + i]), k);
         const uint32_t u = *reinterpret_cast<const uint32_t*>(&m);
         v[2 * i] = __uint_as_float(u << 16), v[2 * i + 1] = __uint_as_float(u & 0xFFFF0000u);
       }
@@ -100,34 +102,32 @@ struct Eight {
   }
 };
 
-// How the rows of x lie: groups of 8 that follow one another through the whole
-// matrix, 16-byte aligned groups in rows of any stride, or neither.
+// How the rows of x lie: half blocks that follow one another through the whole
+// matrix, 16-byte aligned ones in rows of any stride, or neither.
 enum Rows { WHOLE, ALIGNED, ANY };
 
-// A group is 8 values, four neighbours a block: a 16-byte load (two in f32),
-// a maximum over four lanes and a 4-byte store each, so a warp's loads and
-// code stores are whole lines.  A thread has its GROUPS loads in flight
-// together.  What is left to bound it is the number of instructions per group
-// (164 made it 47 us for 16384 x 4096 bf16, of which memory needs 27), so
-// codes and scales are addressed by the group's number alone, two 16-bit
-// magnitudes share a maximum, and a place in the matrix is only worked out
-// where it is needed, without a division per group.
+// A group is 16 values, two neighbours a block: 32 bytes loaded (64 in f32),
+// one maximum over two lanes, 8 bytes stored, so a warp's code stores are
+// whole lines.  A thread has its GROUPS loads in flight together.  Behind
+// memory (27 us for 16384 x 4096 bf16) come the integer instructions of a
+// block's scale and its places: with groups of 8, and a division per group,
+// 47 us; with places by the group's number alone 41 us; hence half blocks.
 template <typename T, int GROUPS, int ROWS>
 __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ld,
-                                                       uint32_t* __restrict__ packed, uint8_t* __restrict__ scales,
+                                                       uint2* __restrict__ packed, uint8_t* __restrict__ scales,
                                                        uint8_t* __restrict__ atoms) {
   launch_dependents();
-  const uint32_t blocks = (cols + 31) / 32, per_row = blocks * 4;
+  const uint32_t blocks = (cols + 31) / 32, per_row = blocks * 2;
   const int64_t first = (int64_t)blockIdx.x * (256 * GROUPS), row0 = first / per_row;
   const int tid = threadIdx.x, count = (int)min((int64_t)(256 * GROUPS), rows * per_row - first);
   const uint32_t t0 = (uint32_t)(first - row0 * per_row) + tid;
   const uint32_t rs = 256 / per_row, gs = 256 - rs * per_row;   // 256 groups on: rows, and groups of a row
-  Eight<T> v[GROUPS];
+  Half<T> v[GROUPS];
   if (ROWS == WHOLE) {
 #pragma unroll
     for (int k = 0; k < GROUPS; ++k) {
       v[k].clear();
-      if (tid + 256 * k < count) v[k].load(x + (first + tid) * 8 + 2048 * k);
+      if (tid + 256 * k < count) v[k].load(x + (first + tid) * 16 + 4096 * k, 16);
     }
   } else {
     int64_t r = row0 + t0 / per_row;
@@ -135,9 +135,9 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, 
 #pragma unroll
     for (int k = 0; k < GROUPS; ++k) {
       v[k].clear();
-      const int left = tid + 256 * k < count ? cols - (int)g * 8 : 0;
-      if (ROWS == ANY) v[k].load_some(x + r * ld + g * 8, left);
-      else if (left > 0) v[k].load(x + r * ld + g * 8);
+      const int left = tid + 256 * k < count ? min(cols - (int)g * 16, 16) : 0;
+      if (ROWS == ANY) v[k].load_some(x + r * ld + g * 16, left);
+      else v[k].load(x + r * ld + g * 16, left);
       r += rs, g += gs;
       if (g >= per_row) g -= per_row, ++r;
     }
@@ -146,14 +146,16 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, 
 #pragma unroll
   for (int k = 0; k < GROUPS; ++k) {
     s[k] = scale_byte(v[k].top());
-    const uint32_t w = s[k] == 255u ? 0u : v[k].codes(inv_scale(s[k]));
+    const float inv = inv_scale(s[k]);
+    uint2 w = make_uint2(v[k].codes(0, inv), v[k].codes(1, inv));
+    if (s[k] == 255u) w = make_uint2(0u, 0u);
     if (tid + 256 * k < count) packed[first + tid + 256 * k] = w;
   }
-  if (tid & 3) return;
+  if (tid & 1) return;
   if (scales) {
 #pragma unroll
     for (int k = 0; k < GROUPS; ++k)
-      if (tid + 256 * k < count) scales[(first + tid) / 4 + 64 * k] = (uint8_t)s[k];
+      if (tid + 256 * k < count) scales[(first + tid) / 2 + 128 * k] = (uint8_t)s[k];
   }
   if (atoms) {
     const uint32_t chunks = (blocks + 3) / 4;
@@ -162,10 +164,10 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, 
 #pragma unroll
     for (int k = 0; k < GROUPS; ++k) {
       if (tid + 256 * k < count) {
-        uint8_t* at = atoms + atom_at(row, g >> 2, chunks);
+        uint8_t* at = atoms + atom_at(row, g >> 1, chunks);
         *at = (uint8_t)s[k];
-        if (g == per_row - 4)   // blocks that fill up the last chunk: any scale but NaN
-            for (uint32_t e = blocks; e < chunks * 4; ++e) at[e - blocks + 1] = 0;
+        if (g == per_row - 2)   // blocks that fill up the last chunk: any scale but NaN
+          for (uint32_t e = blocks; e < chunks * 4; ++e) at[e - blocks + 1] = 0;
       }
       row += rs, g += gs;
       if (g >= per_row) g -= per_row, ++row;
@@ -173,13 +175,19 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, 
   }
 }
 
+// The value of a code (its e2m1 pair already f16) times its scale: exact; the
+// added 0 turns the second code of zero into +0.
+__device__ __forceinline__ float2 values_of(uint32_t h2, float s) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
+  return make_float2(fmaf(f.x, s, 0.0f), fmaf(f.y, s, 0.0f));
+}
+
 // The values of 8 codes a thread: a 4-byte load, 16 or 32 bytes stored, whole
-// lines a warp.  Exact: a code times a power of two; the added 0 turns the
-// second code of zero into +0.
+// lines a warp (rows of the result on 16 bytes, cols a multiple of 8).
 template <typename T, int GROUPS>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restrict__ packed,
                                                          const uint8_t* __restrict__ scales, int64_t rows, int cols,
-                                                         int vec, T* __restrict__ out) {
+                                                         T* __restrict__ out) {
   const uint32_t blocks = (cols + 31) / 32, per_row = blocks * 4;
   const int64_t first = (int64_t)blockIdx.x * (256 * GROUPS), row0 = first / per_row;
   const uint32_t rem = (uint32_t)(first - row0 * per_row) + threadIdx.x;
@@ -188,42 +196,57 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restr
   for (int k = 0; k < GROUPS; ++k) {
     const uint32_t t = rem + 256 * k, r = t / per_row, g = t - r * per_row;
     const int64_t row = row0 + r;
-    w[k] = row < rows ? __ldcs(packed + row * per_row + g) : 0u;
+    w[k] = row < rows ? packed[row * per_row + g] : 0u;
     sc[k] = row < rows ? scales[row * blocks + (g >> 2)] : 0u;
   }
 #pragma unroll
   for (int k = 0; k < GROUPS; ++k) {
     const uint32_t t = rem + 256 * k, r = t / per_row, g = t - r * per_row;
     const int64_t row = row0 + r;
-    if (row >= rows) continue;
+    if (row >= rows || (int)g * 8 >= cols) continue;
     const float s = ds::u8m0_value(sc[k]);
     uint32_t h[4];
     e2m1x8_to_f16x2(w[k], h);
-    float v[8];
+    float2 v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
-      v[2 * j] = fmaf(f.x, s, 0.0f), v[2 * j + 1] = fmaf(f.y, s, 0.0f);
-    }
+    for (int j = 0; j < 4; ++j) v[j] = values_of(h[j], s);
     T* dst = out + row * cols + g * 8;
-    if (vec && (int)(g * 8 + 8) <= cols) {
-      if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-        uint32_t o[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-          o[j] = *reinterpret_cast<const uint32_t*>(&b);
-        }
-        *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
-      }
+    if constexpr (sizeof(T) == 4) {
+      reinterpret_cast<float4*>(dst)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+      reinterpret_cast<float4*>(dst)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
     } else {
+      uint32_t o[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if ((int)(g * 8) + j < cols) dst[j] = (T)v[j];
+      for (int j = 0; j < 4; ++j) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(v[j].x, v[j].y);
+        o[j] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+      *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
     }
+  }
+}
+
+// Any other result: a byte of codes a thread, so that a warp's single stores
+// still fall on neighbouring addresses.
+template <typename T>
+__global__ void __launch_bounds__(256) dequantize_any_kernel(const uint8_t* __restrict__ packed,
+                                                             const uint8_t* __restrict__ scales, int64_t rows, int cols,
+                                                             T* __restrict__ out) {
+  const uint32_t blocks = (cols + 31) / 32, pairs = (cols + 1) / 2;
+  const int64_t first = (int64_t)blockIdx.x * 1024, row0 = first / pairs;
+  const uint32_t rem = (uint32_t)(first - row0 * pairs) + threadIdx.x;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t t = rem + 256 * k, r = t / pairs, g = t - r * pairs;
+    const int64_t row = row0 + r;
+    if (row >= rows) continue;
+    const uint32_t code = packed[row * blocks * 16 + g];
+    const float s = ds::u8m0_value(scales[row * blocks + (g >> 4)]);
+    float lo, hi;
+    tc5::e2m1x2_to_f32x2(code, lo, hi);
+    T* dst = out + row * cols + g * 2;
+    dst[0] = (T)fmaf(lo, s, 0.0f);
+    if ((int)g * 2 + 1 < cols) dst[1] = (T)fmaf(hi, s, 0.0f);
   }
 }
 
@@ -457,11 +480,11 @@ int* err_word() {
   return cudaGetSymbolAddress(&p, g_err) == cudaSuccess ? static_cast<int*>(p) : nullptr;
 }
 
-// Groups of 8 values per thread: four, or one where that leaves SMs idle.
+// Groups of `size` values per thread: four, or one where that leaves SMs idle.
 template <typename F>
-int by_groups(int64_t rows, int64_t cols, F launch) {
-  const int64_t groups = rows * blocks_of(cols) * 4;
-  const int per = groups >= (int64_t)ds::sm_count() * 4 * 1024 ? 4 : 1;
+int by_groups(int64_t rows, int64_t cols, int size, F launch) {
+  const int64_t groups = rows * blocks_of(cols) * (32 / size);
+  const int per = groups >= (int64_t)ds::sm_count() * 2 * 1024 ? 4 : 1;
   const int64_t grid = (groups + 256 * per - 1) / (256 * per);
   DS_REQUIRE(grid < ((int64_t)1 << 31), DS_ERANGE, "mx4: matrix too large");
   if (per == 4) launch(std::integral_constant<int, 4>(), (unsigned)grid);
@@ -474,8 +497,8 @@ int launch_quantize(const void* x, int dtype, int64_t rows, int cols, int64_t ld
   const int es = dtype == DS_F32 ? 4 : 2;
   const bool vec = ds::aligned(x, 16) && cols % 8 == 0 && (rows == 1 || ld * es % 16 == 0);
   const bool whole = vec && cols % 32 == 0 && (rows == 1 || ld == cols);
-  uint32_t* pk = reinterpret_cast<uint32_t*>(packed);
-  const int st = by_groups(rows, cols, [&](auto per, unsigned grid) {
+  uint2* pk = reinterpret_cast<uint2*>(packed);
+  const int st = by_groups(rows, cols, 16, [&](auto per, unsigned grid) {
     constexpr int G = decltype(per)::value;
     auto run = [&](auto* src) {
       using T = std::remove_const_t<std::remove_pointer_t<decltype(src)>>;
@@ -697,17 +720,25 @@ extern "C" int ds_mx4_dequantize(const uint8_t* packed, const uint8_t* scales, i
   DS_REQUIRE(ds::aligned(packed, 16) && ds::aligned(out, out_dtype == DS_F32 ? 4 : 2), DS_EALIGN,
              "mx4_dequantize: codes must be 16-byte aligned, out to its elements");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int vec = ds::aligned(out, 16) && cols * (out_dtype == DS_F32 ? 4 : 2) % 16 == 0;
-  const uint32_t* pk = reinterpret_cast<const uint32_t*>(packed);
-  const int st = by_groups(rows, cols, [&](auto per, unsigned grid) {
-    constexpr int G = decltype(per)::value;
+  const int C = (int)cols;
+  if (ds::aligned(out, 16) && cols % 8 == 0) {
+    const uint32_t* pk = reinterpret_cast<const uint32_t*>(packed);
+    const int st = by_groups(rows, cols, 8, [&](auto per, unsigned grid) {
+      constexpr int G = decltype(per)::value;
+      if (out_dtype == DS_F32)
+        dequantize_kernel<float, G><<<grid, 256, 0, s>>>(pk, scales, rows, C, static_cast<float*>(out));
+      else
+        dequantize_kernel<__nv_bfloat16, G><<<grid, 256, 0, s>>>(pk, scales, rows, C, static_cast<__nv_bfloat16*>(out));
+    });
+    if (st != DS_OK) return st;
+  } else {
+    const int64_t grid = (rows * ((cols + 1) / 2) + 1023) / 1024;
+    DS_REQUIRE(grid < ((int64_t)1 << 31), DS_ERANGE, "mx4_dequantize: matrix too large");
     if (out_dtype == DS_F32)
-      dequantize_kernel<float, G><<<grid, 256, 0, s>>>(pk, scales, rows, (int)cols, vec, static_cast<float*>(out));
+      dequantize_any_kernel<<<(unsigned)grid, 256, 0, s>>>(packed, scales, rows, C, static_cast<float*>(out));
     else
-      dequantize_kernel<__nv_bfloat16, G><<<grid, 256, 0, s>>>(pk, scales, rows, (int)cols, vec,
-                                                               static_cast<__nv_bfloat16*>(out));
-  });
-  if (st != DS_OK) return st;
+      dequantize_any_kernel<<<(unsigned)grid, 256, 0, s>>>(packed, scales, rows, C, static_cast<__nv_bfloat16*>(out));
+  }
   DS_CHECK_LAUNCH("mx4 dequantize_kernel");
   return DS_OK;
 }
