@@ -34,6 +34,33 @@ int sm_count() {
   return cached[dev];
 }
 
+int current_device() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 ? dev : -1;
+}
+
+// Two threads that meet here on a first call both do the work, with the same
+// outcome.
+int allow_smem(SmemOnce* done, const void* kernel, size_t bytes) {
+  const int dev = current_device();
+  if (dev >= 0 && __atomic_load_n(&done->set[dev], __ATOMIC_ACQUIRE)) return DS_OK;
+  DS_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  if (dev >= 0) __atomic_store_n(&done->set[dev], 1, __ATOMIC_RELEASE);
+  return DS_OK;
+}
+
+int* symbol_address(SymbolOnce* known, const void* symbol) {
+  const int dev = current_device();
+  if (dev >= 0) {
+    int* p = __atomic_load_n(&known->at[dev], __ATOMIC_ACQUIRE);
+    if (p) return p;
+  }
+  void* p = nullptr;
+  if (cudaGetSymbolAddress(&p, symbol) != cudaSuccess) return nullptr;
+  if (dev >= 0) __atomic_store_n(&known->at[dev], static_cast<int*>(p), __ATOMIC_RELEASE);
+  return static_cast<int*>(p);
+}
+
 }  // namespace ds
 
 extern "C" const char* ds_last_error_string(void) { return g_last_error; }

@@ -64,24 +64,14 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, 
 // Tensor map of a row-major 16-bit matrix [rows, cols], boxes of 64 columns x
 // box_rows rows.  ld (elements) and base must be 16-byte multiples.
 inline bool map16(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
-  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
-  const cuuint32_t es[2] = {1, 1};
-  return grouped::encode_fn()(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), dims, strides, box, es,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return grouped::encode_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, base, rows, cols, ld * 2, 64, box_rows,
+                            CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // The same of an f32 matrix, boxes of 32 x 32 (128-byte lines).
 inline bool map32(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld) {
-  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)ld * 4};
-  const cuuint32_t box[2] = {32, 32};
-  const cuuint32_t es[2] = {1, 1};
-  return grouped::encode_fn()(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(base), dims, strides, box, es,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return grouped::encode_2d(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base, rows, cols, ld * 4, 32, 32,
+                            CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // ---------------------------------------------------------------- the gated unit

@@ -27,6 +27,24 @@ int cuda_status(cudaError_t e, const char* what);
 // Number of SMs of the current device (cached per device).
 int sm_count();
 
+// Current device, 0 .. 63, or -1.
+int current_device();
+
+// Allows `kernel` `bytes` of dynamic shared memory on the current device.
+// `done`: the kernel's own zero-initialised flags, so that a call after the
+// first on a device costs a load.
+struct SmemOnce {
+  unsigned char set[64];
+};
+int allow_smem(SmemOnce* done, const void* kernel, size_t bytes);
+
+// Address of a __device__ int of the library on the current device, looked up
+// once per device.
+struct SymbolOnce {
+  int* at[64];
+};
+int* symbol_address(SymbolOnce* known, const void* symbol);
+
 }  // namespace ds
 
 #define DS_CHECK_CUDA(expr)                                           \

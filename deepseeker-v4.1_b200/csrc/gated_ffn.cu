@@ -289,14 +289,16 @@ int place(Operand& o, char*& ws, cudaStream_t s) {
 }
 
 int* err_word() {
-  void* p = nullptr;
-  return cudaGetSymbolAddress(&p, g_err) == cudaSuccess ? static_cast<int*>(p) : nullptr;
+  static SymbolOnce known;
+  return ds::symbol_address(&known, &g_err);
 }
 
 template <int MODE, int NT>
 int launch_tiles(const TileParams& p, int slices, cudaStream_t s, bool chained) {
   using C = TileShape<MODE, NT>;
-  DS_CHECK_CUDA(cudaFuncSetAttribute(tile_kernel<MODE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  static SmemOnce once;
+  const int st = ds::allow_smem(&once, reinterpret_cast<const void*>(&tile_kernel<MODE, NT>), C::kSmem);
+  if (st != DS_OK) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((p.M + 127) / 128 * slices), (unsigned)((p.N + NT - 1) / NT));
   cfg.blockDim = dim3(kTileThreads);
@@ -397,7 +399,9 @@ int launch_pairs(PairParams& p, Sides* sides, cudaStream_t s, bool chained) {
     DS_REQUIRE(tiles < ((int64_t)1 << 31), DS_ERANGE, "gated_ffn: too many tiles");
     q.tiles = (int)tiles;
   }
-  DS_CHECK_CUDA(cudaFuncSetAttribute(pair::pair_kernel<EPI, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  static SmemOnce once;
+  const int st = ds::allow_smem(&once, reinterpret_cast<const void*>(&pair::pair_kernel<EPI, NT>), C::kSmem);
+  if (st != DS_OK) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, ds::sm_count() / 2)));
   cfg.blockDim = dim3(pair::kThreads);

@@ -109,6 +109,13 @@ int launch_combine(const float* y, const int32_t* pos, const float* topk_w, cons
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn();
 
+// Encodes a map of a row-major matrix [rows, cols], rows ld_bytes apart, in
+// boxes of box_cols x box_rows (zeros outside).  A thread that has made no
+// runtime call yet (an autograd worker) has no current context, which the
+// encoder needs: it is bound and the call repeated.
+bool encode_2d(CUtensorMap* m, CUtensorMapDataType type, const void* base, int64_t rows, int64_t cols,
+               int64_t ld_bytes, int box_cols, int box_rows, CUtensorMapSwizzle swizzle);
+
 // Activation pieces [rows][row_bytes] (UINT8, 128-byte swizzle) viewed as
 // {128 B, rows, row_bytes / 128}; a box is 128 B x box_rows.
 bool map_pieces(CUtensorMap* m, const void* base, uint64_t rows, uint64_t row_bytes, uint32_t box_rows);

@@ -466,18 +466,14 @@ size_t packed_bytes(int64_t rows, int64_t cols) { return (size_t)rows * blocks_o
 
 // Codes of a matrix as bytes [rows, 16 blocks]; a box is 128 bytes (256 codes) x box_rows.
 bool map_codes(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int box_rows) {
-  const cuuint64_t dims[2] = {(cuuint64_t)blocks_of(cols) * 16, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)blocks_of(cols) * 16};
-  const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
-  const cuuint32_t es[2] = {1, 1};
-  return grouped::encode_fn()(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, es,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const int64_t bytes = blocks_of(cols) * 16;
+  return grouped::encode_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rows, bytes, bytes, 128, box_rows,
+                            CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 int* err_word() {
-  void* p = nullptr;
-  return cudaGetSymbolAddress(&p, g_err) == cudaSuccess ? static_cast<int*>(p) : nullptr;
+  static SymbolOnce known;
+  return ds::symbol_address(&known, &g_err);
 }
 
 // Groups of `size` values per thread: four, or one where that leaves SMs idle.
@@ -518,7 +514,9 @@ int launch_quantize(const void* x, int dtype, int64_t rows, int cols, int64_t ld
 template <int MODE, int NT>
 int launch_tiles(const TileParams& p, int slices, cudaStream_t s, bool chained) {
   using C = TileShape<MODE, NT>;
-  DS_CHECK_CUDA(cudaFuncSetAttribute(tile_kernel<MODE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  static SmemOnce once;
+  const int st = ds::allow_smem(&once, reinterpret_cast<const void*>(&tile_kernel<MODE, NT>), C::kSmem);
+  if (st != DS_OK) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((p.M + 127) / 128 * slices), (unsigned)((p.N + NT - 1) / NT));
   cfg.blockDim = dim3(kTileThreads);
@@ -558,26 +556,16 @@ constexpr int kPairRows = 129;
 
 // Scale atoms as lines of 512 bytes (128 words); a box is two lines.
 bool map_atoms(CUtensorMap* m, const void* base, int64_t rows, int64_t cols) {
-  const cuuint64_t dims[2] = {128, (cuuint64_t)(atoms_bytes(rows, cols) / kAtom)};
-  const cuuint64_t strides[1] = {kAtom};
-  const cuuint32_t box[2] = {128, 2};
-  const cuuint32_t es[2] = {1, 1};
-  return grouped::encode_fn()(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, es,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
-                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return grouped::encode_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, atoms_bytes(rows, cols) / kAtom, 128, kAtom, 128, 2,
+                            CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 // Result [rows, cols] in boxes of 128 bytes x 32 rows; false where its rows do not start on 16 bytes.
 bool map_result(CUtensorMap* m, void* y, int64_t rows, int64_t cols, int dtype) {
-  const int es_ = dtype == DS_F32 ? 4 : 2;
-  if (!ds::aligned(y, 16) || cols * es_ % 16 != 0) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)(cols * es_)};
-  const cuuint32_t box[2] = {(cuuint32_t)(128 / es_), 32};
-  const cuuint32_t es[2] = {1, 1};
-  return grouped::encode_fn()(m, dtype == DS_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2,
-                              y, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const int es = dtype == DS_F32 ? 4 : 2;
+  if (!ds::aligned(y, 16) || cols * es % 16 != 0) return false;
+  return grouped::encode_2d(m, dtype == DS_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, y,
+                            rows, cols, cols * es, 128 / es, 32, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <bool GATED>
@@ -585,7 +573,9 @@ int run_pairs(const PairParams& p, cudaStream_t s, bool chained) {
   constexpr int cols = GATED ? 128 : 256;
   const int64_t tiles = (p.M + 255) / 256 * (int64_t)((p.N + cols - 1) / cols);
   DS_REQUIRE(tiles < ((int64_t)1 << 31), DS_ERANGE, "mx4: too many tiles");
-  DS_CHECK_CUDA(cudaFuncSetAttribute(pairs::pair_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, pairs::kSmem));
+  static SmemOnce once;
+  const int st = ds::allow_smem(&once, reinterpret_cast<const void*>(&pairs::pair_kernel<GATED>), pairs::kSmem);
+  if (st != DS_OK) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, ds::sm_count() / 2)));
   cfg.blockDim = dim3(pairs::kThreads);

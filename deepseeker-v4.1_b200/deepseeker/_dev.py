@@ -1,6 +1,7 @@
 """Small helpers for passing torch tensors through the C ABI."""
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import numpy as np
@@ -10,6 +11,32 @@ import torch
 def stream_handle(device: torch.device | None = None) -> ctypes.c_void_p:
     """cudaStream_t of torch's current stream on `device`."""
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+_SAME = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context in which `device` is the current one; nothing where it is already."""
+    return _SAME if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def raw_stream(device: torch.device) -> int:
+    """cudaStream_t of torch's current stream on `device` (a CUDA tensor's, so with an index) as an integer:
+    what a call of a few microseconds can afford."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def rows_of(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """`t` (2-D) with rows that are contiguous runs, and their distance in elements; a copy where it has none."""
+    rows, cols = t.shape
+    ld, inner = t.stride()
+    if inner == 1 or cols == 1:
+        if rows <= 1:
+            return t, cols
+        if ld >= cols:
+            return t, ld
+    return t.contiguous(), cols
 
 
 def ptr(t: torch.Tensor | None) -> ctypes.c_void_p:

@@ -13,89 +13,87 @@ import ctypes
 import torch
 
 from . import _abi
-from ._dev import stream_handle
+from ._dev import on_device, raw_stream, rows_of, stream_handle
 
 _DTYPES = {torch.bfloat16: _abi.DS_BF16, torch.float16: _abi.DS_F16}
 
 
-def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """A 2-D tensor whose rows are contiguous runs, and their distance in elements."""
-    rows, cols = t.shape
-    if t.stride(1) == 1 or cols == 1:
-        ld = t.stride(0) if rows > 1 else cols
-        if ld >= cols:
-            return t, ld
-    return t.contiguous(), cols
-
-
-def _check(x, w1, w3, w2, limit) -> tuple[int, int]:
+def _check(x, w1, w3, w2, limit) -> int:
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _DTYPES:
         raise ValueError("x must be a bf16 or f16 CUDA tensor")
-    if x.dim() < 1:
-        raise ValueError("x must be [..., hidden]")
+    dev, dtype = x.get_device(), x.dtype
     for name, w in (("w1", w1), ("w3", w3), ("w2", w2)):
-        if not isinstance(w, torch.Tensor) or w.device != x.device or w.dtype != x.dtype or w.dim() != 2:
-            raise ValueError(f"{name} must be a 2-D {x.dtype} tensor on x's device")
+        if not isinstance(w, torch.Tensor) or w.get_device() != dev or w.dtype != dtype or w.dim() != 2:
+            raise ValueError(f"{name} must be a 2-D {dtype} tensor on x's device")
     inter, hidden = w1.shape
-    if x.shape[-1] != hidden or w3.shape != (inter, hidden) or w2.shape != (hidden, inter):
+    if x.dim() < 1 or x.shape[-1] != hidden or w3.shape != (inter, hidden) or w2.shape != (hidden, inter):
         raise ValueError("x [..., H], w1 [I, H], w3 [I, H], w2 [H, I] expected")
     if hidden < 1 or inter < 1:
         raise ValueError("hidden and inter must be at least 1")
     if limit is not None and not limit > 0:
         raise ValueError("limit must be positive, or None for no clamps")
-    return hidden, inter
+    return hidden
 
 
 def _desc(x, w1, w3, w2, limit) -> tuple[_abi.DsGatedFfn, tuple]:
     """The call's descriptor, and the tensors that it points into."""
-    (x, lx), (w1, l1), (w3, l3), (w2, l2) = _rows(x), _rows(w1), _rows(w3), _rows(w2)
-    d = _abi.DsGatedFfn(x.shape[0], w1.shape[1], w1.shape[0], _DTYPES[x.dtype], limit or 0.0, x.data_ptr(),
-                        w1.data_ptr(), w3.data_ptr(), w2.data_ptr(), lx, l1, l3, l2)
+    (x, lx), (w1, l1), (w3, l3), (w2, l2) = rows_of(x), rows_of(w1), rows_of(w3), rows_of(w2)
+    inter, hidden = w1.shape
+    d = _abi.DsGatedFfn(x.shape[0], hidden, inter, _DTYPES[x.dtype], limit or 0.0, x.data_ptr(), w1.data_ptr(),
+                        w3.data_ptr(), w2.data_ptr(), lx, l1, l3, l2)
     return d, (x, w1, w3, w2)
 
 
-def _workspace(size_fn: str, device, *args) -> torch.Tensor:
-    n = ctypes.c_size_t(0)
-    _abi.call(size_fn, *args, ctypes.byref(n))
-    return torch.empty(n.value, dtype=torch.uint8, device=device)
+def _pre_bytes(x, w1) -> int:
+    """Bytes of g and u in f32, which lead the buffer kept for the backward pass; h follows."""
+    return 8 * x.shape[0] * ((w1.shape[0] + 7) // 8 * 8)
 
 
 def _forward(x, w1, w3, w2, limit, keep: bool):
+    """y, and the buffer (pre-activations, h) that the backward pass reads."""
     d, hold = _desc(x, w1, w3, w2, limit)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    h = pre = None
-    if keep:
-        cols = (w1.shape[0] + 7) // 8 * 8
-        h = torch.empty(x.shape[0], cols, dtype=x.dtype, device=x.device)
-        pre = torch.empty(2, x.shape[0], cols, dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        ws = _workspace("ds_gated_ffn_workspace_size", x.device, ctypes.byref(d), int(keep))
-        _abi.call("ds_gated_ffn", ctypes.byref(d), y.data_ptr(), h.data_ptr() if keep else None,
-                  pre.data_ptr() if keep else None, ws.data_ptr(), ws.numel(), stream_handle(x.device))
-    return y, h, pre
+    lib, ref, dev = _abi.lib(), ctypes.byref(d), x.device
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    kept = h = pre = None
+    with on_device(dev):
+        if keep:
+            n = _pre_bytes(x, w1)
+            kept = torch.empty(n + n // 4, dtype=torch.uint8, device=dev)
+            pre = kept.data_ptr()
+            h = pre + n
+        n = ctypes.c_size_t(0)
+        _abi.check(lib.ds_gated_ffn_workspace_size(ref, keep, ctypes.byref(n)), "ds_gated_ffn_workspace_size")
+        ws = torch.empty(n.value, dtype=torch.uint8, device=dev) if n.value else None
+        _abi.check(lib.ds_gated_ffn(ref, y.data_ptr(), h, pre, None if ws is None else ws.data_ptr(), n.value,
+                                    raw_stream(dev)), "ds_gated_ffn")
+    return y, kept
 
 
 class _GatedFFN(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w1, w3, w2, limit):
-        y, h, pre = _forward(x, w1, w3, w2, limit, True)
-        ctx.save_for_backward(x, w1, w3, w2, h, pre)
+        y, kept = _forward(x, w1, w3, w2, limit, True)
+        ctx.save_for_backward(x, w1, w3, w2, kept)
         ctx.limit = limit
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, w1, w3, w2, h, pre = ctx.saved_tensors
+        x, w1, w3, w2, kept = ctx.saved_tensors
         d, hold = _desc(x, w1, w3, w2, ctx.limit)
-        dy, ld = _rows(dy)
-        grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None
+        dy, ld = rows_of(dy)
+        lib, ref, dev = _abi.lib(), ctypes.byref(d), x.device
+        grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if need else None
                  for t, need in zip((x, w1, w3, w2), ctx.needs_input_grad)]
-        with torch.cuda.device(x.device):
-            ws = _workspace("ds_gated_ffn_backward_workspace_size", x.device, ctypes.byref(d), dy.data_ptr(), ld)
-            _abi.call("ds_gated_ffn_backward", ctypes.byref(d), h.data_ptr(), pre.data_ptr(), dy.data_ptr(), ld,
-                      *(None if g is None else g.data_ptr() for g in grads), ws.data_ptr(), ws.numel(),
-                      stream_handle(x.device))
+        pre, n = kept.data_ptr(), ctypes.c_size_t(0)
+        with on_device(dev):
+            _abi.check(lib.ds_gated_ffn_backward_workspace_size(ref, dy.data_ptr(), ld, ctypes.byref(n)),
+                       "ds_gated_ffn_backward_workspace_size")
+            ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
+            _abi.check(lib.ds_gated_ffn_backward(ref, pre + _pre_bytes(x, w1), pre, dy.data_ptr(), ld,
+                                                 *[None if g is None else g.data_ptr() for g in grads],
+                                                 ws.data_ptr(), n.value, raw_stream(dev)), "ds_gated_ffn_backward")
         return (*grads, None)
 
 
@@ -109,11 +107,13 @@ def gated_ffn(x: torch.Tensor, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Ten
     pre-activations (f32), 10 bytes per token and intermediate feature.  The
     gradient of a clamped value is 0.
     """
-    hidden, _ = _check(x, w1, w3, w2, limit)
-    rows = x.reshape(-1, hidden)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w1, w3, w2)):
-        return _GatedFFN.apply(rows, w1, w3, w2, limit).view(x.shape)
-    return _forward(rows, w1, w3, w2, limit, False)[0].view(x.shape)
+    hidden = _check(x, w1, w3, w2, limit)
+    rows = x if x.dim() == 2 else x.reshape(-1, hidden)
+    if torch.is_grad_enabled() and (x.requires_grad or w1.requires_grad or w3.requires_grad or w2.requires_grad):
+        y = _GatedFFN.apply(rows, w1, w3, w2, limit)
+    else:
+        y = _forward(rows, w1, w3, w2, limit, False)[0]
+    return y if x.dim() == 2 else y.view(x.shape)
 
 
 def status(device: torch.device | None = None) -> int:
@@ -121,6 +121,6 @@ def status(device: torch.device | None = None) -> int:
     bounded device wait gave up; outputs are then undefined).  Waits for the stream."""
     err = torch.zeros(1, dtype=torch.int32)
     with torch.cuda.device(device):
-        _abi.call("ds_gated_ffn_status", err.data_ptr(), stream_handle(device))
+        _abi.check(_abi.lib().ds_gated_ffn_status(err.data_ptr(), stream_handle(device)), "ds_gated_ffn_status")
         torch.cuda.current_stream(device).synchronize()
     return int(err[0])

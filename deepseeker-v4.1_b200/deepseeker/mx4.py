@@ -14,8 +14,7 @@ import ctypes
 import torch
 
 from . import _abi
-from ._dev import stream_handle
-from .gated import _rows
+from ._dev import on_device, raw_stream, rows_of, stream_handle
 
 BLOCK = 32
 _DTYPES = {torch.float32: _abi.DS_F32, torch.bfloat16: _abi.DS_BF16, torch.float16: _abi.DS_F16}
@@ -26,7 +25,12 @@ def _blocks(cols: int) -> int:
 
 
 def _atoms_bytes(rows: int, cols: int) -> int:
-    return -(-rows // 128) * -(-cols // 128) * 512
+    return (rows + 127) // 128 * ((cols + 127) // 128) * 512
+
+
+def _workspace_bytes(rows: int, cols: int) -> int:
+    """Codes and atoms of a quantised matrix, each on 256 bytes (ds_mx4_linear_workspace_size)."""
+    return (rows * _blocks(cols) * 16 + 255) // 256 * 256 + (_atoms_bytes(rows, cols) + 255) // 256 * 256
 
 
 class MX4Tensor:
@@ -35,27 +39,30 @@ class MX4Tensor:
     = NaN), ``atoms`` (the scales as the tensor cores read them); ``shape``:
     the shape it stands for, leading dimensions included."""
 
-    __slots__ = ("packed", "scales", "atoms", "rows", "cols", "shape", "_c")
+    __slots__ = ("packed", "scales", "atoms", "rows", "cols", "shape", "device", "_c")
 
     def __init__(self, packed, scales, atoms, shape):
         self.packed, self.scales, self.atoms = packed, scales, atoms
-        self.shape = torch.Size(shape)
-        self.rows, self.cols = packed.shape[0], self.shape[-1]
-        self._c = _abi.DsMx4(packed.data_ptr(), atoms.data_ptr(), self.rows, self.cols)
+        self.shape = shape
+        self.rows, self.cols, self.device = packed.shape[0], shape[-1], packed.device
+        self._c = None
 
-    @property
-    def device(self) -> torch.device:
-        return self.packed.device
+    def _ref(self):
+        if self._c is None:
+            self._c = _abi.DsMx4(self.packed.data_ptr(), self.atoms.data_ptr(), self.rows, self.cols)
+        return ctypes.byref(self._c)
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values that the codes stand for, f32 or bf16 (both exact)."""
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError("dtype must be torch.float32 or torch.bfloat16")
-        out = torch.empty(self.rows, self.cols, dtype=dtype, device=self.device)
-        with torch.cuda.device(self.device):
-            _abi.call("ds_mx4_dequantize", self.packed.data_ptr(), self.scales.data_ptr(), self.rows, self.cols,
-                      out.data_ptr(), _DTYPES[dtype], stream_handle(self.device))
-        return out.view(self.shape)
+        dev = self.device
+        out = torch.empty(self.shape, dtype=dtype, device=dev)
+        with on_device(dev):
+            _abi.check(_abi.lib().ds_mx4_dequantize(self.packed.data_ptr(), self.scales.data_ptr(), self.rows,
+                                                    self.cols, out.data_ptr(), _DTYPES[dtype], raw_stream(dev)),
+                       "ds_mx4_dequantize")
+        return out
 
 
 def _check_x(x) -> None:
@@ -67,21 +74,26 @@ def _check_x(x) -> None:
         raise ValueError("4-bit operators have no backward pass: detach x or use torch.no_grad()")
 
 
+def _matrix(x):
+    """x [..., cols] as rows, and their distance in elements."""
+    return rows_of(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
+
+
 def quantize(x: torch.Tensor) -> MX4Tensor:
     """x [..., cols] -> MX4Tensor.  A block's scale is the smallest power of two
     that brings its largest magnitude to 6 or less (1 for zeros); values round
     to the nearest code, ties to the even one.  A NaN or an infinity makes its
     whole block NaN."""
     _check_x(x)
-    cols = x.shape[-1]
-    rows, ld = _rows(x.reshape(-1, cols))
-    n = rows.shape[0]
-    packed = torch.empty(n, _blocks(cols) * 16, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(n, _blocks(cols), dtype=torch.uint8, device=x.device)
-    atoms = torch.empty(_atoms_bytes(n, cols), dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        _abi.call("ds_mx4_quantize", rows.data_ptr(), _DTYPES[x.dtype], n, cols, ld, packed.data_ptr(),
-                  scales.data_ptr(), atoms.data_ptr(), stream_handle(x.device))
+    rows, ld = _matrix(x)
+    n, cols = rows.shape
+    nb, dev = _blocks(cols), x.device
+    packed = torch.empty((n, nb * 16), dtype=torch.uint8, device=dev)
+    scales = torch.empty((n, nb), dtype=torch.uint8, device=dev)
+    atoms = torch.empty(_atoms_bytes(n, cols), dtype=torch.uint8, device=dev)
+    with on_device(dev):
+        _abi.check(_abi.lib().ds_mx4_quantize(rows.data_ptr(), _DTYPES[x.dtype], n, cols, ld, packed.data_ptr(),
+                                              scales.data_ptr(), atoms.data_ptr(), raw_stream(dev)), "ds_mx4_quantize")
     return MX4Tensor(packed, scales, atoms, x.shape)
 
 
@@ -96,64 +108,54 @@ def from_packed(packed: torch.Tensor, scales: torch.Tensor, cols: int | None = N
     cols = nb * BLOCK if cols is None else cols
     if rows < 1 or cols < 1 or _blocks(cols) != nb or packed.shape != (rows, nb * 16) or packed.device != scales.device:
         raise ValueError("packed [rows, 16 ceil(cols/32)] and scales [rows, ceil(cols/32)] expected, on one device")
-    packed, scales = packed.contiguous(), scales.contiguous()
+    packed, scales, dev = packed.contiguous(), scales.contiguous(), packed.device
     if packed.data_ptr() % 16:
         packed = packed.clone()
-    atoms = torch.empty(_atoms_bytes(rows, cols), dtype=torch.uint8, device=packed.device)
-    with torch.cuda.device(packed.device):
-        _abi.call("ds_mx4_scale_atoms", scales.data_ptr(), rows, cols, atoms.data_ptr(), stream_handle(packed.device))
-    return MX4Tensor(packed, scales, atoms, (rows, cols))
+    atoms = torch.empty(_atoms_bytes(rows, cols), dtype=torch.uint8, device=dev)
+    with on_device(dev):
+        _abi.check(_abi.lib().ds_mx4_scale_atoms(scales.data_ptr(), rows, cols, atoms.data_ptr(), raw_stream(dev)),
+                   "ds_mx4_scale_atoms")
+    return MX4Tensor(packed, scales, atoms, torch.Size((rows, cols)))
 
 
-def _weight(w, name: str, device) -> None:
-    if not isinstance(w, MX4Tensor) or len(w.shape) != 2 or w.device != device:
-        raise ValueError(f"{name} must be a 2-D MX4Tensor on x's device")
-
-
-def _input(x, cols: int):
-    """(tensor kept alive, pointer, atoms pointer, type, rows, row stride) of x, quantised or not."""
+def _input(x, cols: int, out_dtype):
+    """(what keeps it alive, pointer, atoms' pointer, type, rows, row stride, result type) of x, quantised or not."""
     if isinstance(x, MX4Tensor):
-        if x.cols != cols:
-            raise ValueError(f"x must be [..., {cols}]")
-        return x, x.packed.data_ptr(), x.atoms.data_ptr(), _abi.DS_U8, x.rows, 0
-    _check_x(x)
+        got, dtype = (x, x.packed.data_ptr(), x.atoms.data_ptr(), _abi.DS_U8, x.rows, 0), torch.bfloat16
+    else:
+        _check_x(x)
+        rows, ld = _matrix(x)
+        got, dtype = (rows, rows.data_ptr(), None, _DTYPES[x.dtype], rows.shape[0], ld), x.dtype
     if x.shape[-1] != cols:
         raise ValueError(f"x must be [..., {cols}]")
-    rows, ld = _rows(x.reshape(-1, cols))
-    return rows, rows.data_ptr(), None, _DTYPES[x.dtype], rows.shape[0], ld
-
-
-def _out(x, rows: int, cols: int, out_dtype):
     if out_dtype is None:
-        out_dtype = torch.bfloat16 if isinstance(x, MX4Tensor) else x.dtype
+        out_dtype = dtype
     if out_dtype not in _DTYPES:
         raise ValueError("out_dtype must be f32, bf16 or f16")
-    return torch.empty(rows, cols, dtype=out_dtype, device=x.device), _DTYPES[out_dtype]
+    return *got, out_dtype
 
 
-def _device_of(x):
-    if not isinstance(x, MX4Tensor):
-        _check_x(x)
-    return x.device
+def _weight(w, name: str, x) -> None:
+    if not isinstance(w, MX4Tensor) or len(w.shape) != 2:
+        raise ValueError(f"{name} must be a 2-D MX4Tensor")
+    if w.device != getattr(x, "device", None):
+        raise ValueError(f"{name} must be on x's device")
 
 
 def linear(x, w: MX4Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """x [..., K] (a tensor, quantised on the way, or an MX4Tensor) times W^T,
     W [N, K] -> [..., N] in out_dtype (default: x's type; bf16 for an
     MX4Tensor).  Exact up to the f32 accumulation and the final rounding."""
-    dev = _device_of(x)
-    _weight(w, "w", dev)
-    hold, px, pa, dt, rows, ld = _input(x, w.cols)
-    out, odt = _out(x, rows, w.rows, out_dtype)
-    ws = None
-    n = 0
-    if dt != _abi.DS_U8:
-        n = _up(rows * _blocks(w.cols) * 16) + _up(_atoms_bytes(rows, w.cols))
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        _abi.call("ds_mx4_linear", px, pa, dt, rows, ld, ctypes.byref(w._c), out.data_ptr(), odt,
-                  None if ws is None else ws.data_ptr(), n, stream_handle(dev))
-    return out.view(*x.shape[:-1], w.rows)
+    _weight(w, "w", x)
+    hold, px, pa, dt, rows, ld, out_dtype = _input(x, w.cols, out_dtype)
+    dev = w.device
+    out = torch.empty((*x.shape[:-1], w.rows), dtype=out_dtype, device=dev)
+    n = 0 if dt == _abi.DS_U8 else _workspace_bytes(rows, w.cols)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    with on_device(dev):
+        _abi.check(_abi.lib().ds_mx4_linear(px, pa, dt, rows, ld, w._ref(), out.data_ptr(), _DTYPES[out_dtype],
+                                            ws.data_ptr() if n else None, n, raw_stream(dev)), "ds_mx4_linear")
+    return out
 
 
 def gated_ffn(x, w1: MX4Tensor, w3: MX4Tensor, w2: MX4Tensor, limit: float | None = None,
@@ -161,26 +163,23 @@ def gated_ffn(x, w1: MX4Tensor, w3: MX4Tensor, w2: MX4Tensor, limit: float | Non
     """(silu(min(x W1^T, L)) * clip(x W3^T, -L, L)) W2^T with x and the product
     of the gate quantised; w1 and w3 [I, H], w2 [H, I].  Clamps as in
     ``deepseeker.gated.gated_ffn``."""
-    dev = _device_of(x)
     for name, w in (("w1", w1), ("w3", w3), ("w2", w2)):
-        _weight(w, name, dev)
-    if w3.shape != w1.shape or w2.shape != (w1.cols, w1.rows):
+        _weight(w, name, x)
+    hidden, inter = w1.cols, w1.rows
+    if w3.shape != w1.shape or w2.shape != (hidden, inter):
         raise ValueError("w1 [I, H], w3 [I, H], w2 [H, I] expected")
     if limit is not None and not limit > 0:
         raise ValueError("limit must be positive, or None for no clamps")
-    hold, px, pa, dt, rows, ld = _input(x, w1.cols)
-    out, odt = _out(x, rows, w2.rows, out_dtype)
-    n = _up(rows * _blocks(w1.rows) * 16) + _up(_atoms_bytes(rows, w1.rows))
-    n += 0 if dt == _abi.DS_U8 else _up(rows * _blocks(w1.cols) * 16) + _up(_atoms_bytes(rows, w1.cols))
+    hold, px, pa, dt, rows, ld, out_dtype = _input(x, hidden, out_dtype)
+    dev = w1.device
+    out = torch.empty(x.shape, dtype=out_dtype, device=dev)
+    n = _workspace_bytes(rows, inter) + (0 if dt == _abi.DS_U8 else _workspace_bytes(rows, hidden))
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        _abi.call("ds_mx4_gated_ffn", px, pa, dt, rows, ld, ctypes.byref(w1._c), ctypes.byref(w3._c),
-                  ctypes.byref(w2._c), limit or 0.0, out.data_ptr(), odt, ws.data_ptr(), n, stream_handle(dev))
-    return out.view(*x.shape[:-1], w2.rows)
-
-
-def _up(n: int) -> int:
-    return (n + 255) // 256 * 256
+    with on_device(dev):
+        _abi.check(_abi.lib().ds_mx4_gated_ffn(px, pa, dt, rows, ld, w1._ref(), w3._ref(), w2._ref(), limit or 0.0,
+                                               out.data_ptr(), _DTYPES[out_dtype], ws.data_ptr(), n, raw_stream(dev)),
+                   "ds_mx4_gated_ffn")
+    return out
 
 
 def status(device: torch.device | None = None) -> int:
@@ -188,6 +187,6 @@ def status(device: torch.device | None = None) -> int:
     bounded device wait gave up; outputs are then undefined).  Waits for the stream."""
     err = torch.zeros(1, dtype=torch.int32)
     with torch.cuda.device(device):
-        _abi.call("ds_mx4_status", err.data_ptr(), stream_handle(device))
+        _abi.check(_abi.lib().ds_mx4_status(err.data_ptr(), stream_handle(device)), "ds_mx4_status")
         torch.cuda.current_stream(device).synchronize()
     return int(err[0])
