@@ -574,12 +574,12 @@ int run_pairs(const PairParams& p, cudaStream_t s, bool chained) {
   const int64_t tiles = (p.M + 255) / 256 * (int64_t)((p.N + cols - 1) / cols);
   DS_REQUIRE(tiles < ((int64_t)1 << 31), DS_ERANGE, "mx4: too many tiles");
   static SmemOnce once;
-  const int st = ds::allow_smem(&once, reinterpret_cast<const void*>(&pairs::pair_kernel<GATED>), pairs::kSmem);
+  const int st = ds::allow_smem(&once, reinterpret_cast<const void*>(&pairs::pair_kernel<GATED>), pairs::Shape<GATED>::kSmem);
   if (st != DS_OK) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, ds::sm_count() / 2)));
   cfg.blockDim = dim3(pairs::kThreads);
-  cfg.dynamicSmemBytes = pairs::kSmem;
+  cfg.dynamicSmemBytes = pairs::Shape<GATED>::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -45,12 +45,18 @@ using namespace ds::pair;
 constexpr int kOps = 32768;                       // 128 rows of x and of W, 128 bytes each
 constexpr int kSf = 6 * kAtom;                    // x: two atoms along k; W: 2 x two
 constexpr int kStage = kOps + kSf;                // 35 KB
-constexpr int kStages = 4;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 32 * (2 + kEpiWarps);
-constexpr int kSmem = 1024 + kStages * kStage + kEpiWarps * 2 * kBox;
 constexpr int kSfCols = 24;
-static_assert(kStage % 1024 == 0 && kSmem <= 226 * 1024, "shared memory of an SM");
+
+// As many stages as fit beside a result box per epilogue warp (the gated
+// product stores h from registers).
+template <bool GATED>
+struct Shape {
+  static constexpr int kStages = GATED ? 6 : 5;
+  static constexpr int kSmem = 1024 + kStages * kStage + (GATED ? 0 : kEpiWarps * kBox);
+  static_assert(kStage % 1024 == 0 && kSmem <= 226 * 1024, "shared memory of an SM");
+};
 
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                     uint32_t accumulate) {
@@ -138,7 +144,7 @@ __device__ __forceinline__ uint4 quantize_block(const float* h, int& s) {
 
 template <bool GATED>
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_kernel(const __grid_constant__ PairParams p) {
-  constexpr int S = kStages;
+  constexpr int S = Shape<GATED>::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   __shared__ __align__(8) uint64_t full[S], empty[S], accfull, accempty;
@@ -231,9 +237,9 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
   } else {
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3, half = (warp - 2) >> 2;
-    uint8_t* box0 = smem + S * kStage + (warp - 2) * 2 * kBox;
+    uint8_t* box = smem + S * kStage + (warp - 2) * kBox;
     const uint32_t bar = leader_addr(&accempty), acc = tc5::lane_quarter(tb, q);
-    int li = 0, turn = 0;
+    int li = 0;
     for (int tile = first; tile < n_tiles; tile += pairs, ++li) {
       int m0, n0;
       locate<GATED>(p, tile, m0, n0);
@@ -279,10 +285,9 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
         for (int c = 0; c < 4; ++c) {
           const int n = n0 + half * 128 + 32 * c;
           if (mw >= p.M || n >= p.N) continue;
-          uint8_t* box = box0 + (turn & 1) * kBox;
           const bool opens = per == 32 || (c & 1) == 0, closes = per == 32 || (c & 1) || n + 32 >= p.N;
           if (opens) {
-            if (lane == 0) box_wait_read<1>();   // the store before the last has read its box
+            if (lane == 0) box_wait_read<0>();   // the last store has read the box
             __syncwarp();
           }
           if (per == 32) {
@@ -301,7 +306,6 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
               box_store(&p.out, per == 32 ? n : n - 32 * (c & 1), mw, box);
               box_commit();
             }
-            ++turn;
           }
         }
       } else if (m < p.M) {

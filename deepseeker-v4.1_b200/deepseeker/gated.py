@@ -78,23 +78,30 @@ class _GatedFFN(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, w1, w3, w2, kept = ctx.saved_tensors
-        d, hold = _desc(x, w1, w3, w2, ctx.limit)
-        dy, ld = rows_of(dy)
-        lib, ref, dev = _abi.lib(), ctypes.byref(d), x.device
-        grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if need else None
-                 for t, need in zip((x, w1, w3, w2), ctx.needs_input_grad)]
-        pre, n = kept.data_ptr(), ctypes.c_size_t(0)
-        with on_device(dev):
-            _abi.check(lib.ds_gated_ffn_backward_workspace_size(ref, dy.data_ptr(), ld, ctypes.byref(n)),
-                       "ds_gated_ffn_backward_workspace_size")
-            ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
-            _abi.check(lib.ds_gated_ffn_backward(ref, pre + _pre_bytes(x, w1), pre, dy.data_ptr(), ld,
-                                                 *[None if g is None else g.data_ptr() for g in grads],
-                                                 ws.data_ptr(), n.value, raw_stream(dev)), "ds_gated_ffn_backward")
-        return (*grads, None)
+        # a graph of the gradients (create_graph) is refused where it is used; plain passes skip that wrapper's cost
+        return _backward_once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
+
+
+def _backward(ctx, dy):
+    x, w1, w3, w2, kept = ctx.saved_tensors
+    d, hold = _desc(x, w1, w3, w2, ctx.limit)
+    dy, ld = rows_of(dy)
+    lib, ref, dev = _abi.lib(), ctypes.byref(d), x.device
+    grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if need else None
+             for t, need in zip((x, w1, w3, w2), ctx.needs_input_grad)]
+    pre, n = kept.data_ptr(), ctypes.c_size_t(0)
+    with on_device(dev):
+        _abi.check(lib.ds_gated_ffn_backward_workspace_size(ref, dy.data_ptr(), ld, ctypes.byref(n)),
+                   "ds_gated_ffn_backward_workspace_size")
+        ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
+        _abi.check(lib.ds_gated_ffn_backward(ref, pre + _pre_bytes(x, w1), pre, dy.data_ptr(), ld,
+                                             *[None if g is None else g.data_ptr() for g in grads],
+                                             ws.data_ptr(), n.value, raw_stream(dev)), "ds_gated_ffn_backward")
+    return (*grads, None)
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 def gated_ffn(x: torch.Tensor, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Tensor,

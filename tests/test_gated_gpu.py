@@ -195,6 +195,17 @@ def test_shared_and_frozen_weights(cuda):
     assert float((g.double() - gw).norm()) <= 4 * HALF_UNIT[torch.bfloat16] * float(gw.norm())
 
 
+def test_second_derivatives_are_refused(cuda):
+    ins, dy = make(6, 64, 32, torch.bfloat16, cuda)
+    a = [t.detach().requires_grad_() for t in ins]
+    want = both(ins, dy, None)[0]
+    up = dy.detach().requires_grad_()
+    grads = torch.autograd.grad(gated.gated_ffn(*a), a, up, create_graph=True)
+    assert all(torch.equal(g, w) for g, w in zip(grads, want[1:]))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(grads[0].sum(), up)
+
+
 def test_no_tokens(cuda):
     ins, _ = make(3, 64, 32, torch.bfloat16, cuda)
     x = ins[0][:0].detach().requires_grad_()
