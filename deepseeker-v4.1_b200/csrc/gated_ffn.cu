@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
       int g = 0;
       for (int it = it0; it < it1; ++it, ++g) {
         const int s = g % S;
-        if (g >= S && !grouped::wait_or_abort(&empty[s], ((g / S) - 1) & 1, abort, p.err)) break;
+        if (g >= S && !ds::pair::wait(&empty[s], ((g / S) - 1) & 1, abort, p.err)) break;
         const int seg = it / ksteps, k0 = (it - seg * ksteps) * kBK;
         uint8_t* st = smem + s * C::kStage;
         mbar_arrive_expect_tx(&full[s], C::kStage);
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
     const uint64_t a0 = tile_desc<Md::kAMn>(smem_u32(smem)), b0 = tile_desc<false>(smem_u32(smem) + C::kA);
     for (int g = 0; g < it1 - it0; ++g) {
       const int s = g % S;
-      if (!grouped::warp_wait(&full[s], (g / S) & 1, abort, p.err)) break;
+      if (!ds::pair::wait_all(&full[s], (g / S) & 1, abort, p.err)) break;
       tc5::fence_after();
       if (elect_one()) {
         const uint64_t ad = a0 + (uint64_t)((s * C::kStage) >> 4), bd = b0 + (uint64_t)((s * C::kStage) >> 4);
@@ -182,9 +182,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
     // all issued MMAs complete before the accumulators are read or released
     if (elect_one()) tc5::commit(&accfull);
     __syncwarp();
-    grouped::warp_wait(&accfull, 0, abort, p.err);
+    ds::pair::wait_all(&accfull, 0, abort, p.err);
   } else {
-    grouped::warp_wait(&accfull, 0, abort, p.err);
+    ds::pair::wait_all(&accfull, 0, abort, p.err);
   }
   tc5::fence_after();
 

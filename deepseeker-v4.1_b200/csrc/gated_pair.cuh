@@ -169,7 +169,7 @@ __device__ __forceinline__ bool copy_tile(const Rings& r, const Problem& q, int 
   const int ksteps = q.ksteps, its = ksteps * q.segs, am = m0 + 128 * rank, bn = GATE ? n0 : n0 + NT / 2 * rank;
   for (int it = 0; it < its; ++it, ++g) {
     const int s = g % C::kStages;
-    if (g >= C::kStages && !grouped::wait_or_abort(&r.empty[s], ((g / C::kStages) - 1) & 1, r.abort, r.err)) return false;
+    if (g >= C::kStages && !wait(&r.empty[s], ((g / C::kStages) - 1) & 1, r.abort, r.err)) return false;
     const int seg = it >= ksteps ? 1 : 0, k0 = (it - seg * ksteps) * kBK;
     uint8_t* st = r.smem + s * C::kStage;
     const uint32_t bar = leader_addr(&r.full[s]);
@@ -190,7 +190,7 @@ __device__ __forceinline__ bool mma_tile(const Rings& r, int its, int f16, uint3
   const uint64_t a0 = tile_desc<AMN>(smem_u32(r.smem)), b0 = tile_desc<BMN>(smem_u32(r.smem) + kOperand);
   for (int it = 0; it < its; ++it, ++g) {
     const int s = g % C::kStages;
-    if (!grouped::warp_wait(&r.full[s], (g / C::kStages) & 1, r.abort, r.err)) return false;
+    if (!wait_all(&r.full[s], (g / C::kStages) & 1, r.abort, r.err)) return false;
     tc5::fence_after();
     if (elect_one()) {
       const uint64_t ad = a0 + (uint64_t)((s * C::kStage) >> 4), bd = b0 + (uint64_t)((s * C::kStage) >> 4);
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
         int m0, n0;
         const Problem& q = p.pr[locate<NT>(p, tile, m0, n0)];
         const int its = q.ksteps * q.segs, b = i & 1;
-        if (i >= 2 && !grouped::warp_wait(&accempty[b], ((i >> 1) - 1) & 1, abort, p.err)) break;
+        if (i >= 2 && !wait_all(&accempty[b], ((i >> 1) - 1) & 1, abort, p.err)) break;
         tc5::fence_after();
         const uint32_t acc = tb + b * NT;
         if (EPI != GATED && q.a_mn) ok = mma_tile<true, true, NT>(r, its, p.f16, acc, g);
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
         }
       };
       if (hidden && half * 32 < nc) fetch(half * 32);
-      if (!grouped::warp_wait(&accfull[b], (i >> 1) & 1, abort, p.err)) {
+      if (!wait_all(&accfull[b], (i >> 1) & 1, abort, p.err)) {
         if (hidden && half * 32 < nc && lane == 0) mbar_wait_bounded(loaded, loads & 1, 200000000ull);
         break;
       }
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
 #pragma unroll 1
         for (int c = half * 32; c < nc; c += 64) {
           float v[32], gv[32], uv[32];
-          if (!grouped::warp_wait(loaded, loads & 1, abort, p.err)) break;
+          if (!wait_all(loaded, loads & 1, abort, p.err)) break;
           ++loads;
           box_get(box0, lane, gv);
           box_get(box1, lane, uv);

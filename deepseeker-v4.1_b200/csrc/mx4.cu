@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
       int g = 0;
       for (int it = it0; it < it1; ++it, ++g) {
         const int s = g % S;
-        if (g >= S && !grouped::wait_or_abort(&empty[s], ((g / S) - 1) & 1, abort, p.err)) break;
+        if (g >= S && !ds::pair::wait(&empty[s], ((g / S) - 1) & 1, abort, p.err)) break;
         uint8_t* st = smem + s * C::kStage;
         uint8_t* sf = st + C::kOps;
         const int na = min(2, chunks - 2 * it);   // atoms of this stage
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
     const uint64_t ops = tc5::sdesc_sw128(smem_u32(smem));
     for (int g = 0; g < it1 - it0; ++g) {
       const int s = g % S;
-      if (!grouped::warp_wait(&full[s], (g / S) & 1, abort, p.err)) break;
+      if (!ds::pair::wait_all(&full[s], (g / S) & 1, abort, p.err)) break;
       tc5::fence_after();
       if (elect_one()) {
         const int left = p.blocks - 8 * (it0 + g);     // blocks from this stage on
@@ -405,9 +405,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
     // all issued MMAs complete before the accumulators are read or released
     if (elect_one()) tc5::commit(&accfull);
     __syncwarp();
-    grouped::warp_wait(&accfull, 0, abort, p.err);
+    ds::pair::wait_all(&accfull, 0, abort, p.err);
   } else {
-    grouped::warp_wait(&accfull, 0, abort, p.err);
+    ds::pair::wait_all(&accfull, 0, abort, p.err);
   }
   tc5::fence_after();
 

@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
         const int ra = (am >> 7) * chunks, rb = (n0 >> 7) * chunks;   // first atom lines
         for (int it = 0; it < its; ++it, ++g) {
           const int s = g % S;
-          if (g >= S && !grouped::wait_or_abort(&empty[s], ((g / S) - 1) & 1, abort, p.err)) goto drain;
+          if (g >= S && !wait(&empty[s], ((g / S) - 1) & 1, abort, p.err)) goto drain;
           uint8_t* st = smem + s * kStage;
           const uint32_t bar = leader_addr(&full[s]);
           if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kStage);
@@ -212,11 +212,11 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
       const int last = min(4, (p.blocks - 8 * (its - 1) + 1) / 2);   // steps of a tile's last stage
       int g = 0, li = 0;
       for (int tile = first; tile < n_tiles; tile += pairs, ++li) {
-        if (li && !grouped::warp_wait(&accempty, (li - 1) & 1, abort, p.err)) break;
+        if (li && !wait_all(&accempty, (li - 1) & 1, abort, p.err)) break;
         tc5::fence_after();
         for (int it = 0; it < its; ++it, ++g) {
           const int s = g % S;
-          if (!grouped::warp_wait(&full[s], (g / S) & 1, abort, p.err)) goto mma_out;
+          if (!wait_all(&full[s], (g / S) & 1, abort, p.err)) goto mma_out;
           tc5::fence_after();
           if (elect_one()) {
             const uint64_t od = ops + (uint64_t)((s * kStage) >> 4), sd = sf0 + (uint64_t)((s * kStage) >> 4);
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
       int m0, n0;
       locate<GATED>(p, tile, m0, n0);
       const int mw = m0 + 128 * rank + 32 * q, m = mw + lane;
-      if (!grouped::warp_wait(&accfull, li & 1, abort, p.err)) break;
+      if (!wait_all(&accfull, li & 1, abort, p.err)) break;
       tc5::fence_after();
       // linear: columns half * 128 .. + 127; gated: features half * 64 .. + 63, gates first
       float v[4][32];

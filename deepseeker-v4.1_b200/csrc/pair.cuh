@@ -27,6 +27,32 @@ __device__ __forceinline__ void dealloc512(uint32_t base) {
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(base) : "memory");
 }
 
+constexpr uint64_t kWaitNs = 2000000000ull;   // 2 s
+constexpr int kErrTimeout = 2;
+
+// Bounded wait for a phase.  The thread sleeps in try_wait and wakes as the
+// phase completes; the clock and the abort flag are looked at only when that
+// has run out once.  Gives up after kWaitNs or when another role has.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* err) {
+  if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait_sleep(bar, parity, 20000u)) {
+    if (*abort) return false;
+    if (globaltimer_ns() - t0 > kWaitNs) {
+      *abort = 1;
+      atomicOr(err, kErrTimeout);
+      return false;
+    }
+  }
+  return true;
+}
+
+// The same by a whole warp, with one verdict.
+__device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, volatile int* abort, int* err) {
+  return __all_sync(0xffffffffu, wait(bar, parity, abort, err));
+}
+
+// This address in the leader's shared memory.
 __device__ __forceinline__ uint32_t leader_addr(const void* p) {
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
