@@ -10,7 +10,7 @@
 // they are tensor-core operands of the next product (one rounding there adds
 // as much error as the rounding of the result itself).
 //
-// Tile kernel (every product of every size): one CTA computes 128 features
+// Tile kernel (few rows): one CTA computes 128 features
 // (the MMA's lanes) x NT tokens or columns over a slice of the contraction.
 // The slices of one tile are the CTAs of a cluster: they leave their f32
 // partial tiles in shared memory and each adds up a share of the columns
@@ -60,13 +60,15 @@ struct TileShape {
   static constexpr int kA = Md::kMats * 2 * kBoxBytes;
   static constexpr int kB = NT * 128;
   static constexpr int kStage = kA + kB;
-  static constexpr int kStages = std::min(8, 200 * 1024 / kStage);
+  // up to 64 tokens two launches' CTAs fit on an SM, so that the next product's
+  // weights are on their way while this one finishes
+  static constexpr int kStages = std::min(8, (NT == 128 ? 200 : Md::kMats == 2 ? 122 : 100) * 1024 / kStage);
   static constexpr int kSmem = 1024 + kStages * kStage;
   static constexpr int kCols = Md::kMats * NT < 32 ? 32 : Md::kMats * NT;
   static_assert(kStage % 1024 == 0 && kStages * kStage >= Md::kMats * NT * 128 * 4, "stages hold the partial tile");
 };
 
-constexpr int kTileThreads = 192;   // warp 0 copies, warp 1 MMA, warps 2-5 epilogue
+constexpr int kTileThreads = 320;   // warp 0 copies, warp 1 MMA, warps 2-9 epilogue (two a lane quarter)
 
 // What becomes of the elements (m, n0 .. n0 + J - 1) of the accumulator(s), nv
 // of them inside the result.  Lanes are features, so a warp's accesses are
@@ -107,8 +109,38 @@ __device__ __forceinline__ void tile_store(const TileParams& p, int m, int n0, i
   }
 }
 
+// Sums this CTA's share of the columns over the partial tiles [mats][NT][128]
+// of the cluster, in slice order.  The reads of four columns from all slices
+// are in flight together.
+template <int MODE, int NT, int SLICES>
+__device__ __forceinline__ void tile_join(const TileParams& p, float* part, int slice, int turn, int m, int mi) {
+  constexpr int kMats = ModeOf<MODE>::kMats;
+  cg::cluster_group cluster = cg::this_cluster();
+  const float* src[SLICES];
+#pragma unroll
+  for (int r = 0; r < SLICES; ++r) src[r] = cluster.map_shared_rank(part, r) + mi;
+  const int share = (p.N + SLICES - 1) / SLICES, end = min(p.N, (slice + 1) * share);
+  for (int n = slice * share + 4 * turn; n < end; n += 8) {
+    float w[SLICES][kMats][4];
+#pragma unroll
+    for (int r = 0; r < SLICES; ++r)
+#pragma unroll
+      for (int t = 0; t < kMats; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[r][t][j] = src[r][(t * NT + min(n + j, end - 1)) * 128];
+    float v[2][4] = {};
+#pragma unroll
+    for (int r = 0; r < SLICES; ++r)
+#pragma unroll
+      for (int t = 0; t < kMats; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[t][j] += w[r][t][j];
+    tile_store<MODE>(p, m, n, end - n, v[0], v[1]);
+  }
+}
+
 template <int MODE, int NT>
-__global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_constant__ TileParams p) {
+__global__ void __launch_bounds__(kTileThreads, NT == 128 ? 1 : 2) tile_kernel(const __grid_constant__ TileParams p) {
   using Md = ModeOf<MODE>;
   using C = TileShape<MODE, NT>;
   constexpr int S = C::kStages;
@@ -120,7 +152,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
   cg::cluster_group cluster = cg::this_cluster();
   const int slices = cluster.dim_blocks().x, slice = cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int m0 = (blockIdx.x / slices) * 128, n0 = blockIdx.y * NT;
+  const int m0 = (blockIdx.x / slices) * 128;
   const int ksteps = (p.K + kBK - 1) / kBK;
   const int it0 = (int)((int64_t)Md::kSegs * ksteps * slice / slices);
   const int it1 = (int)((int64_t)Md::kSegs * ksteps * (slice + 1) / slices);
@@ -141,20 +173,33 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
   const uint32_t tb = tmem_base;
   volatile int* abort = &abort_flag;
   launch_dependents();
-  wait_prior_grid();
 
   if (warp == 0) {
     if (lane == 0) {
-      int g = 0;
-      for (int it = it0; it < it1; ++it, ++g) {
-        const int s = g % S;
-        if (g >= S && !ds::pair::wait(&empty[s], ((g / S) - 1) & 1, abort, p.err)) break;
-        const int seg = it / ksteps, k0 = (it - seg * ksteps) * kBK;
-        uint8_t* st = smem + s * C::kStage;
-        mbar_arrive_expect_tx(&full[s], C::kStage);
-        load_tile<Md::kAMn, 128>(st, &p.a[seg], m0, k0, &full[s]);
-        if (Md::kMats == 2) load_tile<Md::kAMn, 128>(st + 2 * kBoxBytes, &p.a[1], m0, k0, &full[s]);
-        load_tile<false, NT>(st + C::kA, &p.b[seg], n0, k0, &full[s]);
+      auto weights = [&](int g) {
+        const int it = it0 + g, seg = it / ksteps, k0 = (it - seg * ksteps) * kBK;
+        uint8_t* st = smem + g % S * C::kStage;
+        uint64_t* bar = &full[g % S];
+        mbar_arrive_expect_tx(bar, C::kStage);
+        load_tile<Md::kAMn, 128>(st, &p.a[seg], m0, k0, bar);
+        if (Md::kMats == 2) load_tile<Md::kAMn, 128>(st + 2 * kBoxBytes, &p.a[1], m0, k0, bar);
+      };
+      auto rows = [&](int g) {
+        const int it = it0 + g, seg = it / ksteps, k0 = (it - seg * ksteps) * kBK;
+        load_tile<false, NT>(smem + g % S * C::kStage + C::kA, &p.b[seg], 0, k0, &full[g % S]);
+      };
+      // The weights of the first stages need nothing of the launch before this
+      // one in the stream: that is one of the same call, and the call's first
+      // launch began after all earlier work had ended.
+      const int n = it1 - it0, early = min(S, n);
+      for (int g = 0; g < early; ++g) weights(g);
+      wait_prior_grid();
+      for (int g = 0; g < early; ++g) rows(g);
+      int g = early;
+      for (; g < n; ++g) {
+        if (!ds::pair::wait(&empty[g % S], ((g / S) - 1) & 1, abort, p.err)) break;
+        weights(g);
+        rows(g);
       }
       // never leave with copies in flight into this CTA's shared memory
       for (int j = g - S < 0 ? 0 : g - S; j < g; ++j) mbar_wait_bounded(&full[j % S], (j / S) & 1, 200000000ull);
@@ -189,11 +234,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
   tc5::fence_after();
 
   // ---- epilogue: thread = one feature (lane of tensor memory)
-  const int q = warp & 3, mi = q * 32 + lane, m = m0 + mi;
-  const int nv = min(NT, p.N - n0);
+  wait_prior_grid();
+  const int q = warp & 3, turn = (warp - 2) >> 2, mi = q * 32 + lane, m = m0 + mi;
   float* part = reinterpret_cast<float*>(smem);   // [mats][NT][128]
   if (warp >= 2) {
-    for (int c0 = 0; c0 < nv; c0 += 16) {
+    for (int c0 = 16 * turn; c0 < p.N; c0 += 32) {
       float v[Md::kMats][16];
 #pragma unroll
       for (int t = 0; t < Md::kMats; ++t) tc5::ld_x16_nowait(tc5::lane_quarter(tb + t * NT + c0, q), v[t]);
@@ -204,28 +249,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
 #pragma unroll
           for (int j = 0; j < 16; ++j) part[(t * NT + c0 + j) * 128 + mi] = v[t][j];
       } else if (m < p.M) {
-        tile_store<MODE>(p, m, n0 + c0, nv - c0, v[0], v[Md::kMats - 1]);
+        tile_store<MODE>(p, m, c0, p.N - c0, v[0], v[Md::kMats - 1]);
       }
     }
   }
   if (slices > 1) {
     cluster.sync();
     if (warp >= 2 && m < p.M) {
-      // this CTA's share of the columns, four at a time
-      const int share = (nv + slices - 1) / slices, end = min(nv, (slice + 1) * share);
-      for (int n = slice * share; n < end; n += 4) {
-        float v[2][4] = {};
-        for (int r = 0; r < slices; ++r) {
-          const float* src = cluster.map_shared_rank(part, r) + mi;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (n + j >= end) continue;
-            v[0][j] += src[(n + j) * 128];
-            if (Md::kMats == 2) v[1][j] += src[(NT + n + j) * 128];
-          }
-        }
-        tile_store<MODE>(p, m, n0 + n, end - n, v[0], v[1]);
-      }
+      if (slices == 8) tile_join<MODE, NT, 8>(p, part, slice, turn, m, mi);
+      else if (slices == 4) tile_join<MODE, NT, 4>(p, part, slice, turn, m, mi);
+      else tile_join<MODE, NT, 2>(p, part, slice, turn, m, mi);
     }
     cluster.sync();   // partial tiles stay until every CTA has read them
   }
@@ -300,7 +333,7 @@ int launch_tiles(const TileParams& p, int slices, cudaStream_t s, bool chained) 
   const int st = ds::allow_smem(&once, reinterpret_cast<const void*>(&tile_kernel<MODE, NT>), C::kSmem);
   if (st != DS_OK) return st;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((p.M + 127) / 128 * slices), (unsigned)((p.N + NT - 1) / NT));
+  cfg.gridDim = dim3((unsigned)((p.M + 127) / 128 * slices));
   cfg.blockDim = dim3(kTileThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = s;
@@ -328,7 +361,7 @@ int slices_for(int64_t tiles, int ksteps) {
 
 template <int MODE>
 int run_tiles(const TileParams& p, int nt, cudaStream_t s, bool chained) {
-  const int64_t tiles = (int64_t)((p.M + 127) / 128) * ((p.N + nt - 1) / nt);
+  const int64_t tiles = (p.M + 127) / 128;
   const int slices = slices_for(tiles, ModeOf<MODE>::kSegs * ((p.K + kBK - 1) / kBK));
   if (nt == 16) return launch_tiles<MODE, 16>(p, slices, s, chained);
   if (nt == 32) return launch_tiles<MODE, 32>(p, slices, s, chained);
@@ -338,8 +371,11 @@ int run_tiles(const TileParams& p, int nt, cudaStream_t s, bool chained) {
 
 // ---- pair kernel
 
-// The pair kernel takes the products of at least this many rows; weight
-// gradients always.
+// The pair kernel takes the products of at least this many rows, where its 256
+// are half full (at 96 rows the two are even on 4096 x 2048 and 1024 x 1024,
+// 34 and 16 us, and the tile kernel is ahead on uneven widths and in the
+// backward pass, 51 against 59 us; at 129 it would need a second tile of
+// rows); weight gradients always.
 constexpr int kPairRows = 129;
 
 int64_t tiles_of(const Problem& q, int nt) {

@@ -289,7 +289,9 @@ struct TileShape {
   static constexpr int kOps = kMats * 16384 + NT * 128;              // 256 codes of 128 features and NT rows
   static constexpr int kSf = (kMats + 1) * 2 * kAtom;
   static constexpr int kStage = kOps + (kSf + 1023) / 1024 * 1024;
-  static constexpr int kStages = std::min(6, 200 * 1024 / kStage);
+  // two launches' CTAs fit on an SM, so that the next product's
+  // weights are on their way while this one finishes
+  static constexpr int kStages = std::min(6, (kMats == 2 ? 122 : 100) * 1024 / kStage);
   static constexpr int kSmem = 1024 + kStages * kStage;
   static constexpr int kAcc = kMats * NT;
   static constexpr int kSfCols = (kMats + 1) * 8;
@@ -298,32 +300,85 @@ struct TileShape {
   static_assert(kOps % 1024 == 0 && kStages * kStage >= kMats * NT * 128 * 4, "stages hold the partial tile");
 };
 
-constexpr int kTileThreads = 192;   // warp 0 copies, warp 1 MMA, warps 2-5 epilogue
+constexpr int kTileThreads = 320;   // warp 0 copies, warp 1 MMA, warps 2-9 epilogue (two a lane quarter)
 
-// One element of the tile: row n of x, feature m (lane of a full warp).
-template <int MODE>
-__device__ __forceinline__ void tile_store(const TileParams& p, int m, int n, float v0, float v1) {
+// What becomes of the elements (m, n0 .. n0 + J - 1) of the tile, nv of them
+// inside: rows of x n0.., feature m (lane of a full warp).  The columns go
+// through each step together: a block's maximum, scale and codes are a chain
+// of a few hundred cycles, and one column after the other made the epilogue of
+// 64 rows 15 us long.
+template <int MODE, int J>
+__device__ __forceinline__ void tile_store(const TileParams& p, int m, int n0, int nv, const float (&v0)[J],
+                                           const float (&v1)[J]) {
   if constexpr (MODE == LINEAR) {
     if (m >= p.M) return;
-    const int64_t at = (int64_t)n * p.ldo + m;
-    if (p.out_dtype == DS_F32) static_cast<float*>(p.out)[at] = v0;
-    else if (p.out_dtype == DS_F16) static_cast<__half*>(p.out)[at] = __float2half_rn(v0);
-    else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v0);
+    const int64_t at = (int64_t)n0 * p.ldo + m;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if (j >= nv) continue;
+      if (p.out_dtype == DS_F32) static_cast<float*>(p.out)[at + j * p.ldo] = v0[j];
+      else if (p.out_dtype == DS_F16) static_cast<__half*>(p.out)[at + j * p.ldo] = __float2half_rn(v0[j]);
+      else static_cast<__nv_bfloat16*>(p.out)[at + j * p.ldo] = __float2bfloat16_rn(v0[j]);
+    }
   } else {
-    // lanes past the features hold products with unset scales: no part of the block
-    const float h = m < p.M ? gate_unit(v0, v1, p.limit) : 0.0f;
-    const int s = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7FFFFFFFu));
     const int lane = threadIdx.x & 31, block = m >> 5, blocks = (p.M + 31) / 32, chunks = (blocks + 3) / 4;
-    uint32_t w = s == 255 ? 0u : tc5::f32x2_to_e2m1x2(h * inv_scale(s), 0.0f) & 0xFu;
-    if (w == 8u) w = 0u;
-    w |= __shfl_down_sync(0xffffffffu, w, 1) << 4;
-    if (block < blocks && (lane & 1) == 0) p.hq[((int64_t)n * blocks + block) * 16 + lane / 2] = (uint8_t)w;
-    if (lane == 0) p.hs[atom_at(n, block, chunks)] = (uint8_t)s;
+    float h[J];
+    int s[J];
+    uint32_t w[J];
+    // lanes past the features hold products with unset scales: no part of the block
+#pragma unroll
+    for (int j = 0; j < J; ++j) h[j] = m < p.M ? gate_unit(v0[j], v1[j], p.limit) : 0.0f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) s[j] = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(h[j]) & 0x7FFFFFFFu));
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      w[j] = s[j] == 255 ? 0u : tc5::f32x2_to_e2m1x2(h[j] * inv_scale(s[j]), 0.0f) & 0xFu;
+      if (w[j] == 8u) w[j] = 0u;
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j) w[j] |= __shfl_down_sync(0xffffffffu, w[j], 1) << 4;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if (j >= nv) continue;
+      if (block < blocks && (lane & 1) == 0)
+        p.hq[((int64_t)(n0 + j) * blocks + block) * 16 + lane / 2] = (uint8_t)w[j];
+      if (lane == 0) p.hs[atom_at(n0 + j, block, chunks)] = (uint8_t)s[j];
+    }
+  }
+}
+
+// Sums this CTA's share of the columns over the partial tiles [mats][NT][128]
+// of the cluster, in slice order.  The reads of four columns from all slices
+// are in flight together.
+template <int MODE, int NT, int SLICES>
+__device__ __forceinline__ void tile_join(const TileParams& p, float* part, int slice, int turn, int m, int mi) {
+  constexpr int kMats = TileShape<MODE, NT>::kMats;
+  cg::cluster_group cluster = cg::this_cluster();
+  const float* src[SLICES];
+#pragma unroll
+  for (int r = 0; r < SLICES; ++r) src[r] = cluster.map_shared_rank(part, r) + mi;
+  const int share = (p.N + SLICES - 1) / SLICES, end = min(p.N, (slice + 1) * share);
+  for (int n = slice * share + 4 * turn; n < end; n += 8) {
+    float w[SLICES][kMats][4];
+#pragma unroll
+    for (int r = 0; r < SLICES; ++r)
+#pragma unroll
+      for (int t = 0; t < kMats; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[r][t][j] = src[r][(t * NT + min(n + j, end - 1)) * 128];
+    float v[2][4] = {};
+#pragma unroll
+    for (int r = 0; r < SLICES; ++r)
+#pragma unroll
+      for (int t = 0; t < kMats; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[t][j] += w[r][t][j];
+    tile_store<MODE>(p, m, n, end - n, v[0], v[kMats - 1]);
   }
 }
 
 template <int MODE, int NT>
-__global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_constant__ TileParams p) {
+__global__ void __launch_bounds__(kTileThreads, 2) tile_kernel(const __grid_constant__ TileParams p) {
   using C = TileShape<MODE, NT>;
   constexpr int S = C::kStages, kMats = C::kMats;
   extern __shared__ uint8_t smem_raw[];
@@ -334,7 +389,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
   cg::cluster_group cluster = cg::this_cluster();
   const int slices = cluster.dim_blocks().x, slice = cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int mt = blockIdx.x / slices, m0 = mt * 128, n0 = blockIdx.y * NT;
+  const int mt = blockIdx.x / slices, m0 = mt * 128;
   const int chunks = (p.blocks + 3) / 4, ksteps = (chunks + 1) / 2;   // a stage is two chunks of 128 codes
   const int it0 = (int)((int64_t)ksteps * slice / slices), it1 = (int)((int64_t)ksteps * (slice + 1) / slices);
 
@@ -354,25 +409,38 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
   const uint32_t tb = tmem_base;
   volatile int* abort = &abort_flag;
   launch_dependents();
-  wait_prior_grid();
 
   if (warp == 0) {
     if (lane == 0) {
-      int g = 0;
-      for (int it = it0; it < it1; ++it, ++g) {
-        const int s = g % S;
-        if (g >= S && !ds::pair::wait(&empty[s], ((g / S) - 1) & 1, abort, p.err)) break;
-        uint8_t* st = smem + s * C::kStage;
-        uint8_t* sf = st + C::kOps;
-        const int na = min(2, chunks - 2 * it);   // atoms of this stage
-        mbar_arrive_expect_tx(&full[s], C::kOps + (kMats + 1) * na * kAtom);
+      auto weights = [&](int g) {
+        const int it = it0 + g, na = min(2, chunks - 2 * it);   // atoms of this stage
+        uint8_t* st = smem + g % S * C::kStage;
+        uint64_t* bar = &full[g % S];
+        mbar_arrive_expect_tx(bar, C::kOps + (kMats + 1) * na * kAtom);
 #pragma unroll
         for (int t = 0; t < kMats; ++t) {
-          tma_load_2d(st + t * 16384, &p.a[t], it * 128, m0, &full[s]);
-          bulk_g2s(sf + t * 2 * kAtom, p.sa[t] + ((int64_t)mt * chunks + 2 * it) * kAtom, na * kAtom, &full[s]);
+          tma_load_2d(st + t * 16384, &p.a[t], it * 128, m0, bar);
+          bulk_g2s(st + C::kOps + t * 2 * kAtom, p.sa[t] + ((int64_t)mt * chunks + 2 * it) * kAtom, na * kAtom, bar);
         }
-        tma_load_2d(st + kMats * 16384, &p.b, it * 128, n0, &full[s]);
-        bulk_g2s(sf + kMats * 2 * kAtom, p.sb + ((int64_t)(n0 >> 7) * chunks + 2 * it) * kAtom, na * kAtom, &full[s]);
+      };
+      auto rows = [&](int g) {
+        const int it = it0 + g, na = min(2, chunks - 2 * it);
+        uint8_t* st = smem + g % S * C::kStage;
+        tma_load_2d(st + kMats * 16384, &p.b, it * 128, 0, &full[g % S]);
+        bulk_g2s(st + C::kOps + kMats * 2 * kAtom, p.sb + (int64_t)(2 * it) * kAtom, na * kAtom, &full[g % S]);
+      };
+      // The weights of the first stages need nothing of the launch before this
+      // one in the stream: that is one of the same call, and the call's first
+      // launch began after all earlier work had ended.
+      const int n = it1 - it0, early = min(S, n);
+      for (int g = 0; g < early; ++g) weights(g);
+      wait_prior_grid();
+      for (int g = 0; g < early; ++g) rows(g);
+      int g = early;
+      for (; g < n; ++g) {
+        if (!ds::pair::wait(&empty[g % S], ((g / S) - 1) & 1, abort, p.err)) break;
+        weights(g);
+        rows(g);
       }
       // never leave with copies in flight into this CTA's shared memory
       for (int j = g - S < 0 ? 0 : g - S; j < g; ++j) mbar_wait_bounded(&full[j % S], (j / S) & 1, 200000000ull);
@@ -412,11 +480,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
   tc5::fence_after();
 
   // ---- epilogue: thread = one feature (lane of tensor memory)
-  const int q = warp & 3, mi = q * 32 + lane, m = m0 + mi;
-  const int nv = min(NT, p.N - n0);
+  wait_prior_grid();
+  const int q = warp & 3, turn = (warp - 2) >> 2, mi = q * 32 + lane, m = m0 + mi;
   float* part = reinterpret_cast<float*>(smem);   // [mats][NT][128]
   if (warp >= 2) {
-    for (int c0 = 0; c0 < nv; c0 += 16) {
+    for (int c0 = 16 * turn; c0 < p.N; c0 += 32) {
       float v[kMats][16];
 #pragma unroll
       for (int t = 0; t < kMats; ++t) tc5::ld_x16_nowait(tc5::lane_quarter(tb + t * NT + c0, q), v[t]);
@@ -427,24 +495,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
 #pragma unroll
           for (int j = 0; j < 16; ++j) part[(t * NT + c0 + j) * 128 + mi] = v[t][j];
       } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (c0 + j < nv) tile_store<MODE>(p, m, n0 + c0 + j, v[0][j], v[kMats - 1][j]);
+        tile_store<MODE>(p, m, c0, p.N - c0, v[0], v[kMats - 1]);
       }
     }
   }
   if (slices > 1) {
     cluster.sync();
     if (warp >= 2) {
-      for (int n = slice; n < nv; n += slices) {
-        float v0 = 0.0f, v1 = 0.0f;
-        for (int r = 0; r < slices; ++r) {
-          const float* src = cluster.map_shared_rank(part, r);
-          v0 += src[n * 128 + mi];
-          if (kMats == 2) v1 += src[(NT + n) * 128 + mi];
-        }
-        tile_store<MODE>(p, m, n0 + n, v0, v1);
-      }
+      if (slices == 8) tile_join<MODE, NT, 8>(p, part, slice, turn, m, mi);
+      else if (slices == 4) tile_join<MODE, NT, 4>(p, part, slice, turn, m, mi);
+      else tile_join<MODE, NT, 2>(p, part, slice, turn, m, mi);
     }
     cluster.sync();   // partial tiles stay until every CTA has read them
   }
@@ -518,7 +578,7 @@ int launch_tiles(const TileParams& p, int slices, cudaStream_t s, bool chained) 
   const int st = ds::allow_smem(&once, reinterpret_cast<const void*>(&tile_kernel<MODE, NT>), C::kSmem);
   if (st != DS_OK) return st;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((p.M + 127) / 128 * slices), (unsigned)((p.N + NT - 1) / NT));
+  cfg.gridDim = dim3((unsigned)((p.M + 127) / 128 * slices));
   cfg.blockDim = dim3(kTileThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = s;
@@ -534,25 +594,27 @@ int launch_tiles(const TileParams& p, int slices, cudaStream_t s, bool chained) 
   return DS_OK;
 }
 
-// Rows of x per tile (a single tile below 128, so a tile starts at row 0 of a scale atom).
-int row_tile(int64_t n) { return n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 128; }
+// Rows of x per tile: all of them (at most 64), so a tile starts at row 0 of a scale atom.
+int row_tile(int64_t n) { return n <= 16 ? 16 : n <= 32 ? 32 : 64; }
 
 template <int MODE>
 int run_tiles(const TileParams& p, int nt, cudaStream_t s, bool chained) {
-  const int64_t tiles = (int64_t)((p.M + 127) / 128) * ((p.N + nt - 1) / nt);
+  const int64_t tiles = (p.M + 127) / 128;
   const int ksteps = (p.blocks + 7) / 8;
   int slices = 1;   // enough to give every SM a CTA, at least two stages each
   while (slices < 8 && tiles * slices * 2 <= ds::sm_count() && ksteps / (slices * 2) >= 2) slices *= 2;
   if (nt == 16) return launch_tiles<MODE, 16>(p, slices, s, chained);
   if (nt == 32) return launch_tiles<MODE, 32>(p, slices, s, chained);
-  if (nt == 64) return launch_tiles<MODE, 64>(p, slices, s, chained);
-  return launch_tiles<MODE, 128>(p, slices, s, chained);
+  return launch_tiles<MODE, 64>(p, slices, s, chained);
 }
 
 // ---- pair kernel
 
-// The pair kernel takes products of at least this many rows of x.
-constexpr int kPairRows = 129;
+// The pair kernel takes products of at least this many rows of x: at 64 the
+// tile kernel is ahead (gated block of 4096 x 2048: 15.9 against 21.9 us, of
+// 1024 x 1024 15.1 against 16.9), at 96 behind (25.5 against 22.1, 18.7 against
+// 17.1).
+constexpr int kPairRows = 65;
 
 // Scale atoms as lines of 512 bytes (128 words); a box is two lines.
 bool map_atoms(CUtensorMap* m, const void* base, int64_t rows, int64_t cols) {
