@@ -45,6 +45,7 @@ int allow_smem(SmemOnce* done, const void* kernel, size_t bytes) {
   const int dev = current_device();
   if (dev >= 0 && __atomic_load_n(&done->set[dev], __ATOMIC_ACQUIRE)) return DS_OK;
   DS_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  DS_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
   if (dev >= 0) __atomic_store_n(&done->set[dev], 1, __ATOMIC_RELEASE);
   return DS_OK;
 }

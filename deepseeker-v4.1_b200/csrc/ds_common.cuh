@@ -30,7 +30,9 @@ int sm_count();
 // Current device, 0 .. 63, or -1.
 int current_device();
 
-// Allows `kernel` `bytes` of dynamic shared memory on the current device.
+// Allows `kernel` `bytes` of dynamic shared memory on the current device, and
+// asks for the largest shared-memory share of the SM: with the share that one
+// kernel alone would get, the next launch's CTAs cannot join it on its SMs.
 // `done`: the kernel's own zero-initialised flags, so that a call after the
 // first on a device costs a load.
 struct SmemOnce {

@@ -60,9 +60,11 @@ struct TileShape {
   static constexpr int kA = Md::kMats * 2 * kBoxBytes;
   static constexpr int kB = NT * 128;
   static constexpr int kStage = kA + kB;
-  // up to 64 tokens two launches' CTAs fit on an SM, so that the next product's
-  // weights are on their way while this one finishes
-  static constexpr int kStages = std::min(8, (NT == 128 ? 200 : Md::kMats == 2 ? 122 : 100) * 1024 / kStage);
+  // up to 64 tokens a CTA takes less than half of an SM, so that the next
+  // launch's CTAs join it and their weights are on their way while this one
+  // finishes (one token of 4096 x 2048: 17.3 us, 23 with 200 KB each; above
+  // half they do not join whatever the other launch takes)
+  static constexpr int kStages = std::min(8, (NT == 128 ? 200 : 111) * 1024 / kStage);
   static constexpr int kSmem = 1024 + kStages * kStage;
   static constexpr int kCols = Md::kMats * NT < 32 ? 32 : Md::kMats * NT;
   static_assert(kStage % 1024 == 0 && kStages * kStage >= Md::kMats * NT * 128 * 4, "stages hold the partial tile");

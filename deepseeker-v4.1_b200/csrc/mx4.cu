@@ -289,9 +289,9 @@ struct TileShape {
   static constexpr int kOps = kMats * 16384 + NT * 128;              // 256 codes of 128 features and NT rows
   static constexpr int kSf = (kMats + 1) * 2 * kAtom;
   static constexpr int kStage = kOps + (kSf + 1023) / 1024 * 1024;
-  // two launches' CTAs fit on an SM, so that the next product's
-  // weights are on their way while this one finishes
-  static constexpr int kStages = std::min(6, (kMats == 2 ? 122 : 100) * 1024 / kStage);
+  // less than half of an SM, so that the next launch's CTAs join this one's and
+  // their weights are on their way while it finishes
+  static constexpr int kStages = std::min(6, 111 * 1024 / kStage);
   static constexpr int kSmem = 1024 + kStages * kStage;
   static constexpr int kAcc = kMats * NT;
   static constexpr int kSfCols = (kMats + 1) * 8;
