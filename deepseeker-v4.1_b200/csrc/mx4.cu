@@ -640,7 +640,7 @@ int run_pairs(const PairParams& p, cudaStream_t s, bool chained) {
   if (st != DS_OK) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, ds::sm_count() / 2)));
-  cfg.blockDim = dim3(pairs::kThreads);
+  cfg.blockDim = dim3(pairs::Shape<GATED>::kThreads);
   cfg.dynamicSmemBytes = pairs::Shape<GATED>::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute at[1];

@@ -45,14 +45,16 @@ using namespace ds::pair;
 constexpr int kOps = 32768;                       // 128 rows of x and of W, 128 bytes each
 constexpr int kSf = 6 * kAtom;                    // x: two atoms along k; W: 2 x two
 constexpr int kStage = kOps + kSf;                // 35 KB
-constexpr int kEpiWarps = 8;
-constexpr int kThreads = 32 * (2 + kEpiWarps);
 constexpr int kSfCols = 24;
 
 // As many stages as fit beside a result box per epilogue warp (the gated
-// product stores h from registers).
+// product stores h from registers).  The gated epilogue's arithmetic is as
+// long as a tile's 16 stages, so it gets sixteen warps (with eight the block
+// over 16384 x 4096 x 2048 took 128 us in this launch).
 template <bool GATED>
 struct Shape {
+  static constexpr int kEpiWarps = GATED ? 16 : 8;
+  static constexpr int kThreads = 32 * (2 + kEpiWarps);
   static constexpr int kStages = GATED ? 6 : 5;
   static constexpr int kSmem = 1024 + kStages * kStage + (GATED ? 0 : kEpiWarps * kBox);
   static_assert(kStage % 1024 == 0 && kSmem <= 226 * 1024, "shared memory of an SM");
@@ -143,7 +145,8 @@ __device__ __forceinline__ uint4 quantize_block(const float* h, int& s) {
 }
 
 template <bool GATED>
-__global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_kernel(const __grid_constant__ PairParams p) {
+__global__ void __launch_bounds__(Shape<GATED>::kThreads, 1) __cluster_dims__(2, 1, 1)
+    pair_kernel(const __grid_constant__ PairParams p) {
   constexpr int S = Shape<GATED>::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -162,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
       mbar_init(&empty[s], 1);
     }
     mbar_init(&accfull, 1);
-    mbar_init(&accempty, 2 * kEpiWarps);
+    mbar_init(&accempty, 2 * Shape<GATED>::kEpiWarps);
     abort_flag = 0;
     fence_barrier_init();
   }
@@ -236,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
     }
   } else {
     // ------------------------------------------------------------ epilogue
-    const int q = warp & 3, half = (warp - 2) >> 2;
+    const int q = warp & 3, part = (warp - 2) >> 2;
     uint8_t* box = smem + S * kStage + (warp - 2) * kBox;
     const uint32_t bar = leader_addr(&accempty), acc = tc5::lane_quarter(tb, q);
     int li = 0;
@@ -246,44 +249,37 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
       const int mw = m0 + 128 * rank + 32 * q, m = mw + lane;
       if (!wait_all(&accfull, li & 1, abort, p.err)) break;
       tc5::fence_after();
-      // linear: columns half * 128 .. + 127; gated: features half * 64 .. + 63, gates first
-      float v[4][32];
+      // linear: columns part * 128 .. + 127; gated: features part * 32 .. + 31, gate and up
+      float v[GATED ? 2 : 4][32];
       if (GATED) {
-        ld_x32(acc + half * 64, v[0]);
-        ld_x32(acc + half * 64 + 32, v[1]);
-        ld_x32(acc + 128 + half * 64, v[2]);
-        ld_x32(acc + 128 + half * 64 + 32, v[3]);
+        ld_x32(acc + part * 32, v[0]);
+        ld_x32(acc + 128 + part * 32, v[1]);
       } else {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) ld_x32(acc + half * 128 + 32 * c, v[c]);
+        for (int c = 0; c < 4; ++c) ld_x32(acc + part * 128 + 32 * c, v[c]);
       }
       tc5::wait_ld();
       tc5::fence_before();
       __syncwarp();
       if (lane == 0) arrive_leader(bar);
 
-      if (GATED) {
-        const int blocks = (p.N + 31) / 32, hchunks = (blocks + 3) / 4;
-        const int b0 = (n0 + half * 64) >> 5;
+      if constexpr (GATED) {
+        const int blocks = (p.N + 31) / 32, hchunks = (blocks + 3) / 4, b = (n0 >> 5) + part, left = p.N - b * 32;
+        // features past the result read unset scales: no part of the block
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          // features past the result read unset scales: no part of the block
-          const int left = p.N - (b0 + c) * 32;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[c][j] = j < left ? gate_unit(v[c][j], v[2 + c][j], p.limit) : 0.0f;
-          int s;
-          const uint4 codes = quantize_block(v[c], s);
-          if (m < p.M) {
-            if (b0 + c < blocks) *reinterpret_cast<uint4*>(p.hq + ((int64_t)m * blocks + b0 + c) * 16) = codes;
-            if (b0 + c < hchunks * 4) p.hs[atom_at(m, b0 + c, hchunks)] = (uint8_t)s;
-          }
+        for (int j = 0; j < 32; ++j) v[0][j] = j < left ? gate_unit(v[0][j], v[1][j], p.limit) : 0.0f;
+        int s;
+        const uint4 codes = quantize_block(v[0], s);
+        if (m < p.M) {
+          if (b < blocks) *reinterpret_cast<uint4*>(p.hq + ((int64_t)m * blocks + b) * 16) = codes;
+          p.hs[atom_at(m, b, hchunks)] = (uint8_t)s;   // a tile is a chunk of four blocks
         }
       } else if (p.boxed) {
         const int per = p.out_dtype == DS_F32 ? 32 : 64;   // columns of a box
         const bool f16 = p.out_dtype == DS_F16;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const int n = n0 + half * 128 + 32 * c;
+          const int n = n0 + part * 128 + 32 * c;
           if (mw >= p.M || n >= p.N) continue;
           const bool opens = per == 32 || (c & 1) == 0, closes = per == 32 || (c & 1) || n + 32 >= p.N;
           if (opens) {
@@ -311,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
       } else if (m < p.M) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const int n = n0 + half * 128 + 32 * c;
+          const int n = n0 + part * 128 + 32 * c;
           store_some(p, (int64_t)m * p.ldy + n, v[c], p.N - n);
         }
       }
