@@ -19,7 +19,7 @@
 // 16-wide MMA and the weights stream once.
 #include <algorithm>
 #include <cooperative_groups.h>
-#include <string.h>
+#include <initializer_list>
 
 #include "gated_pair.cuh"
 
@@ -274,20 +274,29 @@ __global__ void __launch_bounds__(kTileThreads, NT == 128 ? 1 : 2) tile_kernel(c
 
 // ---------------------------------------------------------------- operand copies
 
-// Copies a strided 16-bit matrix into rows of ldd (a multiple of 8) elements,
+// Copies strided 16-bit matrices into rows of ldd (a multiple of 8) elements,
 // zeros behind the columns: the form that the tensor maps need of an operand
-// whose base or row stride is no multiple of 16 bytes.
-__global__ void __launch_bounds__(256) pack_kernel(const uint16_t* __restrict__ src, int64_t rows, int cols,
-                                                   int64_t lds, uint16_t* __restrict__ dst, int ldd) {
-  const int64_t n = rows * (ldd / 8);
+// whose base or row stride is no multiple of 16 bytes.  All operands of a call
+// in one launch (blockIdx.y).
+struct PackParams {
+  const uint16_t* src[5];
+  uint16_t* dst[5];
+  int64_t rows[5], lds[5];
+  int cols[5];
+};
+
+__global__ void __launch_bounds__(256) pack_kernel(const PackParams p) {
+  const int z = blockIdx.y, cols = p.cols[z], ldd = (cols + 7) / 8 * 8;
+  const int64_t lds = p.lds[z], n = p.rows[z] * (ldd / 8);
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / (ldd / 8);
     const int c = (int)(i - r * (ldd / 8)) * 8;
+    const uint16_t* src = p.src[z] + r * lds + c;
     uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (c + j < cols) w[j >> 1] |= (uint32_t)src[r * lds + c + j] << (16 * (j & 1));
-    *reinterpret_cast<uint4*>(dst + r * ldd + c) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (c + j < cols) w[j >> 1] |= (uint32_t)src[j] << (16 * (j & 1));
+    *reinterpret_cast<uint4*>(p.dst[z] + r * ldd + c) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -307,19 +316,27 @@ size_t copy_bytes(const Operand& o) {
   return direct(o.p, o.ld) ? 0 : grouped::up((size_t)o.rows * up8(o.cols) * 2, 256);
 }
 
-// Replaces the operand by its packed copy in the workspace where it needs one.
-int place(Operand& o, char*& ws, cudaStream_t s) {
-  const size_t bytes = copy_bytes(o);
-  if (bytes == 0) return DS_OK;
-  const int ldd = (int)up8(o.cols);
-  const int64_t work = o.rows * (ldd / 8);
-  const int grid = (int)std::min<int64_t>((work + 255) / 256, (int64_t)ds::sm_count() * 16);
-  pack_kernel<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(o.p), o.rows, (int)o.cols, o.ld,
-                                   reinterpret_cast<uint16_t*>(ws), ldd);
+// Replaces the operands that need one by their packed copies in the workspace.
+int place(std::initializer_list<Operand*> operands, char*& ws, cudaStream_t s) {
+  PackParams p = {};
+  int n = 0;
+  int64_t most = 0;
+  for (Operand* o : operands) {
+    const size_t bytes = copy_bytes(*o);
+    if (bytes == 0) continue;
+    p.src[n] = static_cast<const uint16_t*>(o->p);
+    p.dst[n] = reinterpret_cast<uint16_t*>(ws);
+    p.rows[n] = o->rows, p.lds[n] = o->ld, p.cols[n] = (int)o->cols;
+    most = std::max<int64_t>(most, o->rows * (up8(o->cols) / 8));
+    o->p = ws;
+    o->ld = up8(o->cols);
+    ws += bytes;
+    ++n;
+  }
+  if (n == 0) return DS_OK;
+  const int grid = (int)std::min<int64_t>((most + 255) / 256, (int64_t)ds::sm_count() * 16);
+  pack_kernel<<<dim3(grid, n), 256, 0, s>>>(p);
   DS_CHECK_LAUNCH("pack_kernel");
-  o.p = ws;
-  o.ld = ldd;
-  ws += bytes;
   return DS_OK;
 }
 
@@ -538,8 +555,7 @@ extern "C" int ds_gated_ffn(const DsGatedFfn* desc, void* y, void* h, float* pre
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
   Parts o = parts_of(desc);
-  for (Operand* q : {&o.x, &o.w1, &o.w3, &o.w2})
-    if ((st = place(*q, ws, s)) != DS_OK) return st;
+  if ((st = place({&o.x, &o.w1, &o.w3, &o.w2}, ws, s)) != DS_OK) return st;
   if (!h) h = ws;
   const int64_t ldm = up8(I);
   int* err = err_word();
@@ -611,8 +627,7 @@ extern "C" int ds_gated_ffn_backward(const DsGatedFfn* desc, const void* h, cons
   char* ws = static_cast<char*>(workspace);
   Parts o = parts_of(desc);
   Operand gy = {dy, T, H, ld_dy};
-  for (Operand* q : {&o.x, &o.w1, &o.w3, &o.w2, &gy})
-    if ((st = place(*q, ws, s)) != DS_OK) return st;
+  if ((st = place({&o.x, &o.w1, &o.w3, &o.w2, &gy}, ws, s)) != DS_OK) return st;
   const int64_t ldm = up8(I);
   void* dg = ws;
   void* du = ws + mid_bytes(desc);

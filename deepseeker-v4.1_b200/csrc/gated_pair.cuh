@@ -94,9 +94,9 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
       : "memory");
 }
 
-// 32 columns of one row, n of them inside the result; vec: 16-byte stores.
-__device__ __forceinline__ void store16(uint16_t* dst, const float (&v)[32], int n, bool vec, int f16) {
-  if (vec && n >= 32) {
+// 32 columns of one row, n of them inside the result; rows start on 16 bytes.
+__device__ __forceinline__ void store16(uint16_t* dst, const float (&v)[32], int n, int f16) {
+  if (n >= 32) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       uint32_t w[4];
@@ -295,7 +295,6 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
       // the two warps of a lane quarter take turns at the columns inside the result
       const int nc = mw < q.M ? min(tile_cols(EPI, NT), q.N - n0) : 0;
       uint16_t* out = static_cast<uint16_t*>(q.c[0]) + (int64_t)m * q.ldc;
-      const bool vec = ((reinterpret_cast<uintptr_t>(q.c[0]) | (uintptr_t)(q.ldc * 2)) & 15) == 0;
       // the pre-activations of 32 columns come in while the accumulator of
       // the previous ones (or the MMAs) are still at work
       auto fetch = [&](int c) {
@@ -334,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
           }
 #pragma unroll
           for (int j = 0; j < 32; ++j) gv[j] = gate_unit(gv[j], uv[j], p.limit);
-          if (row) store16(out + n0 + c, gv, nc - c, vec, p.f16);
+          if (row) store16(out + n0 + c, gv, nc - c, p.f16);
         }
       } else if (hidden) {
         uint16_t* out1 = static_cast<uint16_t*>(q.c[1]) + (int64_t)m * q.ldc;
@@ -356,8 +355,8 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
 #pragma unroll
           for (int j = 0; j < 32; ++j) gate_grad(gv[j], uv[j], v[j], p.limit, gv[j], uv[j]);
           if (row) {
-            store16(out + n0 + c, gv, nc - c, vec, p.f16);
-            store16(out1 + n0 + c, uv, nc - c, vec, p.f16);
+            store16(out + n0 + c, gv, nc - c, p.f16);
+            store16(out1 + n0 + c, uv, nc - c, p.f16);
           }
         }
       } else if (q.boxed) {
@@ -385,17 +384,24 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
           }
         }
       } else {
+        if (lane == 0) box_wait_read<0>();   // a boxed result may still leave from here
 #pragma unroll 1
         for (int c = half * 32; c < nc; c += 64) {
           float v[32];
           __syncwarp();
           ld_x32(acc + c, v);
           tc5::wait_ld();
-          if (row) store16(out + n0 + c, v, nc - c, false, p.f16);
+          by_rows(box0, lane, v, [&](int r, float y) {
+            if (mw + r < q.M && c + lane < nc)
+              static_cast<uint16_t*>(q.c[0])[(int64_t)(mw + r) * q.ldc + n0 + c + lane] = to16(y, p.f16);
+          });
         }
       }
       // the boxes are free again before a later tile's loads overwrite them
-      if (EPI == HIDDEN && !hidden && lane == 0) box_wait_read<0>();
+      if (EPI == HIDDEN && !hidden) {
+        if (lane == 0) box_wait_read<0>();
+        fence_proxy_async_smem();
+      }
       tc5::fence_before();
       __syncwarp();
       if (lane == 0) arrive_leader(leader_addr(&accempty[b]));

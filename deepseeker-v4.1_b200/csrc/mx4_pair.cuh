@@ -105,18 +105,6 @@ __device__ __forceinline__ void locate(const PairParams& p, int tile, int& m0, i
   m0 = (16 * band + in % rows) * 256;
 }
 
-// 32 columns of a row as f32 or 16 bits, n of them inside: the way out where
-// rows do not start on 16 bytes.
-__device__ __forceinline__ void store_some(const PairParams& p, int64_t at, const float* v, int n) {
-#pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    if (j >= n) continue;
-    if (p.out_dtype == DS_F32) static_cast<float*>(p.y)[at + j] = v[j];
-    else if (p.out_dtype == DS_F16) static_cast<__half*>(p.y)[at + j] = __float2half_rn(v[j]);
-    else static_cast<__nv_bfloat16*>(p.y)[at + j] = __float2bfloat16_rn(v[j]);
-  }
-}
-
 __device__ __forceinline__ uint32_t pack16(float lo, float hi, bool f16) {
   if (f16) {
     const __half2 h = __floats2half2_rn(lo, hi);
@@ -304,11 +292,18 @@ __global__ void __launch_bounds__(Shape<GATED>::kThreads, 1) __cluster_dims__(2,
             }
           }
         }
-      } else if (m < p.M) {
+      } else {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const int n = n0 + part * 128 + 32 * c;
-          store_some(p, (int64_t)m * p.ldy + n, v[c], p.N - n);
+          if (mw >= p.M || n >= p.N) continue;
+          by_rows(box, lane, v[c], [&](int r, float y) {
+            if (mw + r >= p.M || n + lane >= p.N) return;
+            const int64_t at = (int64_t)(mw + r) * p.ldy + n + lane;
+            if (p.out_dtype == DS_F32) static_cast<float*>(p.y)[at] = y;
+            else if (p.out_dtype == DS_F16) static_cast<__half*>(p.y)[at] = __float2half_rn(y);
+            else static_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(y);
+          });
         }
       }
       __syncwarp();

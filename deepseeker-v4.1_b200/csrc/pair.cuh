@@ -121,6 +121,20 @@ __device__ __forceinline__ void box_get(uint8_t* box, int lane, float (&v)[32]) 
   }
 }
 
+// 32 f32 columns of 32 rows (lane = row) handed out row by row, lane = column:
+// single stores of any width then fall on neighbouring addresses.  A thread's
+// own stores along its row made a result whose rows do not start on 16 bytes
+// six times slower.  The box must not be in use.
+template <typename Store>
+__device__ __forceinline__ void by_rows(uint8_t* box, int lane, const float (&v)[32], Store store) {
+  __syncwarp();
+  box_put(box, lane, v);
+  __syncwarp();
+#pragma unroll 8
+  for (int r = 0; r < 32; ++r)
+    store(r, *reinterpret_cast<const float*>(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4));
+}
+
 // One thread: the box goes to columns x.., rows y.. (clipped to the matrix).
 __device__ __forceinline__ void box_store(const CUtensorMap* map, int x, int y, const uint8_t* box) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x),

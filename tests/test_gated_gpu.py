@@ -102,6 +102,7 @@ def test_block_and_gradients(T, H, I, dtype, cuda):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("T,H,I", [(2048, 4096, 2048), (777, 2560, 1288), (3000, 1001, 1003), (5001, 640, 1000),
+                                   (2500, 1024, 1003), (2500, 1003, 1024),
                                    (16384, 256, 264)])
 def test_large(T, H, I, dtype, cuda):
     ins, dy = make(T, H, I, dtype, cuda, seed=5, scale=0.25 if dtype == torch.float16 else 1.0)
