@@ -100,7 +100,8 @@ def quantize(x: torch.Tensor) -> MX4Tensor:
 def from_packed(packed: torch.Tensor, scales: torch.Tensor, cols: int | None = None) -> MX4Tensor:
     """MX4Tensor over stored codes u8 [rows, 16 ceil(cols/32)] and scales u8
     [rows, ceil(cols/32)] (used in place where contiguous; the scale atoms are
-    built once here).  ``cols`` defaults to 32 per scale."""
+    built once here, so scales that change later need a new MX4Tensor).
+    ``cols`` defaults to 32 per scale."""
     for name, t in (("packed", packed), ("scales", scales)):
         if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.uint8 or t.dim() != 2:
             raise ValueError(f"{name} must be a 2-D u8 CUDA tensor")

@@ -196,6 +196,17 @@ def test_shared_and_frozen_weights(cuda):
     assert float((g.double() - gw).norm()) <= 4 * HALF_UNIT[torch.bfloat16] * float(gw.norm())
 
 
+def test_broadcast_gradient_and_accumulation(cuda):
+    """A loss that sums y hands down an expanded gradient; a second backward pass adds to .grad."""
+    ins, _ = make(33, 72, 40, torch.bfloat16, cuda)
+    a = [t.detach().requires_grad_() for t in ins]
+    want = both(ins, torch.ones(33, 72, dtype=torch.bfloat16, device=cuda), 2.0)[0]
+    gated.gated_ffn(a[0].view(3, 11, 72), *a[1:], limit=2.0).sum().backward()
+    assert all(torch.equal(t.grad, w) for t, w in zip(a, want[1:]))
+    gated.gated_ffn(*a, limit=2.0).sum().backward()
+    assert all(torch.equal(t.grad, w + w) for t, w in zip(a, want[1:]))
+
+
 def test_second_derivatives_are_refused(cuda):
     ins, dy = make(6, 64, 32, torch.bfloat16, cuda)
     a = [t.detach().requires_grad_() for t in ins]
