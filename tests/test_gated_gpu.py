@@ -267,6 +267,41 @@ def test_in_a_graph(cuda):
     assert torch.equal(out, want)
 
 
+def test_training_step_in_a_graph(cuda):
+    for T in (20, 300):
+        ins, dy = make(T, 256, 136, torch.bfloat16, cuda)
+        want = both(ins, dy, 1.0)[0]
+        a = [t.detach().requires_grad_() for t in ins]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):                                # autograd runs once outside the capture
+            torch.autograd.grad(gated.gated_ffn(*a, limit=1.0), a, dy)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = gated.gated_ffn(*a, limit=1.0)
+            out = [y.detach(), *torch.autograd.grad(y, a, dy)]
+        for o in out:
+            o.zero_()
+        graph.replay()
+        assert all(torch.equal(o, w) for o, w in zip(out, want))
+
+
+def test_two_streams_at_once(cuda):
+    cases = [make(T, 512, 264, torch.bfloat16, cuda, seed=T) for T in (7, 700)]
+    want = [both(ins, dy, None)[0] for ins, dy in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(both(*cases[i], None)[0])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for i in (0, 1) for g in got[i] for a, b in zip(g, want[i]))
+
+
 def test_refusals(cuda):
     (x, w1, w3, w2), _ = make(4, 64, 32, torch.bfloat16, cuda)
     bad = [(x.float(), w1, w3, w2), (x.cpu(), w1, w3, w2), (x, w1.half(), w3, w2), (x, w1, w3[:31], w2),
