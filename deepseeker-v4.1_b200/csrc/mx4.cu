@@ -272,6 +272,9 @@ struct TileParams {
   CUtensorMap a[2], b;         // weights (gated: W1, W3), rows of x
   const uint8_t* sa[2];        // their scale atoms
   const uint8_t* sb;
+  const void* x;               // rows of x that the kernel quantises itself (b and sb unused then)
+  int64_t ldx;
+  int cols, vec;               // vec: every 16 values start on 16 bytes
   int M, N;                    // features, rows of x
   int blocks;                  // blocks of 32 along the contraction
   void* out;                   // LINEAR: out[n * ldo + m]
@@ -377,10 +380,36 @@ __device__ __forceinline__ void tile_join(const TileParams& p, float* part, int 
   }
 }
 
-template <int MODE, int NT>
+// One stage of x (256 columns from c0 on) quantised into the operand tile and
+// its two atoms, by the eight warps of the later epilogue: half a block a
+// thread, 16 rows.  Rows past x hold anything; their results are not stored.
+template <typename X>
+__device__ __forceinline__ void quantize_stage(const TileParams& p, uint8_t* tile, uint8_t* atoms, int c0) {
+  const int t = threadIdx.x - 64, row = t >> 4, hb = t & 15;
+  const int left = row < p.N ? p.cols - (c0 + hb * 16) : 0;
+  const X* src = static_cast<const X*>(p.x) + row * p.ldx + c0 + hb * 16;
+  Half<X> v;
+  v.clear();
+  if (p.vec) v.load(src, min(left, 16));
+  else v.load_some(src, min(left, 16));
+  const int s = scale_byte(v.top());
+  const float inv = inv_scale(s);
+  uint2 w = make_uint2(v.codes(0, inv), v.codes(1, inv));
+  if (s == 255) w = make_uint2(0u, 0u);
+  // 128-byte lines, 16-byte pieces swizzled by the line
+  *reinterpret_cast<uint2*>(tile + row * 128 + (((hb >> 1) ^ (row & 7)) << 4) + (hb & 1) * 8) = w;
+  if ((hb & 1) == 0) atoms[(hb >> 3) * kAtom + grouped::atom_off(row, (hb >> 1) & 3)] = (uint8_t)s;
+}
+
+// X: type of the rows of x that the kernel quantises itself (up to 16: every
+// CTA its slice of the contraction, in place of a launch before this one), or
+// void where x comes as codes.
+template <int MODE, int NT, typename X>
 __global__ void __launch_bounds__(kTileThreads, 2) tile_kernel(const __grid_constant__ TileParams p) {
   using C = TileShape<MODE, NT>;
   constexpr int S = C::kStages, kMats = C::kMats;
+  constexpr bool kRaw = !std::is_void<X>::value;
+  static_assert(!kRaw || NT == 16, "quantize_stage fills 16 rows");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   __shared__ __align__(8) uint64_t full[S], empty[S], accfull;
@@ -395,7 +424,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) tile_kernel(const __grid_cons
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], kRaw ? 9 : 1);   // the copies, and eight quantising warps
       mbar_init(&empty[s], 1);
     }
     mbar_init(&accfull, 1);
@@ -416,7 +445,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) tile_kernel(const __grid_cons
         const int it = it0 + g, na = min(2, chunks - 2 * it);   // atoms of this stage
         uint8_t* st = smem + g % S * C::kStage;
         uint64_t* bar = &full[g % S];
-        mbar_arrive_expect_tx(bar, C::kOps + (kMats + 1) * na * kAtom);
+        mbar_arrive_expect_tx(bar, (kRaw ? kMats * 16384 : C::kOps) + (kRaw ? kMats : kMats + 1) * na * kAtom);
 #pragma unroll
         for (int t = 0; t < kMats; ++t) {
           tma_load_2d(st + t * 16384, &p.a[t], it * 128, m0, bar);
@@ -424,6 +453,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) tile_kernel(const __grid_cons
         }
       };
       auto rows = [&](int g) {
+        if (kRaw) return;
         const int it = it0 + g, na = min(2, chunks - 2 * it);
         uint8_t* st = smem + g % S * C::kStage;
         tma_load_2d(st + kMats * 16384, &p.b, it * 128, 0, &full[g % S]);
@@ -475,6 +505,17 @@ __global__ void __launch_bounds__(kTileThreads, 2) tile_kernel(const __grid_cons
     __syncwarp();
     ds::pair::wait_all(&accfull, 0, abort, p.err);
   } else {
+    if constexpr (kRaw) {
+      wait_prior_grid();
+      for (int g = 0; g < it1 - it0; ++g) {
+        if (g >= S && !ds::pair::wait_all(&empty[g % S], ((g / S) - 1) & 1, abort, p.err)) break;
+        uint8_t* st = smem + g % S * C::kStage;
+        quantize_stage<X>(p, st + kMats * 16384, st + C::kOps + kMats * 2 * kAtom, (it0 + g) * 256);
+        fence_proxy_async_smem();   // the tensor core reads what this thread wrote
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[g % S]);
+      }
+    }
     ds::pair::wait_all(&accfull, 0, abort, p.err);
   }
   tc5::fence_after();
@@ -571,11 +612,23 @@ int launch_quantize(const void* x, int dtype, int64_t rows, int cols, int64_t ld
   return DS_OK;
 }
 
-template <int MODE, int NT>
+// The tile kernel quantises up to this many rows of x itself.
+constexpr int kRawRows = 16;
+
+// Rows of x as a call gives them: values, or codes (DS_U8) with their atoms.
+struct Input {
+  const void* p;
+  const uint8_t* atoms;
+  int dtype;
+  int64_t rows, ld;
+  int cols;
+};
+
+template <int MODE, int NT, typename X>
 int launch_tiles(const TileParams& p, int slices, cudaStream_t s, bool chained) {
   using C = TileShape<MODE, NT>;
   static SmemOnce once;
-  const int st = ds::allow_smem(&once, reinterpret_cast<const void*>(&tile_kernel<MODE, NT>), C::kSmem);
+  const int st = ds::allow_smem(&once, reinterpret_cast<const void*>(&tile_kernel<MODE, NT, X>), C::kSmem);
   if (st != DS_OK) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((p.M + 127) / 128 * slices));
@@ -590,22 +643,33 @@ int launch_tiles(const TileParams& p, int slices, cudaStream_t s, bool chained) 
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = chained ? 2 : 1;
-  DS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, tile_kernel<MODE, NT>, p));
+  DS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, tile_kernel<MODE, NT, X>, p));
   return DS_OK;
 }
 
-// Rows of x per tile: all of them (at most 64), so a tile starts at row 0 of a scale atom.
-int row_tile(int64_t n) { return n <= 16 ? 16 : n <= 32 ? 32 : 64; }
-
+// The slices of the contraction: enough to give every SM a CTA, at least two
+// stages each.
 template <int MODE>
-int run_tiles(const TileParams& p, int nt, cudaStream_t s, bool chained) {
+int run_tiles(TileParams& p, const Input& x, cudaStream_t s, bool chained) {
   const int64_t tiles = (p.M + 127) / 128;
   const int ksteps = (p.blocks + 7) / 8;
-  int slices = 1;   // enough to give every SM a CTA, at least two stages each
+  int slices = 1;
   while (slices < 8 && tiles * slices * 2 <= ds::sm_count() && ksteps / (slices * 2) >= 2) slices *= 2;
-  if (nt == 16) return launch_tiles<MODE, 16>(p, slices, s, chained);
-  if (nt == 32) return launch_tiles<MODE, 32>(p, slices, s, chained);
-  return launch_tiles<MODE, 64>(p, slices, s, chained);
+  p.N = (int)x.rows;
+  if (x.dtype != DS_U8) {
+    p.x = x.p, p.ldx = x.ld, p.cols = x.cols;
+    p.vec = ds::aligned(x.p, 16) && x.cols % 8 == 0 && (x.rows == 1 || x.ld * (x.dtype == DS_F32 ? 4 : 2) % 16 == 0);
+    if (x.dtype == DS_F32) return launch_tiles<MODE, 16, float>(p, slices, s, chained);
+    if (x.dtype == DS_F16) return launch_tiles<MODE, 16, __half>(p, slices, s, chained);
+    return launch_tiles<MODE, 16, __nv_bfloat16>(p, slices, s, chained);
+  }
+  // one tile of all rows, so it starts at row 0 of a scale atom
+  const int nt = x.rows <= 16 ? 16 : x.rows <= 32 ? 32 : 64;
+  DS_REQUIRE(map_codes(&p.b, x.p, x.rows, x.cols, nt), DS_ECUDA, "mx4: tensor map encoding failed");
+  p.sb = x.atoms;
+  if (nt == 16) return launch_tiles<MODE, 16, void>(p, slices, s, chained);
+  if (nt == 32) return launch_tiles<MODE, 32, void>(p, slices, s, chained);
+  return launch_tiles<MODE, 64, void>(p, slices, s, chained);
 }
 
 // ---- pair kernel
@@ -652,51 +716,47 @@ int run_pairs(const PairParams& p, cudaStream_t s, bool chained) {
   return DS_OK;
 }
 
-// y = x W^T of quantised operands.
-int product(const void* x, const uint8_t* x_atoms, int64_t rows, const DsMx4& w, void* y, int out_dtype, int* err,
-            cudaStream_t s, bool chained) {
-  if (rows >= kPairRows) {
+// y = x W^T.
+int product(const Input& x, const DsMx4& w, void* y, int out_dtype, int* err, cudaStream_t s, bool chained) {
+  if (x.rows >= kPairRows) {
     PairParams p = {};
-    const bool ok = map_codes(&p.a, x, rows, w.cols, 128) && map_codes(&p.b[0], w.packed, w.rows, w.cols, 128) &&
-                    map_atoms(&p.sa, x_atoms, rows, w.cols) && map_atoms(&p.sb[0], w.atoms, w.rows, w.cols);
+    const bool ok = map_codes(&p.a, x.p, x.rows, w.cols, 128) && map_codes(&p.b[0], w.packed, w.rows, w.cols, 128) &&
+                    map_atoms(&p.sa, x.atoms, x.rows, w.cols) && map_atoms(&p.sb[0], w.atoms, w.rows, w.cols);
     DS_REQUIRE(ok, DS_ECUDA, "mx4: tensor map encoding failed");
-    p.boxed = map_result(&p.out, y, rows, w.rows, out_dtype);
+    p.boxed = map_result(&p.out, y, x.rows, w.rows, out_dtype);
     p.y = y, p.ldy = w.rows, p.out_dtype = out_dtype;
-    p.M = (int)rows, p.N = (int)w.rows, p.blocks = (int)blocks_of(w.cols), p.err = err;
+    p.M = (int)x.rows, p.N = (int)w.rows, p.blocks = (int)blocks_of(w.cols), p.err = err;
     return run_pairs<false>(p, s, chained);
   }
-  const int nt = row_tile(rows);
   TileParams p = {};
-  const bool ok = map_codes(&p.a[0], w.packed, w.rows, w.cols, 128) && map_codes(&p.b, x, rows, w.cols, nt);
-  DS_REQUIRE(ok, DS_ECUDA, "mx4: tensor map encoding failed");
-  p.sa[0] = w.atoms, p.sb = x_atoms;
-  p.M = (int)w.rows, p.N = (int)rows, p.blocks = (int)blocks_of(w.cols), p.err = err;
+  DS_REQUIRE(map_codes(&p.a[0], w.packed, w.rows, w.cols, 128), DS_ECUDA, "mx4: tensor map encoding failed");
+  p.sa[0] = w.atoms;
+  p.M = (int)w.rows, p.blocks = (int)blocks_of(w.cols), p.err = err;
   p.out = y, p.ldo = w.rows, p.out_dtype = out_dtype;
-  return run_tiles<LINEAR>(p, nt, s, chained);
+  return run_tiles<LINEAR>(p, x, s, chained);
 }
 
 // Codes and atoms of h = the gated unit of x W1^T and x W3^T.
-int gate_up(const void* x, const uint8_t* x_atoms, int64_t rows, const DsMx4& w1, const DsMx4& w3, float limit,
-            uint8_t* hq, uint8_t* hs, int* err, cudaStream_t s, bool chained) {
-  if (rows >= kPairRows) {
+int gate_up(const Input& x, const DsMx4& w1, const DsMx4& w3, float limit, uint8_t* hq, uint8_t* hs, int* err,
+            cudaStream_t s, bool chained) {
+  if (x.rows >= kPairRows) {
     PairParams p = {};
-    const bool ok = map_codes(&p.a, x, rows, w1.cols, 128) && map_codes(&p.b[0], w1.packed, w1.rows, w1.cols, 128) &&
-                    map_codes(&p.b[1], w3.packed, w1.rows, w1.cols, 128) && map_atoms(&p.sa, x_atoms, rows, w1.cols) &&
+    const bool ok = map_codes(&p.a, x.p, x.rows, w1.cols, 128) && map_codes(&p.b[0], w1.packed, w1.rows, w1.cols, 128) &&
+                    map_codes(&p.b[1], w3.packed, w1.rows, w1.cols, 128) && map_atoms(&p.sa, x.atoms, x.rows, w1.cols) &&
                     map_atoms(&p.sb[0], w1.atoms, w1.rows, w1.cols) && map_atoms(&p.sb[1], w3.atoms, w1.rows, w1.cols);
     DS_REQUIRE(ok, DS_ECUDA, "mx4: tensor map encoding failed");
     p.hq = hq, p.hs = hs, p.limit = limit;
-    p.M = (int)rows, p.N = (int)w1.rows, p.blocks = (int)blocks_of(w1.cols), p.err = err;
+    p.M = (int)x.rows, p.N = (int)w1.rows, p.blocks = (int)blocks_of(w1.cols), p.err = err;
     return run_pairs<true>(p, s, chained);
   }
-  const int nt = row_tile(rows);
   TileParams p = {};
   const bool ok = map_codes(&p.a[0], w1.packed, w1.rows, w1.cols, 128) &&
-                  map_codes(&p.a[1], w3.packed, w1.rows, w1.cols, 128) && map_codes(&p.b, x, rows, w1.cols, nt);
+                  map_codes(&p.a[1], w3.packed, w1.rows, w1.cols, 128);
   DS_REQUIRE(ok, DS_ECUDA, "mx4: tensor map encoding failed");
-  p.sa[0] = w1.atoms, p.sa[1] = w3.atoms, p.sb = x_atoms;
-  p.M = (int)w1.rows, p.N = (int)rows, p.blocks = (int)blocks_of(w1.cols), p.err = err;
+  p.sa[0] = w1.atoms, p.sa[1] = w3.atoms;
+  p.M = (int)w1.rows, p.blocks = (int)blocks_of(w1.cols), p.err = err;
   p.hq = hq, p.hs = hs, p.limit = limit;
-  return run_tiles<GATED>(p, nt, s, chained);
+  return run_tiles<GATED>(p, x, s, chained);
 }
 
 int validate_weight(const DsMx4* w, const char* what) {
@@ -723,16 +783,20 @@ size_t quantized_bytes(int64_t rows, int64_t cols) {
   return grouped::up(packed_bytes(rows, cols), 256) + grouped::up(atoms_bytes(rows, cols), 256);
 }
 
-// Codes and atoms of x: as given, or quantised into the workspace.
-int quantized_x(const void*& x, const uint8_t*& atoms, int dtype, int64_t rows, int cols, int64_t ld, uint8_t*& ws,
-                cudaStream_t s) {
-  if (dtype == DS_U8) return DS_OK;
-  uint8_t* sa = ws + grouped::up(packed_bytes(rows, cols), 256);
-  const int st = launch_quantize(x, dtype, rows, cols, ld, ws, nullptr, sa, s);
+// Workspace for x given as values.
+size_t x_bytes(int64_t rows, int64_t cols) { return rows <= kRawRows ? 0 : quantized_bytes(rows, cols); }
+
+// Codes and atoms of x: as given, left to the tile kernel, or quantised into
+// the workspace (then the next launch is chained to this one).
+int quantized_x(Input& x, uint8_t*& ws, bool& chained, cudaStream_t s) {
+  chained = false;
+  if (x.dtype == DS_U8 || x.rows <= kRawRows) return DS_OK;
+  uint8_t* sa = ws + grouped::up(packed_bytes(x.rows, x.cols), 256);
+  const int st = launch_quantize(x.p, x.dtype, x.rows, x.cols, x.ld, ws, nullptr, sa, s);
   if (st != DS_OK) return st;
-  x = ws;
-  atoms = sa;
-  ws += quantized_bytes(rows, cols);
+  x.p = ws, x.atoms = sa, x.dtype = DS_U8;
+  ws += quantized_bytes(x.rows, x.cols);
+  chained = true;
   return DS_OK;
 }
 
@@ -811,7 +875,7 @@ extern "C" int ds_mx4_scale_atoms(const uint8_t* scales, int64_t rows, int64_t c
 extern "C" int ds_mx4_linear_workspace_size(int64_t rows, int64_t cols, size_t* bytes) {
   DS_REQUIRE(bytes && rows >= 0 && cols >= 1, DS_EINVAL,
              "mx4_linear_workspace_size: rows >= 0, cols >= 1 and an output expected");
-  *bytes = quantized_bytes(rows, cols);
+  *bytes = x_bytes(rows, cols);
   return DS_OK;
 }
 
@@ -824,7 +888,7 @@ extern "C" int ds_mx4_linear(const void* x, const uint8_t* x_atoms, int x_dtype,
   DS_REQUIRE(out_dtype == DS_F32 || out_dtype == DS_BF16 || out_dtype == DS_F16, DS_EINVAL,
              "mx4_linear: out must be f32, bf16 or f16");
   if (rows == 0) return DS_OK;
-  const size_t need = x_dtype == DS_U8 ? 0 : quantized_bytes(rows, w->cols);
+  const size_t need = x_dtype == DS_U8 ? 0 : x_bytes(rows, w->cols);
   DS_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), DS_EINVAL,
              "mx4_linear: workspace %zu bytes < required %zu", workspace_bytes, need);
   DS_REQUIRE(out && ds::aligned(out, out_dtype == DS_F32 ? 4 : 2) && ds::aligned(workspace, 256), DS_EALIGN,
@@ -832,17 +896,18 @@ extern "C" int ds_mx4_linear(const void* x, const uint8_t* x_atoms, int x_dtype,
   DS_REQUIRE(ds::grouped::encode_fn() != nullptr, DS_ECUDA, "mx4_linear: cuTensorMapEncodeTiled unavailable");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  if ((st = quantized_x(x, x_atoms, x_dtype, rows, (int)w->cols, ld, ws, s)) != DS_OK) return st;
-
   int* err = err_word();
   DS_REQUIRE(err != nullptr, DS_ECUDA, "mx4_linear: error word unavailable");
-  return product(x, x_atoms, rows, *w, out, out_dtype, err, s, x_dtype != DS_U8);
+  Input in = {x, x_atoms, x_dtype, rows, ld, (int)w->cols};
+  bool chained;
+  if ((st = quantized_x(in, ws, chained, s)) != DS_OK) return st;
+  return product(in, *w, out, out_dtype, err, s, chained);
 }
 
 extern "C" int ds_mx4_gated_ffn_workspace_size(int64_t rows, int64_t hidden, int64_t inter, size_t* bytes) {
   DS_REQUIRE(bytes && rows >= 0 && hidden >= 1 && inter >= 1, DS_EINVAL,
              "mx4_gated_ffn_workspace_size: rows >= 0, hidden >= 1, inter >= 1 and an output expected");
-  *bytes = quantized_bytes(rows, hidden) + quantized_bytes(rows, inter);
+  *bytes = x_bytes(rows, hidden) + quantized_bytes(rows, inter);
   return DS_OK;
 }
 
@@ -860,7 +925,7 @@ extern "C" int ds_mx4_gated_ffn(const void* x, const uint8_t* x_atoms, int x_dty
              "mx4_gated_ffn: out must be f32, bf16 or f16");
   DS_REQUIRE(limit >= 0.0f, DS_EINVAL, "mx4_gated_ffn: limit must be >= 0 (0: no clamps)");
   if (rows == 0) return DS_OK;
-  const size_t need = (x_dtype == DS_U8 ? 0 : quantized_bytes(rows, H)) + quantized_bytes(rows, I);
+  const size_t need = (x_dtype == DS_U8 ? 0 : x_bytes(rows, H)) + quantized_bytes(rows, I);
   DS_REQUIRE(workspace && workspace_bytes >= need, DS_EINVAL, "mx4_gated_ffn: workspace %zu bytes < required %zu",
              workspace_bytes, need);
   DS_REQUIRE(out && ds::aligned(out, out_dtype == DS_F32 ? 4 : 2) && ds::aligned(workspace, 256), DS_EALIGN,
@@ -868,14 +933,16 @@ extern "C" int ds_mx4_gated_ffn(const void* x, const uint8_t* x_atoms, int x_dty
   DS_REQUIRE(ds::grouped::encode_fn() != nullptr, DS_ECUDA, "mx4_gated_ffn: cuTensorMapEncodeTiled unavailable");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  if ((st = quantized_x(x, x_atoms, x_dtype, rows, (int)H, ld, ws, s)) != DS_OK) return st;
-  uint8_t* hq = ws;
-  uint8_t* hs = ws + ds::grouped::up(packed_bytes(rows, I), 256);
-
   int* err = err_word();
   DS_REQUIRE(err != nullptr, DS_ECUDA, "mx4_gated_ffn: error word unavailable");
-  if ((st = gate_up(x, x_atoms, rows, *w1, *w3, limit, hq, hs, err, s, x_dtype != DS_U8)) != DS_OK) return st;
-  return product(hq, hs, rows, *w2, out, out_dtype, err, s, true);
+  Input in = {x, x_atoms, x_dtype, rows, ld, (int)H};
+  bool chained;
+  if ((st = quantized_x(in, ws, chained, s)) != DS_OK) return st;
+  uint8_t* hq = ws;
+  uint8_t* hs = ws + ds::grouped::up(packed_bytes(rows, I), 256);
+  if ((st = gate_up(in, *w1, *w3, limit, hq, hs, err, s, chained)) != DS_OK) return st;
+  const Input h = {hq, hs, DS_U8, rows, 0, (int)I};
+  return product(h, *w2, out, out_dtype, err, s, true);
 }
 
 extern "C" int ds_mx4_status(int32_t* err, void* stream) {

@@ -29,8 +29,13 @@ def _atoms_bytes(rows: int, cols: int) -> int:
 
 
 def _workspace_bytes(rows: int, cols: int) -> int:
-    """Codes and atoms of a quantised matrix, each on 256 bytes (ds_mx4_linear_workspace_size)."""
+    """Codes and atoms of a quantised matrix, each on 256 bytes."""
     return (rows * _blocks(cols) * 16 + 255) // 256 * 256 + (_atoms_bytes(rows, cols) + 255) // 256 * 256
+
+
+def _x_bytes(rows: int, cols: int) -> int:
+    """Workspace for x given as values: up to 16 rows the product quantises itself."""
+    return _workspace_bytes(rows, cols) if rows > 16 else 0
 
 
 class MX4Tensor:
@@ -151,7 +156,7 @@ def linear(x, w: MX4Tensor, out_dtype: torch.dtype | None = None) -> torch.Tenso
     hold, px, pa, dt, rows, ld, out_dtype = _input(x, w.cols, out_dtype)
     dev = w.device
     out = torch.empty((*x.shape[:-1], w.rows), dtype=out_dtype, device=dev)
-    n = 0 if dt == _abi.DS_U8 else _workspace_bytes(rows, w.cols)
+    n = 0 if dt == _abi.DS_U8 else _x_bytes(rows, w.cols)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     with on_device(dev):
         _abi.check(_abi.lib().ds_mx4_linear(px, pa, dt, rows, ld, w._ref(), out.data_ptr(), _DTYPES[out_dtype],
@@ -174,7 +179,7 @@ def gated_ffn(x, w1: MX4Tensor, w3: MX4Tensor, w2: MX4Tensor, limit: float | Non
     hold, px, pa, dt, rows, ld, out_dtype = _input(x, hidden, out_dtype)
     dev = w1.device
     out = torch.empty(x.shape, dtype=out_dtype, device=dev)
-    n = _workspace_bytes(rows, inter) + (0 if dt == _abi.DS_U8 else _workspace_bytes(rows, hidden))
+    n = _workspace_bytes(rows, inter) + (0 if dt == _abi.DS_U8 else _x_bytes(rows, hidden))
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     with on_device(dev):
         _abi.check(_abi.lib().ds_mx4_gated_ffn(px, pa, dt, rows, ld, w1._ref(), w3._ref(), w2._ref(), limit or 0.0,

@@ -495,8 +495,9 @@ typedef struct DsMx4 {
 
 /* out [rows, w->rows] (f32, bf16 or f16, contiguous) = x W^T, f32 accumulate.
  * x_dtype f32 / bf16 / f16: x [rows, w->cols], rows ld elements apart, is
- * quantised into the workspace first (x_atoms NULL); DS_U8: x is codes and
- * x_atoms its atoms, and no workspace is needed.  rows in [0, 2^22]. */
+ * quantised into the workspace first, or up to 16 rows by the product itself
+ * without one (x_atoms NULL); DS_U8: x is codes and x_atoms its atoms, and no
+ * workspace is needed.  rows in [0, 2^22]. */
 int ds_mx4_linear_workspace_size(int64_t rows, int64_t cols, size_t* bytes);
 int ds_mx4_linear(const void* x, const uint8_t* x_atoms, int x_dtype, int64_t rows, int64_t ld, const DsMx4* w,
                   void* out, int out_dtype, void* workspace, size_t workspace_bytes, void* stream);

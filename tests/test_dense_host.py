@@ -72,9 +72,10 @@ def test_mx4_sizes_and_arguments(lib):
         assert lib.ds_mx4_atoms_size(rows, cols, ctypes.byref(n)) == _abi.DS_OK
         assert n.value == -(-rows // 128) * -(-cols // 128) * 512 == mx4._atoms_bytes(rows, cols)
         assert lib.ds_mx4_linear_workspace_size(rows, cols, ctypes.byref(n)) == _abi.DS_OK
-        assert n.value == mx4._workspace_bytes(rows, cols)
-    assert lib.ds_mx4_gated_ffn_workspace_size(7, 100, 60, ctypes.byref(n)) == _abi.DS_OK
-    assert n.value == mx4._workspace_bytes(7, 100) + mx4._workspace_bytes(7, 60)
+        assert n.value == mx4._x_bytes(rows, cols) == (mx4._workspace_bytes(rows, cols) if rows > 16 else 0)
+    for rows in (7, 16, 17, 70):                                        # up to 16 rows x needs none, h always
+        assert lib.ds_mx4_gated_ffn_workspace_size(rows, 100, 60, ctypes.byref(n)) == _abi.DS_OK
+        assert n.value == mx4._x_bytes(rows, 100) + mx4._workspace_bytes(rows, 60)
     assert lib.ds_mx4_atoms_size(1, 0, ctypes.byref(n)) == _abi.DS_EINVAL
     q = lambda *a: lib.ds_mx4_quantize(*a, None)  # noqa: E731
     assert q(256, _abi.DS_U8, 1, 32, 32, 256, 256, 256) == _abi.DS_EINVAL
@@ -91,7 +92,7 @@ def test_mx4_sizes_and_arguments(lib):
     assert lin(256, None, _abi.DS_U8, 1, 0, w, _abi.DS_F32, None, 0) == _abi.DS_EINVAL     # codes without atoms
     assert lin(256, None, _abi.DS_F32, 2, 95, w, _abi.DS_F32, 256, 1 << 20) == _abi.DS_EINVAL
     assert lin(256, None, _abi.DS_F32, 1, 96, w, _abi.DS_U8, 256, 1 << 20) == _abi.DS_EINVAL
-    assert lin(256, None, _abi.DS_F32, 1, 96, w, _abi.DS_F32, 256, 255) == _abi.DS_EINVAL
+    assert lin(256, None, _abi.DS_F32, 17, 96, w, _abi.DS_F32, 256, 255) == _abi.DS_EINVAL
     assert lin(256, None, _abi.DS_F32, (1 << 22) + 1, 96, w, _abi.DS_F32, 256, 1 << 40) == _abi.DS_ERANGE
     assert lin(256, None, _abi.DS_F32, 1, 96, _abi.DsMx4(256, None, 64, 96), _abi.DS_F32, 256, 1 << 20) == _abi.DS_EINVAL
     assert lin(256, None, _abi.DS_F32, 1, 96, _abi.DsMx4(264, 256, 64, 96), _abi.DS_F32, 256, 1 << 20) == _abi.DS_EALIGN
