@@ -41,20 +41,45 @@ def _x_bytes(rows: int, cols: int) -> int:
 class MX4Tensor:
     """A quantised matrix: ``packed`` u8 [rows, 16 ceil(cols/32)] (two codes per
     byte, low nibble first), ``scales`` u8 [rows, ceil(cols/32)] (2^(b-127), 255
-    = NaN), ``atoms`` (the scales as the tensor cores read them); ``shape``:
-    the shape it stands for, leading dimensions included."""
+    = NaN), and the scales as the tensor cores read them; ``shape``: the shape
+    it stands for, leading dimensions included."""
 
-    __slots__ = ("packed", "scales", "atoms", "rows", "cols", "shape", "device", "_c")
+    __slots__ = ("rows", "cols", "shape", "device", "_hold", "_packed", "_scales", "_pp", "_ps", "_pa", "_c")
 
-    def __init__(self, packed, scales, atoms, shape):
-        self.packed, self.scales, self.atoms = packed, scales, atoms
-        self.shape = shape
-        self.rows, self.cols, self.device = packed.shape[0], shape[-1], packed.device
+    def __init__(self, rows, shape, device, hold, packed, scales, atoms, views=(None, None)):
+        """``hold``: what owns the memory at the addresses ``packed``, ``scales`` and ``atoms``."""
+        self.rows, self.cols, self.shape, self.device = rows, shape[-1], shape, device
+        self._hold, self._pp, self._ps, self._pa = hold, packed, scales, atoms
+        self._packed, self._scales = views
         self._c = None
+
+    def _view(self, address: int, cols: int) -> torch.Tensor:
+        at = address - self._hold.data_ptr()
+        return self._hold[at:at + self.rows * cols].view(self.rows, cols)
+
+    @property
+    def packed(self) -> torch.Tensor:
+        if self._packed is None:
+            self._packed = self._view(self._pp, _blocks(self.cols) * 16)
+        return self._packed
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._scales = self._view(self._ps, _blocks(self.cols))
+        return self._scales
+
+    @property
+    def atoms(self) -> torch.Tensor:
+        """[ceil(rows/128) * ceil(cols/128) * 512] bytes (include/deepseeker_b200.h)."""
+        if isinstance(self._hold, tuple):
+            return self._hold[2]
+        at = self._pa - self._hold.data_ptr()
+        return self._hold[at:at + _atoms_bytes(self.rows, self.cols)]
 
     def _ref(self):
         if self._c is None:
-            self._c = _abi.DsMx4(self.packed.data_ptr(), self.atoms.data_ptr(), self.rows, self.cols)
+            self._c = _abi.DsMx4(self._pp, self._pa, self.rows, self.cols)
         return ctypes.byref(self._c)
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -64,8 +89,8 @@ class MX4Tensor:
         dev = self.device
         out = torch.empty(self.shape, dtype=dtype, device=dev)
         with on_device(dev):
-            _abi.check(_abi.lib().ds_mx4_dequantize(self.packed.data_ptr(), self.scales.data_ptr(), self.rows,
-                                                    self.cols, out.data_ptr(), _DTYPES[dtype], raw_stream(dev)),
+            _abi.check(_abi.lib().ds_mx4_dequantize(self._pp, self._ps, self.rows, self.cols, out.data_ptr(),
+                                                    _DTYPES[dtype], raw_stream(dev)),
                        "ds_mx4_dequantize")
         return out
 
@@ -93,13 +118,15 @@ def quantize(x: torch.Tensor) -> MX4Tensor:
     rows, ld = _matrix(x)
     n, cols = rows.shape
     nb, dev = _blocks(cols), x.device
-    packed = torch.empty((n, nb * 16), dtype=torch.uint8, device=dev)
-    scales = torch.empty((n, nb), dtype=torch.uint8, device=dev)
-    atoms = torch.empty(_atoms_bytes(n, cols), dtype=torch.uint8, device=dev)
+    # one buffer: codes, atoms, scales
+    at = (n * nb * 16 + 255) // 256 * 256
+    sc = at + _atoms_bytes(n, cols)
+    buf = torch.empty(sc + n * nb, dtype=torch.uint8, device=dev)
+    p = buf.data_ptr()
     with on_device(dev):
-        _abi.check(_abi.lib().ds_mx4_quantize(rows.data_ptr(), _DTYPES[x.dtype], n, cols, ld, packed.data_ptr(),
-                                              scales.data_ptr(), atoms.data_ptr(), raw_stream(dev)), "ds_mx4_quantize")
-    return MX4Tensor(packed, scales, atoms, x.shape)
+        _abi.check(_abi.lib().ds_mx4_quantize(rows.data_ptr(), _DTYPES[x.dtype], n, cols, ld, p, p + sc, p + at,
+                                              raw_stream(dev)), "ds_mx4_quantize")
+    return MX4Tensor(n, x.shape, dev, buf, p, p + sc, p + at)
 
 
 def from_packed(packed: torch.Tensor, scales: torch.Tensor, cols: int | None = None) -> MX4Tensor:
@@ -121,13 +148,14 @@ def from_packed(packed: torch.Tensor, scales: torch.Tensor, cols: int | None = N
     with on_device(dev):
         _abi.check(_abi.lib().ds_mx4_scale_atoms(scales.data_ptr(), rows, cols, atoms.data_ptr(), raw_stream(dev)),
                    "ds_mx4_scale_atoms")
-    return MX4Tensor(packed, scales, atoms, torch.Size((rows, cols)))
+    return MX4Tensor(rows, torch.Size((rows, cols)), dev, (packed, scales, atoms), packed.data_ptr(), scales.data_ptr(),
+                     atoms.data_ptr(), (packed, scales))
 
 
 def _input(x, cols: int, out_dtype):
     """(what keeps it alive, pointer, atoms' pointer, type, rows, row stride, result type) of x, quantised or not."""
     if isinstance(x, MX4Tensor):
-        got, dtype = (x, x.packed.data_ptr(), x.atoms.data_ptr(), _abi.DS_U8, x.rows, 0), torch.bfloat16
+        got, dtype = (x, x._pp, x._pa, _abi.DS_U8, x.rows, 0), torch.bfloat16
     else:
         _check_x(x)
         rows, ld = _matrix(x)
