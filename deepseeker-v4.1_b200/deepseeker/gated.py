@@ -37,8 +37,12 @@ def _check(x, w1, w3, w2, limit) -> int:
 
 def _desc(x, w1, w3, w2, limit) -> tuple[_abi.DsGatedFfn, tuple]:
     """The call's descriptor, and the tensors that it points into."""
-    (x, lx), (w1, l1), (w3, l3), (w2, l2) = rows_of(x), rows_of(w1), rows_of(w3), rows_of(w2)
     inter, hidden = w1.shape
+    if x.is_contiguous() and w1.is_contiguous() and w3.is_contiguous() and w2.is_contiguous():
+        lx = l1 = l3 = hidden
+        l2 = inter
+    else:
+        (x, lx), (w1, l1), (w3, l3), (w2, l2) = rows_of(x), rows_of(w1), rows_of(w3), rows_of(w2)
     d = _abi.DsGatedFfn(x.shape[0], hidden, inter, _DTYPES[x.dtype], limit or 0.0, x.data_ptr(), w1.data_ptr(),
                         w3.data_ptr(), w2.data_ptr(), lx, l1, l3, l2)
     return d, (x, w1, w3, w2)
