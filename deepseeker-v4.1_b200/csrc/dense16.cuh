@@ -74,6 +74,12 @@ inline bool map32(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, 
                             CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// A 16-bit matrix in boxes of 32 x 32 (64-byte lines).
+inline bool map_slim(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld) {
+  return grouped::encode_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, base, rows, cols, ld * 2, 32, 32,
+                            CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
 // ---------------------------------------------------------------- the gated unit
 
 // h = silu(min(g, L)) * clip(u, -L, L); L = 0: no clamps.  The comparisons

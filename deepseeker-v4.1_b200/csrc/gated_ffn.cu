@@ -408,7 +408,7 @@ Problem* add(PairParams& p, int epi, int64_t M, int64_t N, int64_t k, int segs, 
   Problem& q = p.pr[p.n++];
   q.epi = epi, q.M = (int)M, q.N = (int)N;
   q.ksteps = (int)((k + kBK - 1) / kBK), q.segs = segs;
-  q.c[0] = c, q.ldc = ldc;
+  q.c = c, q.ldc = ldc;
   return &q;
 }
 
@@ -437,7 +437,7 @@ int64_t cycles_of(const PairParams& p, int nt, int pairs) {
 
 template <int EPI, int NT>
 int launch_pairs(PairParams& p, Sides* sides, cudaStream_t s, bool chained) {
-  using C = pair::Shape<NT>;
+  using C = pair::Shape<EPI, NT>;
   int64_t tiles = 0;
   for (int z = 0; z < p.n; ++z) {
     Problem& q = p.pr[z];
@@ -445,10 +445,10 @@ int launch_pairs(PairParams& p, Sides* sides, cudaStream_t s, bool chained) {
     auto side = [&](CUtensorMap* m, const Operand& o, int mn, int rows) {
       return !o.p || map16(m, o.p, o.rows, o.cols, o.ld, mn ? 64 : rows);
     };
-    q.boxed = q.epi == STORE && direct(q.c[0], q.ldc);
+    q.boxed = q.epi == STORE && direct(q.c, q.ldc);
     const bool ok = side(&q.a[0], d.a0, q.a_mn, 128) && side(&q.a[1], d.a1, q.a_mn, 128) &&
                     side(&q.b[0], d.b0, q.b_mn, NT / 2) && side(&q.b[1], d.b1, q.b_mn, NT / 2) &&
-                    (!q.boxed || map16(&q.out, q.c[0], q.M, q.N, q.ldc, 32));
+                    (!q.boxed || map16(&q.out, q.c, q.M, q.N, q.ldc, 32));
     DS_REQUIRE(ok, DS_ECUDA, "gated_ffn: tensor map encoding failed");
     tiles += tiles_of(q, NT);
     DS_REQUIRE(tiles < ((int64_t)1 << 31), DS_ERANGE, "gated_ffn: too many tiles");
@@ -655,14 +655,15 @@ extern "C" int ds_gated_ffn_backward(const DsGatedFfn* desc, const void* h, cons
         if (dw2) grad(p, sd, dw2, H, I, gy, oh);
       } else if (need_mid) {
         Problem* q = add(p, HIDDEN, T, I, H, 1, dg, ldm);
-        q->c[1] = du, q->b_mn = 1;
+        q->b_mn = 1;
         sd[p.n - 1] = {q, gy, o.w2, none, none};
       }
       if (k == 0) p.split = p.n;
     }
     if (p.n) {
-      DS_REQUIRE(map32(&p.g, g, T, I, ldm) && map32(&p.u, u, T, I, ldm), DS_ECUDA,
-                 "gated_ffn_backward: tensor map encoding failed (pre-activations)");
+      DS_REQUIRE(map32(&p.g, g, T, I, ldm) && map32(&p.u, u, T, I, ldm) && map_slim(&p.dg, dg, T, I, ldm) &&
+                     map_slim(&p.du, du, T, I, ldm),
+                 DS_ECUDA, "gated_ffn_backward: tensor map encoding failed (pre-activations)");
       if ((st = run_pairs<HIDDEN>(p, sd, s, false)) != DS_OK) return st;
       chained = true;
     }

@@ -12,11 +12,12 @@
 // Persistent, one cluster per two SMs, 320 threads a CTA: warp 0 copies
 // (both CTAs signal the leader's barrier), warp 1 of the leader issues the
 // MMAs, warps 2-9 empty one NT-column accumulator while the other fills.
-// Lanes are rows here.  The f32 pre-activations go out (and come back in the
-// backward pass) as 32 x 32 boxes through 8 KB of shared memory per epilogue
-// warp: a thread's own 16-byte stores to 32 rows at a time made the epilogue
-// longer than the 64 stages of a tile (gate / up of 8192 x 4096 x 2048: 212
-// us with them, 176 us when nothing was kept).
+// Lanes are rows here.  What the epilogue moves beside the accumulator goes
+// through boxes of 32 rows in shared memory: a thread's own 16-byte accesses
+// touch 32 rows at a time, and with them the gate / up launch that keeps g and
+// u took 227 us instead of 200 (8192 x 4096 x 2048; 110 instead of 66 at a
+// hidden size of 1024), the launch of dg and du 107 instead of 92 (hidden size
+// 1024; with 4096 they are even, as the boxes cost that launch a stage).
 //
 // A launch may hold two groups of problems with different contractions (the
 // gradient of W2 beside that of the hidden values; those of W1 and W3 beside
@@ -34,7 +35,7 @@ enum Epilogue { STORE, GATED, HIDDEN };   // plain result; h (and g, u); dg and 
 struct Problem {
   CUtensorMap a[2], b[2];      // operands of the segments; GATED: b = W1, W3
   CUtensorMap out;             // STORE with boxed = 1: the result in boxes of 64 columns x 32 rows
-  void* c[2];                  // result [m * ldc + n], 16 bit (HIDDEN: dg, du)
+  void* c;                     // result [m * ldc + n], 16 bit
   int64_t ldc;
   int M, N;                    // rows and columns of the result
   int ksteps, segs;            // stages of one segment, segments
@@ -47,6 +48,7 @@ struct PairParams {
   Problem pr[3];
   int n, split;                // problems; the first `split` form group 0
   CUtensorMap g, u;            // f32 pre-activations, boxes of 32 x 32
+  CUtensorMap dg, du;          // HIDDEN: the results, boxes of 32 x 32
   int keep;                    // GATED: write them
   int f16;
   float limit;
@@ -61,13 +63,15 @@ constexpr int kOperand = 2 * kBoxBytes;          // 128 rows x 64
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 32 * (2 + kEpiWarps);
 
-template <int NT>
+template <int EPI, int NT>
 struct Shape {
   // half of B: NT / 2 rows x 64; MN-major boxes are 64 wide whatever NT
   static constexpr int kHalf = NT == 256 ? kOperand : kBoxBytes;
   static constexpr int kStage = kOperand + kHalf;
-  static constexpr int kStages = NT == 256 ? 5 : 6;
-  static constexpr int kSmem = 1024 + kStages * kStage + kEpiWarps * 2 * kBox;
+  // per epilogue warp two boxes of 128-byte lines, for dg and du two of 64 more
+  static constexpr int kBoxes = (EPI == HIDDEN ? 3 : 2) * kBox;
+  static constexpr int kStages = (NT == 256 ? 5 : 6) - (EPI == HIDDEN ? 1 : 0);
+  static constexpr int kSmem = 1024 + kStages * kStage + kEpiWarps * kBoxes;
   static_assert(kSmem <= 226 * 1024, "shared memory of an SM");
 };
 
@@ -109,6 +113,16 @@ __device__ __forceinline__ void store16(uint16_t* dst, const float (&v)[32], int
     for (int j = 0; j < 32; ++j)
       if (j < n) dst[j] = to16(v[j], f16);
   }
+}
+
+// 32 columns of a row (lane = row) into a box of 64-byte lines, 16-byte pieces
+// swizzled by line pairs.
+__device__ __forceinline__ void slim_put(uint8_t* box, int lane, const float (&v)[32], int f16) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    *reinterpret_cast<uint4*>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
+        make_uint4(pack16(v[8 * c], v[8 * c + 1], f16), pack16(v[8 * c + 2], v[8 * c + 3], f16),
+                   pack16(v[8 * c + 4], v[8 * c + 5], f16), pack16(v[8 * c + 6], v[8 * c + 7], f16));
 }
 
 // The i-th tile of pair c.  Group 0 is dealt round robin.  A tile of group 1
@@ -162,9 +176,10 @@ struct Rings {
 };
 
 // The copies of one tile, stages g on.  False: a wait gave up.
-template <bool AMN, bool BMN, bool GATE, int NT>
+template <bool AMN, bool BMN, int EPI, int NT>
 __device__ __forceinline__ bool copy_tile(const Rings& r, const Problem& q, int rank, int m0, int n0, int& g) {
-  using C = Shape<NT>;
+  using C = Shape<EPI, NT>;
+  constexpr bool GATE = EPI == GATED;
   constexpr uint32_t kBytes = kOperand + (BMN ? (NT == 256 ? 2 : 1) * kBoxBytes : NT / 2 * 128);
   const int ksteps = q.ksteps, its = ksteps * q.segs, am = m0 + 128 * rank, bn = GATE ? n0 : n0 + NT / 2 * rank;
   for (int it = 0; it < its; ++it, ++g) {
@@ -183,9 +198,9 @@ __device__ __forceinline__ bool copy_tile(const Rings& r, const Problem& q, int 
 // The MMAs of one tile, issued by an elected lane of a warp-uniform loop with
 // descriptors that differ by constants (held in uniform registers; operand
 // layouts read at run time instead made the 64 stages of a tile a fifth slower).
-template <bool AMN, bool BMN, int NT>
+template <bool AMN, bool BMN, int EPI, int NT>
 __device__ __forceinline__ bool mma_tile(const Rings& r, int its, int f16, uint32_t acc, int& g) {
-  using C = Shape<NT>;
+  using C = Shape<EPI, NT>;
   const uint32_t idesc = idesc16(f16, AMN, BMN, 256, NT);
   const uint64_t a0 = tile_desc<AMN>(smem_u32(r.smem)), b0 = tile_desc<BMN>(smem_u32(r.smem) + kOperand);
   for (int it = 0; it < its; ++it, ++g) {
@@ -206,7 +221,8 @@ __device__ __forceinline__ bool mma_tile(const Rings& r, int its, int f16, uint3
 // EPI: the launch's epilogue beside STORE.
 template <int EPI, int NT>
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_kernel(const __grid_constant__ PairParams p) {
-  constexpr int S = Shape<NT>::kStages;
+  using C = Shape<EPI, NT>;
+  constexpr int S = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   __shared__ __align__(8) uint64_t full[S], empty[S], accfull[2], accempty[2], boxfull[kEpiWarps];
@@ -251,10 +267,10 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
       for (int i = 0, tile; ok && (tile = dealer.tile(i)) >= 0; ++i) {
         int m0, n0;
         const Problem& q = p.pr[locate<NT>(p, tile, m0, n0)];
-        if (EPI == GATED) ok = copy_tile<false, false, true, NT>(r, q, rank, m0, n0, g);
-        else if (q.a_mn) ok = copy_tile<true, true, false, NT>(r, q, rank, m0, n0, g);
-        else if (q.b_mn) ok = copy_tile<false, true, false, NT>(r, q, rank, m0, n0, g);
-        else ok = copy_tile<false, false, false, NT>(r, q, rank, m0, n0, g);
+        if (EPI == GATED) ok = copy_tile<false, false, EPI, NT>(r, q, rank, m0, n0, g);
+        else if (q.a_mn) ok = copy_tile<true, true, EPI, NT>(r, q, rank, m0, n0, g);
+        else if (q.b_mn) ok = copy_tile<false, true, EPI, NT>(r, q, rank, m0, n0, g);
+        else ok = copy_tile<false, false, EPI, NT>(r, q, rank, m0, n0, g);
       }
       // every stage has been read by the MMAs, and the signal of that has
       // arrived, before this CTA's shared memory goes
@@ -272,9 +288,9 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
         if (i >= 2 && !wait_all(&accempty[b], ((i >> 1) - 1) & 1, abort, p.err)) break;
         tc5::fence_after();
         const uint32_t acc = tb + b * NT;
-        if (EPI != GATED && q.a_mn) ok = mma_tile<true, true, NT>(r, its, p.f16, acc, g);
-        else if (EPI != GATED && q.b_mn) ok = mma_tile<false, true, NT>(r, its, p.f16, acc, g);
-        else ok = mma_tile<false, false, NT>(r, its, p.f16, acc, g);
+        if (EPI != GATED && q.a_mn) ok = mma_tile<true, true, EPI, NT>(r, its, p.f16, acc, g);
+        else if (EPI != GATED && q.b_mn) ok = mma_tile<false, true, EPI, NT>(r, its, p.f16, acc, g);
+        else ok = mma_tile<false, false, EPI, NT>(r, its, p.f16, acc, g);
         if (ok && elect_one()) commit(&accfull[b]);
         __syncwarp();
       }
@@ -282,8 +298,9 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
   } else {
     // ------------------------------------------------------------ epilogue
     const int q4 = warp & 3, half = (warp - 2) >> 2;
-    uint8_t* box0 = smem + S * Shape<NT>::kStage + (warp - 2) * 2 * kBox;
+    uint8_t* box0 = smem + S * C::kStage + (warp - 2) * C::kBoxes;
     uint8_t* box1 = box0 + kBox;
+    uint8_t* slim = box1 + kBox;   // HIDDEN: boxes of dg and du
     uint64_t* loaded = &boxfull[warp - 2];
     int loads = 0, turn = 0;
     for (int i = 0, tile; (tile = dealer.tile(i)) >= 0; ++i) {
@@ -294,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
       const uint32_t acc = tc5::lane_quarter(tb + b * NT, q4);
       // the two warps of a lane quarter take turns at the columns inside the result
       const int nc = mw < q.M ? min(tile_cols(EPI, NT), q.N - n0) : 0;
-      uint16_t* out = static_cast<uint16_t*>(q.c[0]) + (int64_t)m * q.ldc;
+      uint16_t* out = static_cast<uint16_t*>(q.c) + (int64_t)m * q.ldc;
       // the pre-activations of 32 columns come in while the accumulator of
       // the previous ones (or the MMAs) are still at work
       auto fetch = [&](int c) {
@@ -336,7 +353,6 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
           if (row) store16(out + n0 + c, gv, nc - c, p.f16);
         }
       } else if (hidden) {
-        uint16_t* out1 = static_cast<uint16_t*>(q.c[1]) + (int64_t)m * q.ldc;
 #pragma unroll 1
         for (int c = half * 32; c < nc; c += 64) {
           float v[32], gv[32], uv[32];
@@ -354,9 +370,16 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
           tc5::wait_ld();
 #pragma unroll
           for (int j = 0; j < 32; ++j) gate_grad(gv[j], uv[j], v[j], p.limit, gv[j], uv[j]);
-          if (row) {
-            store16(out + n0 + c, gv, nc - c, p.f16);
-            store16(out1 + n0 + c, uv, nc - c, p.f16);
+          if (lane == 0) box_wait_read<0>();   // the previous columns have left
+          __syncwarp();
+          slim_put(slim, lane, gv, p.f16);
+          slim_put(slim + kBox / 2, lane, uv, p.f16);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            box_store(&p.dg, n0 + c, mw, slim);
+            box_store(&p.du, n0 + c, mw, slim + kBox / 2);
+            box_commit();
           }
         }
       } else if (q.boxed) {
@@ -393,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
           tc5::wait_ld();
           by_rows(box0, lane, v, [&](int r, float y) {
             if (mw + r < q.M && c + lane < nc)
-              static_cast<uint16_t*>(q.c[0])[(int64_t)(mw + r) * q.ldc + n0 + c + lane] = to16(y, p.f16);
+              static_cast<uint16_t*>(q.c)[(int64_t)(mw + r) * q.ldc + n0 + c + lane] = to16(y, p.f16);
           });
         }
       }
