@@ -568,8 +568,9 @@ extern "C" int ds_gated_ffn(const DsGatedFfn* desc, void* y, void* h, float* pre
     PairParams p = {};
     p.f16 = f16, p.limit = desc->limit, p.err = err, p.keep = pre != nullptr;
     Sides up[1] = {{add(p, GATED, T, I, H, 1, h, ldm), o.x, o.w1, none, o.w3}};
-    DS_REQUIRE(!pre || (map32(&p.g, pre, T, I, ldm) && map32(&p.u, pre_u, T, I, ldm)), DS_ECUDA,
-               "gated_ffn: tensor map encoding failed (pre-activations)");
+    DS_REQUIRE(map_slim(&p.h, h, T, I, ldm) &&
+                   (!pre || (map32(&p.g, pre, T, I, ldm) && map32(&p.u, pre_u, T, I, ldm))),
+               DS_ECUDA, "gated_ffn: tensor map encoding failed (h, pre-activations)");
     if ((st = run_pairs<GATED>(p, up, s, false)) != DS_OK) return st;
     PairParams d = {};
     d.f16 = f16, d.err = err;

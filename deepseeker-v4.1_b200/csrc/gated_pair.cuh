@@ -48,7 +48,7 @@ struct PairParams {
   Problem pr[3];
   int n, split;                // problems; the first `split` form group 0
   CUtensorMap g, u;            // f32 pre-activations, boxes of 32 x 32
-  CUtensorMap dg, du;          // HIDDEN: the results, boxes of 32 x 32
+  CUtensorMap dg, du, h;       // results of HIDDEN and GATED, boxes of 32 x 32
   int keep;                    // GATED: write them
   int f16;
   float limit;
@@ -96,23 +96,6 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
       "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
-}
-
-// 32 columns of one row, n of them inside the result; rows start on 16 bytes.
-__device__ __forceinline__ void store16(uint16_t* dst, const float (&v)[32], int n, int f16) {
-  if (n >= 32) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = pack16(v[8 * c + 2 * j], v[8 * c + 2 * j + 1], f16);
-      *reinterpret_cast<uint4*>(dst + 8 * c) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < n) dst[j] = to16(v[j], f16);
-  }
 }
 
 // 32 columns of a row (lane = row) into a box of 64-byte lines, 16-byte pieces
@@ -306,12 +289,11 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
     for (int i = 0, tile; (tile = dealer.tile(i)) >= 0; ++i) {
       int m0, n0;
       const Problem& q = p.pr[locate<NT>(p, tile, m0, n0)];
-      const int b = i & 1, mw = m0 + 128 * rank + 32 * q4, m = mw + lane;
-      const bool row = m < q.M, hidden = EPI == HIDDEN && q.epi == HIDDEN;
+      const int b = i & 1, mw = m0 + 128 * rank + 32 * q4;
+      const bool hidden = EPI == HIDDEN && q.epi == HIDDEN;
       const uint32_t acc = tc5::lane_quarter(tb + b * NT, q4);
       // the two warps of a lane quarter take turns at the columns inside the result
       const int nc = mw < q.M ? min(tile_cols(EPI, NT), q.N - n0) : 0;
-      uint16_t* out = static_cast<uint16_t*>(q.c) + (int64_t)m * q.ldc;
       // the pre-activations of 32 columns come in while the accumulator of
       // the previous ones (or the MMAs) are still at work
       auto fetch = [&](int c) {
@@ -350,7 +332,15 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
           }
 #pragma unroll
           for (int j = 0; j < 32; ++j) gv[j] = gate_unit(gv[j], uv[j], p.limit);
-          if (row) store16(out + n0 + c, gv, nc - c, p.f16);
+          if (lane == 0) box_wait_read<0>();   // g has left box 0
+          __syncwarp();
+          slim_put(box0, lane, gv, p.f16);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            box_store(&p.h, n0 + c, mw, box0);
+            box_commit();
+          }
         }
       } else if (hidden) {
 #pragma unroll 1
