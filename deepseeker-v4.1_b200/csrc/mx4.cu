@@ -39,12 +39,14 @@ struct Half {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) w[i] = 0u;
   }
-  // The first n, a multiple of 8, 16-byte aligned.
+  // The first n, a multiple of 8, 16-byte aligned; STREAM: first to leave L2.
+  template <bool STREAM = false>
   __device__ __forceinline__ void load(const T* p, int n) {
 #pragma unroll
     for (int i = 0; i < kWords / 4; ++i) {
       if (i * 8 >= n * (kF32 ? 2 : 1)) continue;
-      const uint4 a = reinterpret_cast<const uint4*>(p)[i];
+      const uint4* at = reinterpret_cast<const uint4*>(p) + i;
+      const uint4 a = STREAM ? __ldcs(at) : *at;
       w[4 * i] = a.x, w[4 * i + 1] = a.y, w[4 * i + 2] = a.z, w[4 * i + 3] = a.w;
     }
   }
@@ -116,6 +118,9 @@ template <typename T, int GROUPS, int ROWS>
 __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ld,
                                                        uint2* __restrict__ packed, uint8_t* __restrict__ scales,
                                                        uint8_t* __restrict__ atoms) {
+  // rows of many megabytes pass through, so that the codes stay in L2 for what
+  // reads them next (quantising and dequantising 16384 x 4096: 64 -> 58 us)
+  constexpr bool kStream = GROUPS > 1;
   launch_dependents();
   const uint32_t blocks = (cols + 31) / 32, per_row = blocks * 2;
   const int64_t first = (int64_t)blockIdx.x * (256 * GROUPS), row0 = first / per_row;
@@ -127,7 +132,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, 
 #pragma unroll
     for (int k = 0; k < GROUPS; ++k) {
       v[k].clear();
-      if (tid + 256 * k < count) v[k].load(x + (first + tid) * 16 + 4096 * k, 16);
+      if (tid + 256 * k < count) v[k].template load<kStream>(x + (first + tid) * 16 + 4096 * k, 16);
     }
   } else {
     int64_t r = row0 + t0 / per_row;
@@ -137,7 +142,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, 
       v[k].clear();
       const int left = tid + 256 * k < count ? min(cols - (int)g * 16, 16) : 0;
       if (ROWS == ANY) v[k].load_some(x + r * ld + g * 16, left);
-      else v[k].load(x + r * ld + g * 16, left);
+      else v[k].template load<kStream>(x + r * ld + g * 16, left);
       r += rs, g += gs;
       if (g >= per_row) g -= per_row, ++r;
     }
@@ -182,12 +187,19 @@ __device__ __forceinline__ float2 values_of(uint32_t h2, float s) {
   return make_float2(fmaf(f.x, s, 0.0f), fmaf(f.y, s, 0.0f));
 }
 
+template <bool STREAM>
+__device__ __forceinline__ void put(void* dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  if (STREAM) __stcs(static_cast<uint4*>(dst), make_uint4(a, b, c, d));
+  else *static_cast<uint4*>(dst) = make_uint4(a, b, c, d);
+}
+
 // The values of 8 codes a thread: a 4-byte load, 16 or 32 bytes stored, whole
 // lines a warp (rows of the result on 16 bytes, cols a multiple of 8).
 template <typename T, int GROUPS>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restrict__ packed,
                                                          const uint8_t* __restrict__ scales, int64_t rows, int cols,
                                                          T* __restrict__ out) {
+  constexpr bool kStream = GROUPS > 1;   // many megabytes: first to leave L2
   const uint32_t blocks = (cols + 31) / 32, per_row = blocks * 4;
   const int64_t first = (int64_t)blockIdx.x * (256 * GROUPS), row0 = first / per_row;
   const uint32_t rem = (uint32_t)(first - row0 * per_row) + threadIdx.x;
@@ -212,8 +224,9 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restr
     for (int j = 0; j < 4; ++j) v[j] = values_of(h[j], s);
     T* dst = out + row * cols + g * 8;
     if constexpr (sizeof(T) == 4) {
-      reinterpret_cast<float4*>(dst)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
-      reinterpret_cast<float4*>(dst)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+      put<kStream>(dst, __float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
+      put<kStream>(dst + 4, __float_as_uint(v[2].x), __float_as_uint(v[2].y), __float_as_uint(v[3].x),
+                   __float_as_uint(v[3].y));
     } else {
       uint32_t o[4];
 #pragma unroll
@@ -221,7 +234,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restr
         const __nv_bfloat162 b = __floats2bfloat162_rn(v[j].x, v[j].y);
         o[j] = *reinterpret_cast<const uint32_t*>(&b);
       }
-      *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+      put<kStream>(dst, o[0], o[1], o[2], o[3]);
     }
   }
 }
