@@ -13,7 +13,7 @@ import ctypes
 import torch
 
 from . import _abi
-from ._dev import on_device, raw_stream, rows_of, stream_handle
+from ._dev import new_like, on_device, raw_stream, rows_of, stream_handle
 
 _DTYPES = {torch.bfloat16: _abi.DS_BF16, torch.float16: _abi.DS_F16}
 
@@ -57,7 +57,7 @@ def _forward(x, w1, w3, w2, limit, keep: bool):
     """y, and the buffer (pre-activations, h) that the backward pass reads."""
     d, hold = _desc(x, w1, w3, w2, limit)
     lib, ref, dev = _abi.lib(), ctypes.byref(d), x.device
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y = new_like(x)
     kept = h = pre = None
     with on_device(dev):
         if keep:
@@ -92,8 +92,7 @@ def _backward(ctx, dy):
     d, hold = _desc(x, w1, w3, w2, ctx.limit)
     dy, ld = rows_of(dy)
     lib, ref, dev = _abi.lib(), ctypes.byref(d), x.device
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if need else None
-             for t, need in zip((x, w1, w3, w2), ctx.needs_input_grad)]
+    grads = [new_like(t) if need else None for t, need in zip((x, w1, w3, w2), ctx.needs_input_grad)]
     pre, n = kept.data_ptr(), ctypes.c_size_t(0)
     with on_device(dev):
         _abi.check(lib.ds_gated_ffn_backward_workspace_size(ref, dy.data_ptr(), ld, ctypes.byref(n)),

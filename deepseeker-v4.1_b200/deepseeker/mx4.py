@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from . import _abi
-from ._dev import on_device, raw_stream, rows_of, stream_handle
+from ._dev import new_like, on_device, raw_stream, rows_of, stream_handle
 
 BLOCK = 32
 _DTYPES = {torch.float32: _abi.DS_F32, torch.bfloat16: _abi.DS_BF16, torch.float16: _abi.DS_F16}
@@ -206,7 +206,8 @@ def gated_ffn(x, w1: MX4Tensor, w3: MX4Tensor, w2: MX4Tensor, limit: float | Non
         raise ValueError("limit must be positive, or None for no clamps")
     hold, px, pa, dt, rows, ld, out_dtype = _input(x, hidden, out_dtype)
     dev = w1.device
-    out = torch.empty(x.shape, dtype=out_dtype, device=dev)
+    same = dt == _DTYPES[out_dtype]   # x is a tensor of the result's type and shape
+    out = new_like(x) if same else torch.empty(x.shape, dtype=out_dtype, device=dev)
     n = _workspace_bytes(rows, inter) + (0 if dt == _abi.DS_U8 else _x_bytes(rows, hidden))
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     with on_device(dev):
