@@ -15,6 +15,10 @@
 // wait for a few hundred cycles a tile, where tiles of 128 columns (with two
 // accumulators) would ask 94 bytes a cycle of L2 for each SM instead of 64.
 // Lanes are rows: a thread holds whole blocks of h and quantises them alone.
+//
+// 16384 x 4096 to 4096: 107 us, 5.1 PFLOP/s.  Bounded by what reaches the SMs
+// from L2 (1.17 GB; no kernel here gets more than 12 TB/s) and by the
+// accumulator's hand-over; gate / up of 16384 x 4096 x 2048: 110 us.
 #pragma once
 
 #include "mx4.cuh"
