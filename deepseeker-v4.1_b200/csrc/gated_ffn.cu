@@ -35,8 +35,8 @@ enum Mode { GATE_UP, PLAIN, DHID, DX };
 
 template <int MODE>
 struct ModeOf {
-  static constexpr bool kAMn = MODE == DHID || MODE == DX;                // A stored with m running fastest
-  static constexpr int kMats = MODE == GATE_UP ? 2 : 1;                      // accumulators (W1 and W3 share x)
+  static constexpr bool kAMn = MODE == DHID || MODE == DX;                 // A stored with m running fastest
+  static constexpr int kMats = MODE == GATE_UP ? 2 : 1;                    // accumulators (W1 and W3 share x)
   static constexpr int kSegs = MODE == DX ? 2 : 1;                         // dg W1 and du W3 in one accumulator
 };
 
@@ -48,7 +48,7 @@ struct TileParams {
   int K;                       // contraction of one segment
   int f16;
   float limit;
-  float* g;                    // f32 pre-activations [n * ldp + m]: written (GATED, may be null), read (DHID)
+  float* g;                    // f32 pre-activations [n * ldp + m]: written (GATE_UP, may be null), read (DHID)
   float* u;
   int64_t ldp;
   int* err;

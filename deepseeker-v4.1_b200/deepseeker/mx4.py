@@ -133,7 +133,8 @@ def from_packed(packed: torch.Tensor, scales: torch.Tensor, cols: int | None = N
     """MX4Tensor over stored codes u8 [rows, 16 ceil(cols/32)] and scales u8
     [rows, ceil(cols/32)] (used in place where contiguous; the scale atoms are
     built once here, so scales that change later need a new MX4Tensor).
-    ``cols`` defaults to 32 per scale."""
+    ``cols`` defaults to 32 per scale; the codes behind an uneven end have to
+    be 0, as ``quantize`` leaves them: products add them up."""
     for name, t in (("packed", packed), ("scales", scales)):
         if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.uint8 or t.dim() != 2:
             raise ValueError(f"{name} must be a 2-D u8 CUDA tensor")
