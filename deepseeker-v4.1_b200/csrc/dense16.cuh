@@ -113,6 +113,119 @@ __device__ __forceinline__ void gate_grad(float g, float u, float dh, float limi
   }
 }
 
+// ---------------------------------------------------------------- values close to the limit
+//
+// The derivative of a clamp jumps at the limit, so which side of it an exact
+// sum lies on decides over a whole gradient.  The tensor core's sum may lie on
+// the other side: each step of 16 along the contraction cuts what its partial
+// sum holds below f32's last place, and some of the products that it aligns.
+// With S = |x_t|_2 |w_i|_2, which bounds the products' magnitudes together, a
+// sum that ends near L has partial sums up to (S + L) / 2, and the errors of
+// its n steps stay below (n + 1) 2^-23 (S + L): measured are 0.37 of that for
+// products of one sign, 0.02 for normal data of 4096 terms.  Values no further
+// than that from the limit are added up again in 64 bits by a warp (products
+// of 16-bit values are exact in f32) and stored on the side where they belong.
+// Only the stored g and u change: h is continuous at the limit.
+//
+// The tile kernel settles them itself.  The pair kernel lists them for a launch
+// of their own: unit variance and a limit of 1.5 leave one value in 640 of 8192
+// x 4096 x 2048 (a limit of 10 none), and its few epilogue warps would take 320
+// us for what the whole GPU does in 55.  Where the list overflows, that launch
+// looks through all stored values instead.
+
+struct Near {
+  const uint16_t* x;           // null: no clamps, or nothing is kept
+  const uint16_t* w[2];        // W1, W3
+  int64_t ldx, ldw[2];         // multiples of 8, bases on 16 bytes
+  const float* nx;             // 2-norms of the rows of x, W1 and W3
+  const float* nw[2];
+  int K, f16;
+  float limit, per;            // per: largest error of a sum, in units of S + L
+  uint64_t* list;              // pair kernel: i | z << 31 | t << 32 of values to be settled
+  unsigned long long* count;   // how many there are, those without room included
+  uint32_t room;
+};
+
+__device__ __forceinline__ float from16(uint32_t bits, int f16) {
+  return f16 ? __half2float(__ushort_as_half((uint16_t)bits)) : __uint_as_float(bits << 16);
+}
+
+// The exact sum for row t of x and row i of matrix z, by a warp, up to the
+// rounding of 64-bit additions.
+__device__ __forceinline__ double near_sum(const Near& p, int z, int64_t t, int64_t i) {
+  const uint16_t *a = p.x + t * p.ldx, *b = z ? p.w[1] + i * p.ldw[1] : p.w[0] + i * p.ldw[0];
+  const int lane = threadIdx.x & 31;
+  double even = 0.0, odd = 0.0;
+#pragma unroll 4
+  for (int k = lane * 8; k + 8 <= p.K; k += 256) {
+    const uint4 va = *reinterpret_cast<const uint4*>(a + k), vb = *reinterpret_cast<const uint4*>(b + k);
+    const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      even += (double)(from16(wa[j] & 0xFFFFu, p.f16) * from16(wb[j] & 0xFFFFu, p.f16));
+      odd += (double)(from16(wa[j] >> 16, p.f16) * from16(wb[j] >> 16, p.f16));
+    }
+  }
+  const int k = p.K / 8 * 8 + lane;   // an uneven end
+  if (k < p.K) even += (double)(from16(a[k], p.f16) * from16(b[k], p.f16));
+  even += odd;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) even += __shfl_xor_sync(0xffffffffu, even, o);
+  return even;
+}
+
+// A settled value: rounded away from or towards zero, so that it does not
+// cross the limit.
+__device__ __forceinline__ float near_round(double v, float limit) {
+  return fabs(v) <= (double)limit ? __double2float_rz(v) : v > 0 ? __double2float_ru(v) : __double2float_rd(v);
+}
+
+// How far from the limit a value is settled; a norm that is no number or
+// passes f32 settles nothing (the sums are then no numbers either).
+__device__ __forceinline__ float near_band(const Near& p, float nx, float nw) {
+  const float b = p.per * (nx * nw + p.limit);
+  return b <= 3.0e38f ? b : -1.0f;
+}
+__device__ __forceinline__ bool near_g(const Near& p, float g, float band) { return fabsf(g - p.limit) <= band; }
+__device__ __forceinline__ bool near_u(const Near& p, float u, float band) { return fabsf(fabsf(u) - p.limit) <= band; }
+
+// Settles the values of a warp whose bits are set in `near`, one after the
+// other by all lanes.  at(lane, bit): row of x and row of the matrix;
+// put(bit, v): the lane that the value belongs to keeps it.
+template <typename At, typename Put>
+__device__ __forceinline__ void near_settle(const Near& p, int z, uint32_t near, At at, Put put) {
+  const int lane = threadIdx.x & 31;
+  for (uint32_t any; (any = __ballot_sync(0xffffffffu, near != 0)) != 0;) {
+    const int src = __ffs(any) - 1, bit = __ffs(__shfl_sync(0xffffffffu, near, src)) - 1;
+    int64_t t, i;
+    at(src, bit, t, i);
+    const double v = near_sum(p, z, t, i);
+    if (lane != src) continue;
+    put(bit, near_round(v, p.limit));
+    near &= near - 1;
+  }
+  __syncwarp();
+}
+
+// Lists the values of a warp whose bits are set in near[0] and near[1] (lane:
+// row t of x, bit: row i0 + bit of the matrix), as far as there is room.
+__device__ __forceinline__ void near_list(const Near& p, uint32_t (&near)[2], int64_t t, int i0) {
+  const int lane = threadIdx.x & 31, mine = __popc(near[0]) + __popc(near[1]);
+  if (!__any_sync(0xffffffffu, mine)) return;
+  uint32_t at = mine;                    // this lane's values end at `at`
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_up_sync(0xffffffffu, at, o);
+    if (lane >= o) at += v;
+  }
+  unsigned long long to = lane == 31 ? atomicAdd(p.count, (unsigned long long)at) : 0ull;
+  to = __shfl_sync(0xffffffffu, to, 31) + at - mine;
+#pragma unroll
+  for (int z = 0; z < 2; ++z)
+    for (; near[z] && to < p.room; near[z] &= near[z] - 1)
+      p.list[to++] = (uint64_t)t << 32 | (uint32_t)z << 31 | (uint32_t)(i0 + __ffs(near[z]) - 1);
+}
+
 // f32 -> 16-bit (round to nearest even), the low half of the result.
 __device__ __forceinline__ uint16_t to16(float v, int f16) {
   return f16 ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));

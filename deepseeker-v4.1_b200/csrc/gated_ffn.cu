@@ -8,7 +8,11 @@
 // in f32 between the passes, so that the gated unit and its derivative see
 // no rounded input; h, dg and du are rounded once to the 16-bit type, because
 // they are tensor-core operands of the next product (one rounding there adds
-// as much error as the rounding of the result itself).
+// as much error as the rounding of the result itself).  With clamps, g and u
+// too close to the limit for a f32 sum are settled in 64 bits (Near), as a
+// derivative that is there or not depends on it: 900 us instead of 877 for a
+// training step of 8192 x 4096 x 2048 with a limit of 10 (21 of them for the
+// row norms), 940 with one of 1.5 and pre-activations of unit variance.
 //
 // Tile kernel (up to 128 rows): one CTA computes 128 features (the MMA's
 // lanes) of all tokens over a slice of the contraction.
@@ -51,6 +55,7 @@ struct TileParams {
   float* g;                    // f32 pre-activations [n * ldp + m]: written (GATE_UP, may be null), read (DHID)
   float* u;
   int64_t ldp;
+  Near near;                   // GATE_UP
   int* err;
 };
 
@@ -75,7 +80,8 @@ struct TileShape {
 constexpr int kTileThreads = 320;   // warp 0 copies, warp 1 MMA, warps 2-9 epilogue (two a lane quarter)
 
 // What becomes of the elements (m, n0 .. n0 + J - 1) of the accumulator(s), nv
-// of them inside the result.  Lanes are features, so a warp's accesses are
+// of them inside the result (none for a feature outside; whole warps call).
+// Lanes are features, so a warp's accesses are
 // runs of 32; all reads come before the first write, which could alias them
 // for all the compiler knows (one column after the other, the reads' latency
 // made the hidden gradient of 1024 x 4096 x 2048 five times slower).
@@ -110,6 +116,23 @@ __device__ __forceinline__ void tile_store(const TileParams& p, int m, int n0, i
       }
       out[j * p.ldo] = to16(MODE == GATE_UP ? gate_unit(v0[j], v1[j], p.limit) : v0[j], p.f16);
     }
+    if constexpr (MODE == GATE_UP) {
+      if (!p.near.x) return;
+#pragma unroll 1
+      for (int z = 0; z < 2; ++z) {
+        const float nw = nv > 0 ? p.near.nw[z][m] : 0.0f;
+        uint32_t near = 0;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          if (j >= nv) continue;
+          const float band = near_band(p.near, p.near.nx[n0 + j], nw);
+          near |= (uint32_t)(z ? near_u(p.near, v1[j], band) : near_g(p.near, v0[j], band)) << j;
+        }
+        near_settle(p.near, z, near,
+                    [&](int src, int bit, int64_t& t, int64_t& i) { t = n0 + bit, i = m - (int)(threadIdx.x & 31) + src; },
+                    [&](int bit, float v) { (z ? p.u : p.g)[at + bit * p.ldp] = v; });
+      }
+    }
   }
 }
 
@@ -139,7 +162,7 @@ __device__ __forceinline__ void tile_join(const TileParams& p, float* part, int 
       for (int t = 0; t < kMats; ++t)
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[t][j] += w[r][t][j];
-    tile_store<MODE>(p, m, n, end - n, v[0], v[1]);
+    tile_store<MODE>(p, m, n, m < p.M ? end - n : 0, v[0], v[1]);
   }
 }
 
@@ -252,14 +275,14 @@ __global__ void __launch_bounds__(kTileThreads, NT == 128 ? 1 : 2) tile_kernel(c
         for (int t = 0; t < Md::kMats; ++t)
 #pragma unroll
           for (int j = 0; j < 16; ++j) part[(t * NT + c0 + j) * 128 + mi] = v[t][j];
-      } else if (m < p.M) {
-        tile_store<MODE>(p, m, c0, p.N - c0, v[0], v[Md::kMats - 1]);
+      } else {
+        tile_store<MODE>(p, m, c0, m < p.M ? p.N - c0 : 0, v[0], v[Md::kMats - 1]);
       }
     }
   }
   if (slices > 1) {
     cluster.sync();
-    if (warp >= 2 && m < p.M) {
+    if (warp >= 2) {
       if (slices == 8) tile_join<MODE, NT, 8>(p, part, slice, turn, m, mi);
       else if (slices == 4) tile_join<MODE, NT, 4>(p, part, slice, turn, m, mi);
       else tile_join<MODE, NT, 2>(p, part, slice, turn, m, mi);
@@ -299,6 +322,94 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackParams p) {
     for (int j = 0; j < 8; ++j)
       if (c + j < cols) w[j >> 1] |= (uint32_t)src[j] << (16 * (j & 1));
     *reinterpret_cast<uint4*>(p.dst[z] + r * ldd + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// ---------------------------------------------------------------- values close to the limit
+
+// 2-norms of the rows of x, W1 and W3, a warp a row, rather 2^-10 too large
+// than too small: how far a sum may be off (Near).  Memory-bound: 100 MB in 21
+// us for 8192 x 4096 x 2048.  Empties the list.
+struct NormParams {
+  const uint16_t* p[3];
+  int64_t ld[3];
+  int64_t end[3];              // rows so far, in the order of the norms
+  int K, f16;
+  float* out;
+  unsigned long long* count;
+};
+
+__device__ __forceinline__ float sum_squares(const uint16_t* row, int K, int f16, float scale) {
+  const int lane = threadIdx.x & 31;
+  float s = 0.0f;
+#pragma unroll 4
+  for (int k = lane * 8; k + 8 <= K; k += 256) {
+    const uint4 v = *reinterpret_cast<const uint4*>(row + k);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float a = from16(w[j] & 0xFFFFu, f16) * scale, b = from16(w[j] >> 16, f16) * scale;
+      s = fmaf(a, a, fmaf(b, b, s));
+    }
+  }
+  const int k = K / 8 * 8 + lane;   // an uneven end
+  if (k < K) {
+    const float a = from16(row[k], f16) * scale;
+    s = fmaf(a, a, s);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
+__global__ void __launch_bounds__(256) norm_kernel(const NormParams p) {
+  launch_dependents();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.count = 0ull;
+  const int64_t r = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5);
+  if (r >= p.end[2]) return;
+  const uint16_t* row = r < p.end[0]   ? p.p[0] + r * p.ld[0]
+                        : r < p.end[1] ? p.p[1] + (r - p.end[0]) * p.ld[1]
+                                       : p.p[2] + (r - p.end[1]) * p.ld[2];
+  float s = 0.0f, scale = 1.0f;
+  // a sum past f32's range (either end): again with the row brought inside
+  for (int pass = 0; pass < 2; ++pass) {
+    s = sum_squares(row, p.K, p.f16, scale);
+    if (pass || (s >= 1e-30f && s <= 1e37f)) break;
+    scale = s < 1e-30f ? 0x1p70f : 0x1p-70f;
+  }
+  if ((threadIdx.x & 31) == 0) p.out[r] = sqrtf(s) / scale * (1.0f + 0x1p-10f);
+}
+
+// The listed values, a warp each, into the kept pre-activations [2][rows][ldp].
+// More than the list holds: each warp goes through whole rows.
+__global__ void __launch_bounds__(256) settle_kernel(const Near p, float* pre, int64_t ldp, int rows, int cols) {
+  launch_dependents();
+  wait_prior_grid();
+  const int lane = threadIdx.x & 31;
+  const int64_t plane = rows * ldp, warp = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5), warps = gridDim.x * (int64_t)8;
+  const unsigned long long n = *p.count;
+  if (n <= p.room) {
+    for (int64_t e = warp; e < (int64_t)n; e += warps) {
+      const uint64_t v = p.list[e];
+      const int64_t t = (int64_t)(v >> 32), i = (int64_t)(v & 0x7FFFFFFFu);
+      const int z = (int)(v >> 31 & 1);
+      const float settled = near_round(near_sum(p, z, t, i), p.limit);
+      if (lane == 0) pre[z * plane + t * ldp + i] = settled;
+    }
+    return;
+  }
+  for (int64_t e = warp; e < 2 * (int64_t)rows; e += warps) {
+    const int z = e >= rows;
+    const int64_t row = e - (z ? rows : 0);
+    const float nx = p.nx[row], *nw = z ? p.nw[1] : p.nw[0];
+    for (int c0 = 0; c0 < cols; c0 += 32) {
+      const int c = c0 + lane;
+      float* at = pre + z * plane + row * ldp + c;
+      uint32_t near = 0;
+      if (c < cols) near = z ? near_u(p, *at, near_band(p, nx, nw[c])) : near_g(p, *at, near_band(p, nx, nw[c]));
+      near_settle(p, z, near, [&](int src, int, int64_t& t, int64_t& i) { t = row, i = c0 + src; },
+                  [&](int, float v) { *at = v; });
+    }
   }
 }
 
@@ -520,14 +631,74 @@ Parts parts_of(const DsGatedFfn* d) {
 
 size_t mid_bytes(const DsGatedFfn* d) { return grouped::up((size_t)d->tokens * up8(d->inter) * 2, 256); }
 
-size_t forward_bytes(const DsGatedFfn* d, bool own_h) {
+// The operands' packed copies.
+size_t packed_bytes(const DsGatedFfn* d) {
   const Parts o = parts_of(d);
-  return copy_bytes(o.x) + copy_bytes(o.w1) + copy_bytes(o.w3) + copy_bytes(o.w2) + (own_h ? mid_bytes(d) : 0);
+  return copy_bytes(o.x) + copy_bytes(o.w1) + copy_bytes(o.w3) + copy_bytes(o.w2);
+}
+
+// Values close to the limit that are listed before they are settled: one in
+// 32, far more than data leaves there by chance; none for the tile kernel.
+size_t near_room(const DsGatedFfn* d) {
+  return d->tokens < kPairRows ? 0 : std::min<size_t>((size_t)d->tokens * d->inter / 32, 1u << 30);
+}
+
+size_t norm_bytes(const DsGatedFfn* d) {
+  return grouped::up((size_t)(d->tokens + 2 * (int64_t)d->inter) * 4, 256);
+}
+
+// With clamps: row norms of x, W1 and W3, the list and its length.
+size_t near_bytes(const DsGatedFfn* d) {
+  return d->limit > 0.0f ? norm_bytes(d) + 256 + grouped::up(near_room(d) * 8, 256) : 0;
+}
+
+size_t forward_bytes(const DsGatedFfn* d, bool own_h) {
+  return packed_bytes(d) + near_bytes(d) + (own_h ? mid_bytes(d) : 0);
 }
 
 size_t backward_bytes(const DsGatedFfn* d, const void* dy, int64_t ld_dy) {
   const Operand g = {dy, d->tokens, d->hidden, ld_dy};
-  return forward_bytes(d, false) + copy_bytes(g) + 2 * mid_bytes(d);
+  return packed_bytes(d) + copy_bytes(g) + 2 * mid_bytes(d);
+}
+
+// What settles the kept pre-activations that lie close to the limit; the
+// launch that writes them is chained to the one of the norms.
+int prepare_near(Near& p, const DsGatedFfn* d, const Parts& o, char* ws, cudaStream_t s) {
+  const int64_t T = d->tokens, I = d->inter;
+  float* norms = reinterpret_cast<float*>(ws);
+  p.count = reinterpret_cast<unsigned long long*>(ws + norm_bytes(d));
+  p.list = reinterpret_cast<uint64_t*>(ws + norm_bytes(d) + 256);
+  p.room = (uint32_t)near_room(d);
+  NormParams n = {};
+  const Operand* const rows[3] = {&o.x, &o.w1, &o.w3};
+  for (int z = 0; z < 3; ++z) {
+    n.p[z] = static_cast<const uint16_t*>(rows[z]->p), n.ld[z] = rows[z]->ld;
+    n.end[z] = T + z * I;
+  }
+  n.K = d->hidden, n.f16 = d->dtype == DS_F16, n.out = norms, n.count = p.count;
+  norm_kernel<<<(unsigned)((n.end[2] + 7) / 8), 256, 0, s>>>(n);
+  DS_CHECK_LAUNCH("norm_kernel");
+  p.x = n.p[0], p.w[0] = n.p[1], p.w[1] = n.p[2];
+  p.ldx = n.ld[0], p.ldw[0] = n.ld[1], p.ldw[1] = n.ld[2];
+  p.nx = norms, p.nw[0] = norms + T, p.nw[1] = norms + T + I;
+  p.K = n.K, p.f16 = n.f16, p.limit = d->limit;
+  p.per = (float)((d->hidden + 15) / 16 + 1) * 0x1p-23f;
+  return DS_OK;
+}
+
+// Settles what the launch before has listed.
+int settle_listed(const Near& p, float* pre, int64_t ldp, int rows, int cols, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>((p.room + 7) / 8, (int64_t)ds::sm_count() * 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  DS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, settle_kernel, p, pre, ldp, rows, cols));
+  return DS_OK;
 }
 
 }  // namespace
@@ -558,6 +729,10 @@ extern "C" int ds_gated_ffn(const DsGatedFfn* desc, void* y, void* h, float* pre
   char* ws = static_cast<char*>(workspace);
   Parts o = parts_of(desc);
   if ((st = place({&o.x, &o.w1, &o.w3, &o.w2}, ws, s)) != DS_OK) return st;
+  Near near = {};
+  const bool clamped = pre && desc->limit > 0.0f;
+  if (clamped && (st = prepare_near(near, desc, o, ws, s)) != DS_OK) return st;
+  ws += near_bytes(desc);
   if (!h) h = ws;
   const int64_t ldm = up8(I);
   int* err = err_word();
@@ -568,12 +743,13 @@ extern "C" int ds_gated_ffn(const DsGatedFfn* desc, void* y, void* h, float* pre
 
   if (T >= kPairRows) {
     PairParams p = {};
-    p.f16 = f16, p.limit = desc->limit, p.err = err, p.keep = pre != nullptr;
+    p.f16 = f16, p.limit = desc->limit, p.err = err, p.keep = pre != nullptr, p.near = near;
     Sides up[1] = {{add(p, GATED, T, I, H, 1, h, ldm), o.x, o.w1, none, o.w3}};
     DS_REQUIRE(map_slim(&p.h, h, T, I, ldm) &&
                    (!pre || (map32(&p.g, pre, T, I, ldm) && map32(&p.u, pre_u, T, I, ldm))),
                DS_ECUDA, "gated_ffn: tensor map encoding failed (h, pre-activations)");
-    if ((st = run_pairs<GATED>(p, up, s, false)) != DS_OK) return st;
+    if ((st = run_pairs<GATED>(p, up, s, clamped)) != DS_OK) return st;
+    if (near.room && (st = settle_listed(near, pre, ldm, T, I, s)) != DS_OK) return st;
     PairParams d = {};
     d.f16 = f16, d.err = err;
     Sides down[1] = {{add(d, STORE, T, H, I, 1, y, H), oh, o.w2, none, none}};
@@ -587,8 +763,8 @@ extern "C" int ds_gated_ffn(const DsGatedFfn* desc, void* y, void* h, float* pre
   DS_REQUIRE(ok, DS_ECUDA, "gated_ffn: tensor map encoding failed (gate / up)");
   p.M = I, p.N = T, p.K = H;
   p.out[0] = h, p.ldo = ldm;
-  p.g = pre, p.u = pre_u, p.ldp = ldm;
-  if ((st = run_tiles<GATE_UP>(p, nt, s, false)) != DS_OK) return st;
+  p.g = pre, p.u = pre_u, p.ldp = ldm, p.near = near;
+  if ((st = run_tiles<GATE_UP>(p, nt, s, clamped)) != DS_OK) return st;
   ok = map16(&p.a[0], o.w2.p, H, I, o.w2.ld, 128) && map16(&p.b[0], h, T, I, ldm, nt);
   DS_REQUIRE(ok, DS_ECUDA, "gated_ffn: tensor map encoding failed (down)");
   p.M = H, p.K = I;

@@ -54,6 +54,7 @@ struct PairParams {
   CUtensorMap g, u;            // f32 pre-activations, boxes of 32 x 32
   CUtensorMap dg, du, h;       // results of HIDDEN and GATED, boxes of 32 x 32
   int keep;                    // GATED: write them
+  Near near;
   int f16;
   float limit;
   int* err;
@@ -110,6 +111,27 @@ __device__ __forceinline__ void slim_put(uint8_t* box, int lane, const float (&v
     *reinterpret_cast<uint4*>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
         make_uint4(pack16(v[8 * c], v[8 * c + 1], f16), pack16(v[8 * c + 2], v[8 * c + 3], f16),
                    pack16(v[8 * c + 4], v[8 * c + 5], f16), pack16(v[8 * c + 6], v[8 * c + 7], f16));
+}
+
+// Lists the values of 32 rows (lane = row, from m0 on) and `cols` columns (from
+// n0 on) that lie close to the limit.  The distance goes by the largest weight
+// norm of the columns.
+__device__ __forceinline__ void near_find(const Near& p, int lane, const float (&g)[32], const float (&u)[32], int m0,
+                                          int rows, int n0, int cols) {
+  const bool row = m0 + lane < rows;
+  const float nx = row ? p.nx[m0 + lane] : 0.0f;
+  uint32_t near[2] = {0u, 0u};
+#pragma unroll
+  for (int z = 0; z < 2; ++z) {
+    // bits of non-negative values (and of NaN above them) order as the values
+    const uint32_t w = lane < cols ? __float_as_uint(p.nw[z][n0 + lane]) : 0u;
+    const float band = near_band(p, nx, __uint_as_float(__reduce_max_sync(0xffffffffu, w)));
+#pragma unroll
+    for (int j = 0; j < 32; ++j) near[z] |= (uint32_t)(z ? near_u(p, u[j], band) : near_g(p, g[j], band)) << j;
+    near[z] &= cols < 32 ? (1u << cols) - 1u : 0xffffffffu;
+    if (!row) near[z] = 0u;
+  }
+  near_list(p, near, m0 + lane, n0);
 }
 
 // The i-th tile of pair c.  Group 0 is dealt round robin.  A tile of group 1
@@ -326,6 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) pair_ke
             __syncwarp();
             box_put(box0, lane, gv);
             box_put(box1, lane, uv);
+            if (p.near.x) near_find(p.near, lane, gv, uv, mw, q.M, n0 + c, nc - c);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {

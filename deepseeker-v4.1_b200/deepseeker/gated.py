@@ -115,7 +115,8 @@ def gated_ffn(x: torch.Tensor, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Ten
     (both sides), as in ``moe_layer``; None for none.  Differentiable in x and
     the weights: between the passes the block keeps h (16 bits) and both
     pre-activations (f32), 10 bytes per token and intermediate feature.  The
-    gradient of a clamped value is 0.
+    gradient of a clamped value is 0, that of one that equals the limit (taken
+    in f32) is not; the exact sums decide, not their f32 rounding.
     """
     hidden = _check(x, w1, w3, w2, limit)
     rows = x if x.dim() == 2 else x.reshape(-1, hidden)

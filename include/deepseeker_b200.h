@@ -424,7 +424,10 @@ int ds_ep_destroy(DsEp* ep);
  *   g = x W1^T, u = x W3^T, h = silu(min(g, L)) * clip(u, -L, L), y = h W2^T.
  * Products accumulate in f32; h and the gradients of g and u are rounded once
  * to the 16-bit type, g and u are kept in f32 between the passes.  NaN passes
- * through the clamps.  Any sizes, row strides and 2-byte alignments; operands
+ * through the clamps.  A clamped value has no gradient, one that equals the
+ * limit has one, and the exact sums decide: with clamps, kept values of g and u
+ * that f32 sums cannot place are summed up in 64 bits and stored on the side of
+ * the limit where they belong.  Any sizes, row strides and 2-byte alignments; operands
  * whose base is no multiple of 16 bytes or whose row stride is no multiple of
  * 8 elements are first copied into the workspace.  Results do not depend on
  * timing (no atomics). */
