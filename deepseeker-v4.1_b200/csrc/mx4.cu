@@ -785,7 +785,7 @@ int validate_weight(const DsMx4* w, const char* what) {
 }
 
 int validate_x(const void* x, const uint8_t* atoms, int dtype, int64_t rows, int cols, int64_t ld, const char* what) {
-  DS_REQUIRE(dtype == DS_F32 || dtype == DS_BF16 || dtype == DS_F16 || (dtype == DS_U8 && atoms), DS_EINVAL,
+  DS_REQUIRE(dtype == DS_F32 || dtype == DS_BF16 || dtype == DS_F16 || (dtype == DS_U8 && (rows == 0 || atoms)), DS_EINVAL,
              "%s: x must be f32, bf16 or f16, or codes (u8) with atoms", what);
   DS_REQUIRE(rows >= 0 && rows <= (1 << 22), DS_ERANGE, "%s: rows must be in [0, 2^22]", what);
   DS_REQUIRE(rows == 0 || x, DS_EINVAL, "%s: null x", what);
