@@ -6,6 +6,7 @@ import ctypes
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 
 def stream_handle(device: torch.device | None = None) -> ctypes.c_void_p:
@@ -42,6 +43,12 @@ def rows_of(t: torch.Tensor) -> tuple[torch.Tensor, int]:
 def new_like(t: torch.Tensor) -> torch.Tensor:
     """A contiguous tensor of t's shape and type (empty_like takes a third of empty's time and keeps strides)."""
     return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def has_tangent(*ts) -> bool:
+    """Whether one of `ts` carries a forward-mode derivative, which a result made through the C ABI would lose."""
+    return forward_ad._current_level >= 0 and any(
+        isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
 def ptr(t: torch.Tensor | None) -> ctypes.c_void_p:

@@ -4,7 +4,8 @@
 
 the block that a layer's shared expert or a layer without routing evaluates
 (the reference's ``shared_fn``, src/deepseeker/mlx_runner.py:776-781), for
-prompts, single tokens and training.  ``gated_ffn`` takes part in autograd.
+prompts, single tokens and training.  ``gated_ffn`` takes part in autograd
+(reverse mode; operands with forward-mode derivatives are refused).
 """
 from __future__ import annotations
 
@@ -13,7 +14,7 @@ import ctypes
 import torch
 
 from . import _abi
-from ._dev import new_like, on_device, raw_stream, rows_of, stream_handle
+from ._dev import has_tangent, new_like, on_device, raw_stream, rows_of, stream_handle
 
 _DTYPES = {torch.bfloat16: _abi.DS_BF16, torch.float16: _abi.DS_F16}
 
@@ -32,6 +33,8 @@ def _check(x, w1, w3, w2, limit) -> int:
         raise ValueError("hidden and inter must be at least 1")
     if limit is not None and not limit > 0:
         raise ValueError("limit must be positive, or None for no clamps")
+    if has_tangent(x, w1, w3, w2):
+        raise ValueError("gated_ffn has no forward-mode derivatives: an operand is a dual tensor")
     return hidden
 
 

@@ -5,7 +5,8 @@
   linear       x W^T on the tensor cores' 4-bit rate, x quantised on the way or already
   gated_ffn    the gated block (deepseeker.gated) over quantised weights
 
-Serving only: the results have no gradients, and an input that asks for one is refused.
+Serving only: the results have no derivatives, and an input that asks for one
+(a gradient, or a forward-mode tangent) is refused.
 """
 from __future__ import annotations
 
@@ -14,7 +15,7 @@ import ctypes
 import torch
 
 from . import _abi
-from ._dev import new_like, on_device, raw_stream, rows_of, stream_handle
+from ._dev import has_tangent, new_like, on_device, raw_stream, rows_of, stream_handle
 
 BLOCK = 32
 _DTYPES = {torch.float32: _abi.DS_F32, torch.bfloat16: _abi.DS_BF16, torch.float16: _abi.DS_F16}
@@ -102,6 +103,8 @@ def _check_x(x) -> None:
         raise ValueError("x must be [..., cols] with at least one column")
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("4-bit operators have no backward pass: detach x or use torch.no_grad()")
+    if has_tangent(x):
+        raise ValueError("4-bit operators have no forward-mode derivatives: x is a dual tensor")
 
 
 def _matrix(x):
