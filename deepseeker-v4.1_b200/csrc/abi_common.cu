@@ -62,6 +62,20 @@ int* symbol_address(SymbolOnce* known, const void* symbol) {
   return static_cast<int*>(p);
 }
 
+namespace {
+__global__ void take_word_kernel(int* word, int* out) { *out = atomicExch(word, 0); }
+}  // namespace
+
+int take_error_word(int* word, int32_t* err, cudaStream_t s) {
+  int* got = nullptr;
+  DS_CHECK_CUDA(cudaMallocAsync(reinterpret_cast<void**>(&got), sizeof(int), s));
+  take_word_kernel<<<1, 1, 0, s>>>(word, got);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) e = cudaMemcpyAsync(err, got, sizeof(int), cudaMemcpyDefault, s);
+  const cudaError_t freed = cudaFreeAsync(got, s);
+  return e != cudaSuccess ? cuda_status(e, "take_error_word") : freed != cudaSuccess ? cuda_status(freed, "take_error_word") : DS_OK;
+}
+
 }  // namespace ds
 
 extern "C" const char* ds_last_error_string(void) { return g_last_error; }

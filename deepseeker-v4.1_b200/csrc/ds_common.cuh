@@ -47,6 +47,11 @@ struct SymbolOnce {
 };
 int* symbol_address(SymbolOnce* known, const void* symbol);
 
+// Reads an error word on the device into *err (host or device memory) and
+// clears it, in one atomic step: what a kernel on another stream reports
+// meanwhile is in this answer or in the next.
+int take_error_word(int* word, int32_t* err, cudaStream_t s);
+
 }  // namespace ds
 
 #define DS_CHECK_CUDA(expr)                                           \

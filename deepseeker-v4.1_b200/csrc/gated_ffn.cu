@@ -892,8 +892,5 @@ extern "C" int ds_gated_ffn_status(int32_t* err, void* stream) {
   DS_REQUIRE(err != nullptr, DS_EINVAL, "gated_ffn_status: null output");
   int* w = err_word();
   DS_REQUIRE(w != nullptr, DS_ECUDA, "gated_ffn_status: error word unavailable");
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  DS_CHECK_CUDA(cudaMemcpyAsync(err, w, sizeof(int), cudaMemcpyDefault, s));
-  DS_CHECK_CUDA(cudaMemsetAsync(w, 0, sizeof(int), s));
-  return DS_OK;
+  return ds::take_error_word(w, err, static_cast<cudaStream_t>(stream));
 }

@@ -459,8 +459,9 @@ int ds_gated_ffn_backward(const DsGatedFfn* desc, const void* h, const float* pr
                           int64_t ld_dy, void* dx, void* dw1, void* dw3, void* dw2, void* workspace,
                           size_t workspace_bytes, void* stream);
 /* Copies the current device's error word of these calls into *err (host or
- * device memory; read it after the stream has finished) and clears it.  Bit 1:
- * a bounded device wait gave up, and that call's outputs are undefined. */
+ * device memory; read it after the stream has finished) and clears it, in one
+ * step: a call on another stream that gives up meanwhile is in this answer or in
+ * the next.  Bit 1: a bounded device wait gave up, and that call's outputs are undefined. */
 int ds_gated_ffn_status(int32_t* err, void* stream);
 
 /* ---------------------------------------------------------------------------
