@@ -9,6 +9,10 @@ import torch
 from torch.autograd import forward_ad
 
 
+#: A clamp's limit is above this: what is not rounds to 0 in f32, which stands for no clamps.
+LEAST_LIMIT = 2.0 ** -150
+
+
 def stream_handle(device: torch.device | None = None) -> ctypes.c_void_p:
     """cudaStream_t of torch's current stream on `device`."""
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)

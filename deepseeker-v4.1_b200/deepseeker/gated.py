@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from . import _abi
-from ._dev import has_tangent, new_like, on_device, raw_stream, rows_of, stream_handle
+from ._dev import LEAST_LIMIT, has_tangent, new_like, on_device, raw_stream, rows_of, stream_handle
 
 _DTYPES = {torch.bfloat16: _abi.DS_BF16, torch.float16: _abi.DS_F16}
 
@@ -31,8 +31,8 @@ def _check(x, w1, w3, w2, limit) -> int:
         raise ValueError("x [..., H], w1 [I, H], w3 [I, H], w2 [H, I] expected")
     if hidden < 1 or inter < 1:
         raise ValueError("hidden and inter must be at least 1")
-    if limit is not None and not limit > 0:
-        raise ValueError("limit must be positive, or None for no clamps")
+    if limit is not None and not limit > LEAST_LIMIT:
+        raise ValueError("limit must be positive in f32, or None for no clamps")
     if has_tangent(x, w1, w3, w2):
         raise ValueError("gated_ffn has no forward-mode derivatives: an operand is a dual tensor")
     return hidden

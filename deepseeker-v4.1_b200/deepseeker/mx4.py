@@ -15,7 +15,7 @@ import ctypes
 import torch
 
 from . import _abi
-from ._dev import has_tangent, new_like, on_device, raw_stream, rows_of, stream_handle
+from ._dev import LEAST_LIMIT, has_tangent, new_like, on_device, raw_stream, rows_of, stream_handle
 
 BLOCK = 32
 _DTYPES = {torch.float32: _abi.DS_F32, torch.bfloat16: _abi.DS_BF16, torch.float16: _abi.DS_F16}
@@ -206,8 +206,8 @@ def gated_ffn(x, w1: MX4Tensor, w3: MX4Tensor, w2: MX4Tensor, limit: float | Non
     hidden, inter = w1.cols, w1.rows
     if w3.shape != w1.shape or w2.shape != (hidden, inter):
         raise ValueError("w1 [I, H], w3 [I, H], w2 [H, I] expected")
-    if limit is not None and not limit > 0:
-        raise ValueError("limit must be positive, or None for no clamps")
+    if limit is not None and not limit > LEAST_LIMIT:
+        raise ValueError("limit must be positive in f32, or None for no clamps")
     hold, px, pa, dt, rows, ld, out_dtype = _input(x, hidden, out_dtype)
     dev = w1.device
     same = dt == _DTYPES[out_dtype]   # x is a tensor of the result's type and shape
