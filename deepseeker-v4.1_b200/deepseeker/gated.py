@@ -17,6 +17,7 @@ from . import _abi
 from ._dev import LEAST_LIMIT, has_tangent, new_like, on_device, raw_stream, rows_of, stream_handle
 
 _DTYPES = {torch.bfloat16: _abi.DS_BF16, torch.float16: _abi.DS_F16}
+_MOST = 1 << 17   # hidden, inter
 
 
 def _check(x, w1, w3, w2, limit) -> int:
@@ -29,8 +30,8 @@ def _check(x, w1, w3, w2, limit) -> int:
     inter, hidden = w1.shape
     if x.dim() < 1 or x.shape[-1] != hidden or w3.shape != (inter, hidden) or w2.shape != (hidden, inter):
         raise ValueError("x [..., H], w1 [I, H], w3 [I, H], w2 [H, I] expected")
-    if hidden < 1 or inter < 1:
-        raise ValueError("hidden and inter must be at least 1")
+    if not (1 <= hidden <= _MOST and 1 <= inter <= _MOST):   # before they become 32-bit fields
+        raise ValueError("hidden and inter must be in [1, 2^17]")
     if limit is not None and not limit > LEAST_LIMIT:
         raise ValueError("limit must be positive in f32, or None for no clamps")
     if has_tangent(x, w1, w3, w2):

@@ -28,3 +28,13 @@ def test_a_limit_that_f32_rounds_to_zero(cuda):
         assert float(gated.gated_ffn(x, *ws, limit=limit).abs().max()) == 0
         assert float(mx4.gated_ffn(x, *q, limit=limit).abs().max()) == 0
     assert torch.equal(gated.gated_ffn(x, *ws, limit=1e300), gated.gated_ffn(x, *ws))
+
+
+def test_sizes_that_32_bits_would_wrap(cuda):
+    """2^32 + 64 columns are not 64 (broadcast operands: nothing of that size is allocated)."""
+    one = torch.zeros(1, 1, dtype=torch.bfloat16, device=cuda)
+    for n in (2 ** 32 + 64, 2 ** 31, 2 ** 17 + 1):
+        with pytest.raises(ValueError, match="2.17"):
+            gated.gated_ffn(one.expand(1, n), one.expand(1, n), one.expand(1, n), one.expand(n, 1))
+        with pytest.raises(ValueError, match="2.17"):
+            gated.gated_ffn(one, one.expand(n, 1), one.expand(n, 1), one.expand(1, n))
