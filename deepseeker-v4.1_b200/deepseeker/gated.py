@@ -121,6 +121,12 @@ def gated_ffn(x: torch.Tensor, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Ten
     pre-activations (f32), 10 bytes per token and intermediate feature.  The
     gradient of a clamped value is 0, that of one that equals the limit (taken
     in f32) is not; the exact sums decide, not their f32 rounding.
+
+    h and the gradients of both projections are operands of the next products
+    and have their type.  In f16 one beyond 65,504 is infinite, and so is (or
+    becomes NaN) what it enters: its row of y and dx, its column of a weight's
+    gradient.  A ``limit`` up to 255 keeps h (at most limit^2) inside; without
+    one, blocks whose h may grow that large belong in bf16.
     """
     hidden = _check(x, w1, w3, w2, limit)
     rows = x if x.dim() == 2 else x.reshape(-1, hidden)

@@ -423,7 +423,8 @@ int ds_ep_destroy(DsEp* ep);
  * backward pass):
  *   g = x W1^T, u = x W3^T, h = silu(min(g, L)) * clip(u, -L, L), y = h W2^T.
  * Products accumulate in f32; h and the gradients of g and u are rounded once
- * to the 16-bit type, g and u are kept in f32 between the passes.  NaN passes
+ * to the 16-bit type (in f16 beyond 65,504 to an infinity, which h cannot reach
+ * with L <= 255), g and u are kept in f32 between the passes.  NaN passes
  * through the clamps.  A clamped value has no gradient, one that equals the
  * limit has one, and the exact sums decide: with clamps, kept values of g and u
  * that f32 sums cannot place are summed up in 64 bits and stored on the side of
