@@ -66,8 +66,8 @@ __device__ __forceinline__ void copy_atom(uint32_t taddr, uint32_t saddr) {
 }
 
 // The gated unit (ds_gated_ffn's), from f32 sums: the clamps keep a NaN; the
-// fast exponential and division are good to about 2^-20, and what follows
-// rounds to three bits.
+// fast exponential's error grows with |g| (2^-22 near 0, below 2^-16 at 88), and
+// what follows rounds to three bits.
 __device__ __forceinline__ float gate_unit(float g, float u, float limit) {
   if (limit > 0.0f) {
     g = g > limit ? limit : g;

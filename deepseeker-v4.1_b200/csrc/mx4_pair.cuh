@@ -16,9 +16,10 @@
 // accumulators) would ask 94 bytes a cycle of L2 for each SM instead of 64.
 // Lanes are rows: a thread holds whole blocks of h and quantises them alone.
 //
-// 16384 x 4096 to 4096: 107 us, 5.1 PFLOP/s.  Bounded by what reaches the SMs
-// from L2 (1.17 GB; no kernel here gets more than 12 TB/s) and by the
-// accumulator's hand-over; gate / up of 16384 x 4096 x 2048: 110 us.
+// 16384 x 4096 to 4096: 107 us, 5.1 PFLOP/s; gate / up of 16384 x 4096 x 2048:
+// 110 us.  A tile takes 12.4 k cycles for 8.2 k of MMAs: about 1.5 k are the
+// accumulator's hand-over, the rest stages that arrive late (1.17 GB from L2, 11
+// TB/s; what L2 could give has not been measured apart).
 #pragma once
 
 #include "mx4.cuh"
