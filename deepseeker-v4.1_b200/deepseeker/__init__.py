@@ -9,6 +9,7 @@ Modules mirror the reference package's hot-path surface:
   grouped      `plan_groups` and the grouped expert FFN
   moe_align    device sort-and-pad alignment
   gated        dense gated feed-forward block over 16-bit weights, with its backward pass
+  norm         layer norm with its backward pass
   mx4          microscaled 4-bit dense operators: quantisation, product, gated block
   ep           expert-parallel dispatch / combine over torch.distributed
   loader       checkpoint manifest / shards -> resident expert banks
@@ -16,4 +17,4 @@ Modules mirror the reference package's hot-path surface:
 All compute runs in libdeepseeker_b200.so (CUDA, sm_100a), loaded lazily on the
 first operator call; there is no CPU fallback.
 """
-__all__ = ["metal_fp4", "mlx_weights", "requant", "variant_q3", "moe", "grouped", "moe_align", "gated", "mx4", "ep", "loader"]
+__all__ = ["metal_fp4", "mlx_weights", "requant", "variant_q3", "moe", "grouped", "moe_align", "gated", "norm", "mx4", "ep", "loader"]

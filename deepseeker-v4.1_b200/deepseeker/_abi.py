@@ -110,6 +110,11 @@ SIGNATURES: dict[str, tuple] = {
     "ds_mx4_gated_ffn": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, POINTER(DsMx4), POINTER(DsMx4),
                                  POINTER(DsMx4), c_float, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
     "ds_mx4_status": (c_int, [c_void_p, c_void_p]),
+    "ds_layer_norm": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, c_float, c_void_p,
+                              c_void_p, c_void_p]),
+    "ds_layer_norm_backward_workspace_size": (c_int, [c_int64, c_int64, POINTER(c_size_t)]),
+    "ds_layer_norm_backward": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_void_p, c_void_p,
+                                       c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -518,6 +518,29 @@ int ds_mx4_gated_ffn(const void* x, const uint8_t* x_atoms, int x_dtype, int64_t
 /* As ds_gated_ffn_status, for the calls of this group. */
 int ds_mx4_status(int32_t* err, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Layer norm over the last dimension, forward and backward (the reference has
+ * an RMS norm only, src/deepseeker/mlx_forward.py:45, and no backward pass):
+ *   mean = sum x / H, r = 1 / sqrt(sum (x - mean)^2 / H + eps),
+ *   xh = (x - mean) r, y = xh w + b.
+ * x, y, dy, dx are f32, bf16 or f16; weight and bias (either may be NULL: 1
+ * and 0) and their gradients f32 or of x's type.  Sums and statistics are f32,
+ * results rounded once.  Squares of differences to the mean have to stay
+ * inside f32 (magnitudes up to about 1e19 / sqrt(H)).  Any sizes, row strides
+ * and alignments to the element.  Results do not depend on timing. */
+/* x [rows, cols], rows ld elements apart, rows in [0, 2^31), cols in [1, 2^20]
+ * -> y contiguous.  stats [rows, 2] f32 (mean, r) is what a backward pass
+ * reads; NULL where none follows. */
+int ds_layer_norm(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* weight,
+                  const void* bias, int param_dtype, float eps, void* y, float* stats, void* stream);
+/* From dy (rows ld_dy elements apart) and the forward pass's stats: dx
+ * contiguous, dweight and dbias [cols] of param_dtype; NULL skips one.  The
+ * workspace is needed for dweight and dbias only. */
+int ds_layer_norm_backward_workspace_size(int64_t rows, int64_t cols, size_t* bytes);
+int ds_layer_norm_backward(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* weight,
+                           int param_dtype, const float* stats, const void* dy, int64_t ld_dy, void* dx,
+                           void* dweight, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
