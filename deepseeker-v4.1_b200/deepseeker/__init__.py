@@ -6,6 +6,7 @@ Modules mirror the reference package's hot-path surface:
   requant      q3 payload conversion API of scripts/requant_experts_3bit.py
   variant_q3   DEEPSEEKER_VARIANT selection
   moe          routing, resident expert banks, fused decode MoE layer, `moe_layer`
+  balance      balance loss of a router and its counts per expert, with gradients
   grouped      `plan_groups` and the grouped expert FFN
   moe_align    device sort-and-pad alignment
   gated        dense gated feed-forward block over 16-bit weights, with its backward pass
@@ -17,4 +18,4 @@ Modules mirror the reference package's hot-path surface:
 All compute runs in libdeepseeker_b200.so (CUDA, sm_100a), loaded lazily on the
 first operator call; there is no CPU fallback.
 """
-__all__ = ["metal_fp4", "mlx_weights", "requant", "variant_q3", "moe", "grouped", "moe_align", "gated", "norm", "mx4", "ep", "loader"]
+__all__ = ["metal_fp4", "mlx_weights", "requant", "variant_q3", "moe", "balance", "grouped", "moe_align", "gated", "norm", "mx4", "ep", "loader"]

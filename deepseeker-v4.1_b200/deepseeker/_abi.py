@@ -44,6 +44,12 @@ class DsMx4(Structure):
     _fields_ = [("packed", c_void_p), ("atoms", c_void_p), ("rows", c_int64), ("cols", c_int64)]
 
 
+class DsBalance(Structure):
+    _fields_ = [("logits", c_void_p), ("tokens", c_int64), ("ld", c_int64), ("dtype", c_int32), ("experts", c_int32),
+                ("top_k", c_int32), ("kind", c_int32), ("ids", c_void_p), ("valid", c_void_p), ("offsets", c_void_p),
+                ("offsets_i64", c_int32), ("sequences", c_int64)]
+
+
 # name -> (restype, argtypes); every symbol include/deepseeker_b200.h declares
 SIGNATURES: dict[str, tuple] = {
     "ds_last_error_string": (c_char_p, []),
@@ -115,6 +121,9 @@ SIGNATURES: dict[str, tuple] = {
     "ds_layer_norm_backward_workspace_size": (c_int, [c_int64, c_int64, POINTER(c_size_t)]),
     "ds_layer_norm_backward": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_void_p, c_void_p,
                                        c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "ds_balance_loss_workspace_size": (c_int, [POINTER(DsBalance), POINTER(c_size_t)]),
+    "ds_balance_loss": (c_int, [POINTER(DsBalance), c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "ds_balance_loss_backward": (c_int, [POINTER(DsBalance), c_void_p, c_void_p, c_void_p, c_void_p]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -541,6 +541,40 @@ int ds_layer_norm_backward(const void* x, int dtype, int64_t rows, int64_t cols,
                            int param_dtype, const float* stats, const void* dy, int64_t ld_dy, void* dx,
                            void* dweight, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Balance loss of a router, its counts per expert and its gradient (the
+ * reference only serves; its routers, src/deepseeker/mlx_forward.py:62-81, are
+ * ds_route_topk).  Per sequence, over its n valid tokens:
+ *   c_e = how often e was chosen, P_e = 1/n sum_t p_te,
+ *   loss = sum_e (c_e E / (k n)) P_e   (1 when both are even),
+ * p_te = softmax(l_t)_e, or s_te / sum_e s_te with s = sqrt(softplus(l)).  The
+ * gradient takes c_e as given.  Sums of p are f32; results do not depend on
+ * timing.  A row whose scores are all 0 in f32 (logits of
+ * -infinity; for the root of softplus from about -200 on) has p = 0 and no
+ * gradient. */
+typedef struct DsBalance {
+  const void* logits;         /* [T, E], rows ld elements apart                      */
+  int64_t tokens, ld;         /* T: T * top_k < 2^31                                  */
+  int32_t dtype;              /* DS_F32, DS_BF16, DS_F16: logits and their gradient   */
+  int32_t experts, top_k;     /* E in [1, 1024], k in [1, 32]                         */
+  int32_t kind;               /* DS_ROUTE_SOFTMAX or DS_ROUTE_SQRTSOFTPLUS            */
+  const int32_t* ids;         /* [T, k] contiguous; outside [0, E): no expert         */
+  const uint8_t* valid;       /* [T] or NULL; 0: the row is not looked at             */
+  const void* offsets;        /* [sequences + 1] ascending rows; NULL: one sequence   */
+  int32_t offsets_i64;        /* offsets are int64, else int32                        */
+  int64_t sequences;          /* S in [0, 2^24], 1 without offsets                    */
+} DsBalance;
+
+int ds_balance_loss_workspace_size(const DsBalance* desc, size_t* bytes);
+/* loss [S] (0 for a sequence without valid tokens), counts [S, E], and coef
+ * [S, E] = c_e E / (k n^2), which the backward pass reads. */
+int ds_balance_loss(const DsBalance* desc, float* loss, int32_t* counts, float* coef, void* workspace,
+                    size_t workspace_bytes, void* stream);
+/* dlogits [T, E] contiguous, of the logits' type, from dloss [S]: 0 in rows
+ * that are not valid or belong to no sequence.  ids is not read. */
+int ds_balance_loss_backward(const DsBalance* desc, const float* coef, const float* dloss, void* dlogits,
+                             void* stream);
+
 #ifdef __cplusplus
 }
 #endif
