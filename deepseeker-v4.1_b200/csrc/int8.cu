@@ -1,0 +1,580 @@
+// 8-bit integer dense operators: quantisation of rows, and the product of a
+// matrix quantised by row (token) with one quantised by row (output channel):
+//
+//   y[n, m] = (sum_k qx[n, k] qw[m, k]) sx[n] sw[m],
+//
+// sums exact in 32-bit integers (K < 2^17), on tcgen05 kind::i8.
+//
+// Tile kernel (few rows, or few tiles): one CTA computes 128 features (lanes
+// of the accumulator) x NT rows of x over a slice of the contraction; the
+// slices of a tile are the CTAs of a cluster and are added through distributed
+// shared memory.  More rows: int8_pair.cuh.
+#include <algorithm>
+#include <cooperative_groups.h>
+
+#include "int8_pair.cuh"
+
+namespace ds {
+namespace int8 {
+namespace {
+
+namespace cg = cooperative_groups;
+using namespace ds::rows;
+
+__device__ int g_err;   // bit 1: a bounded wait gave up
+
+// ---------------------------------------------------------------- quantisation
+
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* red) {
+  v = __reduce_max_sync(0xffffffffu, v);
+  const int warps = blockDim.x >> 5;
+  if (warps == 1) return v;
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return __reduce_max_sync(0xffffffffu, lane < warps ? red[lane] : 0u);
+}
+
+// One row per blockDim.x threads, V times VEC values each.
+template <typename T, int VEC, int V>
+__global__ void __launch_bounds__(1024) quantize_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ld,
+                                                        uint8_t* __restrict__ codes, int64_t pitch,
+                                                        float* __restrict__ scales) {
+  __shared__ uint32_t red[32];
+  launch_dependents();
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= rows) return;   // whole rows: a warp, or the block
+  Pack<T, VEC> k[V];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = (i * blockDim.x + threadIdx.x) * VEC;
+    if (c < cols) k[i].load(x + row * ld + c);
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = (i * blockDim.x + threadIdx.x) * VEC;
+    if (c >= cols) continue;
+    float v[VEC];
+    k[i].get(v);
+    // bits of non-negative values order as the values, infinities and NaN above
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+  }
+  const float s = scale_of(row_max(top, red));
+  if (threadIdx.x == 0) scales[row] = s;
+  const bool plain = s >= 1.17549435e-38f;
+  const float inv = 1.0f / s;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = (i * blockDim.x + threadIdx.x) * VEC;
+    if (c >= cols) continue;
+    float v[VEC];
+    k[i].get(v);
+    uint32_t q[VEC];
+    if (plain) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) q[j] = code_of(v[j], s, inv);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) q[j] = code_of_small(v[j], s);
+    }
+    uint8_t* at = codes + row * pitch + c;
+    if constexpr (VEC == 1) {
+      *at = (uint8_t)q[0];
+    } else {
+      uint32_t w[VEC / 4];
+#pragma unroll
+      for (int j = 0; j < VEC / 4; ++j)
+        w[j] = q[4 * j] | q[4 * j + 1] << 8 | q[4 * j + 2] << 16 | q[4 * j + 3] << 24;
+      if constexpr (VEC == 8) *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
+      else *reinterpret_cast<uint32_t*>(at) = w[0];
+    }
+  }
+}
+
+// Rows that no block's registers hold: read twice, one value a thread.
+template <typename T>
+__global__ void __launch_bounds__(1024) quantize_long_kernel(const T* __restrict__ x, int cols, int64_t ld,
+                                                             uint8_t* __restrict__ codes, int64_t pitch,
+                                                             float* __restrict__ scales) {
+  __shared__ uint32_t red[32];
+  launch_dependents();
+  const int64_t row = blockIdx.x;
+  const T* src = x + row * ld;
+  uint32_t top = 0;
+  for (int c = threadIdx.x; c < cols; c += blockDim.x) top = max(top, __float_as_uint((float)src[c]) & 0x7FFFFFFFu);
+  const float s = scale_of(row_max(top, red)), inv = 1.0f / s;
+  if (threadIdx.x == 0) scales[row] = s;
+  const bool plain = s >= 1.17549435e-38f;
+  for (int c = threadIdx.x; c < cols; c += blockDim.x)
+    codes[row * pitch + c] = (uint8_t)(plain ? code_of((float)src[c], s, inv) : code_of_small((float)src[c], s));
+}
+
+// Values of codes, VEC a thread: 8 (the result's rows on 16 bytes), or one.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ codes, int64_t pitch,
+                                                         const float* __restrict__ scales, int64_t rows, int cols,
+                                                         T* __restrict__ out) {
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= rows) return;
+  const float s = scales[row];
+  for (int c = threadIdx.x * VEC; c < cols; c += blockDim.x * VEC) {
+    const uint8_t* at = codes + row * pitch + c;
+    T* dst = out + row * cols + c;
+    if constexpr (VEC == 1) {
+      *dst = narrow<T>((float)(int8_t)*at * s);
+    } else {
+      const uint2 w = *reinterpret_cast<const uint2*>(at);
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = (float)(int8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3))) * s;
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float half[4] = {v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
+          put<T, 4>(dst + 4 * h, half);
+        }
+      } else {
+        put<T, 8>(dst, v);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- product of few rows
+
+struct TileParams {
+  CUtensorMap a, b;            // codes of the weights, of x
+  const float *sw, *sx;
+  int M, N;                    // features, rows of x
+  int ksteps;                  // stages of 128 codes
+  void* out;                   // out[n * ldo + m]
+  int64_t ldo;
+  int out_dtype;
+  int* err;
+};
+
+template <int NT>
+struct TileShape {
+  static constexpr int kStage = 16384 + NT * 128;
+  // less than half of an SM, so that the next launch's CTAs join this one's and
+  // their weights are on their way while it finishes
+  static constexpr int kStages = std::min(6, 110 * 1024 / kStage);
+  static constexpr int kSmem = 1024 + kStages * kStage;
+  static constexpr int kCols = NT < 32 ? 32 : NT;
+  static_assert(kStages * kStage >= NT * 128 * 4, "stages hold the partial tile");
+};
+
+constexpr int kTileThreads = 320;   // warp 0 copies, warp 1 MMA, warps 2-9 epilogue (two a lane quarter)
+
+// Elements (m, n0 .. n0 + J - 1) of the result, nv of them inside.
+template <int J>
+__device__ __forceinline__ void tile_store(const TileParams& p, int m, float sw, int n0, int nv, const int (&v)[J]) {
+  if (m >= p.M) return;
+  const int64_t at = (int64_t)n0 * p.ldo + m;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    if (j >= nv) continue;
+    const float y = scaled(v[j], p.sx[n0 + j], sw);
+    if (p.out_dtype == DS_F32) static_cast<float*>(p.out)[at + j * p.ldo] = y;
+    else if (p.out_dtype == DS_F16) static_cast<__half*>(p.out)[at + j * p.ldo] = __float2half_rn(y);
+    else static_cast<__nv_bfloat16*>(p.out)[at + j * p.ldo] = __float2bfloat16_rn(y);
+  }
+}
+
+// Sums this CTA's share of the tile's `rows` rows over the partial tiles
+// [NT][128] of the cluster.  The reads of four rows from all slices are in
+// flight together.
+template <int NT, int SLICES>
+__device__ __forceinline__ void tile_join(const TileParams& p, int* part, int slice, int turn, int m, int mi, float sw,
+                                          int n0, int rows) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int* src[SLICES];
+#pragma unroll
+  for (int r = 0; r < SLICES; ++r) src[r] = cluster.map_shared_rank(part, r) + mi;
+  const int share = (rows + SLICES - 1) / SLICES, end = min(rows, (slice + 1) * share);
+  for (int n = slice * share + 4 * turn; n < end; n += 8) {
+    int w[SLICES][4];
+#pragma unroll
+    for (int r = 0; r < SLICES; ++r)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[r][j] = src[r][min(n + j, end - 1) * 128];
+    int v[4] = {};
+#pragma unroll
+    for (int r = 0; r < SLICES; ++r)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += w[r][j];
+    tile_store(p, m, sw, n0 + n, end - n, v);
+  }
+}
+
+template <int NT>
+__global__ void __launch_bounds__(kTileThreads, 2) tile_kernel(const __grid_constant__ TileParams p) {
+  using C = TileShape<NT>;
+  constexpr int S = C::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  __shared__ __align__(8) uint64_t full[S], empty[S], accfull;
+  __shared__ uint32_t tmem_base;
+  __shared__ int abort_flag;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int slices = cluster.dim_blocks().x, slice = cluster.block_rank();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int mts = (p.M + 127) / 128, tile = blockIdx.x / slices;
+  const int m0 = tile % mts * 128, n0 = tile / mts * NT, rows = min(NT, p.N - n0);
+  const int it0 = (int)((int64_t)p.ksteps * slice / slices), its = (int)((int64_t)p.ksteps * (slice + 1) / slices) - it0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(&accfull, 1);
+    abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) tc5::alloc(&tmem_base, C::kCols);
+  tc5::fence_before();
+  __syncthreads();
+  tc5::fence_after();
+  const uint32_t tb = tmem_base;
+  volatile int* abort = &abort_flag;
+  launch_dependents();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      auto weights = [&](int g) {
+        mbar_arrive_expect_tx(&full[g % S], C::kStage);
+        tma_load_2d(smem + g % S * C::kStage, &p.a, (it0 + g) * 128, m0, &full[g % S]);
+      };
+      auto codes = [&](int g) {
+        tma_load_2d(smem + g % S * C::kStage + 16384, &p.b, (it0 + g) * 128, n0, &full[g % S]);
+      };
+      // The weights of the first stages need nothing of the launch before this
+      // one in the stream: that is one of the same call, and the call's first
+      // launch began after all earlier work had ended.
+      const int early = min(S, its);
+      for (int g = 0; g < early; ++g) weights(g);
+      wait_prior_grid();
+      for (int g = 0; g < early; ++g) codes(g);
+      int g = early;
+      for (; g < its; ++g) {
+        if (!ds::pair::wait(&empty[g % S], ((g / S) - 1) & 1, abort, p.err)) break;
+        weights(g);
+        codes(g);
+      }
+      // never leave with copies in flight into this CTA's shared memory
+      for (int j = g - S < 0 ? 0 : g - S; j < g; ++j) mbar_wait_bounded(&full[j % S], (j / S) & 1, 200000000ull);
+    }
+  } else if (warp == 1) {
+    const uint64_t ops = tc5::sdesc_sw128(smem_u32(smem));
+    constexpr uint32_t id = idesc(128, NT);
+    for (int g = 0; g < its; ++g) {
+      const int s = g % S;
+      if (!ds::pair::wait_all(&full[s], (g / S) & 1, abort, p.err)) break;
+      tc5::fence_after();
+      if (elect_one()) {
+        const uint64_t ad = ops + (uint64_t)((s * C::kStage) >> 4), bd = ad + (16384 >> 4);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) mma(tb, ad + 2 * kk, bd + 2 * kk, id, (g | kk) != 0);
+        tc5::commit(&empty[s]);
+      }
+      __syncwarp();
+    }
+    // all issued MMAs complete before the accumulators are read or released
+    if (elect_one()) tc5::commit(&accfull);
+    __syncwarp();
+    ds::pair::wait_all(&accfull, 0, abort, p.err);
+  } else {
+    ds::pair::wait_all(&accfull, 0, abort, p.err);
+  }
+  tc5::fence_after();
+
+  // ---- epilogue: thread = one feature (lane of tensor memory)
+  wait_prior_grid();
+  const int q = warp & 3, turn = (warp - 2) >> 2, mi = q * 32 + lane, m = m0 + mi;
+  int* part = reinterpret_cast<int*>(smem);   // [NT][128]
+  const float sw = warp >= 2 && m < p.M ? p.sw[m] : 0.0f;
+  if (warp >= 2) {
+    for (int c0 = 16 * turn; c0 < rows; c0 += 32) {
+      float f[16];
+      int v[16];
+      tc5::ld_x16_nowait(tc5::lane_quarter(tb + c0, q), f);
+      tc5::wait_ld();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = __float_as_int(f[j]);
+      if (slices > 1) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) part[(c0 + j) * 128 + mi] = v[j];
+      } else {
+        tile_store(p, m, sw, n0 + c0, rows - c0, v);
+      }
+    }
+  }
+  if (slices > 1) {
+    cluster.sync();
+    if (warp >= 2) {
+      if (slices == 8) tile_join<NT, 8>(p, part, slice, turn, m, mi, sw, n0, rows);
+      else if (slices == 4) tile_join<NT, 4>(p, part, slice, turn, m, mi, sw, n0, rows);
+      else tile_join<NT, 2>(p, part, slice, turn, m, mi, sw, n0, rows);
+    }
+    cluster.sync();   // partial tiles stay until every CTA has read them
+  }
+  tc5::fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc5::fence_after();
+    tc5::dealloc(tb, C::kCols);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+
+constexpr int kMostCols = (1 << 17) - 1;   // 2^14 K stays inside an s32 sum
+
+int64_t pitch_of(int64_t cols) { return (cols + kPitch - 1) / kPitch * kPitch; }
+
+// Codes of a matrix [rows, cols], rows pitch bytes apart, in boxes of 128 codes
+// x box_rows (zeros outside).
+bool map_codes(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t pitch, int box_rows) {
+  return grouped::encode_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rows, cols, pitch, 128, box_rows,
+                            CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int* err_word() {
+  static SymbolOnce known;
+  return ds::symbol_address(&known, &g_err);
+}
+
+int launch_quantize(const void* x, int dtype, int64_t rows, int cols, int64_t ld, uint8_t* codes, int64_t pitch,
+                    float* scales, cudaStream_t s) {
+  const int es = elements(dtype);
+  const bool vec = vectors(x, rows, cols, ld, es);
+  by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    const T* src = static_cast<const T*>(x);
+    if (cols > 32 * 1024) {
+      quantize_long_kernel<T><<<(unsigned)rows, 1024, 0, s>>>(src, cols, ld, codes, pitch, scales);
+      return;
+    }
+    const Shape sh = shape_of(cols, vec ? 16 / es : 1, 16, 1024);
+    const dim3 block(sh.threads, sh.rows);
+    const unsigned grid = (unsigned)((rows + sh.rows - 1) / sh.rows);
+    by_shape<T, 32>(sh, [&](auto w, auto v) {
+      quantize_kernel<T, decltype(w)::value, decltype(v)::value>
+          <<<grid, block, 0, s>>>(src, rows, cols, ld, codes, pitch, scales);
+    });
+  });
+  DS_CHECK_LAUNCH("int8 quantize_kernel");
+  return DS_OK;
+}
+
+// Rows of x as a call gives them: values, or codes (DS_I8) with their scales.
+struct Input {
+  const void* p;
+  const float* scales;
+  int dtype;
+  int64_t rows, ld;
+  int cols;
+};
+
+template <int NT>
+int launch_tiles(TileParams& p, const Input& x, const DsInt8& w, int slices, cudaStream_t s, bool chained) {
+  using C = TileShape<NT>;
+  const bool ok = map_codes(&p.a, w.codes, w.rows, w.cols, w.pitch, 128) &&
+                  map_codes(&p.b, x.p, x.rows, x.cols, x.ld, NT);
+  DS_REQUIRE(ok, DS_ECUDA, "int8: tensor map encoding failed");
+  static SmemOnce once;
+  const int st = ds::allow_smem(&once, reinterpret_cast<const void*>(&tile_kernel<NT>), C::kSmem);
+  if (st != DS_OK) return st;
+  const int64_t tiles = (p.M + 127) / 128 * (int64_t)((p.N + NT - 1) / NT);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * slices));
+  cfg.blockDim = dim3(kTileThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)slices;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = chained ? 2 : 1;
+  DS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, tile_kernel<NT>, p));
+  return DS_OK;
+}
+
+// Result [rows, cols] in boxes of 128 bytes x 32 rows; false where its rows do not start on 16 bytes.
+bool map_result(CUtensorMap* m, void* y, int64_t rows, int64_t cols, int dtype) {
+  const int es = elements(dtype);
+  if (!ds::aligned(y, 16) || cols * es % 16 != 0) return false;
+  return grouped::encode_2d(m, dtype == DS_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, y,
+                            rows, cols, cols * es, 128 / es, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int NT>
+int launch_pairs(PairParams& p, const Input& x, const DsInt8& w, cudaStream_t s, bool chained) {
+  using C = pairs::Shape<NT>;
+  const bool ok = map_codes(&p.a, x.p, x.rows, x.cols, x.ld, 128) &&
+                  map_codes(&p.b, w.codes, w.rows, w.cols, w.pitch, NT / 2);
+  DS_REQUIRE(ok, DS_ECUDA, "int8: tensor map encoding failed");
+  const int64_t tiles = (p.M + 255) / 256 * (int64_t)((p.N + NT - 1) / NT);
+  DS_REQUIRE(tiles < ((int64_t)1 << 31), DS_ERANGE, "int8: too many tiles");
+  static SmemOnce once;
+  const int st = ds::allow_smem(&once, reinterpret_cast<const void*>(&pairs::pair_kernel<NT>), C::kSmem);
+  if (st != DS_OK) return st;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, ds::sm_count() / 2)));
+  cfg.blockDim = dim3(pairs::kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = chained ? 1 : 0;
+  DS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, pairs::pair_kernel<NT>, p));
+  return DS_OK;
+}
+
+// y = x W^T.
+int product(const Input& x, const DsInt8& w, void* y, int out_dtype, int* err, cudaStream_t s, bool chained) {
+  const int ksteps = (int)((w.cols + 127) / 128);
+  if (x.rows > 128) {
+    PairParams p = {};
+    p.sx = x.scales, p.sw = w.scales, p.y = y, p.ldy = w.rows, p.out_dtype = out_dtype;
+    p.boxed = map_result(&p.out, y, x.rows, w.rows, out_dtype);
+    p.M = (int)x.rows, p.N = (int)w.rows, p.ksteps = ksteps, p.err = err;
+    const int64_t rows = (x.rows + 255) / 256, pairs = ds::sm_count() / 2;
+    // whole waves of tiles, the wider the less is read from L2 for a product
+    auto cost = [&](int nt, int stage) { return (rows * ((w.rows + nt - 1) / nt) + pairs - 1) / pairs * stage; };
+    const int64_t c256 = cost(256, 8), c128 = cost(128, 5), c64 = cost(64, 4);
+    if (c256 <= c128 && c256 <= c64) return launch_pairs<256>(p, x, w, s, chained);
+    if (c128 <= c64) return launch_pairs<128>(p, x, w, s, chained);
+    return launch_pairs<64>(p, x, w, s, chained);
+  }
+  TileParams p = {};
+  p.sw = w.scales, p.sx = x.scales, p.M = (int)w.rows, p.N = (int)x.rows, p.ksteps = ksteps, p.err = err;
+  p.out = y, p.ldo = w.rows, p.out_dtype = out_dtype;
+  const int64_t tiles = (w.rows + 127) / 128;
+  int slices = 1;
+  while (slices < 8 && tiles * slices * 2 <= ds::sm_count() && ksteps / (slices * 2) >= 2) slices *= 2;
+  if (x.rows <= 16) return launch_tiles<16>(p, x, w, slices, s, chained);
+  if (x.rows <= 32) return launch_tiles<32>(p, x, w, slices, s, chained);
+  if (x.rows <= 64) return launch_tiles<64>(p, x, w, slices, s, chained);
+  return launch_tiles<128>(p, x, w, slices, s, chained);
+}
+
+size_t quantized_bytes(int64_t rows, int64_t cols) {
+  return grouped::up((size_t)rows * pitch_of(cols), 256) + grouped::up((size_t)rows * 4, 256);
+}
+
+}  // namespace
+}  // namespace int8
+}  // namespace ds
+
+using namespace ds::int8;
+
+extern "C" int ds_int8_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ld, int8_t* codes,
+                                int64_t pitch, float* scales, void* stream) {
+  DS_REQUIRE(x_dtype == DS_F32 || x_dtype == DS_BF16 || x_dtype == DS_F16, DS_EINVAL,
+             "int8_quantize: x must be f32, bf16 or f16");
+  DS_REQUIRE(rows >= 0 && rows < ((int64_t)1 << 31) && cols >= 1 && cols <= kMostCols, DS_ERANGE,
+             "int8_quantize: rows must be in [0, 2^31), cols in [1, 2^17)");
+  DS_REQUIRE(rows <= 1 || ld >= cols, DS_EINVAL, "int8_quantize: row stride below cols");
+  DS_REQUIRE(pitch >= cols && pitch % kPitch == 0, DS_EINVAL,
+             "int8_quantize: the codes' rows must be a multiple of 16 bytes apart, and hold cols");
+  if (rows == 0) return DS_OK;
+  DS_REQUIRE(x && codes && scales, DS_EINVAL, "int8_quantize: null pointer");
+  DS_REQUIRE(ds::aligned(x, ds::rows::elements(x_dtype)) && ds::aligned(codes, 16) && ds::aligned(scales, 4), DS_EALIGN,
+             "int8_quantize: x and scales must be aligned to their elements, codes to 16 bytes");
+  return launch_quantize(x, x_dtype, rows, (int)cols, ld, reinterpret_cast<uint8_t*>(codes), pitch, scales,
+                         static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int ds_int8_dequantize(const int8_t* codes, int64_t pitch, const float* scales, int64_t rows, int64_t cols,
+                                  void* out, int out_dtype, void* stream) {
+  DS_REQUIRE(out_dtype == DS_F32 || out_dtype == DS_BF16 || out_dtype == DS_F16, DS_EINVAL,
+             "int8_dequantize: out must be f32, bf16 or f16");
+  DS_REQUIRE(rows >= 0 && rows < ((int64_t)1 << 31) && cols >= 1 && cols <= kMostCols, DS_ERANGE,
+             "int8_dequantize: rows must be in [0, 2^31), cols in [1, 2^17)");
+  DS_REQUIRE(pitch >= cols && pitch % kPitch == 0, DS_EINVAL,
+             "int8_dequantize: the codes' rows must be a multiple of 16 bytes apart, and hold cols");
+  if (rows == 0) return DS_OK;
+  const int es = ds::rows::elements(out_dtype);
+  DS_REQUIRE(codes && scales && out, DS_EINVAL, "int8_dequantize: null pointer");
+  DS_REQUIRE(ds::aligned(codes, 16) && ds::aligned(scales, 4) && ds::aligned(out, es), DS_EALIGN,
+             "int8_dequantize: codes must be 16-byte aligned, scales and out to their elements");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const uint8_t* src = reinterpret_cast<const uint8_t*>(codes);
+  const bool vec = ds::aligned(out, 16) && cols % 8 == 0;
+  const int n = (int)(vec ? cols / 8 : cols), threads = std::min(256, (n + 31) / 32 * 32);
+  const dim3 block(threads, 256 / threads);
+  const unsigned grid = (unsigned)((rows + block.y - 1) / block.y);
+  ds::rows::by_type(out_dtype, [&](auto t) {
+    using T = decltype(t);
+    T* dst = static_cast<T*>(out);
+    if (vec) dequantize_kernel<T, 8><<<grid, block, 0, s>>>(src, pitch, scales, rows, (int)cols, dst);
+    else dequantize_kernel<T, 1><<<grid, block, 0, s>>>(src, pitch, scales, rows, (int)cols, dst);
+  });
+  DS_CHECK_LAUNCH("int8 dequantize_kernel");
+  return DS_OK;
+}
+
+extern "C" int ds_int8_linear_workspace_size(int64_t rows, int64_t cols, size_t* bytes) {
+  DS_REQUIRE(bytes && rows >= 0 && cols >= 1, DS_EINVAL,
+             "int8_linear_workspace_size: rows >= 0, cols >= 1 and an output expected");
+  *bytes = quantized_bytes(rows, cols);
+  return DS_OK;
+}
+
+extern "C" int ds_int8_linear(const void* x, const float* x_scales, int x_dtype, int64_t rows, int64_t ld,
+                              const DsInt8* w, void* out, int out_dtype, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+  DS_REQUIRE(w && w->codes && w->scales, DS_EINVAL, "int8_linear: null weight");
+  DS_REQUIRE(w->rows >= 1 && w->rows <= (1 << 20) && w->cols >= 1 && w->cols <= kMostCols, DS_ERANGE,
+             "int8_linear: weight rows must be in [1, 2^20], cols in [1, 2^17)");
+  DS_REQUIRE(w->pitch >= w->cols && w->pitch % kPitch == 0, DS_EINVAL,
+             "int8_linear: the weight's rows must be a multiple of 16 bytes apart, and hold its cols");
+  DS_REQUIRE(ds::aligned(w->codes, 16) && ds::aligned(w->scales, 4), DS_EALIGN,
+             "int8_linear: weight codes must be 16-byte aligned, scales to 4");
+  DS_REQUIRE(x_dtype == DS_F32 || x_dtype == DS_BF16 || x_dtype == DS_F16 || x_dtype == DS_I8, DS_EINVAL,
+             "int8_linear: x must be f32, bf16 or f16, or codes (i8) with scales");
+  const bool coded = x_dtype == DS_I8;
+  DS_REQUIRE(rows >= 0 && rows <= (1 << 22), DS_ERANGE, "int8_linear: rows must be in [0, 2^22]");
+  DS_REQUIRE(out_dtype == DS_F32 || out_dtype == DS_BF16 || out_dtype == DS_F16, DS_EINVAL,
+             "int8_linear: out must be f32, bf16 or f16");
+  if (rows == 0) return DS_OK;
+  DS_REQUIRE(x && (!coded || x_scales), DS_EINVAL, "int8_linear: null x");
+  DS_REQUIRE(coded ? ld >= w->cols && ld % kPitch == 0 : rows <= 1 || ld >= w->cols, DS_EINVAL,
+             "int8_linear: row stride of x below its columns, or that of its codes not a multiple of 16");
+  DS_REQUIRE(coded ? ds::aligned(x, 16) && ds::aligned(x_scales, 4) : ds::aligned(x, ds::rows::elements(x_dtype)),
+             DS_EALIGN, "int8_linear: x must be aligned to its elements, codes to 16 bytes");
+  const size_t need = coded ? 0 : quantized_bytes(rows, w->cols);
+  DS_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), DS_EINVAL,
+             "int8_linear: workspace %zu bytes < required %zu", workspace_bytes, need);
+  DS_REQUIRE(out && ds::aligned(out, ds::rows::elements(out_dtype)) && ds::aligned(workspace, 256), DS_EALIGN,
+             "int8_linear: out must be aligned to its elements, the workspace to 256 bytes");
+  DS_REQUIRE(ds::grouped::encode_fn() != nullptr, DS_ECUDA, "int8_linear: cuTensorMapEncodeTiled unavailable");
+  int* err = err_word();
+  DS_REQUIRE(err != nullptr, DS_ECUDA, "int8_linear: error word unavailable");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  Input in = {x, x_scales, x_dtype, rows, ld, (int)w->cols};
+  if (!coded) {
+    uint8_t* codes = static_cast<uint8_t*>(workspace);
+    float* scales = reinterpret_cast<float*>(codes + ds::grouped::up((size_t)rows * pitch_of(w->cols), 256));
+    const int st = launch_quantize(x, x_dtype, rows, in.cols, ld, codes, pitch_of(w->cols), scales, s);
+    if (st != DS_OK) return st;
+    in.p = codes, in.scales = scales, in.ld = pitch_of(w->cols);
+  }
+  return product(in, *w, out, out_dtype, err, s, !coded);
+}
+
+extern "C" int ds_int8_status(int32_t* err, void* stream) {
+  DS_REQUIRE(err != nullptr, DS_EINVAL, "int8_status: null output");
+  int* w = err_word();
+  DS_REQUIRE(w != nullptr, DS_ECUDA, "int8_status: error word unavailable");
+  return ds::take_error_word(w, err, static_cast<cudaStream_t>(stream));
+}

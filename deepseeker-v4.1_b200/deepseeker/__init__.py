@@ -12,10 +12,11 @@ Modules mirror the reference package's hot-path surface:
   gated        dense gated feed-forward block over 16-bit weights, with its backward pass
   norm         layer norm with its backward pass
   mx4          microscaled 4-bit dense operators: quantisation, product, gated block
+  int8         8-bit integer dense operators: quantisation, product
   ep           expert-parallel dispatch / combine over torch.distributed
   loader       checkpoint manifest / shards -> resident expert banks
 
 All compute runs in libdeepseeker_b200.so (CUDA, sm_100a), loaded lazily on the
 first operator call; there is no CPU fallback.
 """
-__all__ = ["metal_fp4", "mlx_weights", "requant", "variant_q3", "moe", "balance", "grouped", "moe_align", "gated", "norm", "mx4", "ep", "loader"]
+__all__ = ["metal_fp4", "mlx_weights", "requant", "variant_q3", "moe", "balance", "grouped", "moe_align", "gated", "norm", "mx4", "int8", "ep", "loader"]

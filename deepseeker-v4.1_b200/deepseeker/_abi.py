@@ -14,7 +14,7 @@ LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libdeepseeker_b200.so"
 # status codes
 DS_OK, DS_EINVAL, DS_EALIGN, DS_ERANGE, DS_ECUDA, DS_ETIMEOUT, DS_ENOTSUP = range(7)
 # element types
-DS_F32, DS_BF16, DS_F16, DS_U8 = range(4)
+DS_F32, DS_BF16, DS_F16, DS_U8, DS_I8 = range(5)
 # weight formats
 DS_FMT_FP4, DS_FMT_Q3, DS_FMT_BF16 = range(3)
 # routing kinds
@@ -48,6 +48,10 @@ class DsBalance(Structure):
     _fields_ = [("logits", c_void_p), ("tokens", c_int64), ("ld", c_int64), ("dtype", c_int32), ("experts", c_int32),
                 ("top_k", c_int32), ("kind", c_int32), ("ids", c_void_p), ("valid", c_void_p), ("offsets", c_void_p),
                 ("offsets_i64", c_int32), ("sequences", c_int64)]
+
+
+class DsInt8(Structure):
+    _fields_ = [("codes", c_void_p), ("scales", c_void_p), ("rows", c_int64), ("cols", c_int64), ("pitch", c_int64)]
 
 
 # name -> (restype, argtypes); every symbol include/deepseeker_b200.h declares
@@ -124,6 +128,12 @@ SIGNATURES: dict[str, tuple] = {
     "ds_balance_loss_workspace_size": (c_int, [POINTER(DsBalance), POINTER(c_size_t)]),
     "ds_balance_loss": (c_int, [POINTER(DsBalance), c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "ds_balance_loss_backward": (c_int, [POINTER(DsBalance), c_void_p, c_void_p, c_void_p, c_void_p]),
+    "ds_int8_quantize": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
+    "ds_int8_dequantize": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p]),
+    "ds_int8_linear_workspace_size": (c_int, [c_int64, c_int64, POINTER(c_size_t)]),
+    "ds_int8_linear": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, POINTER(DsInt8), c_void_p, c_int, c_void_p,
+                               c_size_t, c_void_p]),
+    "ds_int8_status": (c_int, [c_void_p, c_void_p]),
 }
 
 _lib: ctypes.CDLL | None = None

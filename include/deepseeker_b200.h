@@ -49,6 +49,7 @@ extern "C" {
 #define DS_BF16 1
 #define DS_F16 2
 #define DS_U8 3
+#define DS_I8 4
 
 /* ---- weight formats ---------------------------------------------------- */
 #define DS_FMT_FP4 0
@@ -574,6 +575,41 @@ int ds_balance_loss(const DsBalance* desc, float* loss, int32_t* counts, float* 
  * that are not valid or belong to no sequence.  ids is not read. */
 int ds_balance_loss_backward(const DsBalance* desc, const float* coef, const float* dloss, void* dlogits,
                              void* stream);
+
+/* ---------------------------------------------------------------------------
+ * 8-bit integer dense operators, one f32 scale per row of either operand (a
+ * token's activations, an output channel's weights; the reference has no
+ * product in this format).  Of a row of K < 2^17 values: s = max |x| / 127
+ * rounded to f32, code q = the whole number nearest to the exact x / s, the
+ * even one of two, clipped to +-127 (0 where s is 0).  A row with a NaN or an
+ * infinity has scale NaN and codes 0, so products with it are NaN.  Codes of a
+ * row lie together, rows `pitch` bytes apart, a multiple of 16 (what lies
+ * between is neither read as a value nor written). */
+int ds_int8_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ld, int8_t* codes, int64_t pitch,
+                     float* scales, void* stream);
+/* out [rows, cols] f32, bf16 or f16 contiguous = code * scale, rounded to f32
+ * and then to out's type. */
+int ds_int8_dequantize(const int8_t* codes, int64_t pitch, const float* scales, int64_t rows, int64_t cols, void* out,
+                       int out_dtype, void* stream);
+
+typedef struct DsInt8 {
+  const int8_t* codes;        /* 16-byte aligned                                    */
+  const float* scales;        /* [rows]                                             */
+  int64_t rows, cols;         /* 1 .. 2^20, 1 .. 2^17 - 1                           */
+  int64_t pitch;              /* bytes from row to row, a multiple of 16            */
+} DsInt8;
+
+/* out [rows, w->rows] (f32, bf16 or f16, contiguous) = x W^T: the sum of
+ * products of codes, exact in 32-bit integers, converted to f32, times both
+ * scales (the smaller first), rounded to out's type.  x_dtype f32 / bf16 / f16:
+ * x [rows, w->cols], rows ld elements apart, is quantised into the workspace
+ * first (x_scales NULL); DS_I8: x is codes, rows ld bytes apart (a multiple of
+ * 16), x_scales their scales, and no workspace is needed.  rows in [0, 2^22]. */
+int ds_int8_linear_workspace_size(int64_t rows, int64_t cols, size_t* bytes);
+int ds_int8_linear(const void* x, const float* x_scales, int x_dtype, int64_t rows, int64_t ld, const DsInt8* w,
+                   void* out, int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
+/* As ds_gated_ffn_status, for the calls of this group. */
+int ds_int8_status(int32_t* err, void* stream);
 
 #ifdef __cplusplus
 }
