@@ -31,64 +31,81 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* red) {
   if (warps == 1) return v;
   const int lane = threadIdx.x & 31;
   if (lane == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
+  row_barrier();
   return __reduce_max_sync(0xffffffffu, lane < warps ? red[lane] : 0u);
 }
 
-// One row per blockDim.x threads, V times VEC values each.
-template <typename T, int VEC, int V>
-__global__ void __launch_bounds__(1024) quantize_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ld,
-                                                        uint8_t* __restrict__ codes, int64_t pitch,
-                                                        float* __restrict__ scales) {
-  __shared__ uint32_t red[32];
+// Bits of the largest magnitude of a vector as f32 (bits of non-negative values
+// order as the values, infinities and NaN above).
+template <typename T, int VEC>
+__device__ __forceinline__ uint32_t top_of(const Pack<T, VEC>& k) {
+  if constexpr (VEC == 8) {
+    uint32_t t = __vmaxu2(__vmaxu2(k.raw.x & 0x7FFF7FFFu, k.raw.y & 0x7FFF7FFFu),
+                          __vmaxu2(k.raw.z & 0x7FFF7FFFu, k.raw.w & 0x7FFF7FFFu));
+    t = max(t & 0xFFFFu, t >> 16);
+    return std::is_same<T, __half>::value ? __float_as_uint(__half2float(__ushort_as_half((uint16_t)t))) : t << 16;
+  } else {
+    float v[VEC];
+    k.get(v);
+    uint32_t t = 0;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) t = max(t, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+    return t;
+  }
+}
+
+// A block takes rows blockIdx.x, + gridDim.x ..., blockDim.y at a time, V times
+// VEC values a thread; THREADS: of a row, which they fill, or 0.  The next row is
+// loaded while this one is coded.  16384 x 4096 bf16: 35 us, 5.8 TB/s; with 16
+// values a thread instead of 32 37 us, without the row ahead 65.
+template <typename T, int VEC, int V, int THREADS>
+__global__ void __maxnreg__(VEC > 1 && V * VEC <= 32 ? 80 : 128) quantize_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ld,
+                                                       uint8_t* __restrict__ codes, int64_t pitch,
+                                                       float* __restrict__ scales) {
+  __shared__ uint32_t red[kMostRows][2][32];
   launch_dependents();
-  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  if (row >= rows) return;   // whole rows: a warp, or the block
+  const int64_t step = (int64_t)gridDim.x * blockDim.y;
+  auto column = [&](int i) { return (int)(i * (THREADS ? THREADS : blockDim.x) + threadIdx.x) * VEC; };
+  auto inside = [&](int i) { return THREADS || column(i) < cols; };
   Pack<T, VEC> k[V];
-  uint32_t top = 0;
+  auto fetch = [&](int64_t row) {
+    if (row >= rows) return;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = (i * blockDim.x + threadIdx.x) * VEC;
-    if (c < cols) k[i].load(x + row * ld + c);
-  }
+    for (int i = 0; i < V; ++i)
+      if (inside(i)) k[i].load(x + row * ld + column(i));
+  };
+  int turn = 0;
+  int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  for (fetch(row); row < rows; row += step, turn ^= 1) {
+    float v[V][VEC];
+    uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = (i * blockDim.x + threadIdx.x) * VEC;
-    if (c >= cols) continue;
-    float v[VEC];
-    k[i].get(v);
-    // bits of non-negative values order as the values, infinities and NaN above
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-  }
-  const float s = scale_of(row_max(top, red));
-  if (threadIdx.x == 0) scales[row] = s;
-  const bool plain = s >= 1.17549435e-38f;
-  const float inv = 1.0f / s;
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = (i * blockDim.x + threadIdx.x) * VEC;
-    if (c >= cols) continue;
-    float v[VEC];
-    k[i].get(v);
-    uint32_t q[VEC];
-    if (plain) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) q[j] = code_of(v[j], s, inv);
-    } else {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) q[j] = code_of_small(v[j], s);
+    for (int i = 0; i < V; ++i) {
+      if (!inside(i)) continue;
+      top = max(top, top_of(k[i]));
+      k[i].get(v[i]);
     }
-    uint8_t* at = codes + row * pitch + c;
-    if constexpr (VEC == 1) {
-      *at = (uint8_t)q[0];
-    } else {
-      uint32_t w[VEC / 4];
+    fetch(row + step);   // on its way during the rest
+    const float s = scale_of(row_max(top, red[threadIdx.y][turn]));
+    if (threadIdx.x == 0) scales[row] = s;
+    const Coder coder(s);
 #pragma unroll
-      for (int j = 0; j < VEC / 4; ++j)
-        w[j] = q[4 * j] | q[4 * j + 1] << 8 | q[4 * j + 2] << 16 | q[4 * j + 3] << 24;
-      if constexpr (VEC == 8) *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
-      else *reinterpret_cast<uint32_t*>(at) = w[0];
+    for (int i = 0; i < V; ++i) {
+      if (!inside(i)) continue;
+      uint32_t q[VEC];
+      coder.codes(v[i], q);
+      uint8_t* at = codes + row * pitch + column(i);
+      if constexpr (VEC == 1) {
+        *at = (uint8_t)q[0];
+      } else {
+        uint32_t w[VEC / 4];
+#pragma unroll
+        for (int j = 0; j < VEC / 4; ++j)
+          w[j] = __byte_perm(__byte_perm(q[4 * j], q[4 * j + 1], 0x0040), __byte_perm(q[4 * j + 2], q[4 * j + 3], 0x0040),
+                             0x5410);
+        if constexpr (VEC == 8) *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t*>(at) = w[0];
+      }
     }
   }
 }
@@ -104,11 +121,15 @@ __global__ void __launch_bounds__(1024) quantize_long_kernel(const T* __restrict
   const T* src = x + row * ld;
   uint32_t top = 0;
   for (int c = threadIdx.x; c < cols; c += blockDim.x) top = max(top, __float_as_uint((float)src[c]) & 0x7FFFFFFFu);
-  const float s = scale_of(row_max(top, red)), inv = 1.0f / s;
+  const float s = scale_of(row_max(top, red));
   if (threadIdx.x == 0) scales[row] = s;
-  const bool plain = s >= 1.17549435e-38f;
-  for (int c = threadIdx.x; c < cols; c += blockDim.x)
-    codes[row * pitch + c] = (uint8_t)(plain ? code_of((float)src[c], s, inv) : code_of_small((float)src[c], s));
+  const Coder coder(s);
+  for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+    float v[1] = {(float)src[c]};
+    uint32_t q[1];
+    coder.codes(v, q);
+    codes[row * pitch + c] = (uint8_t)q[0];
+  }
 }
 
 // Values of codes, VEC a thread: 8 (the result's rows on 16 bytes), or one.
@@ -354,16 +375,17 @@ int launch_quantize(const void* x, int dtype, int64_t rows, int cols, int64_t ld
   by_type(dtype, [&](auto t) {
     using T = decltype(t);
     const T* src = static_cast<const T*>(x);
-    if (cols > 32 * 1024) {
+    if (cols > (vec ? 64 * 1024 / es : 8 * 1024)) {
       quantize_long_kernel<T><<<(unsigned)rows, 1024, 0, s>>>(src, cols, ld, codes, pitch, scales);
       return;
     }
-    const Shape sh = shape_of(cols, vec ? 16 / es : 1, 16, 1024);
-    const dim3 block(sh.threads, sh.rows);
-    const unsigned grid = (unsigned)((rows + sh.rows - 1) / sh.rows);
-    by_shape<T, 32>(sh, [&](auto w, auto v) {
-      quantize_kernel<T, decltype(w)::value, decltype(v)::value>
-          <<<grid, block, 0, s>>>(src, rows, cols, ld, codes, pitch, scales);
+    // 16 values a thread (eight single ones); many rows are shared out in 32, as
+    // the maximum over a row's threads takes much of the work otherwise
+    const bool many = vec && rows >= 4 * (int64_t)ds::sm_count();
+    const Shape sh = shape_of(cols, vec ? 16 / es : 1, many ? 32 : vec ? 16 : 8, 512, 256);
+    by_shape<T, 2 * sizeof(T), 8>(sh, cols, [&](auto w, auto v, auto threads) {
+      launch_rows<quantize_kernel<T, decltype(w)::value, decltype(v)::value, decltype(threads)::value>>(
+          sh, rows, s, src, rows, cols, ld, codes, pitch, scales);
     });
   });
   DS_CHECK_LAUNCH("int8 quantize_kernel");

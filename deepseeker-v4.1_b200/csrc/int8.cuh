@@ -26,28 +26,51 @@ __device__ __forceinline__ float scale_of(uint32_t top) {
   return top >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(top) / 127.0f;
 }
 
-// Code of x in the low byte of the result, by the scale s >= 2^-126 and inv =
-// 1 / s.  x inv is off by a few parts in 2^24, so its rounding n (in the low
-// bits of a sum with 1.5 * 2^23) is wrong by one at most, next to the middle
-// of two codes; x - n s is exact (both are multiples of half the last place of
-// s, and |x| <= 127.5 s), so comparing twice of it with s settles the code.
-__device__ __forceinline__ uint32_t code_of(float x, float s, float inv) {
-  constexpr float kMagic = 12582912.0f;
-  const float r = fmaf(x, inv, kMagic);
-  const float d = fmaf(-(r - kMagic), s, x), t = 2.0f * fabsf(d);
-  uint32_t q = __float_as_uint(r);
-  if (t > s || (t == s && (q & 1u))) q += d > 0.0f ? 1u : 0xFFFFFFFFu;
-  return q & 0xFFu;
-}
+// A row's scale as codes are formed with it.  Small ones (their inverse may
+// leave f32) and the values go through a factor of 2^64, which is exact; a row
+// whose scale is 0 or no number has codes 0.
+struct Coder {
+  float s, inv;
+  bool small, none;
 
-// The same for smaller scales, whose inverse may leave f32: the quotient in 64
-// bits, which shows a tie only where there is one.  A scale of 0 has codes 0,
-// and so has one that is no number.
-__device__ __noinline__ uint32_t code_of_small(float x, float s) {
-  if (!(s > 0.0f)) return 0u;
-  const double q = rint((double)x / (double)s);
-  return (uint32_t)(int)fmin(fmax(q, -127.0), 127.0) & 0xFFu;
-}
+  __device__ __forceinline__ explicit Coder(float scale) : s(scale) {
+    small = !(scale >= 7.8886091e-31f);   // 2^-100
+    none = !(scale > 0.0f);
+    if (small) s = none ? 1.0f : scale * 18446744073709551616.0f;
+    inv = 1.0f / s;
+  }
+  // Codes of v, in the low bytes of q.  x inv is off by a few parts in 2^24, so
+  // its rounding n (in the low bits of a sum with 1.5 * 2^23) is wrong by one at
+  // most, next to the middle of two codes; x - n s is exact (both are multiples
+  // of half the last place of s, and |x| <= 127.5 s), so comparing twice of it
+  // with s settles the code, where any of them asks for it.
+  template <int VEC>
+  __device__ __forceinline__ void codes(float (&v)[VEC], uint32_t (&q)[VEC]) const {
+    using rows::Values;
+    constexpr float kMagic = 12582912.0f;
+    if (small) {
+      // a scale without its low bits may leave more than 127 of it
+      const float most = 127.0f * s;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] = none ? 0.0f : fminf(fmaxf(v[j] * 18446744073709551616.0f, -most), most);
+    }
+    const Values<VEC> x(v), r = fma(x, Values<VEC>(inv), Values<VEC>(kMagic));
+    float d[VEC], n[VEC], far = 0.0f;
+    fma(r + Values<VEC>(-kMagic), Values<VEC>(-s), x).get(d);
+    r.get(n);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      q[j] = __float_as_uint(n[j]);
+      far = fmaxf(far, fabsf(d[j]));
+    }
+    if (2.0f * far < s) return;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const float t = 2.0f * fabsf(d[j]);
+      if (t > s || (t == s && (q[j] & 1u))) q[j] += d[j] > 0.0f ? 1u : 0xFFFFFFFFu;
+    }
+  }
+};
 
 // Instruction descriptor, kind::i8: s8 operands, s32 accumulators.
 __device__ __forceinline__ constexpr uint32_t idesc(int m, int n) {

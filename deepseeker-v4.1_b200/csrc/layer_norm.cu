@@ -49,72 +49,87 @@ struct Forward {
   float eps;
 };
 
-// One row per blockDim.x threads, V times VEC values each.
-template <typename T, typename P, int VEC, int V>
-__global__ void __launch_bounds__(1024) forward_kernel(const Forward p) {
-  __shared__ float red[2][32];
-  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  if (row >= p.rows) return;   // whole rows: a warp, or the block
-  const T* x = static_cast<const T*>(p.x) + row * p.ld;
+// 1 / sqrt(a), to the last bits by one step of Newton's method.
+__device__ __forceinline__ float inverse_root(float a) {
+  const float y = rsqrtf(a);
+  return fmaf(0.5f * y, fmaf(-a * y, y, 1.0f), y);
+}
+
+// A block takes rows blockIdx.x, + gridDim.x ..., blockDim.y at a time, V times
+// VEC values a thread; THREADS: of a row, which they fill, or 0.  Up to 16
+// values, the parameters of a thread's columns stay in its registers.
+//
+// 16384 x 4096 bf16: 51 us, 5.2 TB/s (a plain copy of it: 43.5).  Behind memory
+// come instructions: a row takes 250 in each warp beside its values (two sums,
+// places, the root), so 16 values a thread, 80 registers (three blocks of 256
+// threads an SM; with 64 or 96 59 us) and the next row loaded while this one is
+// summed.  Measured beside it: no row ahead 72 us, eight values a thread 60, 32
+// 54, 64 with the parameters in shared memory 60, rows through a ring in shared
+// memory 64.
+template <typename T, typename P, int VEC, int V, int THREADS>
+__global__ void __maxnreg__(VEC > 1 && V * VEC <= 16 ? 80 : 128) forward_kernel(const Forward p) {
+  __shared__ float red[kMostRows][2][32];
   const P* w = static_cast<const P*>(p.w);
   const P* b = static_cast<const P*>(p.b);
-  float v[V][VEC];
-  {
-    Pack<T, VEC> k[V];
+  const float inv = 1.0f / p.cols;
+  const int64_t step = (int64_t)gridDim.x * blockDim.y;
+  auto column = [&](int i) { return (int)(i * (THREADS ? THREADS : blockDim.x) + threadIdx.x) * VEC; };
+  auto inside = [&](int i) { return THREADS || column(i) < p.cols; };
+  constexpr bool kKeep = V * VEC <= 16;
+  Values<VEC> kw[kKeep ? V : 1], kb[kKeep ? V : 1];
+  auto fetch_params = [&](int i, int to) {
+    float f[VEC];
+    kw[to] = Values<VEC>(1.0f), kb[to] = Values<VEC>(0.0f);
+    if (w) params<P, VEC>(w + column(i), f), kw[to] = Values<VEC>(f);
+    if (b) params<P, VEC>(b + column(i), f), kb[to] = Values<VEC>(f);
+  };
+  if constexpr (kKeep) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (inside(i)) fetch_params(i, i);
+  }
+  Pack<T, VEC> k[V];
+  auto fetch = [&](int64_t row) {
+    if (row >= p.rows) return;
+    const T* x = static_cast<const T*>(p.x) + row * p.ld;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (inside(i)) k[i].load(x + column(i));
+  };
+  int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  for (fetch(row); row < p.rows; row += step) {
+    Values<VEC> v[V], s(0.0f);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int c = (i * blockDim.x + threadIdx.x) * VEC;
-      if (c < p.cols) k[i].load(x + c);
+      if (!inside(i)) continue;
+      float f[VEC];
+      k[i].get(f);
+      v[i] = Values<VEC>(f);
+      s = s + v[i];
     }
+    fetch(row + step);   // on its way during the rest
+    const float mean = row_sum(total(s), red[threadIdx.y][0]) * inv;
+    const Values<VEC> less(-mean);
+    s = Values<VEC>(0.0f);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int c = (i * blockDim.x + threadIdx.x) * VEC;
-      if (c < p.cols) {
-        k[i].get(v[i]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[i][j] = 0.0f;
-      }
+      if (!inside(i)) continue;
+      v[i] = v[i] + less;
+      s = fma(v[i], v[i], s);
     }
-  }
-  float s = 0.0f;
+    const float r = inverse_root(row_sum(total(s), red[threadIdx.y][1]) * inv + p.eps);
+    if (p.stats && threadIdx.x == 0) p.stats[row] = make_float2(mean, r);
+    T* y = static_cast<T*>(p.y) + row * p.cols;
+    const Values<VEC> rs(r);
 #pragma unroll
-  for (int i = 0; i < V; ++i)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) s += v[i][j];
-  const float mean = row_sum(s, red[0]) / p.cols;
-  s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = (i * blockDim.x + threadIdx.x) * VEC;
-    if (c >= p.cols) continue;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      v[i][j] -= mean;
-      s = fmaf(v[i][j], v[i][j], s);
+    for (int i = 0; i < V; ++i) {
+      if (!inside(i)) continue;
+      const int at = kKeep ? i : 0;
+      float f[VEC];
+      if constexpr (!kKeep) fetch_params(i, 0);
+      fma(v[i] * rs, kw[at], kb[at]).get(f);
+      put<T, VEC>(y + column(i), f);
     }
-  }
-  const float r = 1.0f / sqrtf(row_sum(s, red[1]) / p.cols + p.eps);
-  if (p.stats && threadIdx.x == 0) p.stats[row] = make_float2(mean, r);
-  T* y = static_cast<T*>(p.y) + row * p.cols;
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = (i * blockDim.x + threadIdx.x) * VEC;
-    if (c >= p.cols) continue;
-    float k[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[i][j] *= r;
-    if (w) {
-      params<P, VEC>(w + c, k);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[i][j] *= k[j];
-    }
-    if (b) {
-      params<P, VEC>(b + c, k);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[i][j] += k[j];
-    }
-    put<T, VEC>(y + c, v[i]);
   }
 }
 
@@ -134,7 +149,7 @@ __global__ void __launch_bounds__(1024) forward_long_kernel(const Forward p) {
     const float d = (float)x[c] - mean;
     s = fmaf(d, d, s);
   }
-  const float r = 1.0f / sqrtf(row_sum(s, red[1]) / p.cols + p.eps);
+  const float r = inverse_root(row_sum(s, red[1]) / p.cols + p.eps);
   if (p.stats && threadIdx.x == 0) p.stats[row] = make_float2(mean, r);
   T* y = static_cast<T*>(p.y) + row * p.cols;
   for (int c = threadIdx.x; c < p.cols; c += blockDim.x) {
@@ -154,98 +169,191 @@ struct Backward {
   int cols;
 };
 
-// A block takes rows blockIdx.x, + gridDim.x ... (a warp each, or the block
-// one); its threads keep their columns' sums for the parameters, so x and dy
-// are read once for dx, dw and db together.  The next row is on its way while
-// this one is summed.
-template <typename T, typename P, int VEC, int V>
-__global__ void __launch_bounds__(512) backward_kernel(const Backward p) {
-  extern __shared__ float sums[];   // blockDim.y > 1: [2][cols] of a warp
-  __shared__ float2 red[2][32];
-  const T* x = static_cast<const T*>(p.x);
-  const T* dy = static_cast<const T*>(p.dy);
-  const P* w = static_cast<const P*>(p.w);
+// Sums of N values (2 or 4) over the threads of a row, for all of them.  Within
+// a warp a lane keeps half of the values at each of the first steps, so that N
+// sums take little more than one; red: [warps][N], where a row has several.
+template <int N>
+__device__ __forceinline__ void row_sums(float (&a)[N], float* red) {
   const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  float k[2] = {a[0], a[1]};
+  if constexpr (N == 4) {
+    const bool high = lane & 16;
+    k[0] = (high ? a[2] : a[0]) + __shfl_xor_sync(0xffffffffu, high ? a[0] : a[2], 16);
+    k[1] = (high ? a[3] : a[1]) + __shfl_xor_sync(0xffffffffu, high ? a[1] : a[3], 16);
+  }
+  constexpr int kBit = N == 4 ? 8 : 16;   // lane n * kBit ends up with value n
+  const bool high = lane & kBit;
+  float v = (high ? k[1] : k[0]) + __shfl_xor_sync(0xffffffffu, high ? k[0] : k[1], kBit);
+#pragma unroll
+  for (int o = kBit / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  int at = kBit;
+  if (warps > 1) {
+    if (lane % kBit == 0) red[(threadIdx.x >> 5) * N + lane / kBit] = v;
+    __syncthreads();
+    v = 0.0f;   // lane n + N m: value n of warps m, m + 32 / N ...
+    for (int i = lane; i < warps * N; i += 32) v += red[i];
+#pragma unroll
+    for (int o = N; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    at = 1;
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n) a[n] = __shfl_sync(0xffffffffu, v, n * at);
+}
+
+// How the backward kernel takes its rows: kRows at a time, in vectors through
+// slots, two turns ahead, single values through registers.
+template <int VEC, int V>
+struct Turn {
+  static constexpr bool kRing = VEC > 1;
+  static constexpr int kRows = kRing && V <= 2 ? 2 : 1;
+  static constexpr int kSlots = kRows * 2 * V;                          // x and dy, of a stage
+  static constexpr int kBytes = kRing ? kStages * kSlots * 16 : 0;      // a thread
+};
+
+// A block takes rows in turns (a warp each, or the block one of each turn); its
+// threads keep their columns' sums for the parameters, so x and dy are read
+// once for dx, dw and db together.
+template <typename T, typename P, int VEC, int V, int THREADS>
+__global__ void __launch_bounds__(512) backward_kernel(const Backward p) {
+  using U = Turn<VEC, V>;
+  constexpr int R = U::kRows, S = kStages;
+  extern __shared__ uint4 ring[];
+  __shared__ float red[2][16 * 2 * R];
+  const P* w = static_cast<const P*>(p.w);
   const float inv = 1.0f / p.cols;
-  float kw[V][VEC], aw[V][VEC], ab[V][VEC];
+  const Slots slots(ring);
+  auto column = [&](int i) { return (int)(i * (THREADS ? THREADS : blockDim.x) + threadIdx.x) * VEC; };
+  auto inside = [&](int i) { return THREADS || column(i) < p.cols; };
+  Values<VEC> kw[V], aw[V], ab[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int c = (i * blockDim.x + threadIdx.x) * VEC;
+    float v[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) aw[i][j] = ab[i][j] = 0.0f, kw[i][j] = 1.0f;
-    if (w && c < p.cols) params<P, VEC>(w + c, kw[i]);
+    for (int j = 0; j < VEC; ++j) v[j] = 1.0f;
+    if (w && inside(i)) params<P, VEC>(w + column(i), v);
+    kw[i] = Values<VEC>(v);
+    aw[i] = ab[i] = Values<VEC>(0.0f);
   }
-  Pack<T, VEC> nx[V], nd[V];
-  float2 nst = make_float2(0.0f, 0.0f);
-  auto fetch = [&](int64_t row) {
-    nst = p.stats[row];
+  const int64_t step = (int64_t)gridDim.x * blockDim.y * R, first = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * R;
+  Pack<T, VEC> held[U::kRing ? 1 : 2 * V];   // single values of the next row
+  float2 next[R];                            // its mean and r
+  auto fetch = [&](int stage, int64_t row) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = (i * blockDim.x + threadIdx.x) * VEC;
-      if (c >= p.cols) continue;
-      nx[i].load(x + row * p.ld + c);
-      nd[i].load(dy + row * p.ld_dy + c);
-    }
-  };
-  const int64_t step = (int64_t)gridDim.x * blockDim.y;
-  int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  if (row < p.rows) fetch(row);
-  for (int turn = 0; row < p.rows; row += step, turn ^= 1) {   // blockDim.y > 1 only with a warp a row
-    const float2 st = nst;
-    float xh[V][VEC], g[V][VEC];
-    float s1 = 0.0f, s2 = 0.0f;
+    for (int r = 0; r < R; ++r) {
+      if (row + r >= p.rows) continue;
+      const T* x = static_cast<const T*>(p.x) + (row + r) * p.ld;
+      const T* dy = static_cast<const T*>(p.dy) + (row + r) * p.ld_dy;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = (i * blockDim.x + threadIdx.x) * VEC;
-      if (c < p.cols) {
-        nx[i].get(xh[i]);
-        nd[i].get(g[i]);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          xh[i][j] = (xh[i][j] - st.x) * st.y;
-          aw[i][j] = fmaf(g[i][j], xh[i][j], aw[i][j]);
-          ab[i][j] += g[i][j];
-          g[i][j] *= kw[i][j];
-          s1 += g[i][j];
-          s2 = fmaf(g[i][j], xh[i][j], s2);
+      for (int i = 0; i < V; ++i) {
+        if (!inside(i)) continue;
+        const int c = column(i);
+        if constexpr (U::kRing) {
+          slots.copy(stage * U::kSlots + r * 2 * V + i, x + c);
+          slots.copy(stage * U::kSlots + r * 2 * V + V + i, dy + c);
+        } else {
+          held[i].load(x + c), held[V + i].load(dy + c);
         }
       }
     }
-    if (row + step < p.rows) fetch(row + step);
-    if (!p.dx) continue;
-    s1 = warp_sum(s1), s2 = warp_sum(s2);
-    if (warps > 1) {
-      if (lane == 0) red[turn][threadIdx.x >> 5] = make_float2(s1, s2);
-      __syncthreads();
-      const float2 o = lane < warps ? red[turn][lane] : make_float2(0.0f, 0.0f);
-      s1 = warp_sum(o.x), s2 = warp_sum(o.y);
+    if constexpr (U::kRing) slots.commit();
+  };
+  auto stats = [&](int64_t row) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) next[r] = row + r < p.rows ? p.stats[row + r] : make_float2(0.0f, 0.0f);
+  };
+#pragma unroll
+  for (int i = 0; i < (U::kRing ? S - 1 : 1); ++i) fetch(i, first + i * step);
+  stats(first);
+  int stage = 0, turn = 0;
+  for (int64_t row = first; row < p.rows; row += step, turn ^= 1) {   // blockDim.y > 1 only with a warp a row
+    float2 st[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) st[r] = next[r];
+    Pack<T, VEC> due[U::kRing ? 1 : 2 * V];   // single values of this row
+    const int here = stage;
+    if constexpr (U::kRing) {
+      slots.wait<S - 2>();
+      // into the stage whose rows the turn before this has used
+      fetch(here ? here - 1 : S - 1, row + (S - 1) * step);
+      stage = here + 1 == S ? 0 : here + 1;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2 * V; ++i) due[i] = held[i];
+      fetch(0, row + step);
     }
-    s1 *= inv, s2 *= inv;
-    T* dx = static_cast<T*>(p.dx) + row * p.cols;
+    stats(row + step);
+    // dy and xh, from the slots both times that they are asked for (registers
+    // that held them would be missing elsewhere)
+    auto at = [&](int r, int i, Values<VEC>& d, Values<VEC>& xh) {
+      Pack<T, VEC> kx, kd;
+      if constexpr (U::kRing) {
+        kx.raw = slots.read(here * U::kSlots + r * 2 * V + i);
+        kd.raw = slots.read(here * U::kSlots + r * 2 * V + V + i);
+      } else {
+        kx = due[i], kd = due[V + i];
+      }
+      float v[VEC];
+      kd.get(v);
+      d = Values<VEC>(v);
+      kx.get(v);
+      xh = fma(Values<VEC>(v), Values<VEC>(st[r].y), Values<VEC>(-st[r].x * st[r].y));
+    };
+    float sums[2 * R];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = (i * blockDim.x + threadIdx.x) * VEC;
-      if (c >= p.cols) continue;
+    for (int r = 0; r < R; ++r) {
+      Values<VEC> s1(0.0f), s2(0.0f);
+      if (r == 0 || row + r < p.rows) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) g[i][j] = st.y * (g[i][j] - s1 - xh[i][j] * s2);
-      put<T, VEC>(dx + c, g[i]);
+        for (int i = 0; i < V; ++i) {
+          if (!inside(i)) continue;
+          Values<VEC> d, xh;
+          at(r, i, d, xh);
+          aw[i] = fma(d, xh, aw[i]);
+          ab[i] = ab[i] + d;
+          d = d * kw[i];
+          s1 = s1 + d;
+          s2 = fma(d, xh, s2);
+        }
+      }
+      sums[2 * r] = total(s1), sums[2 * r + 1] = total(s2);
+    }
+    if (!p.dx) continue;
+    row_sums(sums, red[turn]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (r && row + r >= p.rows) continue;
+      const Values<VEC> m1(-sums[2 * r] * inv), m2(-sums[2 * r + 1] * inv), rs(st[r].y);
+      T* dx = static_cast<T*>(p.dx) + (row + r) * p.cols;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (!inside(i)) continue;
+        Values<VEC> d, xh;
+        at(r, i, d, xh);
+        float v[VEC];
+        (fma(d, kw[i], fma(xh, m2, m1)) * rs).get(v);
+        put<T, VEC>(dx + column(i), v);
+      }
     }
   }
   launch_dependents();
   if (!p.part) return;
   float* part = p.part + (int64_t)blockIdx.x * 2 * p.cols;
   if (blockDim.y > 1) {
-    // the warps add their sums one after the other
+    // the warps add their sums one after the other, where the ring was
+    float* sums = reinterpret_cast<float*>(ring);   // [2][cols]
+    __syncthreads();
     for (int y = 0; y < blockDim.y; ++y) {
       if (threadIdx.y == y) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const int c = (i * blockDim.x + threadIdx.x) * VEC;
-          if (c >= p.cols) continue;
+          if (!inside(i)) continue;
+          const int c = column(i);
+          float vw[VEC], vb[VEC];
+          aw[i].get(vw), ab[i].get(vb);
 #pragma unroll
           for (int j = 0; j < VEC; ++j) {
-            sums[c + j] = y ? sums[c + j] + aw[i][j] : aw[i][j];
-            sums[p.cols + c + j] = y ? sums[p.cols + c + j] + ab[i][j] : ab[i][j];
+            sums[c + j] = y ? sums[c + j] + vw[j] : vw[j];
+            sums[p.cols + c + j] = y ? sums[p.cols + c + j] + vb[j] : vb[j];
           }
         }
       }
@@ -256,15 +364,17 @@ __global__ void __launch_bounds__(512) backward_kernel(const Backward p) {
   }
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int c = (i * blockDim.x + threadIdx.x) * VEC;
-    if (c >= p.cols) continue;
+    if (!inside(i)) continue;
+    const int c = column(i);
+    float vw[VEC], vb[VEC];
+    aw[i].get(vw), ab[i].get(vb);
     if constexpr (VEC == 1) {
-      part[c] = aw[i][0], part[p.cols + c] = ab[i][0];
+      part[c] = vw[0], part[p.cols + c] = vb[0];
     } else {
 #pragma unroll
       for (int j = 0; j < VEC; j += 4) {   // cols is a multiple of VEC, so both halves lie on 16 bytes
-        *reinterpret_cast<float4*>(part + c + j) = make_float4(aw[i][j], aw[i][j + 1], aw[i][j + 2], aw[i][j + 3]);
-        *reinterpret_cast<float4*>(part + p.cols + c + j) = make_float4(ab[i][j], ab[i][j + 1], ab[i][j + 2], ab[i][j + 3]);
+        *reinterpret_cast<float4*>(part + c + j) = make_float4(vw[j], vw[j + 1], vw[j + 2], vw[j + 3]);
+        *reinterpret_cast<float4*>(part + p.cols + c + j) = make_float4(vb[j], vb[j + 1], vb[j + 2], vb[j + 3]);
       }
     }
   }
@@ -339,7 +449,17 @@ __global__ void __launch_bounds__(512) join_kernel(const float* __restrict__ par
 
 // ---------------------------------------------------------------- host side
 
-constexpr int kMostForward = 32 * 1024, kMostBackward = 16 * 512;
+// Features of rows that registers hold, 16 for each of 512 threads (in vectors
+// the forward pass takes eight of them, 64 KB).
+constexpr int kMost = 16 * 512;
+
+Shape forward_shape(int cols, int vec) { return shape_of(cols, vec, vec > 1 ? 16 : 8, 512, 32); }
+
+Shape backward_shape(int cols, int vec) {
+  Shape s = shape_of(cols, vec, vec > 1 ? 16 : 8, 512, 256);
+  if (s.threads > 32) s.rows = 1;
+  return s;
+}
 
 // f(type of x, type of the parameters)
 template <typename F>
@@ -352,8 +472,10 @@ void by_types(int dtype, int param_dtype, F f) {
 
 // Blocks of the backward pass, each with its sums.
 int backward_blocks(int64_t rows, const Shape& s) {
-  const int64_t most = (int64_t)ds::sm_count() * std::max(1, 1024 / (s.threads * s.rows));
-  return (int)std::min<int64_t>(most, (rows + s.rows - 1) / s.rows);
+  const int turn = s.rows * (s.vec > 1 && s.v <= 2 ? 2 : 1);   // Turn::kRows
+  // 128 registers a thread fill an SM with 512
+  const int64_t most = (int64_t)ds::sm_count() * std::max(1, 512 / (s.threads * s.rows));
+  return (int)std::min<int64_t>(most, (rows + turn - 1) / turn);
 }
 
 // Row groups of columns_kernel.
@@ -363,10 +485,10 @@ int column_blocks(int64_t rows, int cols) {
 }
 
 int backward_parts(int64_t rows, int cols) {
-  if (cols > kMostBackward) return column_blocks(rows, cols);
+  if (cols > kMost) return column_blocks(rows, cols);
   // whichever way the operands are aligned
   int n = 0;
-  for (int vec : {1, 4, 8}) n = std::max(n, backward_blocks(rows, shape_of(cols, vec, 16, 512)));
+  for (int vec : {1, 4, 8}) n = std::max(n, backward_blocks(rows, backward_shape(cols, vec)));
   return n;
 }
 
@@ -385,6 +507,7 @@ int validate(int dtype, int param_dtype, int64_t rows, int64_t cols, int64_t ld,
 }  // namespace ds
 
 using namespace ds::norm;
+using ds::SmemOnce;
 
 extern "C" int ds_layer_norm(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* weight,
                              const void* bias, int param_dtype, float eps, void* y, float* stats, void* stream) {
@@ -403,15 +526,13 @@ extern "C" int ds_layer_norm(const void* x, int dtype, int64_t rows, int64_t col
   by_types(dtype, param_dtype, [&](auto t, auto pt) {
     using T = decltype(t);
     using P = decltype(pt);
-    if (cols > kMostForward) {
+    if (cols > (vec ? 64 * 1024 / es : kMost)) {
       forward_long_kernel<T, P><<<(unsigned)rows, 1024, 0, s>>>(p);
       return;
     }
-    const Shape sh = shape_of((int)cols, vec ? 16 / es : 1, 16, 1024);
-    const dim3 block(sh.threads, sh.rows);
-    const unsigned grid = (unsigned)((rows + sh.rows - 1) / sh.rows);
-    by_shape<T, 32>(sh, [&](auto w, auto v) {
-      forward_kernel<T, P, decltype(w)::value, decltype(v)::value><<<grid, block, 0, s>>>(p);
+    const Shape sh = forward_shape((int)cols, vec ? 16 / es : 1);
+    by_shape<T, sizeof(T), 8>(sh, (int)cols, [&](auto w, auto v, auto threads) {
+      launch_rows<forward_kernel<T, P, decltype(w)::value, decltype(v)::value, decltype(threads)::value>>(sh, rows, s, p);
     });
   });
   DS_CHECK_LAUNCH("layer_norm forward_kernel");
@@ -451,20 +572,28 @@ extern "C" int ds_layer_norm_backward(const void* x, int dtype, int64_t rows, in
     by_types(dtype, param_dtype, [&](auto t, auto pt) {
       using T = decltype(t);
       using P = decltype(pt);
-      if (cols > kMostBackward) {
+      if (cols > kMost) {
         if (dx) backward_long_kernel<T, P><<<(unsigned)rows, 1024, 0, s>>>(p);
         blocks = column_blocks(rows, (int)cols);
         if (sums) columns_kernel<T><<<dim3((unsigned)((cols + 255) / 256), (unsigned)blocks), 256, 0, s>>>(p);
         return;
       }
-      const Shape sh = shape_of((int)cols, vec ? 16 / es : 1, 16, 512);
+      const Shape sh = backward_shape((int)cols, vec ? 16 / es : 1);
       const dim3 block(sh.threads, sh.rows);
       blocks = backward_blocks(rows, sh);
-      const size_t smem = sh.rows > 1 ? 2 * cols * sizeof(float) : 0;
-      by_shape<T, 16>(sh, [&](auto w, auto v) {
-        backward_kernel<T, P, decltype(w)::value, decltype(v)::value><<<blocks, block, smem, s>>>(p);
+      by_shape<T, sizeof(T), sizeof(T)>(sh, (int)cols, [&](auto w, auto v, auto threads) {
+        constexpr int W = decltype(w)::value, V = decltype(v)::value;
+        static SmemOnce once;
+        const auto kernel = &backward_kernel<T, P, W, V, decltype(threads)::value>;
+        int smem = Turn<W, V>::kBytes * sh.threads * sh.rows;
+        if (sh.rows > 1) smem = std::max(smem, (int)(2 * cols * sizeof(float)));
+        if (smem > 40 * 1024 &&
+            (st = ds::allow_smem(&once, reinterpret_cast<const void*>(kernel), Turn<W, V>::kBytes * 512)) != DS_OK)
+          return;
+        kernel<<<blocks, block, smem, s>>>(p);
       });
     });
+    if (st != DS_OK) return st;
     DS_CHECK_LAUNCH("layer_norm backward_kernel");
   }
   if (sums) {

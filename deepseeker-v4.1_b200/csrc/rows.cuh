@@ -66,24 +66,161 @@ __device__ __forceinline__ void put(T* p, const float (&v)[VEC]) {
   }
 }
 
+// Arithmetic on VEC values, two an instruction where there are two.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// VEC values, as pairs.
+template <int VEC>
+struct Values {
+  static constexpr int kPairs = VEC / 2;
+  uint64_t p[kPairs];
+  __device__ __forceinline__ Values() {}
+  __device__ __forceinline__ explicit Values(float all) {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) p[i] = two(all, all);
+  }
+  __device__ __forceinline__ explicit Values(const float (&v)[VEC]) {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) p[i] = two(v[2 * i], v[2 * i + 1]);
+  }
+  __device__ __forceinline__ void get(float (&v)[VEC]) const {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) split(p[i], v[2 * i], v[2 * i + 1]);
+  }
+};
+template <>
+struct Values<1> {
+  float p;
+  __device__ __forceinline__ Values() {}
+  __device__ __forceinline__ explicit Values(float v) : p(v) {}
+  __device__ __forceinline__ explicit Values(const float (&v)[1]) : p(v[0]) {}
+  __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = p; }
+};
+template <int VEC>
+__device__ __forceinline__ Values<VEC> operator+(const Values<VEC>& a, const Values<VEC>& b) {
+  Values<VEC> r;
+  if constexpr (VEC == 1) {
+    r.p = a.p + b.p;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) r.p[i] = add2(a.p[i], b.p[i]);
+  }
+  return r;
+}
+template <int VEC>
+__device__ __forceinline__ Values<VEC> operator*(const Values<VEC>& a, const Values<VEC>& b) {
+  Values<VEC> r;
+  if constexpr (VEC == 1) {
+    r.p = a.p * b.p;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) r.p[i] = mul2(a.p[i], b.p[i]);
+  }
+  return r;
+}
+template <int VEC>
+__device__ __forceinline__ Values<VEC> fma(const Values<VEC>& a, const Values<VEC>& b, const Values<VEC>& c) {
+  Values<VEC> r;
+  if constexpr (VEC == 1) {
+    r.p = fmaf(a.p, b.p, c.p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) r.p[i] = fma2(a.p[i], b.p[i], c.p[i]);
+  }
+  return r;
+}
+
+template <int VEC>
+__device__ __forceinline__ float total(const Values<VEC>& a) {
+  if constexpr (VEC == 1) {
+    return a.p;
+  } else {
+    uint64_t s = a.p[0];
+#pragma unroll
+    for (int i = 1; i < VEC / 2; ++i) s = add2(s, a.p[i]);
+    float lo, hi;
+    split(s, lo, hi);
+    return lo + hi;
+  }
+}
+
+// Slots of 16 bytes in shared memory, [slot][thread], that a thread fills with
+// asynchronous copies and reads itself, so it waits for nothing but its own:
+// rows on their way while others are in the registers, which alone do not hold
+// the 50 KB that an SM needs in flight.
+struct Slots {
+  uint32_t mine, pitch;
+  __device__ __forceinline__ explicit Slots(const void* smem)
+      : mine(static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + (threadIdx.y * blockDim.x + threadIdx.x) * 16),
+        pitch(blockDim.x * blockDim.y * 16) {}
+  __device__ __forceinline__ void copy(int slot, const void* src) const {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine + slot * pitch), "l"(src) : "memory");
+  }
+  static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  // All committed copies but those of the last N commits are here.
+  template <int N>
+  static __device__ __forceinline__ void wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+  }
+  __device__ __forceinline__ uint4 read(int slot) const {
+    uint4 q;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+                 : "r"(mine + slot * pitch)
+                 : "memory");
+    return q;
+  }
+};
+
+constexpr int kStages = 3;   // rows, or turns of rows, in a thread's slots
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// Sum over the threads of a row: a warp (any number of them in a block), or
-// the whole block, which then meets once.  The same value, bit for bit, in
-// every thread.
+// The warps of a row (threadIdx.y of several in a block) meet; a row of one
+// warp needs none of this.
+__device__ __forceinline__ void row_barrier() {
+  asm volatile("bar.sync %0, %1;" ::"r"(threadIdx.y + 1), "r"(blockDim.x) : "memory");
+}
+
+// Sum over the threads of a row, the same value, bit for bit, in every thread.
+// red: 32 words of the row's.
 __device__ __forceinline__ float row_sum(float v, float* red) {
   v = warp_sum(v);
   const int warps = blockDim.x >> 5;
   if (warps == 1) return v;
   const int lane = threadIdx.x & 31;
   if (lane == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
+  row_barrier();
   return warp_sum(lane < warps ? red[lane] : 0.0f);
 }
+
+constexpr int kMostRows = 8;   // of a block
 
 // ---------------------------------------------------------------- host side
 
@@ -93,20 +230,18 @@ struct Shape {
   int vec, v, threads, rows;
 };
 
-// Values per thread: up to `per`, so that 32 threads and more share a row;
-// beyond 1024 (backward: 512) threads more.
-inline Shape shape_of(int cols, int vec, int per, int most_threads) {
+// A thread takes up to `per` values before a row gets more than a warp, and
+// more only where `most_threads` threads do not hold the row; rows share a block
+// of up to block_threads.
+inline Shape shape_of(int cols, int vec, int per, int most_threads, int block_threads) {
   Shape s;
   s.vec = vec;
   const int n = (cols + vec - 1) / vec;
   s.v = 1;
   while (s.v * vec < per && s.v * 32 < n) s.v *= 2;
-  s.threads = 32;
-  while (s.threads < most_threads && s.threads * s.v < n) s.threads *= 2;
-  while (s.threads * s.v < n) s.v *= 2;
-  // the last doubling may have left whole warps idle
+  while (s.v * most_threads < n) s.v *= 2;
   s.threads = ((n + s.v - 1) / s.v + 31) / 32 * 32;
-  s.rows = s.threads == 32 ? 8 : 1;
+  s.rows = std::max(1, std::min(kMostRows, block_threads / s.threads));
   return s;
 }
 
@@ -117,21 +252,67 @@ void by_type(int dtype, F f) {
   else f(__nv_bfloat16());
 }
 
-// f(values per vector, vectors per thread)
-template <typename T, int MOST, typename F>
-void by_shape(const Shape& s, F f) {
-  constexpr int kVec = 16 / sizeof(T);
-  auto go = [&](auto vec) {
-    constexpr int W = decltype(vec)::value;
-    if (s.v == 1) f(vec, std::integral_constant<int, 1>());
-    else if (s.v == 2) f(vec, std::integral_constant<int, 2>());
-    else if (s.v == 4) f(vec, std::integral_constant<int, std::min(4, MOST / W)>());
-    else if (s.v == 8) f(vec, std::integral_constant<int, std::min(8, MOST / W)>());
-    else if (s.v == 16) f(vec, std::integral_constant<int, std::min(16, MOST / W)>());
-    else f(vec, std::integral_constant<int, std::min(32, MOST / W)>());
-  };
-  if (s.vec == 1) go(std::integral_constant<int, 1>());
-  else go(std::integral_constant<int, kVec>());
+// f(values per vector, vectors per thread, threads of a row) with constants: up
+// to MOST vectors of 16 bytes or 16 single values.  Rows that FILLED vectors a
+// thread fill get their number of threads as a constant, others 0: offsets that
+// are constants and no checks of columns are worth a sixth of a pass over rows
+// of 4096.
+template <typename T, int FILLED, int MOST, typename F>
+void by_shape(const Shape& s, int cols, F f) {
+  using std::integral_constant;
+  const integral_constant<int, 16 / (int)sizeof(T)> vec;
+  const integral_constant<int, 1> one;
+  const integral_constant<int, 0> any;
+  if (s.vec == 1) {
+    if (s.v == 1) f(one, one, any);
+    else if (s.v == 2) f(one, integral_constant<int, 2>(), any);
+    else if (s.v == 4) f(one, integral_constant<int, 4>(), any);
+    else if (s.v == 8) f(one, integral_constant<int, 8>(), any);
+    else f(one, integral_constant<int, 16>(), any);
+  } else if (s.v == FILLED && s.vec * s.v * s.threads == cols && s.threads <= 512) {
+    const integral_constant<int, FILLED> v;
+    if (s.threads == 32) f(vec, v, integral_constant<int, 32>());
+    else if (s.threads == 64) f(vec, v, integral_constant<int, 64>());
+    else if (s.threads == 128) f(vec, v, integral_constant<int, 128>());
+    else if (s.threads == 160) f(vec, v, integral_constant<int, 160>());
+    else if (s.threads == 256) f(vec, v, integral_constant<int, 256>());
+    else if (s.threads == 320) f(vec, v, integral_constant<int, 320>());
+    else if (s.threads == 512) f(vec, v, integral_constant<int, 512>());
+    else f(vec, v, any);
+  } else if (s.v == 1) {
+    f(vec, one, any);
+  } else if (s.v == 2) {
+    f(vec, integral_constant<int, 2>(), any);
+  } else if (s.v == 4) {
+    f(vec, integral_constant<int, std::min(4, MOST)>(), any);
+  } else {
+    f(vec, integral_constant<int, std::min(8, MOST)>(), any);
+  }
+}
+
+// Blocks of `kernel` that an SM holds, asked for once per size.
+struct Residency {
+  unsigned char known[33];   // by warps
+};
+inline int resident(Residency* r, const void* kernel, int threads, size_t smem) {
+  unsigned char* at = &r->known[threads / 32];
+  if (const int n = __atomic_load_n(at, __ATOMIC_RELAXED)) return n;
+  int n = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) {
+    (void)cudaGetLastError();
+    return 1;
+  }
+  __atomic_store_n(at, (unsigned char)n, __ATOMIC_RELAXED);
+  return n;
+}
+
+// Launches KERNEL, which takes rows blockIdx.x, + gridDim.x ..., on as many
+// blocks as are resident at a time.
+template <auto KERNEL, typename... A>
+void launch_rows(const Shape& sh, int64_t rows, cudaStream_t s, const A&... args) {
+  static Residency known;
+  const int64_t most = (int64_t)ds::sm_count() * resident(&known, reinterpret_cast<const void*>(KERNEL), sh.threads * sh.rows, 0);
+  KERNEL<<<(unsigned)std::min<int64_t>((rows + sh.rows - 1) / sh.rows, most), dim3(sh.threads, sh.rows), 0, s>>>(args...);
 }
 
 inline bool vectors(const void* p, int64_t rows, int64_t cols, int64_t ld, int es) {

@@ -276,11 +276,12 @@ def test_many_values(cuda):
     w = torch.ones(cols, dtype=F32, device=cuda, requires_grad=True)
     y = norm.layer_norm(x.requires_grad_(), w)
     at = torch.tensor([0, 4096, 1 << 19, rows - 2, rows - 1], device=cuda)
-    assert torch.equal(y[at], norm.layer_norm(x[at]))
+    # (sums over many rows and over few are shared out among threads differently, so not bit by bit)
+    xs = x.detach()[at]
+    want = formula(xs, None, None, 1e-5, xs)
+    check(y.detach()[at], want["y"], "y")
     dx, = torch.autograd.grad(y, x, x.detach())
-    a = x.detach()[at].requires_grad_()
-    want, = torch.autograd.grad(norm.layer_norm(a, w), a, x.detach()[at])
-    assert torch.equal(dx[at], want)
+    check(dx[at], want["dx"], "dx")
 
 
 def test_refusals(cuda):
