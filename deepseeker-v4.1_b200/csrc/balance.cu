@@ -21,6 +21,7 @@
 #include "ds_common.cuh"
 #include "ptx.cuh"
 #include "route.cuh"
+#include "rows.cuh"
 
 namespace ds {
 namespace balance {
@@ -28,6 +29,11 @@ namespace {
 
 namespace cg = cooperative_groups;
 using namespace ds::ptx;
+using ds::rows::add2;
+using ds::rows::fma2;
+using ds::rows::mul2;
+using ds::rows::split;
+using ds::rows::two;
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 
@@ -127,10 +133,50 @@ __device__ __forceinline__ float group_sum(float v, int lanes) {
   return v;
 }
 
+// 2^x, sqrt(x), 1 / sqrt(x) and 1 / x of the special function unit, off by a few
+// units in the last place of f32 (results below 2^-126 become 0).
+__device__ __forceinline__ float fast_exp2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float fast_sqrt(float x) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float fast_rsqrt(float x) {
+  float r;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float fast_inverse(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// log(1 + t) / t on [0, 1]: the polynomial of degree 8 with the least largest
+// relative error (a fit in 64 bits: 3e-8; 3 units of f32 with its roundings).
+__device__ __forceinline__ uint64_t log1p_ratio2(uint64_t t) {
+  constexpr float k[9] = {0.9999999403953552f, -0.4999949336051941f, 0.3331909477710724f, -0.2484297752380371f,
+                          0.1910598874092102f, -0.1366320699453354f, 0.07822549343109131f, -0.029504956677556038f,
+                          0.005232623778283596f};
+  uint64_t r = two(k[8], k[8]);
+#pragma unroll
+  for (int i = 7; i >= 0; --i) r = fma2(r, t, two(k[i], k[i]));
+  return r;
+}
+
 // A row's logits -> a (in place), its slope da / dl where asked for.  Columns
-// past the row hold -infinity, which gives a = 0 and slope 0.
+// past the row hold -infinity, which gives a = 0 and slope 0.  sqrt(softplus)
+// takes 14 instructions and two of the special function unit a value, 18 and
+// three with its slope (expf, log1pf, sqrtf and divisions: 50 to 70, and the
+// passes over 65536 x 384 three times as long as their memory).
 template <bool SOFTMAX, bool SLOPE, int N>
 __device__ __forceinline__ void scores(float (&v)[N], float (&slope)[SLOPE && !SOFTMAX ? N : 1], int lanes) {
+  static_assert(N % 2 == 0, "pairs");
+  constexpr float kLog2e = 1.44269504f;
   if constexpr (SOFTMAX) {
     float m = v[0];
 #pragma unroll
@@ -138,17 +184,33 @@ __device__ __forceinline__ void scores(float (&v)[N], float (&slope)[SLOPE && !S
     for (int o = 1; o < lanes; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (m == -INFINITY) m = 0.0f;   // no expert is left: every a is 0
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = expf(v[j] - m);
+    for (int j = 0; j < N; j += 2) {
+      float x, y;
+      split(mul2(add2(two(v[j], v[j + 1]), two(-m, -m)), two(kLog2e, kLog2e)), x, y);
+      v[j] = fast_exp2(x), v[j + 1] = fast_exp2(y);
+    }
   } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float l = v[j];
-      // below -17 softplus(l) is exp(l) in f32, and its root stays above 0 for longer
-      const float h = expf(-0.5f * fabsf(l)), t = h * h;
-      const bool low = l < -17.0f;
-      const float a = low ? h : sqrtf(fmaxf(l, 0.0f) + log1pf(t));
-      if constexpr (SLOPE) slope[j] = low ? 0.5f * h : (l >= 0.0f ? 0.5f : 0.5f * t) / ((1.0f + t) * a);
-      v[j] = a;   // a NaN comes through the logarithm
+    for (int j = 0; j < N; j += 2) {
+      float h[2], s[2], t[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) h[i] = fast_exp2(fabsf(v[j + i]) * (-0.5f * kLog2e));   // exp(-|l| / 2)
+      const uint64_t h2 = two(h[0], h[1]), t2 = mul2(h2, h2);
+      // softplus(l) = max(l, 0) + log(1 + exp(-|l|))
+      split(fma2(t2, log1p_ratio2(t2), two(fmaxf(v[j], 0.0f), fmaxf(v[j + 1], 0.0f))), s[0], s[1]);
+      split(t2, t[0], t[1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float l = v[j + i];
+        const bool low = l < -17.0f;   // softplus(l) is exp(l) in f32, and its root stays above 0 for longer
+        if constexpr (SLOPE) {
+          const float root = fast_rsqrt(s[i]);
+          v[j + i] = low ? h[i] : s[i] * root;
+          slope[j + i] = low ? 0.5f * h[i] : (l >= 0.0f ? 0.5f : 0.5f * t[i]) * root * fast_inverse(1.0f + t[i]);
+        } else {
+          v[j + i] = low ? h[i] : fast_sqrt(s[i]);
+        }
+      }
     }
   }
 }
@@ -196,9 +258,14 @@ __device__ __forceinline__ void unpack(const Pack<T, VEC> (&k)[NV], float (&v)[N
   }
 }
 
-// Loss and coefficients of expert e of a sequence of n valid tokens.
-__device__ __forceinline__ double finish(const Params& p, int64_t s, int e, float sum, int count, int n) {
-  const double c = n ? (double)count * p.experts / ((double)p.top_k * n * n) : 0.0;
+// E / (k n^2) of a sequence of n valid tokens, 0 without any.
+__device__ __forceinline__ double factor_of(const Params& p, int n) {
+  return n ? (double)p.experts / ((double)p.top_k * n * n) : 0.0;
+}
+
+// Stores count and coefficient of expert e; its part of the loss.
+__device__ __forceinline__ double finish(const Params& p, int64_t s, int e, float sum, int count, double factor) {
+  const double c = count * factor;
   p.counts[s * p.experts + e] = count;
   p.coef[s * p.experts + e] = (float)c;
   return c * sum;
@@ -210,8 +277,14 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
+// Blocks of an SM, by the registers that a lane's values ask for.
+__host__ __device__ constexpr int blocks_of(int vec, int nv) {
+  const int n = vec == 1 ? 2 * nv : vec * nv;   // single values need their places too
+  return n <= 12 ? 4 : n <= 16 ? 3 : n <= 32 ? 2 : 1;
+}
+
 template <typename T, bool SOFTMAX, int VEC, int NV>
-__global__ void __launch_bounds__(kThreads) forward_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, blocks_of(VEC, NV)) forward_kernel(const Params p) {
   constexpr int N = NV * VEC;
   extern __shared__ uint8_t smem[];
   float* sums = reinterpret_cast<float*>(smem);                       // [kWarps][experts]
@@ -227,9 +300,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Params p) {
     for (int e = threadIdx.x; e < p.experts; e += kThreads) hist[e] = 0;
     if (threadIdx.x == 0) valid_rows = 0;
     __syncthreads();
-    float acc[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] = 0.0f;
+    uint64_t acc[N / 2] = {};
     int n = 0;
     Pack<T, VEC> next[NV];
     bool ok = false;
@@ -238,50 +309,58 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Params p) {
       if (ok) fetch<T, VEC, NV>(next, logits + row * p.ld, l, G, p.experts);
     };
     ask(from + slot);
+    // the chosen experts, while the first rows are on their way
+    const int chosen = (int)((to - from) * p.top_k);
+    const int32_t* ids = p.ids + from * p.top_k;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < chosen; i += kThreads) {
+      const int id = ids[i];
+      if ((unsigned)id < (unsigned)p.experts && (!p.valid || p.valid[from + i / p.top_k])) atomicAdd(&hist[id], 1);
+    }
     for (int64_t first = from; first < to; first += per_pass) {
       const int64_t row = first + slot;
       const bool live = ok;
       float v[N], none[1];
       unpack<T, VEC, NV>(next, v, l, G, p.experts, live);
       ask(row + per_pass);
-      if (live) {
-        n += l == 0;
-        for (int i = l; i < p.top_k; i += G) {
-          const int id = p.ids[row * p.top_k + i];
-          if ((unsigned)id < (unsigned)p.experts) atomicAdd(&hist[id], 1);
-        }
-      }
+      n += live && l == 0;
       scores<SOFTMAX, false, N>(v, none, G);
-      float z = 0.0f;
+      uint64_t z2 = 0;
 #pragma unroll
-      for (int j = 0; j < N; ++j) z += v[j];
-      z = group_sum(z, G);
+      for (int j = 0; j < N; j += 2) z2 = add2(z2, two(v[j], v[j + 1]));
+      float z, y;
+      split(z2, z, y);
+      z = group_sum(z + y, G);
       const float inv = z == 0.0f ? 0.0f : 1.0f / z;   // a row without scores has no shares
 #pragma unroll
-      for (int j = 0; j < N; ++j) acc[j] = fmaf(v[j], inv, acc[j]);
+      for (int j = 0; j < N; j += 2) acc[j / 2] = fma2(two(v[j], v[j + 1]), two(inv, inv), acc[j / 2]);
     }
+    float part[N];
+#pragma unroll
+    for (int j = 0; j < N; j += 2) split(acc[j / 2], part[j], part[j + 1]);
     // lanes of the same column, then the warps
 #pragma unroll
     for (int j = 0; j < N; ++j)
-      for (int o = G; o < 32; o <<= 1) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
+      for (int o = G; o < 32; o <<= 1) part[j] += __shfl_xor_sync(0xffffffffu, part[j], o);
     if (lane < G) {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const int c = column<VEC>(j, l, G);
-        if (c < p.experts) sums[warp * p.experts + c] = acc[j];
+        if (c < p.experts) sums[warp * p.experts + c] = part[j];
       }
     }
     n = __reduce_add_sync(0xffffffffu, n);
     if (lane == 0 && n) atomicAdd(&valid_rows, n);
     __syncthreads();
     uint32_t* rec = p.records + (blockIdx.x + s) * record_words(p);
+    const double factor = p.single ? factor_of(p, valid_rows) : 0.0;
     double loss = 0.0;
     for (int e = threadIdx.x; e < p.experts; e += kThreads) {
       float t = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) t += sums[w * p.experts + e];
       if (p.single) {
-        loss += finish(p, 0, e, t, hist[e], valid_rows);
+        loss += finish(p, 0, e, t, hist[e], factor);
       } else {
         rec[e] = __float_as_uint(t);
         rec[p.experts + e] = (uint32_t)hist[e];
@@ -318,32 +397,38 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Params p) {
   wait_prior_grid();
   const uint32_t* rec = p.records + s * words;   // + block * words
   int n = 0;
-  for (int64_t b = b0 + threadIdx.x; b < b1; b += 32 * kJoinWarps) n += (int)rec[b * words + 2 * p.experts];
-  n = __reduce_add_sync(0xffffffffu, n);
-  if (lane == 0) ints[warp][32] = n;
-  __syncthreads();
-  n = 0;
-#pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) n += ints[w][32];
-  double loss = 0.0;
+  double loss = 0.0, factor = 0.0;
   for (int tile = rank; tile < tiles; tile += parts) {
+    const bool first = tile == rank;
     const int e = tile * 32 + lane;
     float t = 0.0f;
     int c = 0;
+    if (first)   // beside the sums' loads
+      for (int64_t b = b0 + threadIdx.x; b < b1; b += 32 * kJoinWarps) n += (int)rec[b * words + 2 * p.experts];
     if (e < p.experts) {
-#pragma unroll 4
+#pragma unroll 8
       for (int64_t b = b0 + warp; b < b1; b += kJoinWarps) {
         t += __uint_as_float(rec[b * words + e]);
         c += (int)rec[b * words + p.experts + e];
       }
     }
     sums[warp][lane] = t, ints[warp][lane] = c;
+    if (first) {
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (lane == 0) ints[warp][32] = n;
+    }
     __syncthreads();
     if (warp == 0) {
+      if (first) {
+        n = 0;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) n += ints[w][32];
+        factor = factor_of(p, n);
+      }
       t = 0.0f, c = 0;
 #pragma unroll
       for (int w = 0; w < kJoinWarps; ++w) t += sums[w][lane], c += ints[w][lane];
-      if (e < p.experts) loss += finish(p, s, e, t, c, n);
+      if (e < p.experts) loss += finish(p, s, e, t, c, factor);
     }
     __syncthreads();
   }
@@ -361,7 +446,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Params p) {
 }
 
 template <typename T, bool SOFTMAX, int VEC, int NV>
-__global__ void __launch_bounds__(kThreads) backward_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, blocks_of(VEC, NV)) backward_kernel(const Params p) {
   constexpr int N = NV * VEC;
   const int lane = threadIdx.x & 31, G = p.lanes, l = lane & (G - 1);
   const int per_pass = kThreads / G, slot = threadIdx.x / G;
@@ -391,9 +476,18 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const Params p) {
       unpack<T, VEC, NV>(next, v, l, G, p.experts, live);
       ask(row + per_pass);
       scores<SOFTMAX, true, N>(v, slope, G);
-      float z = 0.0f, d = 0.0f;
+      uint64_t z2 = 0, d2 = 0;
 #pragma unroll
-      for (int j = 0; j < N; ++j) z += v[j], d = fmaf(v[j], c[j], d);
+      for (int j = 0; j < N; j += 2) {
+        const uint64_t a = two(v[j], v[j + 1]);
+        z2 = add2(z2, a);
+        d2 = fma2(a, two(c[j], c[j + 1]), d2);
+      }
+      float z, d, y;
+      split(z2, z, y);
+      z += y;
+      split(d2, d, y);
+      d += y;
       for (int o = 1; o < G; o <<= 1) {
         z += __shfl_xor_sync(0xffffffffu, z, o);
         d += __shfl_xor_sync(0xffffffffu, d, o);
@@ -401,7 +495,10 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const Params p) {
       const float inv = z == 0.0f ? 0.0f : 1.0f / z, k = live ? g * inv : 0.0f;
       d *= inv;
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = k * (SOFTMAX ? v[j] : slope[SOFTMAX ? 0 : j]) * (c[j] - d);
+      for (int j = 0; j < N; j += 2) {
+        const uint64_t a = SOFTMAX ? two(v[j], v[j + 1]) : two(slope[SOFTMAX ? 0 : j], slope[SOFTMAX ? 0 : j + 1]);
+        split(mul2(mul2(two(k, k), a), add2(two(c[j], c[j + 1]), two(-d, -d))), v[j], v[j + 1]);
+      }
       if (row < to) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -429,6 +526,9 @@ Layout layout_of(int experts, bool vec) {
   a.lanes = 1;
   while (a.lanes < 32 && (n + a.lanes - 1) / a.lanes > most) a.lanes *= 2;
   a.nv = (n + a.lanes - 1) / a.lanes;
+  // as by_layout rounds it up
+  if (vec) a.nv = a.nv <= 4 ? a.nv : 8;
+  else a.nv = a.nv <= 4 ? 4 : a.nv <= 8 ? 8 : a.nv <= 16 ? 16 : 32;
   return a;
 }
 
@@ -465,9 +565,9 @@ bool vectors(const void* p, int experts, int64_t tokens, int64_t ld, int dtype) 
   return experts % 4 == 0 && (tokens <= 1 || ld % 4 == 0) && ds::aligned(p, dtype == DS_F32 ? 16 : 8);
 }
 
-// Rows of a block: whole passes, and enough blocks for three or more on every SM.
+// Rows of a block: whole passes, and as many blocks as are resident at a time.
 int64_t rows_per_block(int64_t tokens, const Layout& a) {
-  const int64_t pass = kThreads / a.lanes, most = (int64_t)ds::sm_count() * 4;
+  const int64_t pass = kThreads / a.lanes, most = (int64_t)ds::sm_count() * blocks_of(a.vec, a.nv);
   return ((tokens + most - 1) / most + pass - 1) / pass * pass;
 }
 
@@ -553,7 +653,7 @@ extern "C" int ds_balance_loss(const DsBalance* desc, float* loss, int32_t* coun
     DS_CHECK_LAUNCH("balance forward_kernel");
   }
   if (p.single) return DS_OK;
-  const int parts = d.sequences * 8 <= ds::sm_count() ? 8 : 1;
+  const int parts = d.sequences <= 512 ? 8 : 1;   // a block alone takes the experts 32 after 32
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(d.sequences * parts));
   cfg.blockDim = dim3(32 * kJoinWarps);

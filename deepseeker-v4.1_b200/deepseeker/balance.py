@@ -87,10 +87,13 @@ class _BalanceLoss(torch.autograd.Function):
         ctx.save_for_backward(logits, valid, offsets, kept)
         ctx.kind = kind
         ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)   # of the counts, which have none
         return loss, counts
 
     @staticmethod
     def backward(ctx, dloss, _):
+        if dloss is None:
+            return None, None, None, None, None
         # a graph of the gradients (create_graph) is refused where it is used; plain passes skip that wrapper's cost
         return _backward_once(ctx, dloss) if torch.is_grad_enabled() else _backward(ctx, dloss)
 
