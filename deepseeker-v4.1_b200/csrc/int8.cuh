@@ -72,6 +72,11 @@ struct Coder {
   }
 };
 
+// The low bytes of four codes as a word.
+__device__ __forceinline__ uint32_t pack_codes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
 // Instruction descriptor, kind::i8: s8 operands, s32 accumulators.
 __device__ __forceinline__ constexpr uint32_t idesc(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);

@@ -30,6 +30,11 @@ def _workspace_bytes(rows: int, cols: int) -> int:
     return _up(rows * _up(cols, 16), 256) + _up(4 * rows, 256)
 
 
+def _x_bytes(rows: int, cols: int) -> int:
+    """Workspace for x given as values: a single row the product quantises itself."""
+    return _workspace_bytes(rows, cols) if rows > 1 else 0
+
+
 class Int8Tensor:
     """A quantised matrix: ``codes`` i8 and ``scales`` f32 of its rows (value =
     code * scale; scale NaN for a row that held a NaN or an infinity); ``shape``:
@@ -155,8 +160,8 @@ def linear(x, w: Int8Tensor, out_dtype: torch.dtype | None = None) -> torch.Tens
     if out_dtype not in _DTYPES:
         raise ValueError("out_dtype must be f32, bf16 or f16")
     if ps is None:
-        n = _workspace_bytes(rows, w.cols)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        n = _x_bytes(rows, w.cols)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     out = torch.empty((*x.shape[:-1], w.rows), dtype=out_dtype, device=dev)
     with on_device(dev):
         _abi.check(_abi.lib().ds_int8_linear(px, ps, dt, rows, ld, w._ref(), out.data_ptr(), _DTYPES[out_dtype],

@@ -603,8 +603,9 @@ typedef struct DsInt8 {
  * products of codes, exact in 32-bit integers, converted to f32, times both
  * scales (the smaller first), rounded to out's type.  x_dtype f32 / bf16 / f16:
  * x [rows, w->cols], rows ld elements apart, is quantised into the workspace
- * first (x_scales NULL); DS_I8: x is codes, rows ld bytes apart (a multiple of
- * 16), x_scales their scales, and no workspace is needed.  rows in [0, 2^22]. */
+ * first (x_scales NULL; a single row by the product itself, without one);
+ * DS_I8: x is codes, rows ld bytes apart (a multiple of 16), x_scales their
+ * scales, and no workspace is needed.  rows in [0, 2^22]. */
 int ds_int8_linear_workspace_size(int64_t rows, int64_t cols, size_t* bytes);
 int ds_int8_linear(const void* x, const float* x_scales, int x_dtype, int64_t rows, int64_t ld, const DsInt8* w,
                    void* out, int out_dtype, void* workspace, size_t workspace_bytes, void* stream);

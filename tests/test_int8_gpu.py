@@ -145,7 +145,8 @@ def check(y, want):
     assert y.shape == want.shape and bool((err <= bound).all()), (float((err - bound).max()), float(err.max()))
 
 
-PRODUCTS = [(1, 1, 1), (1, 32, 128), (1, 4096, 4096), (2, 64, 1), (15, 33, 40), (16, 256, 128), (17, 999, 513),
+PRODUCTS = [(1, 1, 1), (2, 15, 9), (3, 17, 5), (4, 500, 1300), (5, 4096, 300), (7, 10000, 33), (8, 64, 5000),
+            (9, 100, 130), (12, 1100, 257), (1, 32, 128), (1, 4096, 4096), (2, 64, 1), (15, 33, 40), (16, 256, 128), (17, 999, 513),
             (32, 130, 96), (33, 160, 264), (64, 1, 7), (65, 288, 640), (100, 1001, 777), (128, 512, 128), (129, 544, 200),
             (200, 2000, 72), (300, 2560, 136), (1111, 96, 1280), (1, 20000, 24), (257, 384, 256), (2048, 128, 384),
             (520, 1024, 4096), (3000, 257, 2049)]

@@ -43,7 +43,7 @@ def test_dequantize_arguments(lib):
     assert call(rows=0, codes=None, out=None) == _abi.DS_OK
 
 
-def linear(lib, x=256, xs=None, dtype=BF16, rows=4, ld=40, out=256, to=BF16, ws=256, n=1 << 20, null=False, **w):
+def linear(lib, x=256, xs=None, dtype=BF16, rows=20, ld=40, out=256, to=BF16, ws=256, n=1 << 20, null=False, **w):
     d = dict(codes=256, scales=256, rows=8, cols=40, pitch=48)
     d.update(w.get("w", {}))
     return lib.ds_int8_linear(x, xs, dtype, rows, ld, None if null else ctypes.byref(_abi.DsInt8(**d)), out, to, ws, n,
@@ -59,7 +59,7 @@ def linear(lib, x=256, xs=None, dtype=BF16, rows=4, ld=40, out=256, to=BF16, ws=
     (dict(dtype=I8, xs=256, ld=32, rows=1), _abi.DS_EINVAL), (dict(dtype=I8, xs=256, ld=48, x=264), _abi.DS_EALIGN),
     (dict(dtype=I8, xs=258, ld=48), _abi.DS_EALIGN), (dict(rows=-1), _abi.DS_ERANGE),
     (dict(rows=(1 << 22) + 1), _abi.DS_ERANGE), (dict(ld=39), _abi.DS_EINVAL), (dict(to=U8), _abi.DS_EINVAL),
-    (dict(x=None), _abi.DS_EINVAL), (dict(x=257), _abi.DS_EALIGN), (dict(n=511), _abi.DS_EINVAL),
+    (dict(x=None), _abi.DS_EINVAL), (dict(x=257), _abi.DS_EALIGN), (dict(n=20 * 48 + 64 + 256 - 1), _abi.DS_EINVAL),
     (dict(ws=None), _abi.DS_EINVAL), (dict(ws=264), _abi.DS_EALIGN), (dict(out=None), _abi.DS_EALIGN),
     (dict(out=257), _abi.DS_EALIGN)])
 def test_linear_arguments(lib, kw, status):
@@ -69,9 +69,10 @@ def test_linear_arguments(lib, kw, status):
 
 def test_sizes(lib):
     n = ctypes.c_size_t(0)
-    for rows, cols in ((0, 1), (1, 1), (5, 16), (7, 17), (129, 4096)):
+    for rows, cols in ((0, 1), (1, 1), (2, 16), (3, 16), (8, 40), (9, 17), (16, 17), (17, 17), (129, 4096)):
         assert lib.ds_int8_linear_workspace_size(rows, cols, ctypes.byref(n)) == _abi.DS_OK
-        assert n.value == int8._workspace_bytes(rows, cols)
+        assert n.value == int8._x_bytes(rows, cols) == (
+            int8._workspace_bytes(rows, cols) if rows > 1 else 0)
     assert lib.ds_int8_linear_workspace_size(1, 0, ctypes.byref(n)) == _abi.DS_EINVAL
     assert lib.ds_int8_linear_workspace_size(1, 1, None) == _abi.DS_EINVAL
     assert lib.ds_int8_status(None, None) == _abi.DS_EINVAL
