@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(512) join_kernel(const float* __restrict__ par
 // the forward pass takes eight of them, 64 KB).
 constexpr int kMost = 16 * 512;
 
-Shape forward_shape(int cols, int vec) { return shape_of(cols, vec, vec > 1 ? 16 : 8, 512, 32); }
+Shape forward_shape(int cols, int vec) { return shape_of(cols, vec, vec > 1 ? 16 : 8, 512, 128); }
 
 Shape backward_shape(int cols, int vec) {
   Shape s = shape_of(cols, vec, vec > 1 ? 16 : 8, 512, 256);
@@ -513,7 +513,7 @@ extern "C" int ds_layer_norm(const void* x, int dtype, int64_t rows, int64_t col
                              const void* bias, int param_dtype, float eps, void* y, float* stats, void* stream) {
   int st = validate(dtype, param_dtype, rows, cols, ld, "layer_norm");
   if (st != DS_OK) return st;
-  DS_REQUIRE(eps >= 0.0f, DS_EINVAL, "layer_norm: eps must be >= 0");
+  DS_REQUIRE(eps >= 0.0f && eps <= 3.4e38f, DS_EINVAL, "layer_norm: eps must be a number >= 0");
   if (rows == 0) return DS_OK;
   const int es = elements(dtype), ps = elements(param_dtype);
   DS_REQUIRE(x && y, DS_EINVAL, "layer_norm: null pointer");

@@ -14,6 +14,7 @@ autograd (reverse mode; the counts are taken as given).
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -63,20 +64,29 @@ def _desc(logits, ids, kind, valid, offsets) -> tuple[_abi.DsBalance, tuple]:
     return d, (logits, ids, valid, offsets)
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(device: int, tokens: int, experts: int, sequences: int) -> int:
+    """Workspace of a call on `device`, the current one (sizes follow its SMs)."""
+    d = _abi.DsBalance(256, tokens, experts, _abi.DS_F32, experts, 1, _abi.DS_ROUTE_SOFTMAX, 256, None, 256, 0, sequences)
+    n = ctypes.c_size_t(0)
+    _abi.check(_abi.lib().ds_balance_loss_workspace_size(ctypes.byref(d), ctypes.byref(n)), "ds_balance_loss_workspace_size")
+    return n.value
+
+
 def _forward(logits, ids, kind, valid, offsets):
     """loss, counts, and the coefficients that the backward pass reads."""
     d, hold = _desc(logits, ids, kind, valid, offsets)
-    dev, lib, ref, n = logits.device, _abi.lib(), ctypes.byref(d), ctypes.c_size_t(0)
-    lead = () if offsets is None else (d.sequences,)
+    dev, sequences, experts = logits.device, d.sequences, d.experts
+    lead = () if offsets is None else (sequences,)
+    loss = torch.empty(lead, dtype=torch.float32, device=dev)
+    counts = torch.empty((*lead, experts), dtype=torch.int32, device=dev)
+    at = 4 * sequences * experts
     with on_device(dev):
-        loss = torch.empty(lead, dtype=torch.float32, device=dev)
-        counts = torch.empty((*lead, d.experts), dtype=torch.int32, device=dev)
-        _abi.check(lib.ds_balance_loss_workspace_size(ref, ctypes.byref(n)), "ds_balance_loss_workspace_size")
-        # the coefficients, then the workspace
-        at = 4 * d.sequences * d.experts
-        kept = torch.empty(at + n.value, dtype=torch.uint8, device=dev)
-        _abi.check(lib.ds_balance_loss(ref, loss.data_ptr(), counts.data_ptr(), kept.data_ptr(), kept.data_ptr() + at,
-                                       n.value, raw_stream(dev)), "ds_balance_loss")
+        n = _workspace_bytes(dev.index, d.tokens, experts, sequences)
+        kept = torch.empty(at + n, dtype=torch.uint8, device=dev)   # the coefficients, then the workspace
+        p = kept.data_ptr()
+        _abi.check(_abi.lib().ds_balance_loss(ctypes.byref(d), loss.data_ptr(), counts.data_ptr(), p, p + at, n,
+                                              raw_stream(dev)), "ds_balance_loss")
     return loss, counts, kept
 
 

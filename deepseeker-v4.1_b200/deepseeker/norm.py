@@ -9,7 +9,7 @@ derivatives are refused).
 from __future__ import annotations
 
 import ctypes
-import math
+import functools
 
 import torch
 
@@ -18,6 +18,7 @@ from ._dev import has_tangent, new_like, on_device, raw_stream, rows_of
 
 _DTYPES = {torch.float32: _abi.DS_F32, torch.bfloat16: _abi.DS_BF16, torch.float16: _abi.DS_F16}
 _MOST = 1 << 20   # features
+_MOST_EPS = 2.0 ** 127
 
 
 def _check(x, weight, bias, eps) -> torch.dtype:
@@ -37,8 +38,8 @@ def _check(x, weight, bias, eps) -> torch.dtype:
         if dtype is not None and t.dtype != dtype:
             raise ValueError("weight and bias must have one type")
         dtype = t.dtype
-    if not 0 <= eps < math.inf:
-        raise ValueError("eps must be a number >= 0")
+    if not 0 <= eps < _MOST_EPS:
+        raise ValueError("eps must be a number >= 0 that f32 holds")
     if has_tangent(x, weight, bias):
         raise ValueError("layer_norm has no forward-mode derivatives: an operand is a dual tensor")
     return dtype or torch.float32
@@ -46,6 +47,15 @@ def _check(x, weight, bias, eps) -> torch.dtype:
 
 def _dense(t):
     return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(device: int, rows: int, cols: int) -> int:
+    """Workspace of a backward pass with parameters on `device`, the current one (sizes follow its SMs)."""
+    n = ctypes.c_size_t(0)
+    _abi.check(_abi.lib().ds_layer_norm_backward_workspace_size(rows, cols, ctypes.byref(n)),
+               "ds_layer_norm_backward_workspace_size")
+    return n.value
 
 
 def _forward(x, weight, bias, eps, kind, keep: bool):
@@ -83,16 +93,15 @@ def _backward(ctx, dy):
     need_x, need_w, need_b = ctx.needs_input_grad[:3]
     dx = new_like(x) if need_x else None
     dw, db = (torch.empty(cols, dtype=ctx.kind, device=dev) if need else None for need in (need_w, need_b))
-    lib, n, ws = _abi.lib(), ctypes.c_size_t(0), None
+    n, ws = 0, None
     with on_device(dev):
         if need_w or need_b:
-            _abi.check(lib.ds_layer_norm_backward_workspace_size(rows, cols, ctypes.byref(n)),
-                       "ds_layer_norm_backward_workspace_size")
-            ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
-        _abi.check(lib.ds_layer_norm_backward(
+            n = _workspace_bytes(dev.index, rows, cols)
+            ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        _abi.check(_abi.lib().ds_layer_norm_backward(
             xr.data_ptr(), _DTYPES[x.dtype], rows, cols, ld, None if weight is None else weight.data_ptr(),
             _DTYPES[ctx.kind], stats.data_ptr(), dr.data_ptr(), ld_dy,
-            *[None if t is None else t.data_ptr() for t in (dx, dw, db, ws)], n.value, raw_stream(dev)),
+            *[None if t is None else t.data_ptr() for t in (dx, dw, db, ws)], n, raw_stream(dev)),
             "ds_layer_norm_backward")
     return dx, dw, db, None, None
 

@@ -290,7 +290,7 @@ def test_refusals(cuda):
                 (x, w, w.bfloat16()), (x[0, 0],), (x[:, :0],), ("x",)):
         with pytest.raises(ValueError):
             norm.layer_norm(*bad)
-    for eps in (-1e-5, float("nan"), float("inf")):
+    for eps in (-1e-5, float("nan"), float("inf"), 1e39):
         with pytest.raises(ValueError):
             norm.layer_norm(x, eps=eps)
     a = x.float().requires_grad_()

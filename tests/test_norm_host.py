@@ -27,7 +27,7 @@ def forward(lib, x=256, dtype=BF16, rows=4, cols=64, ld=64, w=256, b=256, kind=F
     (dict(dtype=U8), _abi.DS_EINVAL), (dict(kind=F16), _abi.DS_EINVAL), (dict(dtype=F32, kind=BF16), _abi.DS_EINVAL),
     (dict(rows=-1), _abi.DS_ERANGE), (dict(rows=1 << 31), _abi.DS_ERANGE), (dict(cols=0), _abi.DS_ERANGE),
     (dict(cols=(1 << 20) + 1, ld=1 << 21), _abi.DS_ERANGE), (dict(ld=63), _abi.DS_EINVAL),
-    (dict(eps=-1.0), _abi.DS_EINVAL), (dict(eps=float("nan")), _abi.DS_EINVAL), (dict(x=None), _abi.DS_EINVAL),
+    (dict(eps=-1.0), _abi.DS_EINVAL), (dict(eps=float("nan")), _abi.DS_EINVAL), (dict(eps=float("inf")), _abi.DS_EINVAL), (dict(x=None), _abi.DS_EINVAL),
     (dict(y=None), _abi.DS_EINVAL), (dict(x=257), _abi.DS_EALIGN), (dict(w=258), _abi.DS_EALIGN),
     (dict(stats=260), _abi.DS_EALIGN)])
 def test_forward_arguments(lib, kw, status):
