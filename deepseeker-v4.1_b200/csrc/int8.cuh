@@ -2,7 +2,8 @@
 // scaled result.
 //
 // A row of K values is K codes q in -127 .. 127 (stored ones may be -128) and
-// one f32 scale s = max |x| / 127, rounded to f32; q is the whole number
+// one f32 scale s = max |x| * (1 / 127), both factors and the product in f32 (a
+// unit of its last place from the quotient at most); q is the whole number
 // nearest to the exact quotient x / s, the even one of two.
 #pragma once
 
@@ -23,7 +24,7 @@ constexpr int kPitch = 16;
 // The scale of a row whose largest magnitude has these bits: NaN for a NaN or
 // an infinity, which stand above all numbers.
 __device__ __forceinline__ float scale_of(uint32_t top) {
-  return top >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(top) / 127.0f;
+  return top >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(top) * (1.0f / 127.0f);
 }
 
 // A row's scale as codes are formed with it.  Small ones (their inverse may

@@ -100,9 +100,9 @@ def _matrix(x):
 
 
 def quantize(x: torch.Tensor) -> Int8Tensor:
-    """x [..., cols] -> Int8Tensor.  A row's scale is its largest magnitude over
-    127 (rounded to f32), a code the whole number nearest to the exact quotient,
-    ties to the even one.  A NaN or an infinity makes its whole row NaN."""
+    """x [..., cols] -> Int8Tensor.  A row's scale is its largest magnitude times
+    1 / 127 (in f32), a code the whole number nearest to the exact quotient of
+    value and scale, ties to the even one.  A NaN or an infinity makes its whole row NaN."""
     _check_x(x)
     rows, ld = _matrix(x)
     n, cols = rows.shape

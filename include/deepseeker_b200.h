@@ -579,9 +579,9 @@ int ds_balance_loss_backward(const DsBalance* desc, const float* coef, const flo
 /* ---------------------------------------------------------------------------
  * 8-bit integer dense operators, one f32 scale per row of either operand (a
  * token's activations, an output channel's weights; the reference has no
- * product in this format).  Of a row of K < 2^17 values: s = max |x| / 127
- * rounded to f32, code q = the whole number nearest to the exact x / s, the
- * even one of two, clipped to +-127 (0 where s is 0).  A row with a NaN or an
+ * product in this format).  Of a row of K < 2^17 values: s = max |x| * (1 / 127)
+ * in f32 (factor and product rounded), code q = the whole number nearest to the
+ * exact x / s, the even one of two, clipped to +-127 (0 where s is 0).  A row with a NaN or an
  * infinity has scale NaN and codes 0, so products with it are NaN.  Codes of a
  * row lie together, rows `pitch` bytes apart, a multiple of 16 (what lies
  * between is neither read as a value nor written). */

@@ -26,7 +26,7 @@ def emulate(x):
     x = x.detach().cpu().double()
     top = x.abs().amax(1)
     bad = ~torch.isfinite(top)
-    scale = torch.where(bad, torch.full_like(top, math.nan), top / 127).float()
+    scale = torch.where(bad, torch.full_like(top, math.nan), top).float() * torch.tensor(1 / 127)   # f32 throughout
     s = torch.where(bad | (scale == 0), torch.ones_like(top), scale.double())
     q = torch.round((x / s[:, None]).nan_to_num(0, 0, 0)).clamp(-127, 127)
     return torch.where((bad | (scale == 0))[:, None], torch.zeros_like(q), q).to(torch.int8), scale
