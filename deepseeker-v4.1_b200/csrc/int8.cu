@@ -587,10 +587,9 @@ int launch_tiles(TileParams& p, const Input& x, const DsInt8& w, int slices, cud
   return DS_OK;
 }
 
-// Result [rows, cols] in boxes of 128 bytes x 32 rows; false where its rows do not start on 16 bytes.
+// Result [rows, cols], whose rows start on 16 bytes, in boxes of 128 bytes x 32 rows.
 bool map_result(CUtensorMap* m, void* y, int64_t rows, int64_t cols, int dtype) {
   const int es = elements(dtype);
-  if (!ds::aligned(y, 16) || cols * es % 16 != 0) return false;
   return grouped::encode_2d(m, dtype == DS_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, y,
                             rows, cols, cols * es, 128 / es, 32, CU_TENSOR_MAP_SWIZZLE_128B);
 }
@@ -674,9 +673,11 @@ int launch_rows_kernel(const Input& x, const DsInt8& w, void* y, int out_dtype, 
 // 17.5).  The tile kernel shares a contraction out among up to eight CTAs; it
 // wins where it is long and the result small (8192 x 512, 512 rows: 12 us, the
 // pair kernel 20).
-int64_t pair_ns(int64_t rows, int64_t cols, int ksteps, int nt) {
+// Results whose rows do not start on 16 bytes (boxed false) leave it row by row:
+// 20 ns a column and wave more.
+int64_t pair_ns(int64_t rows, int64_t cols, int ksteps, int nt, bool boxed) {
   const int64_t tiles = (rows + 255) / 256 * ((cols + nt - 1) / nt), pairs = ds::sm_count() / 2;
-  return 4800 + (tiles + pairs - 1) / pairs * ksteps * (nt == 256 ? 360 : nt == 128 ? 270 : 234);
+  return 4800 + (tiles + pairs - 1) / pairs * (ksteps * (nt == 256 ? 360 : nt == 128 ? 270 : 234) + (boxed ? 0 : 20 * nt));
 }
 
 // `slices`: of the contraction, enough to give every SM a CTA, at least two stages each.
@@ -694,13 +695,16 @@ int product(const Input& x, const DsInt8& w, void* y, int out_dtype, int* err, c
   const int ksteps = (int)((w.cols + 127) / 128), nt = x.rows <= 16 ? 16 : x.rows <= 32 ? 32 : x.rows <= 64 ? 64 : 128;
   int slices, wide = 256;
   const int64_t by_tiles = tile_ns(x.rows, w.rows, ksteps, nt, &slices);
-  int64_t by_pairs = pair_ns(x.rows, w.rows, ksteps, 256);
-  for (int n : {128, 64})
-    if (pair_ns(x.rows, w.rows, ksteps, n) < by_pairs) by_pairs = pair_ns(x.rows, w.rows, ksteps, n), wide = n;
+  const bool boxed = ds::aligned(y, 16) && w.rows * elements(out_dtype) % 16 == 0;
+  int64_t by_pairs = pair_ns(x.rows, w.rows, ksteps, 256, boxed);
+  for (int n : {128, 64}) {
+    const int64_t t = pair_ns(x.rows, w.rows, ksteps, n, boxed);
+    if (t < by_pairs) by_pairs = t, wide = n;
+  }
   if (x.rows > 64 && by_pairs < by_tiles) {
     PairParams p = {};
     p.sx = x.scales, p.sw = w.scales, p.y = y, p.ldy = w.rows, p.out_dtype = out_dtype;
-    p.boxed = map_result(&p.out, y, x.rows, w.rows, out_dtype);
+    p.boxed = boxed && map_result(&p.out, y, x.rows, w.rows, out_dtype);
     p.M = (int)x.rows, p.N = (int)w.rows, p.ksteps = ksteps, p.err = err;
     if (wide == 256) return launch_pairs<256>(p, x, w, s, chained);
     if (wide == 128) return launch_pairs<128>(p, x, w, s, chained);
