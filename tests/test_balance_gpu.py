@@ -285,6 +285,42 @@ def test_streams_and_graph(cuda):
         assert all(torch.equal(a, b) for a, b in zip((loss, counts, dl), want))
 
 
+def test_calls_at_once(cuda):
+    cases = []
+    for T, E, k, ends in ((3000, 128, 8, [0, 5, 2000, 3000]), (61, 16, 2, None), (900, 1024, 4, [0, 900])):
+        l, ids = data(T, E, k, F32, cuda, seed=T)
+        off = None if ends is None else torch.tensor(ends, device=cuda)
+        cases.append((l, ids, "sqrtsoftplus", torch.ones((), device=cuda) if off is None else torch.ones(len(ends) - 1, device=cuda),
+                      off))
+    want = [run(*c[:4], offsets=c[4]) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for c, s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                got.append(run(*c[:4], offsets=c[4]))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for g, w in zip(got, want) for x, y in zip(g, w))
+
+
+def test_counts_alone_and_loss_alone(cuda):
+    """Either result may be left unused; a loss in a larger sum gets its own gradient."""
+    l, ids = data(50, 20, 3, F32, cuda)
+    leaf = l.clone().requires_grad_()
+    loss, counts = balance.balance_loss(leaf, ids)
+    total = loss * 0.25 + leaf.sum() * 0.0
+    total.backward()
+    want = run(l, ids, "softmax", torch.tensor(0.25, device=cuda))
+    assert torch.equal(leaf.grad, want[2]) and torch.equal(counts, want[1])
+    leaf.grad = None
+    for _ in range(2):                                                  # the same graph twice
+        loss, _ = balance.balance_loss(leaf, ids)
+        loss.backward(retain_graph=True)
+        loss.backward()
+    assert bool((leaf.grad - 4 * run(l, ids, "softmax", torch.tensor(1.0, device=cuda))[2]).abs().max() <= 1e-7)
+
+
 def test_refusals(cuda):
     l, ids = data(8, 16, 2, F32, cuda)
     ok = dict(valid=torch.ones(8, dtype=torch.bool, device=cuda), offsets=torch.tensor([0, 8], device=cuda))

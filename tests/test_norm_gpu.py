@@ -276,12 +276,55 @@ def test_many_values(cuda):
     w = torch.ones(cols, dtype=F32, device=cuda, requires_grad=True)
     y = norm.layer_norm(x.requires_grad_(), w)
     at = torch.tensor([0, 4096, 1 << 19, rows - 2, rows - 1], device=cuda)
-    # (sums over many rows and over few are shared out among threads differently, so not bit by bit)
     xs = x.detach()[at]
     want = formula(xs, None, None, 1e-5, xs)
     check(y.detach()[at], want["y"], "y")
     dx, = torch.autograd.grad(y, x, x.detach())
     check(dx[at], want["dx"], "dx")
+
+
+@pytest.mark.parametrize("cols", [96, 1000, 4096, 8200, 40000])
+def test_a_row_does_not_depend_on_the_others(cols, cuda):
+    x, dy = data(1500, cols, BF16, cuda), data(1500, cols, BF16, cuda, seed=3)
+    w, b = data(1, cols, F32, cuda, seed=1)[0], data(1, cols, F32, cuda, seed=2)[0]
+    whole = train(x, w, b, dy)
+    for lo, hi in ((0, 1), (7, 9), (1490, 1500)):
+        part = train(x[lo:hi], w, b, dy[lo:hi])
+        assert torch.equal(part["y"], whole["y"][lo:hi]) and torch.equal(part["dx"], whole["dx"][lo:hi])
+
+
+def test_calls_at_once(cuda):
+    """Eager steps on three streams, then two captured steps replayed side by side."""
+    cases = [(data(r, c, BF16, cuda, seed=r), data(1, c, F32, cuda, seed=1)[0], data(1, c, F32, cuda, seed=2)[0],
+              data(r, c, BF16, cuda, seed=r + 1)) for r, c in ((900, 1024), (40, 711), (300, 4096))]
+    want = [train(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for c, s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                got.append(train(*c))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g[n], w[n]) for g, w in zip(got, want) for n in w)
+    from deepseeker import moe
+
+    held, graphs = [], []
+    for x, w, b, dy in cases[:2]:
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with moe.graph_capture(graph):
+            y = norm.layer_norm(*leaves)
+            held.append((leaves, y, torch.autograd.grad(y, leaves, dy)))
+        graphs.append(graph)
+    for _ in range(5):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, y, grads), w in zip(held, want):
+            assert all(torch.equal(t, w[n]) for t, n in zip((y, *grads), ("y", "dx", "dw", "db")))
 
 
 def test_refusals(cuda):
