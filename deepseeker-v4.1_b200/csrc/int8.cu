@@ -5,10 +5,13 @@
 //
 // sums exact in 32-bit integers (K < 2^17), on tcgen05 kind::i8.
 //
-// Tile kernel (few rows, or few tiles): one CTA computes 128 features (lanes
-// of the accumulator) x NT rows of x over a slice of the contraction; the
-// slices of a tile are the CTAs of a cluster and are added through distributed
-// shared memory.  More rows: int8_pair.cuh.
+// Up to four rows: CUDA cores (rows_kernel).  Tile kernel (few rows, or a long
+// contraction and few tiles): one CTA computes 128 features (lanes of the
+// accumulator) x NT rows of x over a slice of the contraction; the slices of a
+// tile are the CTAs of a cluster and are added through distributed shared
+// memory.  64 rows of 4096 to 4096: 8.0 us (16.8 MB of weights, 2.6 us of memory
+// time), bounded by its start, the stages' latency and the join.  More rows:
+// int8_pair.cuh.
 #include <algorithm>
 #include <cooperative_groups.h>
 
@@ -403,7 +406,9 @@ __device__ __forceinline__ uint4 codes_at(const uint8_t* at, int n) {
 // type of x, or int8_t where a launch before this one has quantised it (every
 // block that quantises does all of it: two rows took 12.8 us that way).
 // No cluster, no tensor memory: bounded by the stream of weights and the start
-// of a launch.  The grid is one wave of blocks, see features_of.
+// of a launch.  The grid is one wave of blocks where it
+// can be (by_features).  One row of 4096 to 4096: 8.4 us with its launch, 2.6 of
+// them the weights at memory speed.
 template <typename X, int T, int F>
 __global__ void __launch_bounds__(256) rows_kernel(const VecParams p) {
   __shared__ uint32_t tops[T][8];

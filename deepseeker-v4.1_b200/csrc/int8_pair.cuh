@@ -7,6 +7,10 @@
 // leader issues the MMAs, warps 2-9 empty one accumulator while the other
 // fills.  Lanes are rows: a thread multiplies its row's sums by the row's and
 // the columns' scales and rounds once.
+//
+// 16384 x 4096 to 4096: 154 to 163 us, 3.4 to 3.6 POP/s, bounded by the tensor
+// cores under the power cap (pipe 92 % active at 1.6 GHz; 64 bytes a cycle of L2
+// for each SM at 256 columns).  A tile's epilogue is 1.5 k cycles of its 16 k.
 #pragma once
 
 #include "int8.cuh"

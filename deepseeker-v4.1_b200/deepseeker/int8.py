@@ -53,7 +53,8 @@ class Int8Tensor:
     def codes(self) -> torch.Tensor:
         """i8, of ``shape``; its rows lie ``pitch`` bytes apart."""
         if self._codes is None:
-            rows = self._hold[:self.rows * self.pitch].view(torch.int8).view(self.rows, self.pitch)[:, :self.cols]
+            at = (self._pc - self._ps) // 4
+            rows = self._hold[at:].view(torch.int8).view(self.rows, self.pitch)[:, :self.cols]
             self._codes = rows.unflatten(0, self.shape[:-1]) if len(self.shape) > 1 else rows[0]
         return self._codes
 
@@ -61,8 +62,8 @@ class Int8Tensor:
     def scales(self) -> torch.Tensor:
         """f32, of ``shape`` without the last dimension."""
         if self._scales is None:
-            at = self._ps - self._hold.data_ptr()
-            self._scales = self._hold[at:at + 4 * self.rows].view(torch.float32).view(self.shape[:-1])
+            scales = self._hold[:self.rows]
+            self._scales = scales if len(self.shape) == 2 else scales.view(self.shape[:-1])
         return self._scales
 
     def _ref(self):
@@ -107,13 +108,13 @@ def quantize(x: torch.Tensor) -> Int8Tensor:
     rows, ld = _matrix(x)
     n, cols = rows.shape
     dev, pitch = x.device, _up(cols, 16)
-    at = _up(n * pitch, 256)
-    buf = torch.empty(at + 4 * n, dtype=torch.uint8, device=dev)   # codes, scales
+    at = _up(4 * n, 256)
+    buf = torch.empty((at + n * pitch) // 4, dtype=torch.float32, device=dev)   # scales, codes
     p = buf.data_ptr()
     with on_device(dev):
-        _abi.check(_abi.lib().ds_int8_quantize(rows.data_ptr(), _DTYPES[x.dtype], n, cols, ld, p, pitch, p + at,
+        _abi.check(_abi.lib().ds_int8_quantize(rows.data_ptr(), _DTYPES[x.dtype], n, cols, ld, p + at, pitch, p,
                                                raw_stream(dev)), "ds_int8_quantize")
-    return Int8Tensor(n, x.shape, pitch, dev, buf, p, p + at)
+    return Int8Tensor(n, x.shape, pitch, dev, buf, p + at, p)
 
 
 def from_codes(codes: torch.Tensor, scales: torch.Tensor) -> Int8Tensor:
