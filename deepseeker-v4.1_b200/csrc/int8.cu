@@ -134,7 +134,10 @@ __global__ void __launch_bounds__(1024) quantize_long_kernel(const T* __restrict
 }
 
 // Values of codes, VEC a thread: 8 (the result's rows on 16 bytes), or one.
-template <typename T, int VEC>
+// STREAM: results of many megabytes leave L2 first, so that the codes, which
+// their quantisation may just have left there, do not (16384 x 4096 to bf16 after
+// its quantisation: 34 -> 28.6 us).
+template <typename T, int VEC, bool STREAM>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ codes, int64_t pitch,
                                                          const float* __restrict__ scales, int64_t rows, int cols,
                                                          T* __restrict__ out) {
@@ -155,10 +158,10 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float half[4] = {v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
-          put<T, 4>(dst + 4 * h, half);
+          put<T, 4, STREAM>(dst + 4 * h, half);
         }
       } else {
-        put<T, 8>(dst, v);
+        put<T, 8, STREAM>(dst, v);
       }
     }
   }
@@ -777,8 +780,10 @@ extern "C" int ds_int8_dequantize(const int8_t* codes, int64_t pitch, const floa
   ds::rows::by_type(out_dtype, [&](auto t) {
     using T = decltype(t);
     T* dst = static_cast<T*>(out);
-    if (vec) dequantize_kernel<T, 8><<<grid, block, 0, s>>>(src, pitch, scales, rows, (int)cols, dst);
-    else dequantize_kernel<T, 1><<<grid, block, 0, s>>>(src, pitch, scales, rows, (int)cols, dst);
+    const bool stream = rows * cols * es >= (64 << 20);   // half of L2
+    if (vec && stream) dequantize_kernel<T, 8, true><<<grid, block, 0, s>>>(src, pitch, scales, rows, (int)cols, dst);
+    else if (vec) dequantize_kernel<T, 8, false><<<grid, block, 0, s>>>(src, pitch, scales, rows, (int)cols, dst);
+    else dequantize_kernel<T, 1, false><<<grid, block, 0, s>>>(src, pitch, scales, rows, (int)cols, dst);
   });
   DS_CHECK_LAUNCH("int8 dequantize_kernel");
   return DS_OK;

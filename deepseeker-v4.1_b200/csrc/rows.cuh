@@ -44,25 +44,32 @@ __device__ __forceinline__ T narrow(float v) {
   else return __float2bfloat16_rn(v);
 }
 
-template <typename T, int VEC>
+// STREAM: first to leave L2.
+template <typename T, int VEC, bool STREAM = false>
 __device__ __forceinline__ void put(T* p, const float (&v)[VEC]) {
   if constexpr (VEC == 1) {
     *p = narrow<T>(v[0]);
-  } else if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
   } else {
     uint32_t w[4];
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (std::is_same<T, __half>::value) {
-        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-      } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __half>::value) {
+          const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
       }
     }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    uint4* at = reinterpret_cast<uint4*>(p);
+    const uint4 q = make_uint4(w[0], w[1], w[2], w[3]);
+    if constexpr (STREAM) __stcs(at, q);
+    else *at = q;
   }
 }
 
