@@ -132,7 +132,7 @@ def from_codes(codes: torch.Tensor, scales: torch.Tensor) -> Int8Tensor:
     scales, pitch = scales.contiguous(), codes.stride(0)
     if (cols > 1 and codes.stride(1) != 1) or codes.data_ptr() % 16 or pitch % 16 or pitch < cols:
         pitch = _up(cols, 16)
-        held = torch.zeros((rows, pitch), dtype=torch.int8, device=codes.device)[:, :cols]
+        held = torch.empty((rows, pitch), dtype=torch.int8, device=codes.device)[:, :cols]
         codes = held.copy_(codes)
     return Int8Tensor(rows, torch.Size((rows, cols)), pitch, codes.device, (codes, scales), codes.data_ptr(),
                       scales.data_ptr(), (codes, scales))
