@@ -58,28 +58,56 @@ __device__ __forceinline__ uint32_t top_of(const Pack<T, VEC>& k) {
 }
 
 // A block takes rows blockIdx.x, + gridDim.x ..., blockDim.y at a time, V times
-// VEC values a thread; THREADS: of a row, which they fill, or 0.  The next row is
-// loaded while this one is coded.  16384 x 4096 bf16: 35 us, 5.8 TB/s; with 16
-// values a thread instead of 32 37 us, without the row ahead 65.
-template <typename T, int VEC, int V, int THREADS>
-__global__ void __maxnreg__(VEC > 1 && V * VEC <= 32 ? 80 : 128) quantize_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ld,
-                                                       uint8_t* __restrict__ codes, int64_t pitch,
-                                                       float* __restrict__ scales) {
+// VEC values a thread; THREADS: of a row, which they fill, or 0, or -1: rows of
+// any columns and strides, through lines.  The next row is loaded while this one
+// is coded.  16384 x 4096 bf16: 35 us, 5.8 TB/s; with 16 values a thread instead
+// of 32 37 us, without the row ahead 65.  Through lines 75 us (single values, in
+// registers or through lines, 93 to 112).
+template <typename T, int V, int THREADS>
+__global__ void __maxnreg__(V <= 2 * (int)sizeof(T) ? 80 : 128) quantize_kernel(const T* __restrict__ x, int64_t rows,
+                                                                                int cols, int64_t ld,
+                                                                                uint8_t* __restrict__ codes,
+                                                                                int64_t pitch,
+                                                                                float* __restrict__ scales) {
+  constexpr int VEC = 16 / sizeof(T);
+  constexpr bool kLines = THREADS < 0;
+  extern __shared__ uint4 smem[];
   __shared__ uint32_t red[kMostRows][2][32];
   launch_dependents();
   const int64_t step = (int64_t)gridDim.x * blockDim.y;
-  auto column = [&](int i) { return (int)(i * (THREADS ? THREADS : blockDim.x) + threadIdx.x) * VEC; };
-  auto inside = [&](int i) { return THREADS || column(i) < cols; };
+  auto column = [&](int i) { return (i * (THREADS > 0 ? THREADS : (int)blockDim.x) + (int)threadIdx.x) * VEC; };
+  auto inside = [&](int i) { return THREADS > 0 || column(i) < cols; };
+  Lines<T> lines;
+  lines.template place<kStages>(smem, x, cols);
   Pack<T, VEC> k[V];
-  auto fetch = [&](int64_t row) {
-    if (row >= rows) return;
+  auto fetch = [&](int stage, int64_t row) {
+    if constexpr (kLines) {
+      if (row < rows) lines.copy(stage, x + row * ld);
+      Slots::commit();
+    } else {
+      if (row >= rows) return;
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (inside(i)) k[i].load(x + row * ld + column(i));
+      for (int i = 0; i < V; ++i)
+        if (inside(i)) k[i].load(x + row * ld + column(i));
+    }
   };
-  int turn = 0;
+  int turn = 0, stage = 0;
   int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  for (fetch(row); row < rows; row += step, turn ^= 1) {
+#pragma unroll
+  for (int i = 0; i < (kLines ? kStages - 1 : 1); ++i) fetch(i, row + i * step);
+  for (; row < rows; row += step, turn ^= 1) {
+    if constexpr (kLines) {
+      Slots::wait<kStages - 2>();
+      line_barrier();   // the row is here, and the one before it read
+      fetch(stage ? stage - 1 : kStages - 1, row + (kStages - 1) * step);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (!inside(i)) continue;
+        k[i].raw = lines.vector(stage, x + row * ld, column(i));
+        if (column(i) + VEC > cols) k[i].cut(cols - column(i));
+      }
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
     float v[V][VEC];
     uint32_t top = 0;
 #pragma unroll
@@ -88,7 +116,7 @@ __global__ void __maxnreg__(VEC > 1 && V * VEC <= 32 ? 80 : 128) quantize_kernel
       top = max(top, top_of(k[i]));
       k[i].get(v[i]);
     }
-    fetch(row + step);   // on its way during the rest
+    if constexpr (!kLines) fetch(0, row + step);   // on its way during the rest
     const float s = scale_of(row_max(top, red[threadIdx.y][turn]));
     if (threadIdx.x == 0) scales[row] = s;
     const Coder coder(s);
@@ -98,15 +126,17 @@ __global__ void __maxnreg__(VEC > 1 && V * VEC <= 32 ? 80 : 128) quantize_kernel
       uint32_t q[VEC];
       coder.codes(v[i], q);
       uint8_t* at = codes + row * pitch + column(i);
-      if constexpr (VEC == 1) {
-        *at = (uint8_t)q[0];
-      } else {
-        uint32_t w[VEC / 4];
+      if (kLines && column(i) + VEC > cols) {
 #pragma unroll
-        for (int j = 0; j < VEC / 4; ++j) w[j] = pack_codes(q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]);
-        if constexpr (VEC == 8) *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
-        else *reinterpret_cast<uint32_t*>(at) = w[0];
+        for (int j = 0; j < VEC; ++j)
+          if (column(i) + j < cols) at[j] = (uint8_t)q[j];
+        continue;
       }
+      uint32_t w[VEC / 4];
+#pragma unroll
+      for (int j = 0; j < VEC / 4; ++j) w[j] = pack_codes(q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]);
+      if constexpr (VEC == 8) *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
+      else *reinterpret_cast<uint32_t*>(at) = w[0];
     }
   }
 }
@@ -126,43 +156,59 @@ __global__ void __launch_bounds__(1024) quantize_long_kernel(const T* __restrict
   if (threadIdx.x == 0) scales[row] = s;
   const Coder coder(s);
   for (int c = threadIdx.x; c < cols; c += blockDim.x) {
-    float v[1] = {(float)src[c]};
-    uint32_t q[1];
+    float v[2] = {(float)src[c], 0.0f};
+    uint32_t q[2];
     coder.codes(v, q);
     codes[row * pitch + c] = (uint8_t)q[0];
   }
 }
 
-// Values of codes, VEC a thread: 8 (the result's rows on 16 bytes), or one.
-// STREAM: results of many megabytes leave L2 first, so that the codes, which
-// their quantisation may just have left there, do not (16384 x 4096 to bf16 after
-// its quantisation: 34 -> 28.6 us).
-template <typename T, int VEC, bool STREAM>
+// Values of codes, VEC a thread: eight where the result's rows lie on 16 bytes,
+// otherwise (ANY) the 16 bytes of a granule of the result, whose codes are a
+// window of two.  STREAM: results of many megabytes leave L2 first, so that the
+// codes, which their quantisation may just have left there, do not (16384 x 4096
+// to bf16 after its quantisation: 34 -> 28.6 us).
+template <typename T, bool ANY, bool STREAM>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ codes, int64_t pitch,
                                                          const float* __restrict__ scales, int64_t rows, int cols,
                                                          T* __restrict__ out) {
+  constexpr int PER = 16 / sizeof(T), VEC = ANY ? PER : 8;
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= rows) return;
   const float s = scales[row];
-  for (int c = threadIdx.x * VEC; c < cols; c += blockDim.x * VEC) {
-    const uint8_t* at = codes + row * pitch + c;
-    T* dst = out + row * cols + c;
-    if constexpr (VEC == 1) {
-      *dst = narrow<T>((float)(int8_t)*at * s);
-    } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(at);
-      float v[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = (float)(int8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3))) * s;
-      if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float half[4] = {v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
-          put<T, 4, STREAM>(dst + 4 * h, half);
-        }
-      } else {
-        put<T, 8, STREAM>(dst, v);
+  const uint8_t* from = codes + row * pitch;
+  T* dst = out + row * cols;
+  // columns of the row in its first granule that are another's
+  const int skip = ANY ? (int)(reinterpret_cast<uintptr_t>(dst) & 15) / (int)sizeof(T) : 0;
+  for (int c = (int)threadIdx.x * VEC - skip; c < cols; c += blockDim.x * VEC) {
+    if (ANY && (c < 0 || c + VEC > cols)) {
+      for (int j = max(c, 0); j < min(c + VEC, cols); ++j) dst[j] = narrow<T>((float)(int8_t)from[j] * s);
+      continue;
+    }
+    // c + skip is a multiple of VEC
+    uint32_t w[VEC / 4];
+    if constexpr (VEC == 8) {
+      uint2 q = *reinterpret_cast<const uint2*>(from + c + skip);
+      if (ANY && skip) {
+        const uint2 before = *reinterpret_cast<const uint2*>(from + c + skip - 8);
+        const uint32_t a = skip < 4 ? before.y : before.x, b = skip < 4 ? q.x : before.y, e = skip < 4 ? q.y : q.x;
+        const int bits = 8 * (4 - (skip & 3));
+        q = make_uint2(__funnelshift_rc(a, b, bits), __funnelshift_rc(b, e, bits));
       }
+      w[0] = q.x, w[1] = q.y;
+    } else {
+      w[0] = *reinterpret_cast<const uint32_t*>(from + c + skip);
+      if (skip) w[0] = __funnelshift_r(*reinterpret_cast<const uint32_t*>(from + c + skip - 4), w[0], 8 * (4 - skip));
+    }
+    float v[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = (float)(int8_t)(w[j / 4] >> (8 * (j & 3))) * s;
+#pragma unroll
+    for (int h = 0; h < VEC / PER; ++h) {
+      float part[PER];
+#pragma unroll
+      for (int j = 0; j < PER; ++j) part[j] = v[h * PER + j];
+      put<T, PER, STREAM>(dst + c + h * PER, part);
     }
   }
 }
@@ -539,22 +585,25 @@ int launch_quantize(const void* x, int dtype, int64_t rows, int cols, int64_t ld
                     float* scales, cudaStream_t s) {
   const int es = elements(dtype);
   const bool vec = vectors(x, rows, cols, ld, es);
+  int st = DS_OK;
   by_type(dtype, [&](auto t) {
     using T = decltype(t);
     const T* src = static_cast<const T*>(x);
-    if (cols > (vec ? 64 * 1024 / es : 8 * 1024)) {
+    if (cols > 64 * 1024 / es || (!vec && kStages * Lines<T>::pitch_of(cols) > kMostSmem)) {
       quantize_long_kernel<T><<<(unsigned)rows, 1024, 0, s>>>(src, cols, ld, codes, pitch, scales);
       return;
     }
-    // 16 values a thread (eight single ones); many rows are shared out in 32, as
-    // the maximum over a row's threads takes much of the work otherwise
-    const bool many = vec && rows >= 4 * (int64_t)ds::sm_count();
-    const Shape sh = shape_of(cols, vec ? 16 / es : 1, many ? 32 : vec ? 16 : 8, 512, 256);
-    by_shape<T, 2 * sizeof(T), 8>(sh, cols, [&](auto w, auto v, auto threads) {
-      launch_rows<quantize_kernel<T, decltype(w)::value, decltype(v)::value, decltype(threads)::value>>(
-          sh, rows, s, src, rows, cols, ld, codes, pitch, scales);
+    // 16 values a thread; many rows are shared out in 32, as the maximum over a
+    // row's threads takes much of the work otherwise (but not f32 through lines:
+    // too few registers, 8192 x 4096 with its dequantisation 110 us instead of 88)
+    const bool many = rows >= 4 * (int64_t)ds::sm_count() && (vec || es == 2);
+    const Shape sh = shape_of(cols, 16 / es, many ? 32 : 16, 512, 256);
+    by_shape<T, 2 * sizeof(T), 8, true>(sh, cols, vec, [&](auto, auto v, auto threads) {
+      st = launch_rows<quantize_kernel<T, decltype(v)::value, decltype(threads)::value>>(
+          sh, rows, vec ? 0 : kStages * Lines<T>::pitch_of(cols), s, src, rows, cols, ld, codes, pitch, scales);
     });
   });
+  if (st != DS_OK) return st;
   DS_CHECK_LAUNCH("int8 quantize_kernel");
   return DS_OK;
 }
@@ -774,16 +823,17 @@ extern "C" int ds_int8_dequantize(const int8_t* codes, int64_t pitch, const floa
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const uint8_t* src = reinterpret_cast<const uint8_t*>(codes);
   const bool vec = ds::aligned(out, 16) && cols % 8 == 0;
-  const int n = (int)(vec ? cols / 8 : cols), threads = std::min(256, (n + 31) / 32 * 32);
+  const int n = (int)(vec ? cols / 8 : (cols * es + 14) / 16 + 1), threads = std::min(256, (n + 31) / 32 * 32);
   const dim3 block(threads, 256 / threads);
   const unsigned grid = (unsigned)((rows + block.y - 1) / block.y);
   ds::rows::by_type(out_dtype, [&](auto t) {
     using T = decltype(t);
     T* dst = static_cast<T*>(out);
     const bool stream = rows * cols * es >= (64 << 20);   // half of L2
-    if (vec && stream) dequantize_kernel<T, 8, true><<<grid, block, 0, s>>>(src, pitch, scales, rows, (int)cols, dst);
-    else if (vec) dequantize_kernel<T, 8, false><<<grid, block, 0, s>>>(src, pitch, scales, rows, (int)cols, dst);
-    else dequantize_kernel<T, 1, false><<<grid, block, 0, s>>>(src, pitch, scales, rows, (int)cols, dst);
+    if (vec && stream) dequantize_kernel<T, false, true><<<grid, block, 0, s>>>(src, pitch, scales, rows, (int)cols, dst);
+    else if (vec) dequantize_kernel<T, false, false><<<grid, block, 0, s>>>(src, pitch, scales, rows, (int)cols, dst);
+    else if (stream) dequantize_kernel<T, true, true><<<grid, block, 0, s>>>(src, pitch, scales, rows, (int)cols, dst);
+    else dequantize_kernel<T, true, false><<<grid, block, 0, s>>>(src, pitch, scales, rows, (int)cols, dst);
   });
   DS_CHECK_LAUNCH("int8 dequantize_kernel");
   return DS_OK;

@@ -40,6 +40,14 @@ __device__ __forceinline__ void params(const P* p, float (&v)[VEC]) {
   }
 }
 
+// f(vectors of a thread that are whole), see by_end.
+template <int VEC, int V, int THREADS, typename F>
+__device__ __forceinline__ void by_rows(int cols, F f) {
+  if constexpr (THREADS > 0) f(std::integral_constant<int, V>());
+  else if constexpr (VEC > 1) f(std::integral_constant<int, 0>());
+  else by_end<V>(cols, f);
+}
+
 struct Forward {
   const void *x, *w, *b;
   void* y;
@@ -66,71 +74,100 @@ __device__ __forceinline__ float inverse_root(float a) {
 // summed.  Measured beside it: no row ahead 72 us, eight values a thread 60, 32
 // 54, 64 with the parameters in shared memory 60, rows through a ring in shared
 // memory 64.
+//
+// Rows that do not lie on 16 bytes: single values through lines, 16384 x 4095
+// bf16 90 us, 8192 x 4095 f32 51.  Measured beside it: single values in registers
+// 119 and 65; vectors that are shifted out of the lines and into others 113 to
+// 145 (bf16).
 template <typename T, typename P, int VEC, int V, int THREADS>
-__global__ void __maxnreg__(VEC > 1 && V * VEC <= 16 ? 80 : 128) forward_kernel(const Forward p) {
+__global__ void __maxnreg__(VEC == 1 && V <= 8 ? 64 : V * VEC <= 16 ? 80 : 128) forward_kernel(const Forward p) {
   __shared__ float red[kMostRows][2][32];
   const P* w = static_cast<const P*>(p.w);
   const P* b = static_cast<const P*>(p.b);
   const float inv = 1.0f / p.cols;
   const int64_t step = (int64_t)gridDim.x * blockDim.y;
-  auto column = [&](int i) { return (int)(i * (THREADS ? THREADS : blockDim.x) + threadIdx.x) * VEC; };
-  auto inside = [&](int i) { return THREADS || column(i) < p.cols; };
-  constexpr bool kKeep = V * VEC <= 16;
-  Values<VEC> kw[kKeep ? V : 1], kb[kKeep ? V : 1];
-  auto fetch_params = [&](int i, int to) {
-    float f[VEC];
-    kw[to] = Values<VEC>(1.0f), kb[to] = Values<VEC>(0.0f);
-    if (w) params<P, VEC>(w + column(i), f), kw[to] = Values<VEC>(f);
-    if (b) params<P, VEC>(b + column(i), f), kb[to] = Values<VEC>(f);
-  };
-  if constexpr (kKeep) {
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (inside(i)) fetch_params(i, i);
-  }
-  Pack<T, VEC> k[V];
-  auto fetch = [&](int64_t row) {
-    if (row >= p.rows) return;
-    const T* x = static_cast<const T*>(p.x) + row * p.ld;
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (inside(i)) k[i].load(x + column(i));
-  };
-  int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  for (fetch(row); row < p.rows; row += step) {
-    Values<VEC> v[V], s(0.0f);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      if (!inside(i)) continue;
+  auto column = [](int i) { return column_of<VEC, V, THREADS>(i); };
+  by_rows<VEC, V, THREADS>(p.cols, [&](auto whole) {
+    constexpr int kWhole = decltype(whole)::value;
+    auto inside = [&](int i) { return i < kWhole || ((VEC > 1 || i < kWhole + 4) && column(i) < p.cols); };
+    constexpr bool kKeep = V * VEC <= 16;
+    Values<VEC> kw[kKeep ? V : 1], kb[kKeep ? V : 1];
+    auto fetch_params = [&](int i, int to) {
       float f[VEC];
-      k[i].get(f);
-      v[i] = Values<VEC>(f);
-      s = s + v[i];
-    }
-    fetch(row + step);   // on its way during the rest
-    const float mean = row_sum(total(s), red[threadIdx.y][0]) * inv;
-    const Values<VEC> less(-mean);
-    s = Values<VEC>(0.0f);
+      kw[to] = Values<VEC>(1.0f), kb[to] = Values<VEC>(0.0f);
+      if (w) params<P, VEC>(w + column(i), f), kw[to] = Values<VEC>(f);
+      if (b) params<P, VEC>(b + column(i), f), kb[to] = Values<VEC>(f);
+    };
+    if constexpr (kKeep) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      if (!inside(i)) continue;
-      v[i] = v[i] + less;
-      s = fma(v[i], v[i], s);
+      for (int i = 0; i < V; ++i)
+        if (inside(i)) fetch_params(i, i);
     }
-    const float r = inverse_root(row_sum(total(s), red[threadIdx.y][1]) * inv + p.eps);
-    if (p.stats && threadIdx.x == 0) p.stats[row] = make_float2(mean, r);
-    T* y = static_cast<T*>(p.y) + row * p.cols;
-    const Values<VEC> rs(r);
+    constexpr bool kLines = VEC == 1;
+    extern __shared__ uint4 smem[];
+    Lines<T> lines;
+    lines.template place<kStages>(smem, p.x, p.cols);
+    [[maybe_unused]] Pack<T, VEC> k[kLines ? 1 : V];
+    auto fetch = [&](int stage, int64_t row) {
+      const T* x = static_cast<const T*>(p.x) + row * p.ld;
+      if constexpr (kLines) {
+        if (row < p.rows) lines.copy(stage, x);
+        Slots::commit();
+      } else {
+        if (row >= p.rows) return;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      if (!inside(i)) continue;
-      const int at = kKeep ? i : 0;
-      float f[VEC];
-      if constexpr (!kKeep) fetch_params(i, 0);
-      fma(v[i] * rs, kw[at], kb[at]).get(f);
-      put<T, VEC>(y + column(i), f);
+        for (int i = 0; i < V; ++i)
+          if (inside(i)) k[i].load(x + column(i));
+      }
+    };
+    int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    [[maybe_unused]] int stage = 0;
+#pragma unroll
+    for (int i = 0; i < (kLines ? kStages - 1 : 1); ++i) fetch(i, row + i * step);
+    for (; row < p.rows; row += step) {
+      Values<VEC> v[V], s(0.0f);
+      [[maybe_unused]] const T* here = nullptr;
+      if constexpr (kLines) {
+        Slots::wait<kStages - 2>();
+        line_barrier();   // all of the row is here, and the row before it has been read
+        fetch(stage ? stage - 1 : kStages - 1, row + (kStages - 1) * step);
+        here = lines.at(stage, static_cast<const T*>(p.x) + row * p.ld);
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (!inside(i)) continue;
+        float f[VEC];
+        if constexpr (kLines) f[0] = (float)here[column(i)];
+        else k[i].get(f);
+        v[i] = Values<VEC>(f);
+        s = s + v[i];
+      }
+      if constexpr (!kLines) fetch(0, row + step);   // on its way during the rest
+      const float mean = row_sum(total(s), red[threadIdx.y][0]) * inv;
+      const Values<VEC> less(-mean);
+      s = Values<VEC>(0.0f);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (!inside(i)) continue;
+        v[i] = v[i] + less;
+        s = fma(v[i], v[i], s);
+      }
+      const float r = inverse_root(row_sum(total(s), red[threadIdx.y][1]) * inv + p.eps);
+      if (p.stats && threadIdx.x == 0) p.stats[row] = make_float2(mean, r);
+      T* y = static_cast<T*>(p.y) + row * p.cols;
+      const Values<VEC> rs(r);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (!inside(i)) continue;
+        const int at = kKeep ? i : 0;
+        float f[VEC];
+        if constexpr (!kKeep) fetch_params(i, 0);
+        fma(v[i] * rs, kw[at], kb[at]).get(f);
+        put<T, VEC>(y + column(i), f);
+      }
     }
-  }
+  });
 }
 
 // Rows that no block's registers hold: read three times, one value a thread.
@@ -189,7 +226,7 @@ __device__ __forceinline__ void row_sums(float (&a)[N], float* red) {
   int at = kBit;
   if (warps > 1) {
     if (lane % kBit == 0) red[(threadIdx.x >> 5) * N + lane / kBit] = v;
-    __syncthreads();
+    asm volatile("bar.sync 1;" ::: "memory");   // warps may come from different calls of by_end
     v = 0.0f;   // lane n + N m: value n of warps m, m + 32 / N ...
     for (int i = lane; i < warps * N; i += 32) v += red[i];
 #pragma unroll
@@ -200,14 +237,15 @@ __device__ __forceinline__ void row_sums(float (&a)[N], float* red) {
   for (int n = 0; n < N; ++n) a[n] = __shfl_sync(0xffffffffu, v, n * at);
 }
 
-// How the backward kernel takes its rows: kRows at a time, in vectors through
-// slots, two turns ahead, single values through registers.
+// How the backward kernel takes its rows, two turns ahead: kRows at a time, in
+// vectors through slots, single values through lines.
 template <int VEC, int V>
 struct Turn {
-  static constexpr bool kRing = VEC > 1;
-  static constexpr int kRows = kRing && V <= 2 ? 2 : 1;
+  static constexpr bool kLines = VEC == 1;
+  static constexpr int kRows = !kLines && V <= 2 ? 2 : 1;
   static constexpr int kSlots = kRows * 2 * V;                          // x and dy, of a stage
-  static constexpr int kBytes = kRing ? kStages * kSlots * 16 : 0;      // a thread
+  static constexpr int kBytes = kLines ? 0 : kStages * kSlots * 16;     // a thread
+  static constexpr int kThreads = kLines && V <= 8 ? 1024 : 512;        // that an SM's registers hold
 };
 
 // A block takes rows in turns (a warp each, or the block one of each turn); its
@@ -216,8 +254,11 @@ struct Turn {
 // like the forward pass.  Measured beside it: one row a turn with the next one in
 // registers 47 us, one row a turn through a ring 59, x and dy kept in registers
 // from the first use to the second 40 (and 52 once they spilled).
+//
+// 8192 x 4095, forward and backward: 131 us bf16 (184 with single values in
+// registers), 4096 x 8191 144 (303).
 template <typename T, typename P, int VEC, int V, int THREADS>
-__global__ void __launch_bounds__(512) backward_kernel(const Backward p) {
+__global__ void __launch_bounds__(512, Turn<VEC, V>::kThreads / 512) backward_kernel(const Backward p) {
   using U = Turn<VEC, V>;
   constexpr int R = U::kRows, S = kStages;
   extern __shared__ uint4 ring[];
@@ -225,162 +266,163 @@ __global__ void __launch_bounds__(512) backward_kernel(const Backward p) {
   const P* w = static_cast<const P*>(p.w);
   const float inv = 1.0f / p.cols;
   const Slots slots(ring);
-  auto column = [&](int i) { return (int)(i * (THREADS ? THREADS : blockDim.x) + threadIdx.x) * VEC; };
-  auto inside = [&](int i) { return THREADS || column(i) < p.cols; };
-  Values<VEC> kw[V], aw[V], ab[V];
+  Lines<T> line_x, line_dy;
+  line_x.template place<S>(ring, p.x, p.cols, 0, 2), line_dy.template place<S>(ring, p.dy, p.cols, 1, 2);
+  auto column = [](int i) { return column_of<VEC, V, THREADS>(i); };
+  by_rows<VEC, V, THREADS>(p.cols, [&](auto whole) {
+    constexpr int kWhole = decltype(whole)::value;
+    auto inside = [&](int i) { return i < kWhole || ((VEC > 1 || i < kWhole + 4) && column(i) < p.cols); };
+    Values<VEC> kw[V], aw[V], ab[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    float v[VEC];
+    for (int i = 0; i < V; ++i) {
+      float v[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = 1.0f;
-    if (w && inside(i)) params<P, VEC>(w + column(i), v);
-    kw[i] = Values<VEC>(v);
-    aw[i] = ab[i] = Values<VEC>(0.0f);
-  }
-  const int64_t step = (int64_t)gridDim.x * blockDim.y * R, first = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * R;
-  Pack<T, VEC> held[U::kRing ? 1 : 2 * V];   // single values of the next row
-  float2 next[R];                            // its mean and r
-  auto fetch = [&](int stage, int64_t row) {
+      for (int j = 0; j < VEC; ++j) v[j] = 1.0f;
+      if (w && inside(i)) params<P, VEC>(w + column(i), v);
+      kw[i] = Values<VEC>(v);
+      aw[i] = ab[i] = Values<VEC>(0.0f);
+    }
+    const int64_t step = (int64_t)gridDim.x * blockDim.y * R;
+    const int64_t first = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * R;
+    float2 next[R];   // mean and r of the next rows
+    auto fetch = [&](int stage, int64_t row) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (row + r >= p.rows) continue;
-      const T* x = static_cast<const T*>(p.x) + (row + r) * p.ld;
-      const T* dy = static_cast<const T*>(p.dy) + (row + r) * p.ld_dy;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if (!inside(i)) continue;
-        const int c = column(i);
-        if constexpr (U::kRing) {
-          slots.copy(stage * U::kSlots + r * 2 * V + i, x + c);
-          slots.copy(stage * U::kSlots + r * 2 * V + V + i, dy + c);
+      for (int r = 0; r < R; ++r) {
+        if (row + r >= p.rows) continue;
+        const T* x = static_cast<const T*>(p.x) + (row + r) * p.ld;
+        const T* dy = static_cast<const T*>(p.dy) + (row + r) * p.ld_dy;
+        if constexpr (U::kLines) {
+          line_x.copy(stage, x), line_dy.copy(stage, dy);
         } else {
-          held[i].load(x + c), held[V + i].load(dy + c);
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            if (!inside(i)) continue;
+            const int c = column(i);
+            slots.copy(stage * U::kSlots + r * 2 * V + i, x + c);
+            slots.copy(stage * U::kSlots + r * 2 * V + V + i, dy + c);
+          }
         }
       }
-    }
-    if constexpr (U::kRing) slots.commit();
-  };
-  auto stats = [&](int64_t row) {
+      slots.commit();
+    };
+    auto stats = [&](int64_t row) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) next[r] = row + r < p.rows ? p.stats[row + r] : make_float2(0.0f, 0.0f);
-  };
+      for (int r = 0; r < R; ++r) next[r] = row + r < p.rows ? p.stats[row + r] : make_float2(0.0f, 0.0f);
+    };
 #pragma unroll
-  for (int i = 0; i < (U::kRing ? S - 1 : 1); ++i) fetch(i, first + i * step);
-  stats(first);
-  int stage = 0, turn = 0;
-  for (int64_t row = first; row < p.rows; row += step, turn ^= 1) {   // blockDim.y > 1 only with a warp a row
-    float2 st[R];
+    for (int i = 0; i < S - 1; ++i) fetch(i, first + i * step);
+    stats(first);
+    int stage = 0, turn = 0;
+    for (int64_t row = first; row < p.rows; row += step, turn ^= 1) {   // blockDim.y > 1 only with a warp a row
+      float2 st[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) st[r] = next[r];
-    Pack<T, VEC> due[U::kRing ? 1 : 2 * V];   // single values of this row
-    const int here = stage;
-    if constexpr (U::kRing) {
+      for (int r = 0; r < R; ++r) st[r] = next[r];
+      const int here = stage;
       slots.wait<S - 2>();
+      if constexpr (U::kLines) line_barrier();   // all of the row is here, and the row before it has been used
       // into the stage whose rows the turn before this has used
       fetch(here ? here - 1 : S - 1, row + (S - 1) * step);
       stage = here + 1 == S ? 0 : here + 1;
-    } else {
+      stats(row + step);
+      const T* here_x = line_x.at(here, static_cast<const T*>(p.x) + row * p.ld);
+      const T* here_dy = line_dy.at(here, static_cast<const T*>(p.dy) + row * p.ld_dy);
+      // dy and xh, from shared memory both times that they are asked for (registers
+      // that held them would be missing elsewhere)
+      auto at = [&](int r, int i, Values<VEC>& d, Values<VEC>& xh) {
+        Pack<T, VEC> kx, kd;
+        if constexpr (U::kLines) {
+          kx.raw = here_x[column(i)], kd.raw = here_dy[column(i)];
+        } else {
+          kx.raw = slots.read(here * U::kSlots + r * 2 * V + i);
+          kd.raw = slots.read(here * U::kSlots + r * 2 * V + V + i);
+        }
+        float v[VEC];
+        kd.get(v);
+        d = Values<VEC>(v);
+        kx.get(v);
+        xh = fma(Values<VEC>(v), Values<VEC>(st[r].y), Values<VEC>(-st[r].x * st[r].y));
+      };
+      float sums[2 * R];
 #pragma unroll
-      for (int i = 0; i < 2 * V; ++i) due[i] = held[i];
-      fetch(0, row + step);
-    }
-    stats(row + step);
-    // dy and xh, from the slots both times that they are asked for (registers
-    // that held them would be missing elsewhere)
-    auto at = [&](int r, int i, Values<VEC>& d, Values<VEC>& xh) {
-      Pack<T, VEC> kx, kd;
-      if constexpr (U::kRing) {
-        kx.raw = slots.read(here * U::kSlots + r * 2 * V + i);
-        kd.raw = slots.read(here * U::kSlots + r * 2 * V + V + i);
-      } else {
-        kx = due[i], kd = due[V + i];
+      for (int r = 0; r < R; ++r) {
+        Values<VEC> s1(0.0f), s2(0.0f);
+        if (r == 0 || row + r < p.rows) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            if (!inside(i)) continue;
+            Values<VEC> d, xh;
+            at(r, i, d, xh);
+            aw[i] = fma(d, xh, aw[i]);
+            ab[i] = ab[i] + d;
+            d = d * kw[i];
+            s1 = s1 + d;
+            s2 = fma(d, xh, s2);
+          }
+        }
+        sums[2 * r] = total(s1), sums[2 * r + 1] = total(s2);
       }
-      float v[VEC];
-      kd.get(v);
-      d = Values<VEC>(v);
-      kx.get(v);
-      xh = fma(Values<VEC>(v), Values<VEC>(st[r].y), Values<VEC>(-st[r].x * st[r].y));
-    };
-    float sums[2 * R];
+      if (!p.dx) continue;
+      row_sums(sums, red[turn]);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      Values<VEC> s1(0.0f), s2(0.0f);
-      if (r == 0 || row + r < p.rows) {
+      for (int r = 0; r < R; ++r) {
+        if (r && row + r >= p.rows) continue;
+        const Values<VEC> m1(-sums[2 * r] * inv), m2(-sums[2 * r + 1] * inv), rs(st[r].y);
+        T* dx = static_cast<T*>(p.dx) + (row + r) * p.cols;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           if (!inside(i)) continue;
           Values<VEC> d, xh;
           at(r, i, d, xh);
-          aw[i] = fma(d, xh, aw[i]);
-          ab[i] = ab[i] + d;
-          d = d * kw[i];
-          s1 = s1 + d;
-          s2 = fma(d, xh, s2);
+          float v[VEC];
+          (fma(d, kw[i], fma(xh, m2, m1)) * rs).get(v);
+          put<T, VEC>(dx + column(i), v);
         }
       }
-      sums[2 * r] = total(s1), sums[2 * r + 1] = total(s2);
     }
-    if (!p.dx) continue;
-    row_sums(sums, red[turn]);
+    launch_dependents();
+    if (!p.part) return;
+    float* part = p.part + (int64_t)blockIdx.x * 2 * p.cols;
+    if (blockDim.y > 1) {
+      // the warps add their sums one after the other, where the ring was
+      float* sums = reinterpret_cast<float*>(ring);   // [2][cols]
+      __syncthreads();
+      for (int y = 0; y < blockDim.y; ++y) {
+        if (threadIdx.y == y) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (r && row + r >= p.rows) continue;
-      const Values<VEC> m1(-sums[2 * r] * inv), m2(-sums[2 * r + 1] * inv), rs(st[r].y);
-      T* dx = static_cast<T*>(p.dx) + (row + r) * p.cols;
+          for (int i = 0; i < V; ++i) {
+            if (!inside(i)) continue;
+            const int c = column(i);
+            float vw[VEC], vb[VEC];
+            aw[i].get(vw), ab[i].get(vb);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if (!inside(i)) continue;
-        Values<VEC> d, xh;
-        at(r, i, d, xh);
-        float v[VEC];
-        (fma(d, kw[i], fma(xh, m2, m1)) * rs).get(v);
-        put<T, VEC>(dx + column(i), v);
-      }
-    }
-  }
-  launch_dependents();
-  if (!p.part) return;
-  float* part = p.part + (int64_t)blockIdx.x * 2 * p.cols;
-  if (blockDim.y > 1) {
-    // the warps add their sums one after the other, where the ring was
-    float* sums = reinterpret_cast<float*>(ring);   // [2][cols]
-    __syncthreads();
-    for (int y = 0; y < blockDim.y; ++y) {
-      if (threadIdx.y == y) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          if (!inside(i)) continue;
-          const int c = column(i);
-          float vw[VEC], vb[VEC];
-          aw[i].get(vw), ab[i].get(vb);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            sums[c + j] = y ? sums[c + j] + vw[j] : vw[j];
-            sums[p.cols + c + j] = y ? sums[p.cols + c + j] + vb[j] : vb[j];
+            for (int j = 0; j < VEC; ++j) {
+              sums[c + j] = y ? sums[c + j] + vw[j] : vw[j];
+              sums[p.cols + c + j] = y ? sums[p.cols + c + j] + vb[j] : vb[j];
+            }
           }
         }
+        __syncthreads();
       }
-      __syncthreads();
+      for (int c = threadIdx.y * blockDim.x + threadIdx.x; c < 2 * p.cols; c += blockDim.x * blockDim.y) part[c] = sums[c];
+      return;
     }
-    for (int c = threadIdx.y * blockDim.x + threadIdx.x; c < 2 * p.cols; c += blockDim.x * blockDim.y) part[c] = sums[c];
-    return;
-  }
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if (!inside(i)) continue;
-    const int c = column(i);
-    float vw[VEC], vb[VEC];
-    aw[i].get(vw), ab[i].get(vb);
-    if constexpr (VEC == 1) {
-      part[c] = vw[0], part[p.cols + c] = vb[0];
-    } else {
+    for (int i = 0; i < V; ++i) {
+      if (!inside(i)) continue;
+      const int c = column(i);
+      float vw[VEC], vb[VEC];
+      aw[i].get(vw), ab[i].get(vb);
+      if constexpr (VEC == 1) {
+        part[c] = vw[0], part[p.cols + c] = vb[0];
+      } else {
 #pragma unroll
-      for (int j = 0; j < VEC; j += 4) {   // cols is a multiple of VEC, so both halves lie on 16 bytes
-        *reinterpret_cast<float4*>(part + c + j) = make_float4(vw[j], vw[j + 1], vw[j + 2], vw[j + 3]);
-        *reinterpret_cast<float4*>(part + p.cols + c + j) = make_float4(vb[j], vb[j + 1], vb[j + 2], vb[j + 3]);
+        for (int j = 0; j < VEC; j += 4) {   // cols is a multiple of VEC, so both halves lie on 16 bytes
+          *reinterpret_cast<float4*>(part + c + j) = make_float4(vw[j], vw[j + 1], vw[j + 2], vw[j + 3]);
+          *reinterpret_cast<float4*>(part + p.cols + c + j) = make_float4(vb[j], vb[j + 1], vb[j + 2], vb[j + 3]);
+        }
       }
     }
-  }
+  });
 }
 
 // Rows that no block's registers hold: dx, x and dy read twice.
@@ -456,10 +498,14 @@ __global__ void __launch_bounds__(512) join_kernel(const float* __restrict__ par
 // the forward pass takes eight of them, 64 KB).
 constexpr int kMost = 16 * 512;
 
-Shape forward_shape(int cols, int vec) { return shape_of(cols, vec, vec > 1 ? 16 : 8, 512, 128); }
+Shape forward_shape(int cols, int vec) { return shape_of(cols, vec, 16, 512, 128); }
 
+// Single values: a thread takes eight of rows that are two warps' otherwise, so
+// that more of them wait at a time (training steps, f16: 333 x 711 12.7 us, with 16
+// values 16; 32800 x 1023 156 and 183); longer rows fill an SM with 16, shorter
+// ones are a warp's (127583 x 263: 153 us, with eight 387).
 Shape backward_shape(int cols, int vec) {
-  Shape s = shape_of(cols, vec, vec > 1 ? 16 : 8, 512, 256);
+  Shape s = shape_of(cols, vec, vec == 1 && cols > 512 && cols <= 1024 ? 8 : 16, 512, 256);
   if (s.threads > 32) s.rows = 1;
   return s;
 }
@@ -476,8 +522,8 @@ void by_types(int dtype, int param_dtype, F f) {
 // Blocks of the backward pass, each with its sums.
 int backward_blocks(int64_t rows, const Shape& s) {
   const int turn = s.rows * (s.vec > 1 && s.v <= 2 ? 2 : 1);   // Turn::kRows
-  // 128 registers a thread fill an SM with 512
-  const int64_t most = (int64_t)ds::sm_count() * std::max(1, 512 / (s.threads * s.rows));
+  const int threads = s.vec == 1 && s.v <= 8 ? 1024 : 512;             // Turn::kThreads
+  const int64_t most = (int64_t)ds::sm_count() * std::max(1, threads / (s.threads * s.rows));
   return (int)std::min<int64_t>(most, (rows + turn - 1) / turn);
 }
 
@@ -534,10 +580,12 @@ extern "C" int ds_layer_norm(const void* x, int dtype, int64_t rows, int64_t col
       return;
     }
     const Shape sh = forward_shape((int)cols, vec ? 16 / es : 1);
-    by_shape<T, sizeof(T), 8>(sh, (int)cols, [&](auto w, auto v, auto threads) {
-      launch_rows<forward_kernel<T, P, decltype(w)::value, decltype(v)::value, decltype(threads)::value>>(sh, rows, s, p);
+    by_shape<T, sizeof(T), 8, false>(sh, (int)cols, vec, [&](auto w, auto v, auto threads) {
+      st = launch_rows<forward_kernel<T, P, decltype(w)::value, decltype(v)::value, decltype(threads)::value>>(
+          sh, rows, vec ? 0 : kStages * Lines<T>::pitch_of((int)cols), s, p);
     });
   });
+  if (st != DS_OK) return st;
   DS_CHECK_LAUNCH("layer_norm forward_kernel");
   return DS_OK;
 }
@@ -584,14 +632,15 @@ extern "C" int ds_layer_norm_backward(const void* x, int dtype, int64_t rows, in
       const Shape sh = backward_shape((int)cols, vec ? 16 / es : 1);
       const dim3 block(sh.threads, sh.rows);
       blocks = backward_blocks(rows, sh);
-      by_shape<T, sizeof(T), sizeof(T)>(sh, (int)cols, [&](auto w, auto v, auto threads) {
+      by_shape<T, sizeof(T), sizeof(T), false>(sh, (int)cols, vec, [&](auto w, auto v, auto threads) {
         constexpr int W = decltype(w)::value, V = decltype(v)::value;
         static SmemOnce once;
         const auto kernel = &backward_kernel<T, P, W, V, decltype(threads)::value>;
-        int smem = Turn<W, V>::kBytes * sh.threads * sh.rows;
+        const bool lines = Turn<W, V>::kLines;
+        const int line = 2 * kStages * Lines<T>::pitch_of((int)cols);
+        int smem = lines ? line * sh.rows : Turn<W, V>::kBytes * sh.threads * sh.rows;
         if (sh.rows > 1) smem = std::max(smem, (int)(2 * cols * sizeof(float)));
-        if (smem > 40 * 1024 &&
-            (st = ds::allow_smem(&once, reinterpret_cast<const void*>(kernel), Turn<W, V>::kBytes * 512)) != DS_OK)
+        if (smem > 40 * 1024 && (st = ds::allow_smem(&once, reinterpret_cast<const void*>(kernel), kMostSmem)) != DS_OK)
           return;
         kernel<<<blocks, block, smem, s>>>(p);
       });

@@ -18,6 +18,17 @@ struct Pack {
   Raw raw;
   __device__ __forceinline__ void load(const T* p) { raw = __ldcs(reinterpret_cast<const Raw*>(p)); }
   __device__ __forceinline__ void load_kept(const T* p) { raw = *reinterpret_cast<const Raw*>(p); }
+  // Values from the n-th on become 0.
+  __device__ __forceinline__ void cut(int n) {
+    uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    constexpr int kPer = 4 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (n <= i * kPer) w[i] = 0;
+      else if (kPer == 2 && n == i * kPer + 1) w[i] &= 0xFFFFu;
+    }
+    raw = make_uint4(w[0], w[1], w[2], w[3]);
+  }
   __device__ __forceinline__ void get(float (&v)[VEC]) const {
     if constexpr (VEC == 1) {
       v[0] = (float)raw;
@@ -203,6 +214,73 @@ struct Slots {
 
 constexpr int kStages = 3;   // rows, or turns of rows, in a thread's slots
 
+// Rows that begin or end anywhere, in lines of shared memory: byte for byte as
+// they lie, wherever that is.  A row's threads copy the granules of 16 bytes that
+// hold it, without what lies before the matrix or behind the row: a value on its
+// way in a register would take four bytes whatever its size.
+template <typename T>
+struct Lines {
+  // 16 beyond the granules: vector() reads two
+  __host__ __device__ static constexpr int pitch_of(int cols) {
+    return (cols * (int)sizeof(T) + 31 - (int)sizeof(T)) / 16 * 16 + 16;
+  }
+  const T* matrix;
+  uint8_t* mine;
+  int cols, pitch;
+  // `which` of `of` matrices, STAGES lines of each for each of the block's rows
+  template <int STAGES>
+  __device__ __forceinline__ void place(void* smem, const void* matrix, int cols, int which = 0, int of = 1) {
+    this->matrix = static_cast<const T*>(matrix), this->cols = cols, pitch = pitch_of(cols);
+    mine = static_cast<uint8_t*>(smem) + (threadIdx.y * of + which) * STAGES * pitch;
+  }
+  static __device__ __forceinline__ int skip(const T* row) { return (int)(reinterpret_cast<uintptr_t>(row) & 15); }
+  __device__ __forceinline__ void copy(int stage, const T* row) const {
+    const int bytes = skip(row) + cols * (int)sizeof(T);
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(row) - skip(row);
+    uint8_t* dst = mine + stage * pitch;
+    for (int o = threadIdx.x * 16; o < bytes; o += blockDim.x * 16) {
+      const int n = min(16, bytes - o);
+      if (src + o < reinterpret_cast<const uint8_t*>(matrix)) {   // o = 0
+        for (int b = skip(row); b < n; b += (int)sizeof(T))
+          *reinterpret_cast<T*>(dst + b) = *reinterpret_cast<const T*>(src + b);
+      } else {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                         static_cast<uint32_t>(__cvta_generic_to_shared(dst + o))),
+                     "l"(src + o), "r"(n)
+                     : "memory");
+      }
+    }
+  }
+  // The row, value for value.
+  __device__ __forceinline__ const T* at(int stage, const T* row) const {
+    return reinterpret_cast<const T*>(mine + stage * pitch + skip(row));
+  }
+  // 16 bytes of it, whose first value is c, a multiple of a vector's: parts of two granules.
+  __device__ __forceinline__ uint4 vector(int stage, const T* row, int c) const {
+    const int off = skip(row), bits = (off & 3) * 8;
+    const uint8_t* p = mine + stage * pitch + c * (int)sizeof(T);
+    const uint4 a = *reinterpret_cast<const uint4*>(p), b = *reinterpret_cast<const uint4*>(p + 16);
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    uint4 r;
+    auto from = [&](auto words) {   // the same in all of a row's threads, so a branch
+      constexpr int n = decltype(words)::value;
+      r.x = __funnelshift_r(w[n], w[n + 1], bits);
+      r.y = __funnelshift_r(w[n + 1], w[n + 2], bits);
+      r.z = __funnelshift_r(w[n + 2], w[n + 3], bits);
+      r.w = __funnelshift_r(w[n + 3], w[n + 4], bits);
+    };
+    if (off < 8) {
+      if (off < 4) from(std::integral_constant<int, 0>());
+      else from(std::integral_constant<int, 1>());
+    } else if (off < 12) {
+      from(std::integral_constant<int, 2>());
+    } else {
+      from(std::integral_constant<int, 3>());
+    }
+    return r;
+  }
+};
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -213,6 +291,12 @@ __device__ __forceinline__ float warp_sum(float v) {
 // warp needs none of this.
 __device__ __forceinline__ void row_barrier() {
   asm volatile("bar.sync %0, %1;" ::"r"(threadIdx.y + 1), "r"(blockDim.x) : "memory");
+}
+
+// The same where a row may have one warp.
+__device__ __forceinline__ void line_barrier() {
+  if (blockDim.x == 32) __syncwarp();
+  else row_barrier();
 }
 
 // Sum over the threads of a row, the same value, bit for bit, in every thread.
@@ -228,6 +312,26 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 }
 
 constexpr int kMostRows = 8;   // of a block
+
+// First column of vector i of a thread's V.  Vectors: a row's threads side by
+// side.  Single values: a warp's side by side, V times, so that their places are
+// a constant apart.
+template <int VEC, int V, int THREADS>
+__device__ __forceinline__ int column_of(int i) {
+  if constexpr (VEC == 1) return ((threadIdx.x >> 5) * V + i) * 32 + (threadIdx.x & 31);
+  else return (i * (THREADS ? THREADS : blockDim.x) + threadIdx.x) * VEC;
+}
+
+// f(how many of a warp's V times 32 single values lie in the row: all of these,
+// some of the next four, none of the rest), as a constant.  A warp that has the
+// row's end would otherwise ask for each value and hold up the others (rows of
+// 4064 values in place of 4096: a quarter of the time).
+template <int V, int WHOLE = V, typename F>
+__device__ __forceinline__ void by_end(int cols, F f) {
+  if constexpr (WHOLE <= 0) f(std::integral_constant<int, 0>());
+  else if (((int)(threadIdx.x >> 5) * V + WHOLE) * 32 <= cols) f(std::integral_constant<int, WHOLE>());
+  else by_end<V, WHOLE - 4>(cols, f);
+}
 
 // ---------------------------------------------------------------- host side
 
@@ -260,23 +364,37 @@ void by_type(int dtype, F f) {
 }
 
 // f(values per vector, vectors per thread, threads of a row) with constants: up
-// to MOST vectors of 16 bytes or 16 single values.  Rows that FILLED vectors a
+// to MOST vectors of 16 bytes or 16 single values, or with LINES, -1 threads and
+// vectors for rows that do not lie on 16 bytes.  Rows that FILLED vectors a
 // thread fill get their number of threads as a constant, others 0: offsets that
 // are constants and no checks of columns are worth a sixth of a pass over rows
 // of 4096.
-template <typename T, int FILLED, int MOST, typename F>
-void by_shape(const Shape& s, int cols, F f) {
+template <typename T, int FILLED, int MOST, bool LINES, typename F>
+void by_shape(const Shape& s, int cols, bool vectors, F f) {
   using std::integral_constant;
   const integral_constant<int, 16 / (int)sizeof(T)> vec;
   const integral_constant<int, 1> one;
   const integral_constant<int, 0> any;
-  if (s.vec == 1) {
+  auto by_v = [&](auto threads) {
+    if (s.v == 1) f(vec, one, threads);
+    else if (s.v == 2) f(vec, integral_constant<int, 2>(), threads);
+    else if (s.v == 4) f(vec, integral_constant<int, std::min(4, MOST)>(), threads);
+    else f(vec, integral_constant<int, std::min(8, MOST)>(), threads);
+  };
+  if constexpr (LINES) {
+    if (!vectors) {
+      by_v(integral_constant<int, -1>());
+      return;
+    }
+  } else if (!vectors) {
     if (s.v == 1) f(one, one, any);
     else if (s.v == 2) f(one, integral_constant<int, 2>(), any);
     else if (s.v == 4) f(one, integral_constant<int, 4>(), any);
     else if (s.v == 8) f(one, integral_constant<int, 8>(), any);
     else f(one, integral_constant<int, 16>(), any);
-  } else if (s.v == FILLED && s.vec * s.v * s.threads == cols && s.threads <= 512) {
+    return;
+  }
+  if (s.v == FILLED && s.vec * s.v * s.threads == cols && s.threads <= 512) {
     const integral_constant<int, FILLED> v;
     if (s.threads == 32) f(vec, v, integral_constant<int, 32>());
     else if (s.threads == 64) f(vec, v, integral_constant<int, 64>());
@@ -286,16 +404,12 @@ void by_shape(const Shape& s, int cols, F f) {
     else if (s.threads == 320) f(vec, v, integral_constant<int, 320>());
     else if (s.threads == 512) f(vec, v, integral_constant<int, 512>());
     else f(vec, v, any);
-  } else if (s.v == 1) {
-    f(vec, one, any);
-  } else if (s.v == 2) {
-    f(vec, integral_constant<int, 2>(), any);
-  } else if (s.v == 4) {
-    f(vec, integral_constant<int, std::min(4, MOST)>(), any);
   } else {
-    f(vec, integral_constant<int, std::min(8, MOST)>(), any);
+    by_v(any);
   }
 }
+
+constexpr int kMostSmem = 220 * 1024;   // dynamic, of a block
 
 // Blocks of `kernel` that an SM holds, asked for once per size.
 struct Residency {
@@ -314,12 +428,21 @@ inline int resident(Residency* r, const void* kernel, int threads, size_t smem) 
 }
 
 // Launches KERNEL, which takes rows blockIdx.x, + gridDim.x ..., on as many
-// blocks as are resident at a time.
+// blocks as are resident at a time; smem: bytes for each of a block's rows.
 template <auto KERNEL, typename... A>
-void launch_rows(const Shape& sh, int64_t rows, cudaStream_t s, const A&... args) {
+int launch_rows(const Shape& sh, int64_t rows, int smem, cudaStream_t s, const A&... args) {
   static Residency known;
-  const int64_t most = (int64_t)ds::sm_count() * resident(&known, reinterpret_cast<const void*>(KERNEL), sh.threads * sh.rows, 0);
-  KERNEL<<<(unsigned)std::min<int64_t>((rows + sh.rows - 1) / sh.rows, most), dim3(sh.threads, sh.rows), 0, s>>>(args...);
+  static SmemOnce once;
+  const void* kernel = reinterpret_cast<const void*>(KERNEL);
+  smem *= sh.rows;
+  if (smem > 40 * 1024) {
+    const int st = ds::allow_smem(&once, kernel, kMostSmem);
+    if (st != DS_OK) return st;
+  }
+  const int most = std::min(resident(&known, kernel, sh.threads * sh.rows, 0), 227 * 1024 / (smem + 4 * 1024));
+  const int64_t blocks = std::min<int64_t>((rows + sh.rows - 1) / sh.rows, (int64_t)ds::sm_count() * std::max(1, most));
+  KERNEL<<<(unsigned)blocks, dim3(sh.threads, sh.rows), smem, s>>>(args...);
+  return DS_OK;
 }
 
 inline bool vectors(const void* p, int64_t rows, int64_t cols, int64_t ld, int es) {

@@ -65,6 +65,24 @@ def test_quantize(rows, cols, dtype, cuda):
         assert bool(((got - want).abs() <= (U + torch.finfo(to).eps / 2) * want.abs() + 2.0 ** -25 * (to == F16)).all())
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows", [1, 5, 1900])
+@pytest.mark.parametrize("cols", [1, 2, 7, 8, 9, 17, 64, 255, 257, 1022, 1025, 2049, 4095, 8191, 20001])
+def test_rows_anywhere(cols, rows, dtype, cuda):
+    """Rows that begin and end between 16-byte boundaries, among values that are no numbers; several turns a block."""
+    x = data(rows, cols, cuda, seed=cols, dtype=dtype)
+    codes, scales = emulate(x)
+    want = codes.float() * scales[:, None]
+    for pad, off in ((0, 1), (5, 0), (3, 6)):
+        big = torch.full((rows * (cols + pad) + 2 * off,), float("nan"), dtype=dtype, device=cuda)
+        view = big[off:off + rows * (cols + pad)].view(rows, cols + pad)[:, :cols]
+        view.copy_(x)
+        q = int8.quantize(view)
+        assert torch.equal(q.codes.cpu(), codes) and torch.equal(q.scales.cpu(), scales)
+    for to in (F32, BF16, F16):
+        assert torch.equal(q.dequantize(to).cpu(), want.to(to))   # one product, rounded once more
+
+
 def test_every_tie(cuda):
     """Scale 1: all multiples of 1 / 2, and their neighbours in f32."""
     half = torch.arange(-254, 255, device=cuda).float() / 2

@@ -161,6 +161,34 @@ def test_strides_and_alignments(cols, dtype, cuda):
         check(t, want[name], name)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows", [1, 6, 1400])
+@pytest.mark.parametrize("cols", [1, 7, 31, 32, 33, 127, 129, 256, 257, 511, 513, 640, 1023, 1024, 1025, 2047, 2050, 4094,
+                                  4097, 8191, 8192])
+def test_rows_anywhere(cols, rows, dtype, cuda):
+    """Rows that begin and end between 16-byte boundaries, among values that are no numbers; several turns a block."""
+    x, dy = data(rows, cols, dtype, cuda, seed=cols), data(rows, cols, dtype, cuda, seed=rows + 5)
+    w, b = data(1, cols, F32, cuda, seed=1)[0], data(1, cols, F32, cuda, seed=2)[0]
+    want = formula(x, w, b, 1e-5, dy)
+
+    def placed(t, pad, off):
+        big = torch.full((rows * (cols + pad) + 2 * off,), float("nan"), dtype=dtype, device=cuda)
+        view = big[off:off + rows * (cols + pad)].view(rows, cols + pad)[:, :cols]
+        view.copy_(t)
+        return view
+
+    seen = []
+    for pad, off in ((0, 1), (5, 0), (1, 3)):
+        got = train(placed(x, pad, off), w, b, placed(dy, 3 - pad % 3, off + 2))
+        for name, t in got.items():
+            check(t, want[name], name)
+        seen.append(got)
+    # the order of a row's sums follows from its columns, but for rows that lie on 16 bytes (of the three, the single
+    # one at the beginning of its buffer), which are summed in vectors
+    if rows > 1 or cols * x.element_size() % 16:
+        assert all(torch.equal(seen[0][n], seen[i][n]) for n in want for i in (1, 2))
+
+
 def test_shapes(cuda):
     x = data(24, 80, BF16, cuda)
     w, b = data(1, 80, BF16, cuda, seed=1)[0], data(1, 80, BF16, cuda, seed=2)[0]
