@@ -6,8 +6,9 @@
 //   dw = sum over rows of dy xh,  db = sum over rows of dy
 //
 // Bounded by memory.  A row stays in the registers of the threads that loaded
-// it, so x and dy are read once.  Sums, mean and r are f32; the variance is
-// summed from differences to the mean, so a mean far from 0 costs nothing.
+// it, so x and dy are read once.  Sums, mean and r are f32.  The variance is
+// summed from differences to the mean and xh is off by two roundings of its own
+// in both passes, so a mean far from 0 costs no more than its own rounding.
 #include <algorithm>
 #include <type_traits>
 
@@ -253,7 +254,8 @@ struct Turn {
 // once for dx, dw and db together.  8192 x 4096 bf16: 37.7 us, 5.3 TB/s, bounded
 // like the forward pass.  Measured beside it: one row a turn with the next one in
 // registers 47 us, one row a turn through a ring 59, x and dy kept in registers
-// from the first use to the second 40 (and 52 once they spilled).
+// from the first use to the second 40 (and 52 once they spilled).  4096 x 8192
+// f32, with its join: 72 us; 88 with xh as (x - mean) r.
 //
 // 8192 x 4095, forward and backward: 131 us bf16 (184 with single values in
 // registers), 4096 x 8191 144 (303).
@@ -314,9 +316,16 @@ __global__ void __launch_bounds__(512, Turn<VEC, V>::kThreads / 512) backward_ke
     stats(first);
     int stage = 0, turn = 0;
     for (int64_t row = first; row < p.rows; row += step, turn ^= 1) {   // blockDim.y > 1 only with a warp a row
+      // xh = (x r + high) + low, high + low = -mean r: the rounding of that product
+      // (by one fma, Dekker's TwoProduct) would otherwise be in all of the row's xh,
+      // which it exceeds where x is near the mean and the mean far from 0
       float2 st[R];
+      float high[R], low[R];
 #pragma unroll
-      for (int r = 0; r < R; ++r) st[r] = next[r];
+      for (int r = 0; r < R; ++r) {
+        st[r] = next[r];
+        high[r] = -st[r].x * st[r].y, low[r] = fmaf(-st[r].x, st[r].y, -high[r]);
+      }
       const int here = stage;
       slots.wait<S - 2>();
       if constexpr (U::kLines) line_barrier();   // all of the row is here, and the row before it has been used
@@ -326,8 +335,8 @@ __global__ void __launch_bounds__(512, Turn<VEC, V>::kThreads / 512) backward_ke
       stats(row + step);
       const T* here_x = line_x.at(here, static_cast<const T*>(p.x) + row * p.ld);
       const T* here_dy = line_dy.at(here, static_cast<const T*>(p.dy) + row * p.ld_dy);
-      // dy and xh, from shared memory both times that they are asked for (registers
-      // that held them would be missing elsewhere)
+      // dy and xh - low, from shared memory both times that they are asked for
+      // (registers that held them would be missing elsewhere)
       auto at = [&](int r, int i, Values<VEC>& d, Values<VEC>& xh) {
         Pack<T, VEC> kx, kd;
         if constexpr (U::kLines) {
@@ -340,7 +349,7 @@ __global__ void __launch_bounds__(512, Turn<VEC, V>::kThreads / 512) backward_ke
         kd.get(v);
         d = Values<VEC>(v);
         kx.get(v);
-        xh = fma(Values<VEC>(v), Values<VEC>(st[r].y), Values<VEC>(-st[r].x * st[r].y));
+        xh = fma(Values<VEC>(v), Values<VEC>(st[r].y), Values<VEC>(high[r]));
       };
       float sums[2 * R];
 #pragma unroll
@@ -352,6 +361,7 @@ __global__ void __launch_bounds__(512, Turn<VEC, V>::kThreads / 512) backward_ke
             if (!inside(i)) continue;
             Values<VEC> d, xh;
             at(r, i, d, xh);
+            xh = xh + Values<VEC>(low[r]);
             aw[i] = fma(d, xh, aw[i]);
             ab[i] = ab[i] + d;
             d = d * kw[i];
@@ -366,7 +376,8 @@ __global__ void __launch_bounds__(512, Turn<VEC, V>::kThreads / 512) backward_ke
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         if (r && row + r >= p.rows) continue;
-        const Values<VEC> m1(-sums[2 * r] * inv), m2(-sums[2 * r + 1] * inv), rs(st[r].y);
+        const float mean_gx = -sums[2 * r + 1] * inv;
+        const Values<VEC> m1(fmaf(low[r], mean_gx, -sums[2 * r] * inv)), m2(mean_gx), rs(st[r].y);
         T* dx = static_cast<T*>(p.dx) + (row + r) * p.cols;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
