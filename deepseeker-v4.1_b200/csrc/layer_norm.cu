@@ -85,7 +85,9 @@ __global__ void __maxnreg__(VEC == 1 && V <= 8 ? 64 : V * VEC <= 16 ? 80 : 128) 
   __shared__ float red[kMostRows][2][32];
   const P* w = static_cast<const P*>(p.w);
   const P* b = static_cast<const P*>(p.b);
-  const float inv = 1.0f / p.cols;
+  // 1 / H in two parts: the mean is the rounded quotient.  With one part it can
+  // miss the mean of equal values, and r takes that up to 1 / sqrt(eps) times.
+  const float inv = 1.0f / p.cols, rest = fmaf(-inv, (float)p.cols, 1.0f) / p.cols;
   const int64_t step = (int64_t)gridDim.x * blockDim.y;
   auto column = [](int i) { return column_of<VEC, V, THREADS>(i); };
   by_rows<VEC, V, THREADS>(p.cols, [&](auto whole) {
@@ -145,7 +147,7 @@ __global__ void __maxnreg__(VEC == 1 && V <= 8 ? 64 : V * VEC <= 16 ? 80 : 128) 
         s = s + v[i];
       }
       if constexpr (!kLines) fetch(0, row + step);   // on its way during the rest
-      const float mean = row_sum(total(s), red[threadIdx.y][0]) * inv;
+      const float all = row_sum(total(s), red[threadIdx.y][0]), mean = fmaf(all, inv, all * rest);
       const Values<VEC> less(-mean);
       s = Values<VEC>(0.0f);
 #pragma unroll

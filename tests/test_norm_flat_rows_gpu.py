@@ -46,3 +46,18 @@ def test_gradients_of_flat_rows(cols, dtype, cuda):
         unit = torch.finfo(dtype).eps / 2
         bound = bound + unit * (want.abs() + bound) + (2.0 ** -25 if dtype == F16 else 0.0)
         assert bool(((dx.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("cols", [7, 56, 328, 984, 1000, 1968, 4095, 7872, 8191])
+def test_flat_rows_of_any_width(cols, dtype, cuda):
+    """The mean is the quotient of the sum, not a product with an inverse that was rounded."""
+    for rows, gap in ((1, 0), (126, 0), (1300, 3)):
+        x = flat(rows, cols, gap, dtype, cuda).requires_grad_()
+        g = torch.Generator(device=cuda).manual_seed(cols)
+        w = (1 + 0.3 * torch.randn(cols, generator=g, device=cuda)).requires_grad_()
+        b = torch.randn(cols, generator=g, device=cuda)
+        y = norm.layer_norm(x, w, b)
+        dw, = torch.autograd.grad(y, w, torch.randn(rows, cols, generator=g, device=cuda).to(dtype))
+        assert torch.equal(y.detach(), b.to(dtype).expand(rows, cols))
+        assert not dw.any()
