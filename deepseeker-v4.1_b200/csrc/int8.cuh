@@ -100,10 +100,11 @@ __device__ __forceinline__ void mma2(uint32_t d, uint64_t a, uint64_t b, uint32_
       : "memory");
 }
 
-// sum * a * b in f32: the smaller scale first, so that no step leaves f32
-// where the result does not.  (Comparisons, as fminf would drop a NaN.)
+// sum * a * b in f32: the scale nearer to 0 first (stored ones may be negative),
+// so that no step leaves f32 where the result does not.  (Comparisons, as fminf
+// would drop a NaN.)
 __device__ __forceinline__ float scaled(int sum, float a, float b) {
-  const bool less = a < b;
+  const bool less = fabsf(a) < fabsf(b);
   return (float)sum * (less ? a : b) * (less ? b : a);
 }
 

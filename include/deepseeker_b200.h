@@ -601,7 +601,7 @@ typedef struct DsInt8 {
 
 /* out [rows, w->rows] (f32, bf16 or f16, contiguous) = x W^T: the sum of
  * products of codes, exact in 32-bit integers, converted to f32, times both
- * scales (the smaller first), rounded to out's type.  x_dtype f32 / bf16 / f16:
+ * scales (the one nearer to 0 first), rounded to out's type.  x_dtype f32 / bf16 / f16:
  * x [rows, w->cols], rows ld elements apart, is quantised into the workspace
  * first (x_scales NULL; a single row by the product itself, without one);
  * DS_I8: x is codes, rows ld bytes apart (a multiple of 16), x_scales their

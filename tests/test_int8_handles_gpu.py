@@ -1,0 +1,40 @@
+"""Handles of the 8-bit operators (deepseeker.int8) that quantisation itself does not make: no rows, scales of either
+sign; and what decides between the kernels of few rows.
+
+A product's tolerance: the sum is exact, its conversion to f32 and each scale round once (u = 2^-24 each).
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from deepseeker import int8
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+U = 2.0 ** -24
+
+
+def normal(rows, cols, device, seed=0, dtype=F32):
+    return torch.randn(rows, cols, generator=torch.Generator(device=device).manual_seed(seed), device=device).to(dtype)
+
+
+def product(q, w):
+    sums = q.codes.double() @ w.codes.double().T                        # whole numbers below 2^53
+    return sums * q.scales.double()[:, None] * w.scales.double()
+
+
+def close(y, want):
+    assert y.dtype == F32 and y.shape == want.shape
+    assert bool(((y.double() - want).abs() <= (4 * U + 8 * U * U) * want.abs()).all())   # and the result's own rounding
+
+
+@pytest.mark.parametrize("rows", [1, 3, 12, 40, 300, 2000])
+def test_scales_of_either_sign(rows, cuda):
+    """Scales of stored codes whose product with the sum leaves f32 on the way unless the one nearer to 0 comes first."""
+    codes = (normal(rows, 96, cuda, rows) * 40).clamp(-128, 127).to(torch.int8)
+    wide = (normal(520, 96, cuda, 1) * 40).clamp(-128, 127).to(torch.int8)
+    for a, b in ((-1e36, 1e-30), (1e-30, -1e36), (-1e36, -1e-30), (-1e-30, -1e36), (1e36, 1e-30), (-3.0, 2.0)):
+        q = int8.from_codes(codes, torch.full((rows,), a, device=cuda))
+        w = int8.from_codes(wide, torch.full((520,), b, device=cuda))
+        close(int8.linear(q, w, out_dtype=F32), product(q, w))
