@@ -164,6 +164,8 @@ def linear(x, w: Int8Tensor, out_dtype: torch.dtype | None = None) -> torch.Tens
         n = _x_bytes(rows, w.cols)
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     out = torch.empty((*x.shape[:-1], w.rows), dtype=out_dtype, device=dev)
+    if not w.rows:
+        return out
     with on_device(dev):
         _abi.check(_abi.lib().ds_int8_linear(px, ps, dt, rows, ld, w._ref(), out.data_ptr(), _DTYPES[out_dtype],
                                              None if ws is None else ws.data_ptr(), n, raw_stream(dev)),

@@ -38,3 +38,16 @@ def test_scales_of_either_sign(rows, cuda):
         q = int8.from_codes(codes, torch.full((rows,), a, device=cuda))
         w = int8.from_codes(wide, torch.full((520,), b, device=cuda))
         close(int8.linear(q, w, out_dtype=F32), product(q, w))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_weights_of_no_rows(dtype, cuda):
+    x = normal(6, 40, cuda, dtype=dtype)
+    none = int8.quantize(normal(3, 40, cuda)[:0])
+    for rows in (x, x[:1], x[:0], x[0], x.view(2, 3, 40), int8.quantize(x), int8.quantize(x[:0])):
+        y = int8.linear(rows, none)
+        assert y.shape == (*rows.shape[:-1], 0) and y.dtype == (BF16 if isinstance(rows, int8.Int8Tensor) else dtype)
+    assert int8.linear(x, none, out_dtype=F16).dtype == F16
+    for bad in (x[:, :39], x.double(), x.cpu()):
+        with pytest.raises(ValueError):
+            int8.linear(bad, none)
