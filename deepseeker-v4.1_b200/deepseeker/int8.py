@@ -89,10 +89,14 @@ def _check_x(x) -> None:
         raise ValueError("x must be a f32, bf16 or f16 CUDA tensor (or an Int8Tensor where one is taken)")
     if x.dim() < 1 or not 1 <= x.shape[-1] < _MOST:
         raise ValueError("x must be [..., cols] with cols in [1, 2^17)")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise ValueError("8-bit operators have no backward pass: detach x or use torch.no_grad()")
-    if has_tangent(x):
-        raise ValueError("8-bit operators have no forward-mode derivatives: x is a dual tensor")
+    _check_no_derivative(x, "x")
+
+
+def _check_no_derivative(t, name) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"8-bit operators have no backward pass: detach {name} or use torch.no_grad()")
+    if has_tangent(t):
+        raise ValueError(f"8-bit operators have no forward-mode derivatives: {name} is a dual tensor")
 
 
 def _matrix(x):
@@ -129,6 +133,7 @@ def from_codes(codes: torch.Tensor, scales: torch.Tensor) -> Int8Tensor:
     if (not isinstance(scales, torch.Tensor) or scales.get_device() != codes.get_device()
             or scales.dtype != torch.float32 or scales.shape != (rows,)):
         raise ValueError("scales must be a f32 tensor [rows] on the codes' device")
+    _check_no_derivative(scales, "scales")
     scales, pitch = scales.contiguous(), codes.stride(0)
     if (cols > 1 and codes.stride(1) != 1) or codes.data_ptr() % 16 or pitch % 16 or pitch < cols:
         pitch = _up(cols, 16)

@@ -51,3 +51,16 @@ def test_weights_of_no_rows(dtype, cuda):
     for bad in (x[:, :39], x.double(), x.cpu()):
         with pytest.raises(ValueError):
             int8.linear(bad, none)
+
+
+def test_scales_that_ask_for_a_derivative(cuda):
+    codes = torch.ones(3, 16, dtype=torch.int8, device=cuda)
+    scales = torch.ones(3, device=cuda, requires_grad=True)
+    with pytest.raises(ValueError, match="backward"):
+        int8.from_codes(codes, scales)
+    with torch.no_grad():
+        assert torch.equal(int8.from_codes(codes, scales).dequantize(), torch.ones(3, 16, device=cuda))
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(torch.ones(3, device=cuda), torch.ones(3, device=cuda))
+        with pytest.raises(ValueError, match="forward-mode"):
+            int8.from_codes(codes, dual)
