@@ -498,10 +498,17 @@ __global__ void __launch_bounds__(kThreads, blocks_of(VEC, NV)) backward_kernel(
       }
       const float inv = z == 0.0f ? 0.0f : 1.0f / z, k = live ? g * inv : 0.0f;
       d *= inv;
+      auto slopes = [&](int j) { return SOFTMAX ? two(v[j], v[j + 1]) : two(slope[SOFTMAX ? 0 : j], slope[SOFTMAX ? 0 : j + 1]); };
+      auto differences = [&](int j) { return add2(two(c[j], c[j + 1]), two(-d, -d)); };
+      if (SOFTMAX || fabsf(k) < INFINITY) {
 #pragma unroll
-      for (int j = 0; j < N; j += 2) {
-        const uint64_t a = SOFTMAX ? two(v[j], v[j + 1]) : two(slope[SOFTMAX ? 0 : j], slope[SOFTMAX ? 0 : j + 1]);
-        split(mul2(mul2(two(k, k), a), add2(two(c[j], c[j + 1]), two(-d, -d))), v[j], v[j + 1]);
+        for (int j = 0; j < N; j += 2) split(mul2(mul2(two(k, k), slopes(j)), differences(j)), v[j], v[j + 1]);
+      } else {
+        // sums near the smallest numbers of f32: g / Z leaves f32 where its product
+        // with the slope does not
+#pragma unroll
+        for (int j = 0; j < N; j += 2)
+          split(mul2(mul2(two(inv, inv), slopes(j)), mul2(two(g, g), differences(j))), v[j], v[j + 1]);
       }
       if (row < to) {
 #pragma unroll

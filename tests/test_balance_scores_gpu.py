@@ -1,0 +1,64 @@
+"""Scores of the balance loss (deepseeker.balance) far from a row's largest one.
+
+Tolerances, derived before the first run, u = 2^-24.  A score far from the row's largest is 2^t e^r: 4 u for the
+instruction 2^t (2^-22), a unit for the product with e^r, and 4 u for what f32 leaves out of log 2 (1.9e-9 |t|,
+|t| <= 126).  A row's sum Z of 16 scores of one lane is off by 9 u for its additions and by the error of its largest
+score, 4 u; 1 / Z, the products with the upstream gradient, with the score and with the coefficient's difference,
+the coefficient and that difference round once each, 6 u.  Where the largest score's expert was not chosen, d =
+sum p c is below 1e-8 c, so nothing cancels: 28 u of the gradient's size, rounded up to 32 u.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from deepseeker import balance
+
+pytestmark = pytest.mark.gpu
+F32 = torch.float32
+U = 2.0 ** -24
+
+
+def gradient(l, ids, kind, g):
+    """dlogits of one sequence by the formula in 64 bits, and what its two terms add up to without their signs."""
+    x, (T, E), k = l.double(), l.shape, ids.shape[1]
+    c = torch.bincount(ids.reshape(-1).long(), minlength=E).double() * E / (k * T * T)
+    if kind == "softmax":
+        p = torch.softmax(x, 1)
+        slope = p
+    else:
+        a = torch.logaddexp(x, torch.zeros_like(x)).sqrt()
+        z = a.sum(1, keepdim=True)
+        p, slope = a / z, torch.sigmoid(x) / (2 * a) / z
+    d = (p * c).sum(1, keepdim=True)
+    return g * slope * (c - d), abs(g) * slope * (c + d)
+
+
+def grad(l, ids, kind, g):
+    leaf = l.clone().requires_grad_()
+    loss, _ = balance.balance_loss(leaf, ids, kind=kind)
+    return torch.autograd.grad(loss, leaf, torch.tensor(g, device=l.device))[0]
+
+
+@pytest.mark.parametrize("g", [1.0, 1e6, -1e30])
+def test_low_rows_and_large_gradients(g, cuda):
+    """Rows whose scores are all near the smallest numbers of f32: 1 / Z times the upstream gradient leaves f32, the
+    gradient of the logits does not."""
+    l = torch.linspace(-170, -150, 5 * 16, device=cuda).view(5, 16).clone()
+    l[4] = 1.0
+    ids = torch.tensor([[0, 1], [2, 3], [0, 7], [9, 0], [1, 15]], dtype=torch.int32, device=cuda)
+    got = grad(l, ids, "sqrtsoftplus", g).double()
+    want, size = gradient(l, ids, "sqrtsoftplus", g)
+    # as above, and the differences c - d cancel: the errors of p in d (28 u) count in full
+    assert bool(((got - want).abs() <= 64 * U * size).all())
+
+
+def test_infinite_gradient_leaves_masked_rows_alone(cuda):
+    l = torch.randn(40, 16, generator=torch.Generator(device=cuda).manual_seed(2), device=cuda).requires_grad_()
+    ids = torch.zeros(40, 2, dtype=torch.int32, device=cuda)
+    valid = torch.arange(40, device=cuda) % 3 > 0
+    for kind in ("softmax", "sqrtsoftplus"):
+        for g in (float("inf"), float("nan")):
+            loss, _ = balance.balance_loss(l, ids, kind=kind, valid=valid)
+            dl, = torch.autograd.grad(loss, l, torch.tensor(g, device=cuda))
+            assert not dl[~valid].any() and not torch.isfinite(dl[valid]).any()
