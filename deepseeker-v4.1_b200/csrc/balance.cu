@@ -137,8 +137,8 @@ __device__ __forceinline__ float group_sum(float v, int lanes) {
   return v;
 }
 
-// 2^x, sqrt(x), 1 / sqrt(x) and 1 / x of the special function unit, off by a few
-// units in the last place of f32 (results below 2^-126 become 0).
+// 2^x, sqrt(x), 1 / sqrt(x) and 1 / x of the special function unit, off by four
+// units in the last place of f32 or less (results below 2^-126 become 0).
 __device__ __forceinline__ float fast_exp2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -160,6 +160,28 @@ __device__ __forceinline__ float fast_inverse(float x) {
   return r;
 }
 
+// exp of both x (numbers, no infinities) as 2^t (1 + r): t is x log2 e in f32, a
+// number as good as any near it, and r = x - t log 2 what it leaves of x, within
+// 4e-6 where 2^t is not 0, so that exp(r) is 1 + r (Cody and Waite's reduction with
+// t in the whole number's place).  2^t alone is off by the roundings of t and log2 e
+// too, 58 units in the last place 60 below 0; this by 2^t's four, one of the
+// product, and |t| / 30 for log 2 in f32.  65536 x 384, both passes: 96 us instead
+// of 90.
+__device__ __forceinline__ void exp_of(uint64_t x, float& a, float& b) {
+  constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+  const uint64_t t = mul2(x, two(kLog2e, kLog2e));
+  split(t, a, b);
+  const uint64_t e = two(fast_exp2(a), fast_exp2(b));
+  split(fma2(e, fma2(t, two(-kLn2, -kLn2), x), e), a, b);
+}
+
+// The larger of both, NaN where one is.
+__device__ __forceinline__ float larger(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // log(1 + t) / t on [0, 1]: the polynomial of degree 8 with the least largest
 // relative error (a fit in 64 bits: 3e-8; 3 units of f32 with its roundings).
 __device__ __forceinline__ uint64_t log1p_ratio2(uint64_t t) {
@@ -173,14 +195,15 @@ __device__ __forceinline__ uint64_t log1p_ratio2(uint64_t t) {
 }
 
 // A row's logits -> a (in place), its slope da / dl where asked for.  Columns
-// past the row hold -infinity, which gives a = 0 and slope 0.  sqrt(softplus)
-// takes 14 instructions and two of the special function unit a value, 18 and
-// three with its slope (expf, log1pf, sqrtf and divisions: 50 to 70, and the
-// passes over 65536 x 384 three times as long as their memory).
+// past the row hold -infinity, which gives a = 0 and slope 0 (exponents end at
+// -200, far below where 2^t is 0, so that they stay numbers).  sqrt(softplus) takes
+// 16 instructions and two of the special function unit a value, 20 and three with
+// its slope (expf, log1pf, sqrtf and divisions: 50 to 70, and the passes over 65536
+// x 384 three times as long as their memory).
 template <bool SOFTMAX, bool SLOPE, int N>
 __device__ __forceinline__ void scores(float (&v)[N], float (&slope)[SLOPE && !SOFTMAX ? N : 1], int lanes) {
   static_assert(N % 2 == 0, "pairs");
-  constexpr float kLog2e = 1.44269504f;
+  constexpr float kLeast = -200.0f;
   if constexpr (SOFTMAX) {
     float m = v[0];
 #pragma unroll
@@ -190,18 +213,19 @@ __device__ __forceinline__ void scores(float (&v)[N], float (&slope)[SLOPE && !S
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
       float x, y;
-      split(mul2(add2(two(v[j], v[j + 1]), two(-m, -m)), two(kLog2e, kLog2e)), x, y);
-      v[j] = fast_exp2(x), v[j + 1] = fast_exp2(y);
+      split(add2(two(v[j], v[j + 1]), two(-m, -m)), x, y);
+      exp_of(two(larger(x, kLeast), larger(y, kLeast)), v[j], v[j + 1]);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
       float h[2], s[2], t[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) h[i] = fast_exp2(fabsf(v[j + i]) * (-0.5f * kLog2e));   // exp(-|l| / 2)
+      // exp(-|l| / 2); what is no number stays none in the maximum below
+      const uint64_t least = two(fmaxf(-fabsf(v[j]), 2.0f * kLeast), fmaxf(-fabsf(v[j + 1]), 2.0f * kLeast));
+      exp_of(mul2(least, two(0.5f, 0.5f)), h[0], h[1]);
       const uint64_t h2 = two(h[0], h[1]), t2 = mul2(h2, h2);
       // softplus(l) = max(l, 0) + log(1 + exp(-|l|))
-      split(fma2(t2, log1p_ratio2(t2), two(fmaxf(v[j], 0.0f), fmaxf(v[j + 1], 0.0f))), s[0], s[1]);
+      split(fma2(t2, log1p_ratio2(t2), two(larger(v[j], 0.0f), larger(v[j + 1], 0.0f))), s[0], s[1]);
       split(t2, t[0], t[1]);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {

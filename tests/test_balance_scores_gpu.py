@@ -62,3 +62,15 @@ def test_infinite_gradient_leaves_masked_rows_alone(cuda):
             loss, _ = balance.balance_loss(l, ids, kind=kind, valid=valid)
             dl, = torch.autograd.grad(loss, l, torch.tensor(g, device=cuda))
             assert not dl[~valid].any() and not torch.isfinite(dl[valid]).any()
+
+
+@pytest.mark.parametrize("kind,top,least,most", [("softmax", 0.0, -80.0, -20.0), ("sqrtsoftplus", 3.0, -160.0, -40.0)])
+def test_far_scores(kind, top, least, most, cuda):
+    g = torch.Generator(device=cuda).manual_seed(1)
+    l = least + (most - least) * torch.rand(3000, 16, generator=g, device=cuda)
+    l[:, 5] = top                                                       # never chosen
+    ids = torch.randint(6, 21, (3000, 2), generator=g, device=cuda, dtype=torch.int32) % 16
+    got = grad(l, ids, kind, 1.0).double()
+    want, size = gradient(l, ids, kind, 1.0)
+    far = torch.arange(16, device=cuda) != 5
+    assert bool(((got - want).abs() <= 32 * U * size)[:, far].all()), float(((got - want).abs() / size)[:, far].max() / U)
