@@ -138,7 +138,9 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor, kind: str = "softmax",
 
     loss f32, 0-d or [S], is differentiable in the logits (rows that are not
     valid or in no sequence get 0); counts int32 [E] or [S, E].  A sequence
-    without valid tokens has loss 0.  Sums are f32.
+    without valid tokens has loss 0.  Sums are f32; scores below 2^-126 are 0
+    (square roots of softplus from logits of -174.7 on), and a row of none but
+    such has no shares and no gradient.
     """
     _check(logits, ids, kind, valid, offsets)
     kind = _KINDS[kind]

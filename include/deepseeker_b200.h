@@ -550,9 +550,9 @@ int ds_layer_norm_backward(const void* x, int dtype, int64_t rows, int64_t cols,
  *   loss = sum_e (c_e E / (k n)) P_e   (1 when both are even),
  * p_te = softmax(l_t)_e, or s_te / sum_e s_te with s = sqrt(softplus(l)).  The
  * gradient takes c_e as given.  Sums of p are f32; results do not depend on
- * timing.  A row whose scores are all 0 in f32 (logits of
- * -infinity; for the root of softplus from about -200 on) has p = 0 and no
- * gradient. */
+ * timing.  Scores below 2^-126 are 0, and a row of none but such (logits of
+ * -infinity; for the root of softplus, about exp(l / 2) there, of -174.7 and
+ * less) has p = 0 and no gradient. */
 typedef struct DsBalance {
   const void* logits;         /* [T, E], rows ld elements apart                      */
   int64_t tokens, ld;         /* T: T * top_k < 2^31                                  */

@@ -74,3 +74,21 @@ def test_far_scores(kind, top, least, most, cuda):
     want, size = gradient(l, ids, kind, 1.0)
     far = torch.arange(16, device=cuda) != 5
     assert bool(((got - want).abs() <= 32 * U * size)[:, far].all()), float(((got - want).abs() / size)[:, far].max() / U)
+
+
+def test_bound_of_low_rows(cuda):
+    """exp(l / 2) is a number of f32 (2^-126 and above) down to -174.67: rows above have their shares, rows below none."""
+    ids = torch.tensor([[0, 1], [2, 3], [0, 7]], dtype=torch.int32, device=cuda)
+    l = torch.full((3, 16), -173.5, device=cuda)
+    l[1] += torch.linspace(-1, 0, 16, device=cuda)
+    want, size = gradient(l, ids, "sqrtsoftplus", 1.0)
+    got = grad(l, ids, "sqrtsoftplus", 1.0).double()
+    assert bool(((got - want).abs() <= 64 * U * size).all())
+    loss, counts = balance.balance_loss(l, ids, kind="sqrtsoftplus")
+    # even shares where the logits are even: loss = sum over rows and experts of c / E
+    p = torch.softmax(l.double() / 2, 1)
+    c = counts.double() * 16 / (2 * 9)
+    assert abs(float(loss) - float((p.sum(0) * c).sum())) <= 64 * U * float(loss)
+    l = torch.full((3, 16), -175.5, device=cuda)
+    loss, counts = balance.balance_loss(l, ids, kind="sqrtsoftplus")
+    assert float(loss) == 0 and int(counts.sum()) == 6 and not grad(l, ids, "sqrtsoftplus", 1.0).any()
