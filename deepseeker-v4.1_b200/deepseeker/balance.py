@@ -80,21 +80,20 @@ def _forward(logits, ids, kind, valid, offsets):
     lead = () if offsets is None else (sequences,)
     loss = torch.empty(lead, dtype=torch.float32, device=dev)
     counts = torch.empty((*lead, experts), dtype=torch.int32, device=dev)
-    at = 4 * sequences * experts
+    coef = torch.empty(sequences * experts, dtype=torch.float32, device=dev)
     with on_device(dev):
         n = _workspace_bytes(dev.index, d.tokens, experts, sequences)
-        kept = torch.empty(at + n, dtype=torch.uint8, device=dev)   # the coefficients, then the workspace
-        p = kept.data_ptr()
-        _abi.check(_abi.lib().ds_balance_loss(ctypes.byref(d), loss.data_ptr(), counts.data_ptr(), p, p + at, n,
-                                              raw_stream(dev)), "ds_balance_loss")
-    return loss, counts, kept
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)   # of its own: the coefficients outlive the call
+        _abi.check(_abi.lib().ds_balance_loss(ctypes.byref(d), loss.data_ptr(), counts.data_ptr(), coef.data_ptr(),
+                                              ws.data_ptr(), n, raw_stream(dev)), "ds_balance_loss")
+    return loss, counts, coef
 
 
 class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, kind, valid, offsets):
-        loss, counts, kept = _forward(logits, ids, kind, valid, offsets)
-        ctx.save_for_backward(logits, valid, offsets, kept)
+        loss, counts, coef = _forward(logits, ids, kind, valid, offsets)
+        ctx.save_for_backward(logits, valid, offsets, coef)
         ctx.kind = kind
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)   # of the counts, which have none
@@ -109,12 +108,12 @@ class _BalanceLoss(torch.autograd.Function):
 
 
 def _backward(ctx, dloss):
-    logits, valid, offsets, kept = ctx.saved_tensors
+    logits, valid, offsets, coef = ctx.saved_tensors
     d, hold = _desc(logits, None, ctx.kind, valid, offsets)
     dloss, dev = dloss.contiguous(), logits.device
     dlogits = new_like(logits)
     with on_device(dev):
-        _abi.check(_abi.lib().ds_balance_loss_backward(ctypes.byref(d), kept.data_ptr(), dloss.data_ptr(),
+        _abi.check(_abi.lib().ds_balance_loss_backward(ctypes.byref(d), coef.data_ptr(), dloss.data_ptr(),
                                                        dlogits.data_ptr(), raw_stream(dev)), "ds_balance_loss_backward")
     return dlogits, None, None, None, None
 

@@ -92,3 +92,15 @@ def test_bound_of_low_rows(cuda):
     l = torch.full((3, 16), -175.5, device=cuda)
     loss, counts = balance.balance_loss(l, ids, kind="sqrtsoftplus")
     assert float(loss) == 0 and int(counts.sum()) == 6 and not grad(l, ids, "sqrtsoftplus", 1.0).any()
+
+
+@pytest.mark.parametrize("offsets", [None, [0, 100, 20000]])
+def test_what_is_kept_for_the_backward_pass(offsets, cuda):
+    """The logits and E coefficients a sequence, not the forward pass's workspace."""
+    l = torch.randn(20000, 64, device=cuda).requires_grad_()
+    ids = torch.zeros(20000, 2, dtype=torch.int32, device=cuda)
+    off = None if offsets is None else torch.tensor(offsets, device=cuda)
+    loss, _ = balance.balance_loss(l, ids, offsets=off)
+    held = {t.untyped_storage().data_ptr(): t.untyped_storage().nbytes() for t in loss.grad_fn.saved_tensors if t is not None}
+    del held[l.data_ptr()]
+    assert sum(held.values()) <= (4 * 64 if off is None else 2 * 4 * 64 + 3 * 8)
