@@ -430,8 +430,8 @@ struct VecParams {
   int64_t pitch;
   const float *sw, *sx;        // sx: scales of x where it comes as codes
   const void* x;
-  int64_t ldx;
-  int vec;                     // every 8 values of a row of x start on 16 bytes
+  int64_t ldx;                 // of codes
+  int vec;                     // every 8 values of x start on 16 bytes
   int cols, M, N;              // K, features, rows of x (up to T)
   void* out;
   int64_t ldo;
@@ -452,19 +452,21 @@ __device__ __forceinline__ uint4 codes_at(const uint8_t* at, int n) {
 // Up to T rows of x by F features a block, on CUDA cores: a thread keeps 16
 // columns (of every blockDim.x * 16), so it quantises just what it multiplies,
 // and all F rows of weights are on their way before x has been looked at.  X:
-// type of x, or int8_t where a launch before this one has quantised it (every
-// block that quantises does all of it: two rows took 12.8 us that way).
+// type of x, one row of values, or int8_t where a launch before this one has
+// quantised it (every block that quantises does all of it: two rows took 12.8 us
+// that way).
 // No cluster, no tensor memory: bounded by the stream of weights and the start
 // of a launch.  The grid is one wave of blocks where it
 // can be (by_features).  One row of 4096 to 4096: 8.4 us with its launch, 2.6 of
 // them the weights at memory speed.
 template <typename X, int T, int F>
 __global__ void __launch_bounds__(256) rows_kernel(const VecParams p) {
-  __shared__ uint32_t tops[T][8];
+  constexpr bool kCoded = std::is_same<X, int8_t>::value;
+  static_assert(kCoded || T == 1, "only a single row comes as values");
+  __shared__ uint32_t tops[8];
   __shared__ int part[8][F * T];
   __shared__ float sx[T];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  constexpr bool kCoded = std::is_same<X, int8_t>::value;
   const int f0 = blockIdx.x * F, wide = blockDim.x * 16;
   const X* x = static_cast<const X*>(p.x);
   uint4 w[F];
@@ -476,39 +478,28 @@ __global__ void __launch_bounds__(256) rows_kernel(const VecParams p) {
     }
   };
   weights(threadIdx.x * 16);
-  float scale[T];
+  [[maybe_unused]] float scale;
   if constexpr (kCoded) {
     launch_dependents();
     wait_prior_grid();
     if (threadIdx.x < T) sx[threadIdx.x] = threadIdx.x < p.N ? p.sx[threadIdx.x] : 0.0f;
   } else {
-    uint32_t top[T] = {};
+    uint32_t top = 0;
     for (int c = threadIdx.x * 16; c < p.cols; c += wide) {
 #pragma unroll
-      for (int t = 0; t < T; ++t) {
-        if (t >= p.N) continue;
+      for (int h = 0; h < 16; h += 8) {
+        float v[8];
+        load8(x + c + h, p.cols - c - h, p.vec, v);
 #pragma unroll
-        for (int h = 0; h < 16; h += 8) {
-          float v[8];
-          load8(x + t * p.ldx + c + h, p.cols - c - h, p.vec, v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) top[t] = max(top[t], __float_as_uint(v[j]) & 0x7FFFFFFFu);
-        }
+        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
       }
     }
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-      top[t] = __reduce_max_sync(0xffffffffu, top[t]);
-      if (lane == 0) tops[t][warp] = top[t];
-    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) tops[warp] = top;
     __syncthreads();
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-      uint32_t m = 0;
-      for (int i = 0; i < warps; ++i) m = max(m, tops[t][i]);
-      scale[t] = scale_of(m);
-      if (threadIdx.x == 0) sx[t] = scale[t];
-    }
+    for (int i = 0; i < warps; ++i) top = max(top, tops[i]);
+    scale = scale_of(top);
+    if (threadIdx.x == 0) sx[0] = scale;
   }
   int acc[F][T] = {};
   for (int c = threadIdx.x * 16;; c += wide) {
@@ -520,12 +511,12 @@ __global__ void __launch_bounds__(256) rows_kernel(const VecParams p) {
         if (t < p.N && c < p.cols) k = codes_at(reinterpret_cast<const uint8_t*>(x) + t * p.ldx + c, p.cols - c);
         q[t][0] = k.x, q[t][1] = k.y, q[t][2] = k.z, q[t][3] = k.w;
       } else {
-        const Coder coder(scale[t]);
+        const Coder coder(scale);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float v[8];
           uint32_t k[8];
-          load8(x + t * p.ldx + c + 8 * h, t < p.N ? p.cols - c - 8 * h : 0, p.vec, v);
+          load8(x + c + 8 * h, p.cols - c - 8 * h, p.vec, v);
           coder.codes(v, k);
           q[t][2 * h] = pack_codes(k[0], k[1], k[2], k[3]), q[t][2 * h + 1] = pack_codes(k[4], k[5], k[6], k[7]);
         }
@@ -701,8 +692,10 @@ template <typename X, int T>
 int by_features(const VecParams& p, cudaStream_t s, bool chained) {
   const int64_t wave = 2 * (int64_t)ds::sm_count();
   if (p.M <= 4 * wave) return launch_vec<X, T, 4>(p, s, chained);
-  if (p.M <= 8 * wave || T == 4) return launch_vec<X, T, 8>(p, s, chained);
-  return launch_vec<X, T, T == 4 ? 8 : 16>(p, s, chained);
+  if constexpr (T < 4) {
+    if (p.M > 8 * wave) return launch_vec<X, T, 16>(p, s, chained);
+  }
+  return launch_vec<X, T, 8>(p, s, chained);
 }
 
 int launch_rows_kernel(const Input& x, const DsInt8& w, void* y, int out_dtype, cudaStream_t s, bool chained) {

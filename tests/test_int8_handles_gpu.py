@@ -64,3 +64,19 @@ def test_scales_that_ask_for_a_derivative(cuda):
         dual = torch.autograd.forward_ad.make_dual(torch.ones(3, device=cuda), torch.ones(3, device=cuda))
         with pytest.raises(ValueError, match="forward-mode"):
             int8.from_codes(codes, dual)
+
+
+@pytest.mark.parametrize("K", [33, 300, 1001, 4096])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4])
+def test_few_rows_by_every_width(rows, K, cuda):
+    """Each number of features that a block takes (4, 8 or 16, by how many there are for an SM), whole and with a rest."""
+    wave = 2 * torch.cuda.get_device_properties(cuda).multi_processor_count
+    x = normal(rows, K, cuda, K, BF16)
+    q = int8.quantize(x)
+    for n in (1, 4 * wave, 4 * wave - 3, 4 * wave + 7, 8 * wave, 8 * wave - 5, 8 * wave + 9, 16 * wave + 8):
+        w = int8.quantize(normal(n, K, cuda, n))
+        want = product(q, w)
+        y = int8.linear(x, w, out_dtype=F32)
+        close(y, want)
+        assert torch.equal(int8.linear(q, w, out_dtype=F32), y)
+    assert int8.status() == 0
