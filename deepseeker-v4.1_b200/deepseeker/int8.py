@@ -107,7 +107,12 @@ def _matrix(x):
 def quantize(x: torch.Tensor) -> Int8Tensor:
     """x [..., cols] -> Int8Tensor.  A row's scale is its largest magnitude times
     1 / 127 (in f32), a code the whole number nearest to the exact quotient of
-    value and scale, ties to the even one.  A NaN or an infinity makes its whole row NaN."""
+    value and scale, ties to the even one.  A NaN or an infinity makes its whole row NaN.
+
+    The product is the rule, not the quotient maximum / 127: they differ by a unit
+    of the last place in about one row of twenty, and half of the maximum can then get
+    another code.  What is quantised elsewhere and has to meet these codes takes the
+    product; ``from_codes`` serves codes and scales of either rule as they are."""
     _check_x(x)
     rows, ld = _matrix(x)
     n, cols = rows.shape

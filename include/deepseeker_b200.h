@@ -581,10 +581,13 @@ int ds_balance_loss_backward(const DsBalance* desc, const float* coef, const flo
  * token's activations, an output channel's weights; the reference has no
  * product in this format).  Of a row of K < 2^17 values: s = max |x| * (1 / 127)
  * in f32 (factor and product rounded), code q = the whole number nearest to the
- * exact x / s, the even one of two, clipped to +-127 (0 where s is 0).  A row with a NaN or an
- * infinity has scale NaN and codes 0, so products with it are NaN.  Codes of a
- * row lie together, rows `pitch` bytes apart, a multiple of 16 (what lies
- * between is neither read as a value nor written). */
+ * exact x / s, the even one of two, clipped to +-127 (0 where s is 0).  (The
+ * rounded quotient max |x| / 127 is a unit of the last place away in about one row
+ * of twenty, where half of the maximum can have another code; the operators that
+ * take codes take either.)  A row with a NaN or an infinity has scale NaN and codes
+ * 0, so products with it are NaN.  Codes of a row lie together, rows `pitch` bytes
+ * apart, a multiple of 16 (what lies between is neither read as a value nor
+ * written). */
 int ds_int8_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ld, int8_t* codes, int64_t pitch,
                      float* scales, void* stream);
 /* out [rows, cols] f32, bf16 or f16 contiguous = code * scale, rounded to f32

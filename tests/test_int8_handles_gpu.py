@@ -80,3 +80,20 @@ def test_few_rows_by_every_width(rows, K, cuda):
         close(y, want)
         assert torch.equal(int8.linear(q, w, out_dtype=F32), y)
     assert int8.status() == 0
+
+
+def test_the_scale_is_a_product(cuda):
+    """A row's scale is max * (1 / 127), factor and product rounded to f32.  It can be a unit of the last place from
+    the rounded quotient max / 127, and half of the maximum, next to the middle of two codes, then has another code."""
+    x = torch.tensor([[143.0, 71.5], [144.0, -72.0], [254.0, 127.0], [127.0, 63.5]], device=cuda)
+    for dtype in (F32, BF16, F16):
+        q = int8.quantize(x.to(dtype))
+        assert torch.equal(q.scales, x[:, 0] * torch.tensor(1 / 127, device=cuda))
+        assert q.codes.tolist() == [[127, 64], [127, -64], [127, 64], [127, 64]]
+    quotient = torch.tensor([143 / 127, 144 / 127], dtype=torch.float64).float()     # rounded once: one unit above
+    assert bool((q.scales[:2].cpu() < quotient).all())
+    by_quotient = torch.round(x[:2].cpu().double() / quotient.double()[:, None])
+    assert by_quotient.tolist() == [[127, 63], [127, -63]]
+    # stored codes are taken as they are, whichever rule made them
+    held = int8.from_codes(by_quotient.to(torch.int8).to(cuda), quotient.to(cuda))
+    assert torch.equal(held.dequantize().cpu(), by_quotient.float() * quotient[:, None])
