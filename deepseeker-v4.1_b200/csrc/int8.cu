@@ -165,9 +165,14 @@ __global__ void __launch_bounds__(1024) quantize_long_kernel(const T* __restrict
 
 // Values of codes, VEC a thread: eight where the result's rows lie on 16 bytes,
 // otherwise (ANY) the 16 bytes of a granule of the result, whose codes are a
-// window of two.  STREAM: results of many megabytes leave L2 first, so that the
-// codes, which their quantisation may just have left there, do not (16384 x 4096
-// to bf16 after its quantisation: 34 -> 28.6 us).
+// window of two.  STREAM: the result leaves L2 first, so that the codes, which
+// their quantisation may just have left there, do not; for results that do not fit
+// into L2, whose next reader has to fetch most of them either way.  To bf16 in rows
+// of 4096, with quantisation before it: 16384 of them 65.6 us instead of 71.7,
+// 18432 77.8 (81.9), from 20480 on none is gained (24576: 107.6, 106.8).  Of codes
+// from memory, alone or with a layer norm or a product reading the result: 40.9
+// (40.1), 94.2 (93.6) and 71.7 us (70.9).  With the result inside L2 that reader
+// would pay: 8192 rows and a product 42.5 us instead of 36.9.
 template <typename T, bool ANY, bool STREAM>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ codes, int64_t pitch,
                                                          const float* __restrict__ scales, int64_t rows, int cols,
@@ -822,7 +827,7 @@ extern "C" int ds_int8_dequantize(const int8_t* codes, int64_t pitch, const floa
   ds::rows::by_type(out_dtype, [&](auto t) {
     using T = decltype(t);
     T* dst = static_cast<T*>(out);
-    const bool stream = rows * cols * es >= (64 << 20);   // half of L2
+    const bool stream = rows * cols * es >= (126 << 20);   // L2
     if (vec && stream) dequantize_kernel<T, false, true><<<grid, block, 0, s>>>(src, pitch, scales, rows, (int)cols, dst);
     else if (vec) dequantize_kernel<T, false, false><<<grid, block, 0, s>>>(src, pitch, scales, rows, (int)cols, dst);
     else if (stream) dequantize_kernel<T, true, true><<<grid, block, 0, s>>>(src, pitch, scales, rows, (int)cols, dst);

@@ -97,3 +97,15 @@ def test_the_scale_is_a_product(cuda):
     # stored codes are taken as they are, whichever rule made them
     held = int8.from_codes(by_quotient.to(torch.int8).to(cuda), quotient.to(cuda))
     assert torch.equal(held.dequantize().cpu(), by_quotient.float() * quotient[:, None])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("cols", [4096, 4095])
+def test_values_of_matrices_beyond_l2(cols, dtype, cuda):
+    """Results on both sides of the size from which they are written past L2."""
+    least = 126 * 2 ** 20 // (cols * torch.finfo(dtype).bits // 8)
+    for rows in (least, least + 1):
+        codes = torch.randint(-128, 128, (rows, cols), device=cuda, dtype=torch.int8)
+        scales = torch.rand(rows, device=cuda) + 0.5
+        got = int8.from_codes(codes, scales).dequantize(dtype)
+        assert torch.equal(got, (codes.float() * scales[:, None]).to(dtype))
