@@ -15,9 +15,11 @@
 // rows are p's sums per expert.  Every sum has an order of its own that only
 // sizes and offsets decide; counts are whole numbers.
 //
-// 65536 x 384 f32, sqrt-softplus: forward 35 us, backward 46 (2.9 and 4.4 TB/s):
-// issue slots, 61 and 72 % of them used, come before memory.  16384 x 256,
-// softmax: 8 and 7.5 us, which are the starts and ends of launches.
+// 65536 x 384 f32, sqrt-softplus: forward 38 us, backward 48 (2.6 and 4.2 TB/s).
+// Neither memory (35 % busy) nor issue slots (62 and 72 % used) are full: a warp
+// waits for its own arithmetic, one step of a score after the other, and an SM's 25
+// warps do not cover all of that.  16384 x 256, softmax: 8.4 and 7.8 us, which are
+// the starts and ends of launches.
 #include <algorithm>
 #include <cooperative_groups.h>
 #include <type_traits>
@@ -165,8 +167,8 @@ __device__ __forceinline__ float fast_inverse(float x) {
 // 4e-6 where 2^t is not 0, so that exp(r) is 1 + r (Cody and Waite's reduction with
 // t in the whole number's place).  2^t alone is off by the roundings of t and log2 e
 // too, 58 units in the last place 60 below 0; this by 2^t's four, one of the
-// product, and |t| / 30 for log 2 in f32.  65536 x 384, both passes: 96 us instead
-// of 90.
+// product, and |t| / 30 for log 2 in f32.  A training step of 65536 x 384 takes 91
+// us with it, 86 without.
 __device__ __forceinline__ void exp_of(uint64_t x, float& a, float& b) {
   constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
   const uint64_t t = mul2(x, two(kLog2e, kLog2e));

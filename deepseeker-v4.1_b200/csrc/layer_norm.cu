@@ -259,8 +259,8 @@ struct Turn {
 // from the first use to the second 40 (and 52 once they spilled).  4096 x 8192
 // f32, with its join: 72 us; 88 with xh as (x - mean) r.
 //
-// 8192 x 4095, forward and backward: 131 us bf16 (184 with single values in
-// registers), 4096 x 8191 144 (303).
+// 8192 x 4095, forward and backward: 127 us bf16 (184 with single values in
+// registers), 4096 x 8191 142 (303).
 template <typename T, typename P, int VEC, int V, int THREADS>
 __global__ void __launch_bounds__(512, Turn<VEC, V>::kThreads / 512) backward_kernel(const Backward p) {
   using U = Turn<VEC, V>;
