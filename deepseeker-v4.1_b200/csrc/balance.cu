@@ -522,19 +522,29 @@ __global__ void __launch_bounds__(kThreads, blocks_of(VEC, NV)) backward_kernel(
         z += __shfl_xor_sync(0xffffffffu, z, o);
         d += __shfl_xor_sync(0xffffffffu, d, o);
       }
+      if constexpr (!SOFTMAX) {
+        // Roots that are all next to 0: neither their products with c nor g / Z need
+        // be numbers of f32.  With Z below 2^-13 every logit is below -17 and a root
+        // twice its slope, so both are taken 2^n times as large, Z in [1, 2).
+        const bool small = z < 1.220703125e-4f && z > 0.0f;
+        if (__any_sync(0xffffffffu, small)) {
+          const float up = small ? __uint_as_float((254u - (__float_as_uint(z) >> 23)) << 23) : 1.0f;
+          float e = 0.0f;
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            slope[j] *= up;
+            e = fmaf(slope[j], c[j], e);
+          }
+          e = group_sum(e, G);
+          if (small) z *= up, d = 2.0f * e;
+        }
+      }
       const float inv = z == 0.0f ? 0.0f : 1.0f / z, k = live ? g * inv : 0.0f;
       d *= inv;
-      auto slopes = [&](int j) { return SOFTMAX ? two(v[j], v[j + 1]) : two(slope[SOFTMAX ? 0 : j], slope[SOFTMAX ? 0 : j + 1]); };
-      auto differences = [&](int j) { return add2(two(c[j], c[j + 1]), two(-d, -d)); };
-      if (SOFTMAX || fabsf(k) < INFINITY) {
 #pragma unroll
-        for (int j = 0; j < N; j += 2) split(mul2(mul2(two(k, k), slopes(j)), differences(j)), v[j], v[j + 1]);
-      } else {
-        // sums near the smallest numbers of f32: g / Z leaves f32 where its product
-        // with the slope does not
-#pragma unroll
-        for (int j = 0; j < N; j += 2)
-          split(mul2(mul2(two(inv, inv), slopes(j)), mul2(two(g, g), differences(j))), v[j], v[j + 1]);
+      for (int j = 0; j < N; j += 2) {
+        const uint64_t a = SOFTMAX ? two(v[j], v[j + 1]) : two(slope[SOFTMAX ? 0 : j], slope[SOFTMAX ? 0 : j + 1]);
+        split(mul2(mul2(two(k, k), a), add2(two(c[j], c[j + 1]), two(-d, -d))), v[j], v[j + 1]);
       }
       if (row < to) {
 #pragma unroll

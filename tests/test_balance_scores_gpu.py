@@ -104,3 +104,15 @@ def test_what_is_kept_for_the_backward_pass(offsets, cuda):
     held = {t.untyped_storage().data_ptr(): t.untyped_storage().nbytes() for t in loss.grad_fn.saved_tensors if t is not None}
     del held[l.data_ptr()]
     assert sum(held.values()) <= (4 * 64 if off is None else 2 * 4 * 64 + 3 * 8)
+
+
+def test_low_rows_of_long_sequences(cuda):
+    """Coefficients of a long sequence are small: their products with the smallest scores leave f32, d does not."""
+    g = torch.Generator(device=cuda).manual_seed(4)
+    l = -172 + 12 * torch.rand(60000, 16, generator=g, device=cuda)
+    ids = torch.randint(0, 16, (60000, 2), generator=g, device=cuda, dtype=torch.int32)
+    for up in (1.0, 1e5, 1e-25):
+        got = grad(l, ids, "sqrtsoftplus", up).double()
+        want, size = gradient(l, ids, "sqrtsoftplus", up)
+        # as for low rows; and half the smallest number where the result itself is that small
+        assert bool(((got - want).abs() <= 64 * U * size + 2.0 ** -149).all()), float(((got - want).abs() / size).max() / U)
